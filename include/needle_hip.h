@@ -317,6 +317,138 @@ int32_t nhip_attention_decode_noalloc_dev(const int8_t* d_q, const float* d_q_sc
                                           const int32_t* d_row_first, const int32_t* d_row_count,
                                           int32_t max_chunks, float* d_out, void* stream);
 
+/* --------------------------------------------- paged KV cache (serving) -- */
+
+/* No counterpart in the reference: an int8 KV cache in pages, for servers
+ * whose sequences grow, branch and end at different times.  The pooled cache
+ * above gives every slot its whole capacity and copies a slot position by
+ * position; here a sequence holds pages of `page_size` positions named by its
+ * row of `tables`, sequences share pages, and a page is copied only when one
+ * of its holders writes past a shared part.
+ *
+ * The caller owns every array (device memory; the four pools 16-byte aligned):
+ *   keys         int8 [layers][pages][kv_heads][page_size][qk_dim]
+ *   key_scales   fp32 [layers][pages][kv_heads][page_size]
+ *   values       int8 [layers][pages][kv_heads][page_size/16][v_dim][16]
+ *   value_scales fp32 [layers][pages][kv_heads][page_size]
+ *   tables       int32 [sequences][width]: the page of positions
+ *                [t*page_size, (t+1)*page_size), -1 past the sequence's pages
+ *   lengths      int32 [sequences]: positions held; a sequence holds the
+ *                ceil(length / page_size) pages that its row begins with
+ *   refs         int32 [pages]: how many sequences hold a page (0: free)
+ * A page holds a kv head's positions together, and 16 positions of a value
+ * dimension together, so that both products of attention read matrix
+ * operands straight from the cache.
+ * page_size 16, 32, 64, 128 or 256; (qk_dim, v_dim) (48, 64), (64, 64) or
+ * (128, 128); kv_heads <= 256; layers <= 4096; pages <= 2^20; sequences <=
+ * 65536; width * page_size <= 2^30; a call takes up to 2^24 rows.
+ *
+ * The calls below take this struct by pointer (read during the call), are
+ * asynchronous on `stream` and may be captured in a graph; calls that write
+ * a cache must be ordered with the other calls on it.  A table entry outside
+ * [0, pages) is never followed. */
+typedef struct nhip_paged_cache {
+    int8_t* keys;
+    float* key_scales;
+    int8_t* values;
+    float* value_scales;
+    int32_t* tables;
+    int32_t* lengths;
+    int32_t* refs;
+    int32_t layers, pages, page_size, kv_heads, qk_dim, v_dim, sequences, width;
+} nhip_paged_cache;
+
+/* An empty cache: tables -1, lengths and refs 0 (the pools need no clearing). */
+int32_t nhip_paged_reset_dev(const nhip_paged_cache* c, void* stream);
+
+/* Row r's new key and value, QuantizeInt8 (src/Needle/Scalar.cs:67-74) per kv
+ * head, into layer `layer` at position row_pos[r] of sequence row_seq[r]:
+ * keys d_k[r*ldk + kvh*qk_dim ..], values d_v[r*ldv + kvh*v_dim ..] (fp32;
+ * columns of a wider matrix such as a fused Q/K/V projection's output;
+ * ldk >= kv_heads*qk_dim, ldv >= kv_heads*v_dim).  The position's page must
+ * be held already (nhip_paged_resize_dev) and by this sequence alone; rows
+ * whose sequence, position or page is out of range write nothing.  Two rows
+ * of a call at one position leave it unspecified.  lengths are not read. */
+int32_t nhip_paged_append_dev(const nhip_paged_cache* c, int32_t layer, const float* d_k, int32_t ldk,
+                              const float* d_v, int32_t ldv, const int32_t* d_row_seq, const int32_t* d_row_pos,
+                              int32_t rows, void* stream);
+
+/* Attention of one new token per row: row r's query heads (q int8
+ * [rows][heads][qk_dim] with q_scales [rows][heads], QuantizeInt8 per head)
+ * attend positions row_first[r] .. row_first[r]+row_count[r]-1 of sequence
+ * row_seq[r]; query head h reads kv head h / (heads/kv_heads) and scores are
+ * scaled by 1/sqrt(qk_dim), as in nhip_attention_decode_dev.  out fp32
+ * [rows][heads][v_dim].  Softmax statistics and sums are fp32 and the result
+ * is within 1e-5 of RMS(out) of exact arithmetic; it is the same for the same
+ * call, but not the bits of the reference's order.  max_count bounds every
+ * row_count (it decides how the work is split).  Rows of count 0, and rows
+ * whose sequence or span is out of range or whose count exceeds max_count,
+ * give zeros; positions on pages outside [0, pages) are left out.
+ * heads/kv_heads <= 16; q and out 16-byte aligned.  The workspace needs no
+ * initialisation; calls that may overlap need one each. */
+size_t nhip_paged_decode_workspace(const nhip_paged_cache* c, int32_t rows, int32_t heads, int32_t max_count);
+int32_t nhip_paged_decode_dev(const nhip_paged_cache* c, int32_t layer, const int8_t* d_q, const float* d_q_scales,
+                              int32_t rows, int32_t heads, const int32_t* d_row_seq, const int32_t* d_row_first,
+                              const int32_t* d_row_count, int32_t max_count, void* d_workspace,
+                              size_t workspace_bytes, float* d_out, void* stream);
+
+/* Causal attention of whole prompts, or of their next parts, packed one
+ * behind the other: run i is the rows run_rows[i] .. run_rows[i+1]-1 (device
+ * array [runs+1], ascending), which sit at positions run_pos[i], run_pos[i]+1,
+ * ... of sequence run_seq[i].  Their keys and values are in the cache already
+ * (nhip_paged_append_dev), as are those of the positions before them.  The row
+ * at position p attends [0, p], or with window > 0 [max(0, p-window+1), p].
+ * Everything else as nhip_paged_decode_dev; max_count bounds every position
+ * + 1 (rows beyond give zeros), and rows behind the last run are left as they
+ * are. */
+size_t nhip_paged_prompt_workspace(const nhip_paged_cache* c, int32_t rows, int32_t heads, int32_t runs,
+                                   int32_t max_count);
+int32_t nhip_paged_prompt_dev(const nhip_paged_cache* c, int32_t layer, const int8_t* d_q, const float* d_q_scales,
+                              int32_t rows, int32_t heads, int32_t runs, const int32_t* d_run_rows,
+                              const int32_t* d_run_seq, const int32_t* d_run_pos, int32_t window, int32_t max_count,
+                              void* d_workspace, size_t workspace_bytes, float* d_out, void* stream);
+
+/* Pages.  All of a call's entries act together (as if every entry read the
+ * cache as it was before the call); of entries that name the same sequence
+ * only the first counts, and entries out of range do nothing.  count <= 1024.
+ * The workspace holds nhip_paged_pages_workspace bytes, needs no
+ * initialisation, and one call's is free for the next call of the stream.
+ *
+ * copy     page src[i]'s contents (all layers) to page dst[i]; tables and refs
+ *          stay.  A page may be the source of several entries, but must not be
+ *          the destination of one and named by another.
+ * fork     sequence dst[i] gives up its pages and becomes a copy of the first
+ *          length[i] positions of sequence src[i] (d_length NULL, or a longer
+ *          length: all of it), sharing its pages (refs).  A beam step's
+ *          reorder is one call with dst 0..n-1 and src the beams' parents.
+ * resize   sequence seq[i] takes length[i].  Shorter: pages past it are given
+ *          up.  Longer: if its last page is partly filled and held by others
+ *          too, it gets a copy of that page; then it takes the pages it lacks.
+ *          (Of several entries of one call that grow into the same page, as
+ *          many of the first copy it as leave one holder.)  Pages are taken in
+ *          entry order, the lowest free page first; pages given up in the
+ *          call are free from the next call on.  If the free pages do not
+ *          suffice nothing changes at all.  d_status (may be NULL) int32 [2]:
+ *          the pages missing (0: done; an entry that lacks more than the pool
+ *          has counts as pages + 1), the entries refused (out of range).
+ *          A refused entry keeps its sequence as it is.
+ * free     resize to 0.
+ * compact  moves pages to the front of the pool: with n pages held, the k-th
+ *          free page below n takes the contents and holders of the k-th held
+ *          page from n on.  d_status (may be NULL) int32 [1]: n. */
+size_t nhip_paged_pages_workspace(const nhip_paged_cache* c, int32_t count);
+int32_t nhip_paged_copy_dev(const nhip_paged_cache* c, int32_t count, const int32_t* d_src, const int32_t* d_dst,
+                            void* stream);
+int32_t nhip_paged_fork_dev(const nhip_paged_cache* c, int32_t count, const int32_t* d_dst, const int32_t* d_src,
+                            const int32_t* d_length, void* d_workspace, size_t workspace_bytes, void* stream);
+int32_t nhip_paged_resize_dev(const nhip_paged_cache* c, int32_t count, const int32_t* d_seq,
+                              const int32_t* d_length, int32_t* d_status, void* d_workspace, size_t workspace_bytes,
+                              void* stream);
+int32_t nhip_paged_free_dev(const nhip_paged_cache* c, int32_t count, const int32_t* d_seq, void* d_workspace,
+                            size_t workspace_bytes, void* stream);
+int32_t nhip_paged_compact_dev(const nhip_paged_cache* c, int32_t* d_status, void* d_workspace,
+                               size_t workspace_bytes, void* stream);
+
 /* ------------------------------------ Needle 3 attention inputs (rows) -- */
 
 /* Needle 3's step from a row's raw Q/K/V projections to its int8 query heads

@@ -123,6 +123,19 @@ _PROTOS = {
     "nhip_attention_decode_workspace_init": (_i32, [_vp, _sz, _vp]),
     "nhip_attention_decode_dev": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _vp,
                                          _vp, _i32, _vp, _sz, _vp, _vp]),
+    "nhip_paged_reset_dev": (_i32, [_vp, _vp]),
+    "nhip_paged_append_dev": (_i32, [_vp, _i32, _vp, _i32, _vp, _i32, _vp, _vp, _i32, _vp]),
+    "nhip_paged_decode_workspace": (_sz, [_vp, _i32, _i32, _i32]),
+    "nhip_paged_decode_dev": (_i32, [_vp, _i32, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _i32, _vp, _sz, _vp, _vp]),
+    "nhip_paged_prompt_workspace": (_sz, [_vp, _i32, _i32, _i32, _i32]),
+    "nhip_paged_prompt_dev": (_i32, [_vp, _i32, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _i32, _i32, _vp, _sz, _vp,
+                                     _vp]),
+    "nhip_paged_pages_workspace": (_sz, [_vp, _i32]),
+    "nhip_paged_copy_dev": (_i32, [_vp, _i32, _vp, _vp, _vp]),
+    "nhip_paged_fork_dev": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "nhip_paged_resize_dev": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "nhip_paged_free_dev": (_i32, [_vp, _i32, _vp, _vp, _sz, _vp]),
+    "nhip_paged_compact_dev": (_i32, [_vp, _vp, _vp, _sz, _vp]),
     "nhip_table_release": (_i32, [_vp, _sz, _vp]),
     "nhip_table_cached": (_i32, [_vp, _vp]),
     "nhip_matmul_batch_dev": (_i32, [_vp, _i32, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp]),
