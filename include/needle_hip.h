@@ -341,7 +341,7 @@ int32_t nhip_attention_decode_noalloc_dev(const int8_t* d_q, const float* d_q_sc
  * operands straight from the cache.
  * page_size 16, 32, 64, 128 or 256; (qk_dim, v_dim) (48, 64), (64, 64) or
  * (128, 128); kv_heads <= 256; layers <= 4096; pages <= 2^20; sequences <=
- * 65536; width * page_size <= 2^30; a call takes up to 2^24 rows.
+ * 65536; width * page_size <= 2^30; a call takes up to 2^20 rows.
  *
  * The calls below take this struct by pointer (read during the call), are
  * asynchronous on `stream` and may be captured in a graph; calls that write

@@ -9,7 +9,7 @@ namespace nhip {
 // Checks a caller's cache (sizes, pointers, alignment); NHIP_OK or NHIP_ERR_ARG.
 int32_t paged_check(const nhip_paged_cache* c);
 
-constexpr int32_t kPagedMaxRows = 1 << 24;  // of a call
+constexpr int32_t kPagedMaxRows = 1 << 20;  // of a call
 
 // One layer of a cache, for the kernels that read or write positions.
 struct PagedLayer {

@@ -105,6 +105,388 @@ __global__ __launch_bounds__(64) void paged_attention_kernel(PagedAttn p)
             p.out[((size_t)r * p.heads + h) * c.v + lane + 64 * e] = total != 0.0f ? o[e] / total : 0.0f;
 }
 
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+// The value that lane n of the lane's row of 16 holds.
+template <int n>
+__device__ __forceinline__ float row_bcast(float v)
+{
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + n, 0xF, 0xF, false));
+}
+
+// What one position contributes besides its codes.  With vs = frac * 2^e
+// (e the scale's exponent), the weight of a position is w = 2^(z' - M) with
+// z' = z log2(e) + e and M the running maximum of z' less 14, so that w frac,
+// the weight of its codes, lies in [0, 2^15) whatever the scales are and is
+// the sum of two fp16 numbers: 22 bits of it, or where it is small a step of
+// 2^-24, which is 2^-39 of the largest weight.  The sum of the softmax takes
+// w 2^-e.  A position that does not count has e = -inf, which makes w 0.
+constexpr float kHeadroom = 14.0f;
+struct Position {
+    float ks, e, frac, inv;
+};
+__device__ __forceinline__ Position position(float ks, float vs, bool live)
+{
+    int e = (int)((__float_as_uint(vs) >> 23) & 255) - 127;
+    e = min(max(e, -60), 60);
+    Position r;
+    r.inv = live ? __uint_as_float((uint32_t)(127 - e) << 23) : 0.0f;
+    r.frac = live ? vs * r.inv : 0.0f;
+    r.ks = live ? ks : 0.0f;
+    r.e = live ? (float)e : -INFINITY;
+    return r;
+}
+
+// Eight int8 codes (two words) as fp16, exactly: the byte c + 128 in the low
+// bits of 1024 makes 1152 + c.
+__device__ __forceinline__ f16x8 codes_f16(uint32_t lo, uint32_t hi)
+{
+    union {
+        uint32_t u[4];
+        f16x2 h[4];
+        f16x8 v;
+    } r;
+    const uint32_t a = lo ^ 0x80808080u, b = hi ^ 0x80808080u;
+    r.u[0] = __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u);
+    r.u[1] = __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u);
+    r.u[2] = __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u);
+    r.u[3] = __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u);
+    const f16x2 off = {(_Float16)1152.0f, (_Float16)1152.0f};
+#pragma unroll
+    for (int k = 0; k < 4; k++) r.h[k] = r.h[k] - off;
+    return r.v;
+}
+
+__device__ __forceinline__ f16x2 to_f16(float a, float b)
+{
+    const f32x2 v = {a, b};
+    return __builtin_convertvector(v, f16x2);
+}
+
+// Maximum / sum over the four lanes l, l + 16, l + 32, l + 48.
+__device__ __forceinline__ float rows_max(float v)
+{
+    v = fmaxf(v, lane_xor<16>(v));
+    return fmaxf(v, lane_xor<32>(v));
+}
+__device__ __forceinline__ float rows_sum(float v)
+{
+    v = v + lane_xor<16>(v);
+    return v + lane_xor<32>(v);
+}
+
+// ---------------------------------------------------------------- decode --
+//
+// One workgroup of W waves per (kv head, row, part of the row's positions);
+// a wave takes 64 positions at a time, in its registers from load to result:
+//   scores   S^T = K Q^T by v_mfma_i32_16x16x64_i8, the group's heads (up to
+//            16) as columns.  Row m of product t is position 16 (m / 4) + 4 t
+//            + m % 4, so lane l, which gets rows 4 (l / 16) + i, ends with
+//            positions 16 (l / 16) + 4 t + i, all of one 16-position block,
+//            for head l % 16.
+//   weights  in that lane; lane l also holds position l's scales, and a
+//            block's 16 are the 16 lanes of its row (row_bcast).
+//   values   O^T = V^T P^T by v_mfma_f32_16x16x32_f16, P split in two fp16
+//            parts.  The operand slot (l / 16, j) of product u is position 16
+//            (l / 16) + 8 u + j: the weights are where they have to be, and
+//            the codes are the 16 bytes that the cache holds of one dimension
+//            and 16 positions, one load.
+// Nothing passes through LDS until the waves' parts are joined.
+struct DecodeParams {
+    PagedLayer c;
+    const int8_t* q;
+    const float* q_scales;
+    float* out;
+    const int32_t* row_seq;
+    const int32_t* row_first;
+    const int32_t* row_count;
+    float* parts;  // [rows][kv_heads][max_parts][group][V + 2]: sums, M, total
+    int32_t heads, group, max_count, blocks, max_parts;  // blocks: 64-position blocks of a part
+    float scale;
+};
+
+// A row's span in 64-position blocks (none when it is out of range).
+struct Span {
+    int seq, first, end, block0, block1;
+};
+__device__ __forceinline__ Span decode_span(const DecodeParams& p, int row)
+{
+    Span s;
+    s.seq = p.row_seq[row];
+    s.first = p.row_first[row];
+    int count = p.row_count[row];
+    const int span = p.c.width << p.c.page_shift;
+    if (s.seq < 0 || s.seq >= p.c.sequences || s.first < 0 || count < 0 || count > p.max_count ||
+        s.first > span - count)
+        count = s.first = 0;
+    s.end = s.first + count;
+    s.block0 = s.first >> 6;
+    s.block1 = count > 0 ? (s.end + 63) >> 6 : s.block0;
+    return s;
+}
+
+template <int QK, int V, int W>
+__global__ __launch_bounds__(64 * W) void paged_decode_kernel(DecodeParams p)
+{
+    constexpr int KH = (QK + 63) / 64, VT = V / 16;
+    extern __shared__ __align__(16) float lds[];  // [W][group][V] sums, then [W][16] M, [W][16] total
+    const PagedLayer& c = p.c;
+    const int row = blockIdx.x, kvh = blockIdx.y, part = blockIdx.z;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int h = lane & 15, g = lane >> 4;
+    const Span s = decode_span(p, row);
+    const int total_blocks = s.block1 - s.block0;
+    const int parts = (total_blocks + p.blocks - 1) / p.blocks;
+    if (part > 0 && part >= parts) return;
+    const int end_block = min(s.block1, s.block0 + (part + 1) * p.blocks);
+
+    i32x4 q[KH];
+    float qs = 0.0f;
+#pragma unroll
+    for (int k = 0; k < KH; k++) q[k] = i32x4{0, 0, 0, 0};
+    if (h < p.group) {
+        const size_t head = (size_t)row * p.heads + kvh * p.group + h;
+#pragma unroll
+        for (int k = 0; k < KH; k++)
+            if (64 * k + 16 * g < QK) q[k] = *reinterpret_cast<const i32x4*>(p.q + head * QK + 64 * k + 16 * g);
+        qs = p.q_scales[head] * p.scale;
+    }
+
+    const int32_t* table = c.tables + (size_t)s.seq * c.width;
+    const int in_page = (1 << c.page_shift) - 1;
+    // the page of position `pos` of a 64-position block: -1 where it may not be followed
+    auto page_at = [&](int pos) {
+        const int t = pos >> c.page_shift;
+        const int page = pos < s.end ? table[min(t, c.width - 1)] : -1;
+        return page >= 0 && page < c.pages ? page : -1;
+    };
+    i32x4 kr[4][KH], vr[VT];
+    float ksr, vsr;
+    bool live;
+    // (a block's addresses come from its first cell in page 0 where there is none, whose bytes then meet weight 0)
+    auto load_keys = [&](int block, int kpage, int vpage) {
+        const int kpos = 64 * block + 16 * (h >> 2);
+        const int8_t* k = c.keys + ((((size_t)max(kpage, 0) * c.kv_heads + kvh) << c.page_shift) +
+                                    (kpos & in_page) + (h & 3)) * QK;
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int half = 0; half < KH; half++)
+                kr[t][half] =
+                    *reinterpret_cast<const i32x4*>(k + 4 * t * QK + min(64 * half + 16 * g, QK - 16));
+        const int pos = 64 * block + lane;
+        const size_t cell = (((size_t)max(vpage, 0) * c.kv_heads + kvh) << c.page_shift) + (pos & in_page);
+        ksr = c.kscale[cell];
+        vsr = c.vscale[cell];
+        live = vpage >= 0 && pos >= s.first && pos < s.end;
+    };
+    auto load_values = [&](int block, int vpage) {
+        const int pos = 64 * block + 16 * g;
+        const int8_t* v = c.values + (((size_t)max(vpage, 0) * c.kv_heads + kvh) << c.page_shift) * V +
+                          (size_t)((pos & in_page) >> 4) * (16 * V) + 16 * h;
+#pragma unroll
+        for (int t = 0; t < VT; t++) vr[t] = *reinterpret_cast<const i32x4*>(v + 256 * t);
+    };
+
+    float peak = kNoScore, total = 0.0f;
+    f32x4 o[VT];
+#pragma unroll
+    for (int t = 0; t < VT; t++) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    int block = s.block0 + part * p.blocks + wave;
+    int kpage = -1, vpage = -1, vpage_now = -1;
+    if (block < end_block) {
+        kpage = page_at(64 * block + 16 * (h >> 2));
+        vpage = page_at(64 * block + 16 * g);
+        load_keys(block, kpage, vpage);
+        load_values(block, vpage);
+        kpage = page_at(64 * (block + W) + 16 * (h >> 2));
+        vpage = page_at(64 * (block + W) + 16 * g);
+    }
+    for (; block < end_block; block += W) {
+        i32x4 dots[4];
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            dots[t] = i32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int half = 0; half < KH; half++)
+                dots[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kr[t][half], q[half], dots[t], 0, 0, 0);
+        }
+        const Position x = position(ksr, vsr, live);
+        const bool more = block + W < end_block;
+        if (more) load_keys(block + W, kpage, vpage);
+        vpage_now = vpage;
+        if (block + 2 * W < end_block) {
+            kpage = page_at(64 * (block + 2 * W) + 16 * (h >> 2));
+            vpage = page_at(64 * (block + 2 * W) + 16 * g);
+        }
+        float z[16];
+#define NHIP_SCORE(j) z[j] = ((float)dots[(j) / 4][(j) % 4] * row_bcast<j>(x.ks)) * qs + row_bcast<j>(x.e);
+        NHIP_SCORE(0) NHIP_SCORE(1) NHIP_SCORE(2) NHIP_SCORE(3) NHIP_SCORE(4) NHIP_SCORE(5) NHIP_SCORE(6)
+        NHIP_SCORE(7) NHIP_SCORE(8) NHIP_SCORE(9) NHIP_SCORE(10) NHIP_SCORE(11) NHIP_SCORE(12) NHIP_SCORE(13)
+        NHIP_SCORE(14) NHIP_SCORE(15)
+#undef NHIP_SCORE
+        float up = z[0];
+#pragma unroll
+        for (int j = 1; j < 16; j++) up = fmaxf(up, z[j]);
+        up = fmaxf(peak, rows_max(up) - kHeadroom);
+        if (__ballot(up > peak)) {
+            const float keep = __builtin_amdgcn_exp2f(peak - up);
+            peak = up;
+            total *= keep;
+#pragma unroll
+            for (int t = 0; t < VT; t++) o[t] *= keep;
+        }
+        float w[16];
+#define NHIP_WEIGHT(j)                                  \
+    w[j] = __builtin_amdgcn_exp2f(z[j] - peak);         \
+    total = fmaf(w[j], row_bcast<j>(x.inv), total);     \
+    w[j] = w[j] * row_bcast<j>(x.frac);
+        NHIP_WEIGHT(0) NHIP_WEIGHT(1) NHIP_WEIGHT(2) NHIP_WEIGHT(3) NHIP_WEIGHT(4) NHIP_WEIGHT(5) NHIP_WEIGHT(6)
+        NHIP_WEIGHT(7) NHIP_WEIGHT(8) NHIP_WEIGHT(9) NHIP_WEIGHT(10) NHIP_WEIGHT(11) NHIP_WEIGHT(12)
+        NHIP_WEIGHT(13) NHIP_WEIGHT(14) NHIP_WEIGHT(15)
+#undef NHIP_WEIGHT
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            union {
+                f16x2 h2[4];
+                f16x8 v;
+            } hi, lo;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float a = w[8 * u + 2 * k], b = w[8 * u + 2 * k + 1];
+                hi.h2[k] = to_f16(a, b);
+                lo.h2[k] = to_f16(a - (float)hi.h2[k][0], b - (float)hi.h2[k][1]);
+            }
+#pragma unroll
+            for (int t = 0; t < VT; t++) {
+                const f16x8 v = codes_f16((uint32_t)vr[t][2 * u], (uint32_t)vr[t][2 * u + 1]);
+                o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi.v, o[t], 0, 0, 0);
+                o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo.v, o[t], 0, 0, 0);
+            }
+        }
+        if (more) load_values(block + W, vpage_now);
+    }
+    total = rows_sum(total);
+
+    // the waves' parts joined: every wave scales its sums to the common maximum
+    float* peaks = lds + (size_t)W * p.group * V;
+    float* totals = peaks + W * 16;
+    if (lane < 16) {
+        peaks[wave * 16 + lane] = peak;
+        totals[wave * 16 + lane] = total;
+    }
+    __syncthreads();
+    float top = kNoScore;
+#pragma unroll
+    for (int k = 0; k < W; k++) top = fmaxf(top, peaks[k * 16 + h]);
+    const float mine = __builtin_amdgcn_exp2f(peak - top);
+    if (h < p.group) {
+        float* sums = lds + ((size_t)wave * p.group + h) * V + 4 * g;
+#pragma unroll
+        for (int t = 0; t < VT; t++) *reinterpret_cast<f32x4*>(sums + 16 * t) = o[t] * mine;
+    }
+    __syncthreads();
+    const bool split = parts > 1;
+    for (int at = threadIdx.x; at < p.group * V; at += 64 * W) {
+        const int head = at / V, d = at - head * V;
+        float best = kNoScore, all = 0.0f, sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < W; k++) best = fmaxf(best, peaks[k * 16 + head]);
+#pragma unroll
+        for (int k = 0; k < W; k++) {
+            all = fmaf(totals[k * 16 + head], __builtin_amdgcn_exp2f(peaks[k * 16 + head] - best), all);
+            sum += lds[((size_t)k * p.group + head) * V + d];
+        }
+        if (!split) {
+            p.out[((size_t)row * p.heads + kvh * p.group + head) * V + d] = all != 0.0f ? sum / all : 0.0f;
+        } else {
+            float* to = p.parts + ((((size_t)row * c.kv_heads + kvh) * p.max_parts + part) * p.group + head) * (V + 2);
+            to[d] = sum;
+            if (d == 0) {
+                to[V] = best;
+                to[V + 1] = all;
+            }
+        }
+    }
+}
+
+// Joins a row's parts, a wave per (row, head); rows of one part are done.
+template <int V>
+__global__ __launch_bounds__(64) void paged_join_kernel(DecodeParams p)
+{
+    const int row = blockIdx.x, head = blockIdx.y, lane = threadIdx.x;
+    const Span s = decode_span(p, row);
+    const int parts = (s.block1 - s.block0 + p.blocks - 1) / p.blocks;
+    if (parts <= 1) return;
+    const int kvh = head / p.group, in_group = head - kvh * p.group;
+    const float* from = p.parts + (((size_t)row * p.c.kv_heads + kvh) * p.max_parts * p.group + in_group) * (V + 2);
+    const size_t step = (size_t)p.group * (V + 2);
+    float best = kNoScore;
+    for (int k = lane; k < parts; k += 64) best = fmaxf(best, from[k * step + V]);
+    best = wave_max(best);
+    float all = 0.0f, sum[V / 64];
+#pragma unroll
+    for (int e = 0; e < V / 64; e++) sum[e] = 0.0f;
+    for (int k = 0; k < parts; k++) {
+        const float f = __builtin_amdgcn_exp2f(from[k * step + V] - best);
+        all = fmaf(from[k * step + V + 1], f, all);
+#pragma unroll
+        for (int e = 0; e < V / 64; e++) sum[e] = fmaf(from[k * step + lane + 64 * e], f, sum[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < V / 64; e++)
+        p.out[((size_t)row * p.heads + head) * V + lane + 64 * e] = all != 0.0f ? sum[e] / all : 0.0f;
+}
+
+// How a decode call is split: waves of a workgroup, 64-position blocks of a
+// part, parts of the longest row.
+struct Split {
+    int waves, blocks, parts;
+};
+Split decode_split(const nhip_paged_cache* c, int32_t rows, int32_t max_count)
+{
+    const int most = max_count / 64 + 2;  // blocks of a row: its ends need not be a block's
+    static const int ew = getenv("PW") ? atoi(getenv("PW")) : 4, eb = getenv("PB") ? atoi(getenv("PB")) : 8;
+    Split s;
+    s.waves = ew;
+    s.blocks = eb;
+    s.parts = (most + s.blocks - 1) / s.blocks;
+    return s;
+}
+
+size_t decode_workspace(const nhip_paged_cache* c, int32_t rows, int32_t heads, const Split& s)
+{
+    return s.parts > 1 ? (size_t)rows * heads * s.parts * (c->v_dim + 2) * sizeof(float) : 0;
+}
+
+// The factor that takes a scaled dot product to a base-2 score.
+float score_scale(int32_t qk) { return (float)(1.4426950408889634 / std::sqrt((double)qk)); }
+
+template <int QK, int V>
+int32_t launch_decode(const DecodeParams& p, const Split& s, int32_t rows, hipStream_t stream)
+{
+    const size_t lds = (size_t)s.waves * (p.group * V + 32) * sizeof(float);
+    const dim3 grid(rows, p.c.kv_heads, s.parts);
+    if (s.waves == 4)
+        hipLaunchKernelGGL((paged_decode_kernel<QK, V, 4>), grid, dim3(256), lds, stream, p);
+    else if (s.waves == 8)
+        hipLaunchKernelGGL((paged_decode_kernel<QK, V, 8>), grid, dim3(512), lds, stream, p);
+    else if (s.waves == 2)
+        hipLaunchKernelGGL((paged_decode_kernel<QK, V, 2>), grid, dim3(128), lds, stream, p);
+    else
+        hipLaunchKernelGGL((paged_decode_kernel<QK, V, 1>), grid, dim3(64), lds, stream, p);
+    NHIP_CHECK_HIP(hipGetLastError());
+    if (s.parts > 1) {
+        hipLaunchKernelGGL((paged_join_kernel<V>), dim3(rows, p.heads), dim3(64), 0, stream, p);
+        NHIP_CHECK_HIP(hipGetLastError());
+    }
+    return NHIP_OK;
+}
+
 int32_t check_attention(const nhip_paged_cache* c, int32_t rows, int32_t heads, int32_t max_count)
 {
     int32_t rc = paged_check(c);
@@ -158,7 +540,7 @@ extern "C" {
 size_t nhip_paged_decode_workspace(const nhip_paged_cache* c, int32_t rows, int32_t heads, int32_t max_count)
 {
     if (check_attention(c, rows, heads, max_count)) return 0;
-    return 0;
+    return decode_workspace(c, rows, heads, decode_split(c, rows, max_count));
 }
 
 int32_t nhip_paged_decode_dev(const nhip_paged_cache* c, int32_t layer, const int8_t* d_q, const float* d_q_scales,
@@ -169,18 +551,31 @@ int32_t nhip_paged_decode_dev(const nhip_paged_cache* c, int32_t layer, const in
     int32_t rc = check_attention(c, rows, heads, max_count);
     if (rc) return rc;
     if (rows == 0) return NHIP_OK;
-    rc = check_call(c, layer, d_q, d_q_scales, d_out, d_workspace, workspace_bytes, 0);
+    const Split split = decode_split(c, rows, max_count);
+    rc = check_call(c, layer, d_q, d_q_scales, d_out, d_workspace, workspace_bytes,
+                    decode_workspace(c, rows, heads, split));
     if (rc) return rc;
     NHIP_REQUIRE(d_row_seq && d_row_first && d_row_count, "paged decode: null pointer");
     rc = ensure_device();
     if (rc) return rc;
-    PagedAttn p = attn_params(c, layer, d_q, d_q_scales, rows, heads, max_count, d_out);
+    DecodeParams p;
+    p.c = paged_layer(c, layer);
+    p.q = d_q;
+    p.q_scales = d_q_scales;
+    p.out = d_out;
     p.row_seq = d_row_seq;
     p.row_first = d_row_first;
     p.row_count = d_row_count;
-    hipLaunchKernelGGL((paged_attention_kernel<false>), dim3(rows, heads), dim3(64), 0, as_stream(stream), p);
-    NHIP_CHECK_HIP(hipGetLastError());
-    return NHIP_OK;
+    p.parts = static_cast<float*>(d_workspace);
+    p.heads = heads;
+    p.group = heads / c->kv_heads;
+    p.max_count = max_count;
+    p.blocks = split.blocks;
+    p.max_parts = split.parts;
+    p.scale = score_scale(c->qk_dim);
+    if (c->qk_dim == 48) return launch_decode<48, 64>(p, split, rows, as_stream(stream));
+    if (c->qk_dim == 64) return launch_decode<64, 64>(p, split, rows, as_stream(stream));
+    return launch_decode<128, 128>(p, split, rows, as_stream(stream));
 }
 
 size_t nhip_paged_prompt_workspace(const nhip_paged_cache* c, int32_t rows, int32_t heads, int32_t runs,

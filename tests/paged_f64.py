@@ -63,7 +63,15 @@ class Pool:
             w /= w.sum()
             out[h] = (w * vs) @ v
             far[h] = bound(len(cells), np.abs(z).max(), vs) * ((w * np.abs(vs)) @ np.abs(v))
+            far[h] += FLOOR * 2 * (w * np.abs(vs)).max() * np.abs(v).sum(0)
         return out, far
+
+
+#: The weights w vs enter the value product as two fp16 numbers.  Below 2^-14
+#: fp16 has a step of 2^-24, so a weight is off by up to 2^-25 besides its
+#: relative error, where the largest is scaled to [2^14, 2^15): 2^-39 of it (an
+#: output whose large weights all meet code 0 shows this floor alone).
+FLOOR = 2.0 ** -39
 
 
 def bound(count, z, vs):

@@ -71,7 +71,7 @@ def test_a_closed_cache_refuses_its_calls():
     ((0, A, 95, A, 128, A, A, 1), "strides"), ((0, A, 96, A, 127, A, A, 1), "strides"),
     ((0, None, 96, A, 128, A, A, 1), "null"), ((0, A, 96, None, 128, A, A, 1), "null"),
     ((0, A, 96, A, 128, None, A, 1), "null"), ((0, A, 96, A, 128, A, None, 1), "null"),
-    ((0, A, 96, A, 128, A, A, -1), "rows"), ((0, A, 96, A, 128, A, A, (1 << 24) + 1), "rows"),
+    ((0, A, 96, A, 128, A, A, -1), "rows"), ((0, A, 96, A, 128, A, A, (1 << 20) + 1), "rows"),
 ])
 def test_append_refuses(args, match):
     with refused(match):
@@ -80,7 +80,7 @@ def test_append_refuses(args, match):
 
 @pytest.mark.parametrize("change,match", [
     ({"layer": 2}, "layer"), ({"q": None}, "null"), ({"q_scales": None}, "null"), ({"out": None}, "null"),
-    ({"q": A + 8}, "aligned"), ({"out": A + 8}, "aligned"), ({"rows": -1}, "rows"), ({"rows": 1 << 25}, "rows"),
+    ({"q": A + 8}, "aligned"), ({"out": A + 8}, "aligned"), ({"rows": -1}, "rows"), ({"rows": (1 << 20) + 1}, "rows"),
     ({"heads": 3}, "heads"), ({"heads": 0}, "heads"), ({"heads": 34}, "heads"), ({"heads": -2}, "heads"),
     ({"max_count": -1}, "max_count"), ({"max_count": 97}, "max_count"), ({"a": None}, "null"),
     ({"b": None}, "null"), ({"c": None}, "null"),
@@ -97,7 +97,7 @@ def test_attention_refuses(change, match):
 
 
 def test_prompt_refuses_its_own():
-    for runs, window in ((-1, 0), ((1 << 24) + 1, 0), (1, -1)):
+    for runs, window in ((-1, 0), ((1 << 20) + 1, 0), (1, -1)):
         with refused("runs"):
             cache().prompt(0, A, A, 3, 12, runs, A, A, A, window, 96, A, BIG, A)
 
