@@ -204,7 +204,8 @@ struct DecodeParams {
     const int32_t* row_seq;
     const int32_t* row_first;
     const int32_t* row_count;
-    float* parts;  // [rows][kv_heads][max_parts][group][V + 2]: sums, M, total
+    float* parts;  // [rows][heads][max_parts][V]: a part's sums
+    float* stats;  // [rows][heads][max_parts][2]: its maximum and total
     int32_t heads, group, max_count, blocks, max_parts;  // blocks: 64-position blocks of a part
     float scale;
 };
@@ -230,7 +231,7 @@ __device__ __forceinline__ Span decode_span(const DecodeParams& p, int row)
 }
 
 template <int QK, int V, int W>
-__global__ __launch_bounds__(64 * W) void paged_decode_kernel(DecodeParams p)
+__global__ __launch_bounds__(64 * W, QK <= 64 ? 4 : 2) void paged_decode_kernel(DecodeParams p)
 {
     constexpr int KH = (QK + 63) / 64, VT = V / 16;
     extern __shared__ __align__(16) float lds[];  // [W][group][V] sums, then [W][16] M, [W][16] total
@@ -404,42 +405,57 @@ __global__ __launch_bounds__(64 * W) void paged_decode_kernel(DecodeParams p)
         if (!split) {
             p.out[((size_t)row * p.heads + kvh * p.group + head) * V + d] = all != 0.0f ? sum / all : 0.0f;
         } else {
-            float* to = p.parts + ((((size_t)row * c.kv_heads + kvh) * p.max_parts + part) * p.group + head) * (V + 2);
-            to[d] = sum;
-            if (d == 0) {
-                to[V] = best;
-                to[V + 1] = all;
-            }
+            const size_t at_part = ((size_t)row * p.heads + kvh * p.group + head) * p.max_parts + part;
+            p.parts[at_part * V + d] = sum;
+            if (d == 0) *reinterpret_cast<float2*>(p.stats + 2 * at_part) = make_float2(best, all);
         }
     }
 }
 
-// Joins a row's parts, a wave per (row, head); rows of one part are done.
+constexpr int kMaxParts = 64;  // a lane each where they are joined
+
+// Joins a row's parts, four waves per (row, head), each a quarter of the
+// parts; rows of one part are done.
 template <int V>
-__global__ __launch_bounds__(64) void paged_join_kernel(DecodeParams p)
+__global__ __launch_bounds__(256) void paged_join_kernel(DecodeParams p)
 {
-    const int row = blockIdx.x, head = blockIdx.y, lane = threadIdx.x;
+    __shared__ float factors[kMaxParts], quarters[4][V];
+    const int row = blockIdx.x, head = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Span s = decode_span(p, row);
     const int parts = (s.block1 - s.block0 + p.blocks - 1) / p.blocks;
     if (parts <= 1) return;
-    const int kvh = head / p.group, in_group = head - kvh * p.group;
-    const float* from = p.parts + (((size_t)row * p.c.kv_heads + kvh) * p.max_parts * p.group + in_group) * (V + 2);
-    const size_t step = (size_t)p.group * (V + 2);
-    float best = kNoScore;
-    for (int k = lane; k < parts; k += 64) best = fmaxf(best, from[k * step + V]);
-    best = wave_max(best);
-    float all = 0.0f, sum[V / 64];
+    const size_t first = ((size_t)row * p.heads + head) * p.max_parts;
+    float2 stat = make_float2(kNoScore, 0.0f);
+    if (lane < parts) stat = *reinterpret_cast<const float2*>(p.stats + 2 * (first + lane));
+    const float factor = __builtin_amdgcn_exp2f(stat.x - wave_max(stat.x));
+    if (wave == 0) factors[lane] = factor;
+    float all = factor * stat.y;
+    for (int off = 32; off; off >>= 1) all += __shfl_xor(all, off);
+    __syncthreads();
+    constexpr int E = V / 64;
+    float sum[E];
 #pragma unroll
-    for (int e = 0; e < V / 64; e++) sum[e] = 0.0f;
-    for (int k = 0; k < parts; k++) {
-        const float f = __builtin_amdgcn_exp2f(from[k * step + V] - best);
-        all = fmaf(from[k * step + V + 1], f, all);
+    for (int e = 0; e < E; e++) sum[e] = 0.0f;
+    const float* from = p.parts + first * V + lane;
+    for (int k = wave; k < parts; k += 16) {
+        float x[4][E];
 #pragma unroll
-        for (int e = 0; e < V / 64; e++) sum[e] = fmaf(from[k * step + lane + 64 * e], f, sum[e]);
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+            for (int e = 0; e < E; e++) x[u][e] = from[(size_t)min(k + 4 * u, parts - 1) * V + 64 * e];
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+            for (int e = 0; e < E; e++) sum[e] = k + 4 * u < parts ? fmaf(x[u][e], factors[k + 4 * u], sum[e]) : sum[e];
     }
 #pragma unroll
-    for (int e = 0; e < V / 64; e++)
-        p.out[((size_t)row * p.heads + head) * V + lane + 64 * e] = all != 0.0f ? sum[e] / all : 0.0f;
+    for (int e = 0; e < E; e++) quarters[wave][lane + 64 * e] = sum[e];
+    __syncthreads();
+    if (threadIdx.x < V) {
+        const int d = threadIdx.x;
+        const float t = (quarters[0][d] + quarters[1][d]) + (quarters[2][d] + quarters[3][d]);
+        p.out[((size_t)row * p.heads + head) * V + d] = all != 0.0f ? t / all : 0.0f;
+    }
 }
 
 // How a decode call is split: waves of a workgroup, 64-position blocks of a
@@ -447,14 +463,30 @@ __global__ __launch_bounds__(64) void paged_join_kernel(DecodeParams p)
 struct Split {
     int waves, blocks, parts;
 };
+
+// A wave takes about 1.3 us a block beside 4 us for the launch; joining parts
+// costs 3 us.  So rows of few blocks stay whole: up to 18 (4 rows of 1024
+// positions, 16 kv heads: 7.7 us whole, 8.0 in parts; 2 rows of 1556, 4 kv
+// heads of 128: 15.5 whole, 10.9 in parts), or up to 40 where the workgroups
+// fill half the CUs anyway (16 rows of up to 2048, 16 kv heads: 13.4 us
+// whole, 15.7 in parts).  Longer ones are cut into parts of at least 8 blocks
+// such that the longest rows give 2048 workgroups (32 rows of up to 32768 on 8
+// kv heads of 128: 292 us in parts of 65 blocks, 372 in parts of 8), at most
+// kMaxParts.  Four waves a workgroup where one round of them reaches the end
+// or the workgroups are many, else eight (the 16 rows above: 13.4 and 17.1).
 Split decode_split(const nhip_paged_cache* c, int32_t rows, int32_t max_count)
 {
+    const int64_t units = (int64_t)rows * c->kv_heads;
     const int most = max_count / 64 + 2;  // blocks of a row: its ends need not be a block's
-    static const int ew = getenv("PW") ? atoi(getenv("PW")) : 4, eb = getenv("PB") ? atoi(getenv("PB")) : 8;
     Split s;
-    s.waves = ew;
-    s.blocks = eb;
+    if (most <= 18 || (most <= 40 && units >= 128)) {
+        s.blocks = most;
+    } else {
+        const int64_t even = (most * units + 2047) / 2048, fewest = (most + kMaxParts - 1) / kMaxParts;
+        s.blocks = (int)std::min<int64_t>(most, std::max<int64_t>({8, even, fewest}));
+    }
     s.parts = (most + s.blocks - 1) / s.blocks;
+    s.waves = most <= 10 || units * s.parts >= 512 ? 4 : 8;
     return s;
 }
 
@@ -473,15 +505,11 @@ int32_t launch_decode(const DecodeParams& p, const Split& s, int32_t rows, hipSt
     const dim3 grid(rows, p.c.kv_heads, s.parts);
     if (s.waves == 4)
         hipLaunchKernelGGL((paged_decode_kernel<QK, V, 4>), grid, dim3(256), lds, stream, p);
-    else if (s.waves == 8)
-        hipLaunchKernelGGL((paged_decode_kernel<QK, V, 8>), grid, dim3(512), lds, stream, p);
-    else if (s.waves == 2)
-        hipLaunchKernelGGL((paged_decode_kernel<QK, V, 2>), grid, dim3(128), lds, stream, p);
     else
-        hipLaunchKernelGGL((paged_decode_kernel<QK, V, 1>), grid, dim3(64), lds, stream, p);
+        hipLaunchKernelGGL((paged_decode_kernel<QK, V, 8>), grid, dim3(512), lds, stream, p);
     NHIP_CHECK_HIP(hipGetLastError());
     if (s.parts > 1) {
-        hipLaunchKernelGGL((paged_join_kernel<V>), dim3(rows, p.heads), dim3(64), 0, stream, p);
+        hipLaunchKernelGGL((paged_join_kernel<V>), dim3(rows, p.heads), dim3(256), 0, stream, p);
         NHIP_CHECK_HIP(hipGetLastError());
     }
     return NHIP_OK;
@@ -567,6 +595,7 @@ int32_t nhip_paged_decode_dev(const nhip_paged_cache* c, int32_t layer, const in
     p.row_first = d_row_first;
     p.row_count = d_row_count;
     p.parts = static_cast<float*>(d_workspace);
+    p.stats = p.parts + (size_t)rows * heads * split.parts * c->v_dim;
     p.heads = heads;
     p.group = heads / c->kv_heads;
     p.max_count = max_count;
