@@ -13,109 +13,25 @@ namespace {
 
 constexpr float kNoScore = -1e30f;  // the running maximum before any position: finite, so that a difference is never NaN
 
-struct PagedAttn {
-    PagedLayer c;
-    const int8_t* q;
-    const float* q_scales;
-    float* out;
-    const int32_t* row_seq;
-    const int32_t* row_first;
-    const int32_t* row_count;
-    const int32_t* run_rows;
-    const int32_t* run_seq;
-    const int32_t* run_pos;
-    int32_t rows, heads, group, runs, window, max_count;
-    float scale;  // 1 / sqrt(qk)
-};
-
-// The run that holds row r, or -1.
-__device__ int run_of(const PagedAttn& p, int r)
-{
-    for (int i = 0; i < p.runs; i++)
-        if (r >= p.run_rows[i] && r < p.run_rows[i + 1]) return i;
-    return -1;
-}
-
-// One wave per (row, head): 64 positions at a time, a lane per position for
-// the scores, a lane per value dimension for the sums.
-template <bool PROMPT>
-__global__ __launch_bounds__(64) void paged_attention_kernel(PagedAttn p)
-{
-    const PagedLayer& c = p.c;
-    const int r = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-    const int kvh = h / p.group;
-    const int span = c.width << c.page_shift;
-    int seq, first, count;
-    if constexpr (PROMPT) {
-        const int run = run_of(p, r);
-        if (run < 0) return;
-        seq = p.run_seq[run];
-        const int64_t at = (int64_t)p.run_pos[run] + (r - p.run_rows[run]);
-        const bool ok = p.run_pos[run] >= 0 && at < min(span, p.max_count);
-        first = ok && p.window > 0 ? max(0, (int)at - p.window + 1) : 0;
-        count = ok ? (int)at + 1 - first : 0;
-    } else {
-        seq = p.row_seq[r];
-        first = p.row_first[r];
-        count = p.row_count[r];
-        if (first < 0 || count < 0 || count > p.max_count || first > span - count) count = 0;
-    }
-    if (seq < 0 || seq >= c.sequences) count = 0;
-    const int8_t* q = p.q + ((size_t)r * p.heads + h) * c.qk;
-    const float qs = p.q_scales[(size_t)r * p.heads + h] * p.scale;
-    float peak = kNoScore, total = 0.0f, o[2] = {0.0f, 0.0f};
-    for (int base = 0; base < count; base += 64) {
-        const int s = base + lane, pos = first + s;
-        int page = -1;
-        if (s < count) page = c.tables[(size_t)seq * c.width + (pos >> c.page_shift)];
-        const bool live = page >= 0 && page < c.pages;
-        const int at = pos & ((1 << c.page_shift) - 1);
-        const size_t cell = live ? ((size_t)page * c.kv_heads + kvh) << c.page_shift : 0;
-        float z = -INFINITY, vs = 0.0f;
-        if (live) {
-            int dot = 0;
-            for (int d = 0; d < c.qk; d += 4)
-                dot = __builtin_amdgcn_sdot4(*(const int*)(q + d), *(const int*)(c.keys + (cell + at) * c.qk + d), dot,
-                                             false);
-            z = (float)dot * c.kscale[cell + at] * qs;
-            vs = c.vscale[cell + at];
-        }
-        const float up = fmaxf(peak, wave_max(z));
-        const float keep = expf(peak - up);
-        const float e = live ? expf(z - up) : 0.0f;
-        peak = up;
-        float sum = e;
-        for (int off = 32; off; off >>= 1) sum += __shfl_xor(sum, off);
-        total = total * keep + sum;
-        o[0] *= keep;
-        o[1] *= keep;
-        const float w = live ? e * vs : 0.0f;
-        for (int j = 0; j < 64; j++) {
-            if (!__shfl((int)live, j)) continue;
-            const float wj = __shfl(w, j);
-            const size_t first_cell = ((size_t)(uint32_t)__shfl((int)(cell >> 32), j) << 32) | (uint32_t)__shfl((int)cell, j);
-            const int aj = __shfl(at, j);
-            const int8_t* v = c.values + first_cell * c.v + (size_t)(aj >> 4) * 16 * c.v + (aj & 15);
-            for (int e2 = 0; e2 < 2; e2++)
-                if (lane + 64 * e2 < c.v) o[e2] = fmaf(wj, (float)v[16 * (lane + 64 * e2)], o[e2]);
-        }
-    }
-    for (int e = 0; e < 2; e++)
-        if (lane + 64 * e < c.v)
-            p.out[((size_t)r * p.heads + h) * c.v + lane + 64 * e] = total != 0.0f ? o[e] / total : 0.0f;
-}
-
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
+// v, but the compiler may not pair its operation with a neighbour's (which
+// keeps row_bcast from folding into it).
+__device__ __forceinline__ float alone(float v)
+{
+    asm("" : "+v"(v));
+    return v;
+}
+
 // The value that lane n of the lane's row of 16 holds.
 template <int n>
 __device__ __forceinline__ float row_bcast(float v)
 {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + n, 0xF, 0xF, false));
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x150 + n, 0xF, 0xF, true));
 }
 
 // What one position contributes besides its codes.  With vs = frac * 2^e
@@ -165,6 +81,13 @@ __device__ __forceinline__ f16x2 to_f16(float a, float b)
 {
     const f32x2 v = {a, b};
     return __builtin_convertvector(v, f16x2);
+}
+
+// a and b less their fp16 parts (minus_one: -1 that the compiler does not
+// know, so that each is one v_fma_mix_f32).
+__device__ __forceinline__ f16x2 rest_f16(float a, float b, f16x2 part, float minus_one)
+{
+    return to_f16(fmaf((float)part[0], minus_one, a), fmaf((float)part[1], minus_one, b));
 }
 
 // Maximum / sum over the four lanes l, l + 16, l + 32, l + 48.
@@ -293,6 +216,7 @@ __global__ __launch_bounds__(64 * W, QK <= 64 ? 4 : 2) void paged_decode_kernel(
         for (int t = 0; t < VT; t++) vr[t] = *reinterpret_cast<const i32x4*>(v + 256 * t);
     };
 
+    const float minus_one = alone(-1.0f);
     float peak = kNoScore, total = 0.0f;
     f32x4 o[VT];
 #pragma unroll
@@ -344,8 +268,8 @@ __global__ __launch_bounds__(64 * W, QK <= 64 ? 4 : 2) void paged_decode_kernel(
         float w[16];
 #define NHIP_WEIGHT(j)                                  \
     w[j] = __builtin_amdgcn_exp2f(z[j] - peak);         \
-    total = fmaf(w[j], row_bcast<j>(x.inv), total);     \
-    w[j] = w[j] * row_bcast<j>(x.frac);
+    total = fmaf(row_bcast<j>(x.inv), w[j], total);     \
+    w[j] = alone(row_bcast<j>(x.frac) * w[j]);
         NHIP_WEIGHT(0) NHIP_WEIGHT(1) NHIP_WEIGHT(2) NHIP_WEIGHT(3) NHIP_WEIGHT(4) NHIP_WEIGHT(5) NHIP_WEIGHT(6)
         NHIP_WEIGHT(7) NHIP_WEIGHT(8) NHIP_WEIGHT(9) NHIP_WEIGHT(10) NHIP_WEIGHT(11) NHIP_WEIGHT(12)
         NHIP_WEIGHT(13) NHIP_WEIGHT(14) NHIP_WEIGHT(15)
@@ -360,7 +284,7 @@ __global__ __launch_bounds__(64 * W, QK <= 64 ? 4 : 2) void paged_decode_kernel(
             for (int k = 0; k < 4; k++) {
                 const float a = w[8 * u + 2 * k], b = w[8 * u + 2 * k + 1];
                 hi.h2[k] = to_f16(a, b);
-                lo.h2[k] = to_f16(a - (float)hi.h2[k][0], b - (float)hi.h2[k][1]);
+                lo.h2[k] = rest_f16(a, b, hi.h2[k], minus_one);
             }
 #pragma unroll
             for (int t = 0; t < VT; t++) {
@@ -515,6 +439,397 @@ int32_t launch_decode(const DecodeParams& p, const Split& s, int32_t rows, hipSt
     return NHIP_OK;
 }
 
+// ---------------------------------------------------------------- prompt --
+//
+// A workgroup of four waves takes 128 queries of one kv head and run; a query
+// is a (row, head of the group) pair, row-major, so a tile is whole rows of
+// all the group's heads whatever their number.  It walks the positions its
+// rows attend 64 at a time.  The codes of a tile are staged in LDS by all
+// four waves (keys as they are, values as fp16, each converted once), two
+// tiles deep: the next one's loads are issued before a tile's products and
+// stored after them.  Each wave keeps 32 queries as columns:
+//   scores   S^T = K Q^T by v_mfma_i32_32x32x32_i8; row m = 8 b + 4 g + i of a
+//            product (b = m / 8) is position 16 (b / 2) + 8 g + 4 (b % 2) + i,
+//            so lane (g, query) gets in register r = 4 b + i position
+//            16 (r / 8) + 8 g + r % 8 of its 32.
+//   weights  in that lane.  Its row of 16 lanes holds those 16 positions'
+//            scales, lane r of it register r's (row_bcast folds into the
+//            multiplication), and a query's maximum and total are its lane's.
+//   values   O^T = V^T P^T by v_mfma_f32_32x32x16_f16: registers 8 u .. 8 u + 7
+//            are the eight weights that product u wants of this lane.
+// The weights are 2^(z - M) with M within 2^8 of the running maximum: the sums
+// are rescaled only when a maximum moves further, a few times a row.
+struct PromptParams {
+    PagedLayer c;
+    const int8_t* q;
+    const float* q_scales;
+    float* out;
+    const int32_t* run_rows;
+    const int32_t* run_seq;
+    const int32_t* run_pos;
+    float* parts;  // as DecodeParams'
+    float* stats;
+    int32_t rows, heads, group, runs, window, max_count, blocks, max_parts;
+    float scale;
+};
+
+constexpr int kTileQueries = 128;
+constexpr float kLag = 8.0f;  // log2 of how far a weight may grow past the reference before the sums are rescaled
+
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// Rows [row0, row1) of a run, cut to the call's.
+struct RunRows {
+    int row0, row1;
+};
+__device__ __forceinline__ RunRows run_rows(const PromptParams& p, int run)
+{
+    RunRows r;
+    r.row0 = min(max(p.run_rows[run], 0), p.rows);
+    r.row1 = max(r.row0, min(p.run_rows[run + 1], p.rows));
+    return r;
+}
+
+// The run of tile `tile` (the runs' tiles in order) and the tile's place in
+// it, by one wave, a lane a run; run -1 past the last.
+__device__ __forceinline__ int find_tile(const PromptParams& p, int tile, int& in_run, int& of_run)
+{
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int base = 0; base < p.runs; base += 64) {
+        int n = 0;
+        if (base + lane < p.runs) {
+            const RunRows r = run_rows(p, base + lane);
+            n = (int)(((int64_t)(r.row1 - r.row0) * p.group + kTileQueries - 1) / kTileQueries);
+        }
+        int sum = n;
+        for (int off = 1; off < 64; off <<= 1) {
+            const int up = __shfl_up(sum, off);
+            if (lane >= off) sum += up;
+        }
+        const uint64_t hit = __ballot(before + sum > tile);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            of_run = __builtin_amdgcn_readlane(n, l);
+            in_run = tile - before - (__builtin_amdgcn_readlane(sum, l) - of_run);
+            return base + l;
+        }
+        before += __builtin_amdgcn_readlane(sum, 63);
+    }
+    return -1;
+}
+
+// An int32 of an array that no kernel of the launch writes, by a scalar load.
+__device__ __forceinline__ int32_t scalar_load(const int32_t* a, int64_t i)
+{
+    return ((const __attribute__((address_space(4))) int32_t*)a)[i];
+}
+
+template <int QK, int V>
+__global__ __launch_bounds__(256, QK <= 64 ? 4 : 2) void paged_prompt_kernel(PromptParams p)
+{
+    constexpr int KS = QK <= 64 ? 64 : 128;  // bytes of a key row in LDS
+    constexpr int KK = KS / 32;              // products of 32 key bytes
+    constexpr int DT = V / 32;               // tiles of 32 value dimensions
+    constexpr int KU = KS / 64, VU = V / 64; // 16-byte units a thread stages of each
+    constexpr int KCH = QK / 16;             // units of a key row
+    __shared__ __align__(16) uint8_t lds_k[2][64 * KS];
+    __shared__ __align__(16) uint8_t lds_v[2][V * 128];
+    __shared__ float lds_ks[2][64], lds_vs[2][64];
+    const PagedLayer& c = p.c;
+    // (a tile's kv heads side by side: with 8 of them each XCD keeps one head's positions in its L2)
+    const int tile_of_call = blockIdx.x / c.kv_heads, kvh = blockIdx.x - tile_of_call * c.kv_heads;
+    const int part = blockIdx.y;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 5;
+
+    int in_run, of_run;
+    const int run = __builtin_amdgcn_readfirstlane(find_tile(p, tile_of_call, in_run, of_run));
+    if (run < 0) return;
+    const RunRows rr = run_rows(p, run);
+    const int row0 = __builtin_amdgcn_readfirstlane(rr.row0);
+    const int queries = __builtin_amdgcn_readfirstlane(rr.row1 - rr.row0) * p.group;
+    // the last tiles of a run attend most: they go first
+    const int q0 = __builtin_amdgcn_readfirstlane((of_run - 1 - in_run) * kTileQueries);
+    const int qn = min(kTileQueries, queries - q0);
+    // positions: run_pos belongs to the run's first row as the caller counts
+    // them, which may lie before row 0
+    const int seq = scalar_load(p.run_seq, run), pos_of_run = scalar_load(p.run_pos, run);
+    const int64_t pos0 = (int64_t)pos_of_run + row0 - scalar_load(p.run_rows, run);
+    const int limit = min(c.width << c.page_shift, p.max_count);
+    const bool known = seq >= 0 && seq < c.sequences && pos_of_run >= 0;
+
+    // this lane's query
+    const int query = q0 + 32 * wave + (lane & 31);
+    const bool mine = query < q0 + qn;
+    const int q_row = min(query, queries - 1) / p.group;
+    const int head = kvh * p.group + min(query, queries - 1) - q_row * p.group;
+    const int64_t far_pos = pos0 + q_row;
+    const int q_pos = known && far_pos < limit ? (int)far_pos : -1;  // -1 attends nothing
+    const int q_first = p.window > 0 ? max(q_pos - p.window + 1, 0) : 0;
+    const size_t q_at = (size_t)(row0 + q_row) * p.heads + head;
+    i32x4 q[KK];
+#pragma unroll
+    for (int k = 0; k < KK; k++) {
+        q[k] = i32x4{0, 0, 0, 0};
+        if (32 * k + 16 * g < QK) q[k] = *reinterpret_cast<const i32x4*>(p.q + q_at * QK + 32 * k + 16 * g);
+    }
+    float qs = p.q_scales[q_at] * p.scale;
+    qs = qs == 0.0f ? 1e-30f : qs;  // (a score is then 0, and a position left out still -inf)
+
+    // the wave's and the workgroup's positions (the last query's row is the furthest)
+    auto pos_of = [&](int at) {
+        const int64_t x = pos0 + at / p.group;
+        return known ? (int)(x < limit ? x : limit - 1) : -1;
+    };
+    const int wave_first = __builtin_amdgcn_readfirstlane(pos_of(min(q0 + 32 * wave, queries - 1)));
+    const int wave_last = 32 * wave < qn ? __builtin_amdgcn_readfirstlane(pos_of(min(q0 + 32 * wave + 31, queries - 1)))
+                                         : -1;
+    const int first_pos = __builtin_amdgcn_readfirstlane(pos_of(q0));
+    const int last_pos = __builtin_amdgcn_readfirstlane(pos_of(q0 + qn - 1));
+    const int from = p.window > 0 ? max(first_pos - p.window + 1, 0) : 0;
+    const int tile0 = from >> 6, tile1 = last_pos >= 0 ? (last_pos >> 6) + 1 : tile0;
+    const int begin = tile0 + part * p.blocks;
+    const int end = min(tile1, begin + p.blocks);
+
+    // staging: a wave's units lie in one 16-position block, so its page is a scalar
+    const int in_page = (1 << c.page_shift) - 1;
+    const int k_pos = QK <= 64 ? 16 * wave + lane / KCH : 8 * wave + lane / 8;  // (+ 32 for the second unit)
+    const int k_ch = QK <= 64 ? lane % KCH : lane % 8;
+    const bool k_does = QK != 48 || lane < 48;
+    const int v_block = V == 64 ? wave : wave >> 1;  // (+ 2 for the second unit)
+    const int v_dim = V == 64 ? lane : 64 * (wave & 1) + lane;
+    auto key_swizzle = [](int pos) {
+        return KS == 64 ? ((pos >> 1) & 1) | (((pos >> 3) & 1) << 1) : (pos & 3) | (((pos >> 3) & 1) << 2);
+    };
+    const int32_t* table = c.tables + (size_t)max(seq, 0) * c.width;
+    i32x4 kr[KU], vr[VU];
+    float scale_r = 0.0f;
+    uint64_t live_next = 0, live = 0;
+    auto load = [&](int tile) {
+        int page[4];
+        uint64_t ok = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int t = (64 * tile + 16 * k) >> c.page_shift;
+            page[k] = scalar_load(table, min(t, c.width - 1));
+            const bool good = page[k] >= 0 && page[k] < c.pages;
+            ok |= good ? 0xFFFFull << (16 * k) : 0;
+            page[k] = good ? page[k] : 0;
+        }
+        const int lo = from - 64 * tile, hi = last_pos + 1 - 64 * tile;  // live positions of the tile: [lo, hi)
+        if (lo > 0) ok &= ~0ull << lo;
+        if (hi < 64) ok &= (1ull << hi) - 1;
+        live_next = ok;
+        auto cell = [&](int block) {
+            const int pg = block == 0 ? page[0] : block == 1 ? page[1] : block == 2 ? page[2] : page[3];
+            return (((size_t)pg * c.kv_heads + kvh) << c.page_shift) + ((64 * tile + 16 * block) & in_page);
+        };
+#pragma unroll
+        for (int u = 0; u < KU; u++) {
+            const int block = QK <= 64 ? wave : (wave >> 1) + 2 * u;
+            if (k_does)
+                kr[u] = *reinterpret_cast<const i32x4*>(c.keys + cell(block) * QK + ((k_pos & 15) * QK + 16 * k_ch));
+        }
+#pragma unroll
+        for (int u = 0; u < VU; u++)
+            vr[u] = *reinterpret_cast<const i32x4*>(c.values + cell(v_block + 2 * u) * V + 16 * v_dim);
+        const float* s = lane & 16 ? c.vscale : c.kscale;
+        scale_r = s[cell(wave) + (lane & 15)];
+    };
+    auto store = [&](int buf) {
+#pragma unroll
+        for (int u = 0; u < KU; u++) {
+            const int pos = k_pos + 32 * u;
+            if (k_does) *reinterpret_cast<i32x4*>(lds_k[buf] + pos * KS + 16 * (k_ch ^ key_swizzle(pos))) = kr[u];
+        }
+#pragma unroll
+        for (int u = 0; u < VU; u++) {
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+                *reinterpret_cast<f16x8*>(lds_v[buf] + v_dim * 128 +
+                                          16 * ((2 * (v_block + 2 * u) + e) ^ (v_dim & 7))) =
+                    codes_f16((uint32_t)vr[u][2 * e], (uint32_t)vr[u][2 * e + 1]);
+        }
+        const int pos = 16 * wave + (lane & 15);
+        if (lane < 32) (lane & 16 ? lds_vs : lds_ks)[buf][pos] = (live >> pos) & 1 ? scale_r : 0.0f;
+    };
+
+    f32x16 o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
+    float peak = kNoScore, total[2] = {0.0f, 0.0f};
+    int exponent = -100;  // of the value scales, the largest so far
+    const float minus_one = alone(-1.0f);
+    // where this lane reads: the key row of its A row, the value rows of its dimensions
+    const int m = lane & 31;
+    const int key_row = 16 * (m >> 4) + 8 * ((m >> 2) & 1) + 4 * ((m >> 3) & 1) + (m & 3);
+    const int key_x = g ^ key_swizzle(key_row), value_x = g ^ (lane & 7);
+    const int slot = 16 * ((lane >> 3) & 1) + 8 * g + (lane & 7);  // the position whose scales this lane holds
+
+    if (begin < end) {
+        load(begin);
+        live = live_next;
+        store(0);
+    }
+    __syncthreads();
+    for (int tile = begin; tile < end; tile++) {
+        const int buf = (tile - begin) & 1;
+        const uint64_t live_now = live;
+        const bool more = tile + 1 < end;
+        if (more) load(tile + 1);
+        const bool any = 64 * tile <= wave_last && (p.window == 0 || 64 * tile + 63 >= wave_first - p.window + 1);
+        if (any) {
+            const uint8_t* kb = lds_k[buf] + key_row * KS;
+            i32x16 s[2];
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[t][r] = 0;
+#pragma unroll
+                for (int k = 0; k < KK; k++)
+                    s[t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(
+                        *reinterpret_cast<const i32x4*>(kb + 32 * t * KS + 16 * (key_x ^ (2 * k))), q[k], s[t], 0, 0, 0);
+            }
+            float ks[2], vs[2];
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                ks[t] = lds_ks[buf][32 * t + slot];
+                vs[t] = lds_vs[buf][32 * t + slot];
+            }
+            // the exponent of the value scales follows their largest (infinities and NaN aside)
+            auto exponent_of = [](float x) { return (int)((__float_as_uint(x) >> 23) & 255) - 127; };
+            const int e0 = exponent_of(vs[0]), e1 = exponent_of(vs[1]);
+            if (__ballot((e0 > exponent && e0 < 128) || (e1 > exponent && e1 < 128))) {
+                int e = max(e0 < 128 ? e0 : -100, e1 < 128 ? e1 : -100);
+                for (int off = 32; off; off >>= 1) e = max(e, __shfl_xor(e, off));
+                e = __builtin_amdgcn_readfirstlane(min(e, 100));
+                if (e > exponent) {
+                    const float keep = __uint_as_float((uint32_t)max(127 + exponent - e, 0) << 23);
+#pragma unroll
+                    for (int d = 0; d < DT; d++) o[d] *= keep;
+                    exponent = e;
+                }
+            }
+            const float unit = __uint_as_float((uint32_t)(127 - exponent) << 23);
+            const float vn[2] = {vs[0] * unit, vs[1] * unit};
+            const bool masked = live_now != ~0ull || 64 * tile + 63 > wave_first ||
+                                (p.window > 0 && 64 * tile < wave_last - p.window + 1);
+            float z[2][16];
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+#define NHIP_DOT(r) z[t][r] = alone(row_bcast<r>(ks[t]) * (float)s[t][r]);
+                NHIP_DOT(0) NHIP_DOT(1) NHIP_DOT(2) NHIP_DOT(3) NHIP_DOT(4) NHIP_DOT(5) NHIP_DOT(6) NHIP_DOT(7)
+                NHIP_DOT(8) NHIP_DOT(9) NHIP_DOT(10) NHIP_DOT(11) NHIP_DOT(12) NHIP_DOT(13) NHIP_DOT(14) NHIP_DOT(15)
+#undef NHIP_DOT
+            }
+            uint32_t counts = ~0u;  // bit 16 t + r: this lane's query attends the position
+            if (masked) {
+                counts = 0;
+                const uint64_t bits = live_now >> (8 * g);
+                const int last = q_pos - 64 * tile - 8 * g, first = q_first - 64 * tile - 8 * g;
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        const int at = 32 * t + 16 * (r / 8) + r % 8;
+                        const bool on = at <= last && at >= first && ((bits >> at) & 1);
+                        counts |= on ? 1u << (16 * t + r) : 0;
+                        z[t][r] = on ? z[t][r] : -INFINITY;
+                    }
+            }
+            float up = z[0][0];
+#pragma unroll
+            for (int r = 1; r < 32; r++) up = fmaxf(up, z[r / 16][r % 16]);
+            up = fmaxf(up, lane_xor<32>(up)) * qs;
+            if (__ballot(up - peak > kHeadroom)) {
+                const float to = fmaxf(peak, up - (kHeadroom - kLag));
+                const float keep = __builtin_amdgcn_exp2f(peak - to);
+                peak = to;
+                total[0] *= keep;
+                total[1] *= keep;
+#pragma unroll
+                for (int d = 0; d < DT; d++) o[d] *= keep;
+            }
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                float w[16];
+#define NHIP_WEIGHT(r)                                              \
+    w[r] = __builtin_amdgcn_exp2f(fmaf(z[t][r], qs, -peak));        \
+    total[r & 1] += w[r];                                           \
+    w[r] = alone(row_bcast<r>(vn[t]) * w[r]);
+                NHIP_WEIGHT(0) NHIP_WEIGHT(1) NHIP_WEIGHT(2) NHIP_WEIGHT(3) NHIP_WEIGHT(4) NHIP_WEIGHT(5)
+                NHIP_WEIGHT(6) NHIP_WEIGHT(7) NHIP_WEIGHT(8) NHIP_WEIGHT(9) NHIP_WEIGHT(10) NHIP_WEIGHT(11)
+                NHIP_WEIGHT(12) NHIP_WEIGHT(13) NHIP_WEIGHT(14) NHIP_WEIGHT(15)
+#undef NHIP_WEIGHT
+                if (masked) {  // (a weight of 0 times a scale that is no number)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) w[r] = (counts >> (16 * t + r)) & 1 ? w[r] : 0.0f;
+                }
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    union {
+                        f16x2 h[4];
+                        f16x8 v;
+                    } hi, lo;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const float a = w[8 * u + 2 * k], b = w[8 * u + 2 * k + 1];
+                        hi.h[k] = to_f16(a, b);
+                        lo.h[k] = rest_f16(a, b, hi.h[k], minus_one);
+                    }
+                    const uint8_t* vb = lds_v[buf] + (lane & 31) * 128 + 16 * (value_x ^ (4 * t + 2 * u));
+#pragma unroll
+                    for (int d = 0; d < DT; d++) {
+                        const f16x8 v = *reinterpret_cast<const f16x8*>(vb + 32 * 128 * d);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, hi.v, o[d], 0, 0, 0);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, lo.v, o[d], 0, 0, 0);
+                    }
+                }
+            }
+        }
+        if (more) {
+            live = live_next;
+            store(buf ^ 1);
+        }
+        __syncthreads();
+    }
+
+    float all = total[0] + total[1];
+    all += lane_xor<32>(all);
+    if (!mine) return;
+    if (q_pos < 0) {  // a row out of range, in a tile of others
+        all = 0.0f;
+        peak = kNoScore;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
+    }
+    const float unit = __uint_as_float((uint32_t)(127 + exponent) << 23);
+    float factor;
+    float* to;
+    if (p.max_parts == 1) {
+        factor = all != 0.0f ? unit / all : 0.0f;
+        to = p.out + q_at * V;
+    } else {
+        const size_t at = q_at * p.max_parts + part;
+        factor = unit;
+        to = p.parts + at * V;
+        if (g == 0) *reinterpret_cast<float2*>(p.stats + 2 * at) = make_float2(peak, all);
+    }
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            const f32x4 x = {o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]};
+            *reinterpret_cast<f32x4*>(to + 32 * d + 8 * b + 4 * g) = x * factor;
+        }
+}
+
 int32_t check_attention(const nhip_paged_cache* c, int32_t rows, int32_t heads, int32_t max_count)
 {
     int32_t rc = paged_check(c);
@@ -526,6 +841,12 @@ int32_t check_attention(const nhip_paged_cache* c, int32_t rows, int32_t heads, 
     NHIP_REQUIRE(max_count >= 0 && max_count <= c->width * c->page_size,
                  "paged attention: max_count %d out of range (a sequence holds %d positions)", max_count,
                  c->width * c->page_size);
+    return NHIP_OK;
+}
+
+int32_t check_runs(int32_t runs, int32_t window)
+{
+    NHIP_REQUIRE(runs >= 0 && runs <= kPagedMaxRows && window >= 0, "paged prompt: %d runs, window %d", runs, window);
     return NHIP_OK;
 }
 
@@ -542,20 +863,33 @@ int32_t check_call(const nhip_paged_cache* c, int32_t layer, const int8_t* q, co
     return NHIP_OK;
 }
 
-PagedAttn attn_params(const nhip_paged_cache* c, int32_t layer, const int8_t* q, const float* q_scales, int32_t rows,
-                      int32_t heads, int32_t max_count, float* out)
+// How a prompt call is split: tiles of 128 queries (at most), and where those
+// are few, 64-position blocks of a part and parts of the longest row.
+struct PromptSplit {
+    int64_t tiles;
+    int blocks, parts;
+};
+PromptSplit prompt_split(const nhip_paged_cache* c, int32_t rows, int32_t heads, int32_t runs, int32_t max_count)
 {
-    PagedAttn p{};
-    p.c = paged_layer(c, layer);
-    p.q = q;
-    p.q_scales = q_scales;
-    p.out = out;
-    p.rows = rows;
-    p.heads = heads;
-    p.group = heads / c->kv_heads;
-    p.max_count = max_count;
-    p.scale = 1.0f / std::sqrt((float)c->qk_dim);
-    return p;
+    const int64_t queries = (int64_t)rows * (heads / c->kv_heads);
+    PromptSplit s;
+    s.tiles = queries / kTileQueries + std::min(runs, rows);
+    s.blocks = max_count / 64 + 2;
+    s.parts = 1;
+    return s;
+}
+
+size_t prompt_workspace(const nhip_paged_cache* c, int32_t rows, int32_t heads, const PromptSplit& s)
+{
+    return s.parts > 1 ? (size_t)rows * heads * s.parts * (c->v_dim + 2) * sizeof(float) : 0;
+}
+
+template <int QK, int V>
+int32_t launch_prompt(const PromptParams& p, const PromptSplit& s, hipStream_t stream)
+{
+    hipLaunchKernelGGL((paged_prompt_kernel<QK, V>), dim3(s.tiles * p.c.kv_heads, s.parts), dim3(256), 0, stream, p);
+    NHIP_CHECK_HIP(hipGetLastError());
+    return NHIP_OK;
 }
 
 }  // namespace
@@ -610,9 +944,8 @@ int32_t nhip_paged_decode_dev(const nhip_paged_cache* c, int32_t layer, const in
 size_t nhip_paged_prompt_workspace(const nhip_paged_cache* c, int32_t rows, int32_t heads, int32_t runs,
                                    int32_t max_count)
 {
-    (void)runs;
-    if (check_attention(c, rows, heads, max_count)) return 0;
-    return 0;
+    if (check_attention(c, rows, heads, max_count) || check_runs(runs, 0)) return 0;
+    return prompt_workspace(c, rows, heads, prompt_split(c, rows, heads, runs, max_count));
 }
 
 int32_t nhip_paged_prompt_dev(const nhip_paged_cache* c, int32_t layer, const int8_t* d_q, const float* d_q_scales,
@@ -622,22 +955,40 @@ int32_t nhip_paged_prompt_dev(const nhip_paged_cache* c, int32_t layer, const in
 {
     int32_t rc = check_attention(c, rows, heads, max_count);
     if (rc) return rc;
-    NHIP_REQUIRE(runs >= 0 && runs <= kPagedMaxRows && window >= 0, "paged prompt: %d runs, window %d", runs, window);
+    rc = check_runs(runs, window);
+    if (rc) return rc;
     if (rows == 0 || runs == 0) return NHIP_OK;
-    rc = check_call(c, layer, d_q, d_q_scales, d_out, d_workspace, workspace_bytes, 0);
+    const PromptSplit split = prompt_split(c, rows, heads, runs, max_count);
+    NHIP_REQUIRE(split.tiles * c->kv_heads <= (1 << 23), "paged prompt: %d rows in %d runs of %d kv heads are too many",
+                 rows, runs, c->kv_heads);
+    rc = check_call(c, layer, d_q, d_q_scales, d_out, d_workspace, workspace_bytes,
+                    prompt_workspace(c, rows, heads, split));
     if (rc) return rc;
     NHIP_REQUIRE(d_run_rows && d_run_seq && d_run_pos, "paged prompt: null pointer");
     rc = ensure_device();
     if (rc) return rc;
-    PagedAttn p = attn_params(c, layer, d_q, d_q_scales, rows, heads, max_count, d_out);
+    PromptParams p;
+    p.c = paged_layer(c, layer);
+    p.q = d_q;
+    p.q_scales = d_q_scales;
+    p.out = d_out;
     p.run_rows = d_run_rows;
     p.run_seq = d_run_seq;
     p.run_pos = d_run_pos;
+    p.parts = static_cast<float*>(d_workspace);
+    p.stats = p.parts + (size_t)rows * heads * split.parts * c->v_dim;
+    p.rows = rows;
+    p.heads = heads;
+    p.group = heads / c->kv_heads;
     p.runs = runs;
     p.window = window;
-    hipLaunchKernelGGL((paged_attention_kernel<true>), dim3(rows, heads), dim3(64), 0, as_stream(stream), p);
-    NHIP_CHECK_HIP(hipGetLastError());
-    return NHIP_OK;
+    p.max_count = max_count;
+    p.blocks = split.blocks;
+    p.max_parts = split.parts;
+    p.scale = score_scale(c->qk_dim);
+    if (c->qk_dim == 48) return launch_prompt<48, 64>(p, split, as_stream(stream));
+    if (c->qk_dim == 64) return launch_prompt<64, 64>(p, split, as_stream(stream));
+    return launch_prompt<128, 128>(p, split, as_stream(stream));
 }
 
 }  // extern "C"

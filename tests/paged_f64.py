@@ -44,9 +44,9 @@ class Pool:
         return (self.keys[layer, p, kvh, at], self.key_scales[layer, p, kvh, at],
                 self.values[layer, p, kvh, at // 16, :, at % 16], self.value_scales[layer, p, kvh, at])
 
-    def attend(self, layer, seq, q, q_scales, first, count):
+    def attend(self, layer, seq, q, q_scales, first, count, prompt=False):
         """One row's [heads][v] in 64 bits, and per output the bound of the
-        kernel's error (see `bound`)."""
+        kernel's error (see `bound` and FLOOR)."""
         heads = q.shape[0]
         out, far = np.zeros((heads, self.v)), np.zeros((heads, self.v))
         for h in range(heads):
@@ -63,7 +63,8 @@ class Pool:
             w /= w.sum()
             out[h] = (w * vs) @ v
             far[h] = bound(len(cells), np.abs(z).max(), vs) * ((w * np.abs(vs)) @ np.abs(v))
-            far[h] += FLOOR * 2 * (w * np.abs(vs)).max() * np.abs(v).sum(0)
+            largest = np.nanmax(self.value_scales) * PROMPT_LAG if prompt else (w * np.abs(vs)).max()
+            far[h] += FLOOR * 2 * largest * np.abs(v).sum(0)
         return out, far
 
 
@@ -72,6 +73,10 @@ class Pool:
 #: relative error, where the largest is scaled to [2^14, 2^15): 2^-39 of it (an
 #: output whose large weights all meet code 0 shows this floor alone).
 FLOOR = 2.0 ** -39
+
+#: A prompt's weights are scaled by the running maximum that is up to 2^8 behind
+#: and by the largest value scale of the kv head so far, not by the product.
+PROMPT_LAG = 2.0 ** 8
 
 
 def bound(count, z, vs):

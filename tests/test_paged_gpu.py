@@ -243,7 +243,7 @@ def check_prompt(gpu, layer, q, qs, runs, window, max_count, rows_behind=0):
             p, r = pos + j, run_rows[i] + j
             if 0 <= s < pool.sequences and pos >= 0 and p < min(max_count, pool.width * pool.page):
                 first = max(0, p - window + 1) if window else 0
-                want[r], far[r] = pool.attend(layer, s, q[r], qs[r], first, p + 1 - first)
+                want[r], far[r] = pool.attend(layer, s, q[r], qs[r], first, p + 1 - first, True)
     assert np.array_equal(got[run_rows[-1]:], want[run_rows[-1]:].astype(np.float32))
     close(got[:run_rows[-1]], want[:run_rows[-1]], far[:run_rows[-1]])
     return got
@@ -316,8 +316,8 @@ def test_prompt_ignores_what_run_rows_may_not_say(hip):
     q, qs = queries(rng, 10, 2, 64)
     got = gpu.prompt(0, q, qs, [-5, 4, 2, 2 ** 31 - 1], [0, 1, 2], [8, 0, 3], 0, 128)
     for r in range(10):  # run 0 has rows -5..3 (row r at position 8 + 5 + r), run 1 none, run 2 rows from 2 on
-        want, far = pool.attend(0, 0, q[r], qs[r], 0, 14 + r)
-        alt, alt_far = pool.attend(0, 2, q[r], qs[r], 0, 3 + r - 2 + 1) if r >= 2 else (want, far)
+        want, far = pool.attend(0, 0, q[r], qs[r], 0, 14 + r, True)
+        alt, alt_far = pool.attend(0, 2, q[r], qs[r], 0, 3 + r - 2 + 1, True) if r >= 2 else (want, far)
         ok = [np.abs(got[r] - w) <= f for w, f in ((want, far), (alt, alt_far))]
         assert np.all(ok[1] if r >= 4 else ok[0] | ok[1])
 
@@ -596,7 +596,7 @@ def test_a_server_s_steps(hip, orc):
         k = np.array([history[s][p][layer][0] for p in range(count)], dtype=np.float32).reshape(count, kv, qk)
         x = np.array([history[s][p][layer][1] for p in range(count)], dtype=np.float32).reshape(count, kv, v)
         expected_append(orc, pool, 0, k, x, [0] * count, list(range(count)))
-        return pool.attend(0, 0, q, qs, 0, count)
+        return pool.attend(0, 0, q, qs, 0, count, True)
 
     def feed(spec):
         """spec: (sequence, positions); appends random rows and checks their attention in every layer."""
