@@ -526,8 +526,13 @@ __device__ __forceinline__ int32_t scalar_load(const int32_t* a, int64_t i)
     return ((const __attribute__((address_space(4))) int32_t*)a)[i];
 }
 
+#define NHIP_INLINE __attribute__((always_inline))
+#ifndef NHIP_SCHED
+#define NHIP_SCHED
+#endif
+
 template <int QK, int V>
-__global__ __launch_bounds__(256, QK <= 64 ? 4 : 2) void paged_prompt_kernel(PromptParams p)
+__global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(PromptParams p)
 {
     constexpr int KS = QK <= 64 ? 64 : 128;  // bytes of a key row in LDS
     constexpr int KK = KS / 32;              // products of 32 key bytes
@@ -600,60 +605,77 @@ __global__ __launch_bounds__(256, QK <= 64 ? 4 : 2) void paged_prompt_kernel(Pro
     const bool k_does = QK != 48 || lane < 48;
     const int v_block = V == 64 ? wave : wave >> 1;  // (+ 2 for the second unit)
     const int v_dim = V == 64 ? lane : 64 * (wave & 1) + lane;
-    auto key_swizzle = [](int pos) {
-        return KS == 64 ? ((pos >> 1) & 1) | (((pos >> 3) & 1) << 1) : (pos & 3) | (((pos >> 3) & 1) << 2);
-    };
+    // 16-byte units are spread over the banks such that the 16 lanes that LDS serves together find 16 different places
+    auto key_swizzle = [](int pos) { return KS == 64 ? (pos >> 2) & 3 : (pos >> 1) & 7; };
+    auto value_swizzle = [](int dim) { return (dim >> 1) & 7; };
     const int32_t* table = c.tables + (size_t)max(seq, 0) * c.width;
-    i32x4 kr[KU], vr[VU];
-    float scale_r = 0.0f;
-    uint64_t live_next = 0, live = 0;
-    auto load = [&](int tile) {
+    // the pages of a tile's four 16-position blocks (page 0 for one that may not be followed), and which positions count
+    struct TilePages {
         int page[4];
-        uint64_t ok = 0;
+        uint64_t live;
+    };
+    auto find_pages = [&](int tile) NHIP_INLINE {
+        TilePages r;
+        r.live = 0;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             const int t = (64 * tile + 16 * k) >> c.page_shift;
-            page[k] = scalar_load(table, min(t, c.width - 1));
-            const bool good = page[k] >= 0 && page[k] < c.pages;
-            ok |= good ? 0xFFFFull << (16 * k) : 0;
-            page[k] = good ? page[k] : 0;
+            const int page = scalar_load(table, min(t, c.width - 1));
+            const bool good = page >= 0 && page < c.pages;
+            r.live |= good ? 0xFFFFull << (16 * k) : 0;
+            r.page[k] = good ? page : 0;
         }
-        const int lo = from - 64 * tile, hi = last_pos + 1 - 64 * tile;  // live positions of the tile: [lo, hi)
-        if (lo > 0) ok &= ~0ull << lo;
-        if (hi < 64) ok &= (1ull << hi) - 1;
-        live_next = ok;
-        auto cell = [&](int block) {
-            const int pg = block == 0 ? page[0] : block == 1 ? page[1] : block == 2 ? page[2] : page[3];
-            return (((size_t)pg * c.kv_heads + kvh) << c.page_shift) + ((64 * tile + 16 * block) & in_page);
-        };
+        const int lo = from - 64 * tile, hi = last_pos + 1 - 64 * tile;  // [lo, hi) of the tile
+        if (lo > 0) r.live &= ~0ull << lo;
+        if (hi < 64) r.live &= (1ull << hi) - 1;
+        return r;
+    };
+    auto cell = [&](const TilePages& t, int tile, int block) NHIP_INLINE {
+        const int pg = block == 0 ? t.page[0] : block == 1 ? t.page[1] : block == 2 ? t.page[2] : t.page[3];
+        return (((size_t)pg * c.kv_heads + kvh) << c.page_shift) + ((64 * tile + 16 * block) & in_page);
+    };
+    i32x4 kr[KU], vr[VU];
+    float scale_r = 0.0f;
+    auto load_keys = [&](const TilePages& t, int tile) NHIP_INLINE {
 #pragma unroll
         for (int u = 0; u < KU; u++) {
             const int block = QK <= 64 ? wave : (wave >> 1) + 2 * u;
             if (k_does)
-                kr[u] = *reinterpret_cast<const i32x4*>(c.keys + cell(block) * QK + ((k_pos & 15) * QK + 16 * k_ch));
+                kr[u] = *reinterpret_cast<const i32x4*>(c.keys + cell(t, tile, block) * QK +
+                                                        ((k_pos & 15) * QK + 16 * k_ch));
         }
+    };
+    auto load_values = [&](const TilePages& t, int tile) NHIP_INLINE {
 #pragma unroll
         for (int u = 0; u < VU; u++)
-            vr[u] = *reinterpret_cast<const i32x4*>(c.values + cell(v_block + 2 * u) * V + 16 * v_dim);
+            vr[u] = *reinterpret_cast<const i32x4*>(c.values + cell(t, tile, v_block + 2 * u) * V + 16 * v_dim);
         const float* s = lane & 16 ? c.vscale : c.kscale;
-        scale_r = s[cell(wave) + (lane & 15)];
+        scale_r = s[cell(t, tile, wave) + (lane & 15)];
     };
-    auto store = [&](int buf) {
+    auto store_keys = [&](int buf) NHIP_INLINE {
 #pragma unroll
         for (int u = 0; u < KU; u++) {
             const int pos = k_pos + 32 * u;
             if (k_does) *reinterpret_cast<i32x4*>(lds_k[buf] + pos * KS + 16 * (k_ch ^ key_swizzle(pos))) = kr[u];
         }
+    };
+    auto store_values = [&](int buf, uint64_t live) NHIP_INLINE {
 #pragma unroll
         for (int u = 0; u < VU; u++) {
 #pragma unroll
             for (int e = 0; e < 2; e++)
                 *reinterpret_cast<f16x8*>(lds_v[buf] + v_dim * 128 +
-                                          16 * ((2 * (v_block + 2 * u) + e) ^ (v_dim & 7))) =
+                                          16 * ((2 * (v_block + 2 * u) + e) ^ value_swizzle(v_dim))) =
                     codes_f16((uint32_t)vr[u][2 * e], (uint32_t)vr[u][2 * e + 1]);
         }
+        // A value scale that is no finite number spoils the rows that attend
+        // its position, and no others: their score becomes NaN, the scale 0.
         const int pos = 16 * wave + (lane & 15);
-        if (lane < 32) (lane & 16 ? lds_vs : lds_ks)[buf][pos] = (live >> pos) & 1 ? scale_r : 0.0f;
+        const uint64_t odd = __ballot((__float_as_uint(scale_r) & 0x7F800000u) == 0x7F800000u) >> 16;
+        const bool spoilt = (odd >> (lane & 15)) & 1;
+        float x = spoilt ? (lane & 16 ? 0.0f : NAN) : scale_r;
+        x = (live >> pos) & 1 ? x : 0.0f;
+        if (lane < 32) (lane & 16 ? lds_vs : lds_ks)[buf][pos] = x;
     };
 
     f32x16 o[DT];
@@ -667,135 +689,132 @@ __global__ __launch_bounds__(256, QK <= 64 ? 4 : 2) void paged_prompt_kernel(Pro
     // where this lane reads: the key row of its A row, the value rows of its dimensions
     const int m = lane & 31;
     const int key_row = 16 * (m >> 4) + 8 * ((m >> 2) & 1) + 4 * ((m >> 3) & 1) + (m & 3);
-    const int key_x = g ^ key_swizzle(key_row), value_x = g ^ (lane & 7);
+    const int key_x = g ^ key_swizzle(key_row), value_x = g ^ value_swizzle(lane & 31);
     const int slot = 16 * ((lane >> 3) & 1) + 8 * g + (lane & 7);  // the position whose scales this lane holds
 
     if (begin < end) {
-        load(begin);
-        live = live_next;
-        store(0);
-    }
-    __syncthreads();
-    for (int tile = begin; tile < end; tile++) {
-        const int buf = (tile - begin) & 1;
-        const uint64_t live_now = live;
-        const bool more = tile + 1 < end;
-        if (more) load(tile + 1);
-        const bool any = 64 * tile <= wave_last && (p.window == 0 || 64 * tile + 63 >= wave_first - p.window + 1);
-        if (any) {
-            const uint8_t* kb = lds_k[buf] + key_row * KS;
-            i32x16 s[2];
+        TilePages pages = find_pages(begin);
+        load_keys(pages, begin);
+        load_values(pages, begin);
+        store_keys(0);
+        store_values(0, pages.live);
+        uint64_t live = pages.live;
+        pages = find_pages(min(begin + 1, end - 1));
+        __syncthreads();
+        for (int tile = begin; tile < end; tile++) {
+            const int buf = (tile - begin) & 1;
+            // (past the last tile its own are staged again, and not used)
+            load_keys(pages, min(tile + 1, end - 1));
+            load_values(pages, min(tile + 1, end - 1));
+            const uint64_t live_next = pages.live;
+            pages = find_pages(min(tile + 2, end - 1));
+            if (64 * tile <= wave_last && (p.window == 0 || 64 * tile + 63 >= wave_first - p.window + 1)) {
+                const uint8_t* kb = lds_k[buf] + key_row * KS;
+                i32x16 s[2];
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
+                for (int t = 0; t < 2; t++) {
 #pragma unroll
-                for (int r = 0; r < 16; r++) s[t][r] = 0;
+                    for (int r = 0; r < 16; r++) s[t][r] = 0;
 #pragma unroll
-                for (int k = 0; k < KK; k++)
-                    s[t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(
-                        *reinterpret_cast<const i32x4*>(kb + 32 * t * KS + 16 * (key_x ^ (2 * k))), q[k], s[t], 0, 0, 0);
-            }
-            float ks[2], vs[2];
+                    for (int k = 0; k < KK; k++)
+                        s[t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(
+                            *reinterpret_cast<const i32x4*>(kb + 32 * t * KS + 16 * (key_x ^ (2 * k))), q[k], s[t], 0,
+                            0, 0);
+                }
+                float ks[2], vs[2];
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
-                ks[t] = lds_ks[buf][32 * t + slot];
-                vs[t] = lds_vs[buf][32 * t + slot];
-            }
-            // the exponent of the value scales follows their largest (infinities and NaN aside)
-            auto exponent_of = [](float x) { return (int)((__float_as_uint(x) >> 23) & 255) - 127; };
-            const int e0 = exponent_of(vs[0]), e1 = exponent_of(vs[1]);
-            if (__ballot((e0 > exponent && e0 < 128) || (e1 > exponent && e1 < 128))) {
-                int e = max(e0 < 128 ? e0 : -100, e1 < 128 ? e1 : -100);
-                for (int off = 32; off; off >>= 1) e = max(e, __shfl_xor(e, off));
-                e = __builtin_amdgcn_readfirstlane(min(e, 100));
-                if (e > exponent) {
-                    const float keep = __uint_as_float((uint32_t)max(127 + exponent - e, 0) << 23);
+                for (int t = 0; t < 2; t++) {
+                    ks[t] = lds_ks[buf][32 * t + slot];
+                    vs[t] = lds_vs[buf][32 * t + slot];
+                }
+                // the exponent of the value scales follows their largest
+                const int e01 = (int)(__float_as_uint(fmaxf(fabsf(vs[0]), fabsf(vs[1]))) >> 23) - 127;
+                if (__ballot(e01 > exponent)) {
+                    int e = e01;
+                    for (int off = 32; off; off >>= 1) e = max(e, __shfl_xor(e, off));
+                    e = __builtin_amdgcn_readfirstlane(min(e, 100));
+                    if (e > exponent) {
+                        const float keep = __uint_as_float((uint32_t)max(127 + exponent - e, 0) << 23);
+#pragma unroll
+                        for (int d = 0; d < DT; d++) o[d] *= keep;
+                        exponent = e;
+                    }
+                }
+                const float unit = __uint_as_float((uint32_t)(127 - exponent) << 23);
+                const float vn[2] = {vs[0] * unit, vs[1] * unit};
+                float z[2][16];
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+#define NHIP_DOT(r) z[t][r] = alone(row_bcast<r>(ks[t]) * (float)s[t][r]);
+                    NHIP_DOT(0) NHIP_DOT(1) NHIP_DOT(2) NHIP_DOT(3) NHIP_DOT(4) NHIP_DOT(5) NHIP_DOT(6) NHIP_DOT(7)
+                    NHIP_DOT(8) NHIP_DOT(9) NHIP_DOT(10) NHIP_DOT(11) NHIP_DOT(12) NHIP_DOT(13) NHIP_DOT(14)
+                    NHIP_DOT(15)
+#undef NHIP_DOT
+                }
+                if (live != ~0ull || 64 * tile + 63 > wave_first ||
+                    (p.window > 0 && 64 * tile < wave_last - p.window + 1)) {
+                    const uint64_t bits = live >> (8 * g);
+                    const int last = q_pos - 64 * tile - 8 * g, first = q_first - 64 * tile - 8 * g;
+#pragma unroll
+                    for (int t = 0; t < 2; t++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) {
+                            const int at = 32 * t + 16 * (r / 8) + r % 8;
+                            z[t][r] = at <= last && at >= first && ((bits >> at) & 1) ? z[t][r] : -INFINITY;
+                        }
+                }
+                float up = z[0][0];
+#pragma unroll
+                for (int r = 1; r < 32; r++) up = fmaxf(up, z[r / 16][r % 16]);
+                up = fmaxf(up, lane_xor<32>(up)) * qs;
+                if (__ballot(up - peak > kHeadroom)) {
+                    const float to = fmaxf(peak, up - (kHeadroom - kLag));
+                    const float keep = __builtin_amdgcn_exp2f(peak - to);
+                    peak = to;
+                    total[0] *= keep;
+                    total[1] *= keep;
 #pragma unroll
                     for (int d = 0; d < DT; d++) o[d] *= keep;
-                    exponent = e;
                 }
-            }
-            const float unit = __uint_as_float((uint32_t)(127 - exponent) << 23);
-            const float vn[2] = {vs[0] * unit, vs[1] * unit};
-            const bool masked = live_now != ~0ull || 64 * tile + 63 > wave_first ||
-                                (p.window > 0 && 64 * tile < wave_last - p.window + 1);
-            float z[2][16];
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
-#define NHIP_DOT(r) z[t][r] = alone(row_bcast<r>(ks[t]) * (float)s[t][r]);
-                NHIP_DOT(0) NHIP_DOT(1) NHIP_DOT(2) NHIP_DOT(3) NHIP_DOT(4) NHIP_DOT(5) NHIP_DOT(6) NHIP_DOT(7)
-                NHIP_DOT(8) NHIP_DOT(9) NHIP_DOT(10) NHIP_DOT(11) NHIP_DOT(12) NHIP_DOT(13) NHIP_DOT(14) NHIP_DOT(15)
-#undef NHIP_DOT
-            }
-            uint32_t counts = ~0u;  // bit 16 t + r: this lane's query attends the position
-            if (masked) {
-                counts = 0;
-                const uint64_t bits = live_now >> (8 * g);
-                const int last = q_pos - 64 * tile - 8 * g, first = q_first - 64 * tile - 8 * g;
-#pragma unroll
-                for (int t = 0; t < 2; t++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        const int at = 32 * t + 16 * (r / 8) + r % 8;
-                        const bool on = at <= last && at >= first && ((bits >> at) & 1);
-                        counts |= on ? 1u << (16 * t + r) : 0;
-                        z[t][r] = on ? z[t][r] : -INFINITY;
-                    }
-            }
-            float up = z[0][0];
-#pragma unroll
-            for (int r = 1; r < 32; r++) up = fmaxf(up, z[r / 16][r % 16]);
-            up = fmaxf(up, lane_xor<32>(up)) * qs;
-            if (__ballot(up - peak > kHeadroom)) {
-                const float to = fmaxf(peak, up - (kHeadroom - kLag));
-                const float keep = __builtin_amdgcn_exp2f(peak - to);
-                peak = to;
-                total[0] *= keep;
-                total[1] *= keep;
-#pragma unroll
-                for (int d = 0; d < DT; d++) o[d] *= keep;
-            }
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                float w[16];
-#define NHIP_WEIGHT(r)                                              \
-    w[r] = __builtin_amdgcn_exp2f(fmaf(z[t][r], qs, -peak));        \
-    total[r & 1] += w[r];                                           \
+                for (int t = 0; t < 2; t++) {
+                    float w[16];
+#define NHIP_WEIGHT(r)                                       \
+    w[r] = __builtin_amdgcn_exp2f(fmaf(z[t][r], qs, -peak)); \
+    total[r & 1] += w[r];                                    \
     w[r] = alone(row_bcast<r>(vn[t]) * w[r]);
-                NHIP_WEIGHT(0) NHIP_WEIGHT(1) NHIP_WEIGHT(2) NHIP_WEIGHT(3) NHIP_WEIGHT(4) NHIP_WEIGHT(5)
-                NHIP_WEIGHT(6) NHIP_WEIGHT(7) NHIP_WEIGHT(8) NHIP_WEIGHT(9) NHIP_WEIGHT(10) NHIP_WEIGHT(11)
-                NHIP_WEIGHT(12) NHIP_WEIGHT(13) NHIP_WEIGHT(14) NHIP_WEIGHT(15)
+                    NHIP_WEIGHT(0) NHIP_WEIGHT(1) NHIP_WEIGHT(2) NHIP_WEIGHT(3) NHIP_WEIGHT(4) NHIP_WEIGHT(5)
+                    NHIP_WEIGHT(6) NHIP_WEIGHT(7) NHIP_WEIGHT(8) NHIP_WEIGHT(9) NHIP_WEIGHT(10) NHIP_WEIGHT(11)
+                    NHIP_WEIGHT(12) NHIP_WEIGHT(13) NHIP_WEIGHT(14) NHIP_WEIGHT(15)
 #undef NHIP_WEIGHT
-                if (masked) {  // (a weight of 0 times a scale that is no number)
 #pragma unroll
-                    for (int r = 0; r < 16; r++) w[r] = (counts >> (16 * t + r)) & 1 ? w[r] : 0.0f;
-                }
+                    for (int u = 0; u < 2; u++) {
+                        union {
+                            f16x2 h[4];
+                            f16x8 v;
+                        } hi, lo;
 #pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    union {
-                        f16x2 h[4];
-                        f16x8 v;
-                    } hi, lo;
+                        for (int k = 0; k < 4; k++) {
+                            const float a = w[8 * u + 2 * k], b = w[8 * u + 2 * k + 1];
+                            hi.h[k] = to_f16(a, b);
+                            lo.h[k] = rest_f16(a, b, hi.h[k], minus_one);
+                        }
+                        const uint8_t* vb = lds_v[buf] + (lane & 31) * 128 + 16 * (value_x ^ (4 * t + 2 * u));
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const float a = w[8 * u + 2 * k], b = w[8 * u + 2 * k + 1];
-                        hi.h[k] = to_f16(a, b);
-                        lo.h[k] = rest_f16(a, b, hi.h[k], minus_one);
-                    }
-                    const uint8_t* vb = lds_v[buf] + (lane & 31) * 128 + 16 * (value_x ^ (4 * t + 2 * u));
-#pragma unroll
-                    for (int d = 0; d < DT; d++) {
-                        const f16x8 v = *reinterpret_cast<const f16x8*>(vb + 32 * 128 * d);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, hi.v, o[d], 0, 0, 0);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, lo.v, o[d], 0, 0, 0);
+                        for (int d = 0; d < DT; d++) {
+                            const f16x8 v = *reinterpret_cast<const f16x8*>(vb + 32 * 128 * d);
+                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, hi.v, o[d], 0, 0, 0);
+                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, lo.v, o[d], 0, 0, 0);
+                        }
                     }
                 }
+                NHIP_SCHED
             }
-        }
-        if (more) {
+            store_keys(buf ^ 1);
+            store_values(buf ^ 1, live_next);
             live = live_next;
-            store(buf ^ 1);
+            __syncthreads();
         }
-        __syncthreads();
     }
 
     float all = total[0] + total[1];
