@@ -527,9 +527,6 @@ __device__ __forceinline__ int32_t scalar_load(const int32_t* a, int64_t i)
 }
 
 #define NHIP_INLINE __attribute__((always_inline))
-#ifndef NHIP_SCHED
-#define NHIP_SCHED
-#endif
 
 template <int QK, int V>
 __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(PromptParams p)
@@ -541,7 +538,8 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
     constexpr int KCH = QK / 16;             // units of a key row
     __shared__ __align__(16) uint8_t lds_k[2][64 * KS];
     __shared__ __align__(16) uint8_t lds_v[2][V * 128];
-    __shared__ float lds_ks[2][64], lds_vs[2][64];
+    __shared__ float lds_ks[4][64], lds_vs[4][64];
+    __shared__ uint16_t lds_live[4][4];
     const PagedLayer& c = p.c;
     // (a tile's kv heads side by side: with 8 of them each XCD keeps one head's positions in its L2)
     const int tile_of_call = blockIdx.x / c.kv_heads, kvh = blockIdx.x - tile_of_call * c.kv_heads;
@@ -594,88 +592,72 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
     const int first_pos = __builtin_amdgcn_readfirstlane(pos_of(q0));
     const int last_pos = __builtin_amdgcn_readfirstlane(pos_of(q0 + qn - 1));
     const int from = p.window > 0 ? max(first_pos - p.window + 1, 0) : 0;
+    const int from_window = p.window > 0 ? p.window - 1 : 1 << 30;  // positions before its own that a row attends
     const int tile0 = from >> 6, tile1 = last_pos >= 0 ? (last_pos >> 6) + 1 : tile0;
     const int begin = tile0 + part * p.blocks;
     const int end = min(tile1, begin + p.blocks);
 
-    // staging: a wave's units lie in one 16-position block, so its page is a scalar
+    // Staging: a wave brings one 16-position block of a tile, so its page is a
+    // scalar, looked up a tile ahead.  Units are spread over the banks such
+    // that the 16 lanes LDS serves together find 16 different places.
     const int in_page = (1 << c.page_shift) - 1;
-    const int k_pos = QK <= 64 ? 16 * wave + lane / KCH : 8 * wave + lane / 8;  // (+ 32 for the second unit)
-    const int k_ch = QK <= 64 ? lane % KCH : lane % 8;
+    const int k_pos = lane / KCH, k_ch = lane % KCH;  // (+ 8 positions for a second unit)
     const bool k_does = QK != 48 || lane < 48;
-    const int v_block = V == 64 ? wave : wave >> 1;  // (+ 2 for the second unit)
-    const int v_dim = V == 64 ? lane : 64 * (wave & 1) + lane;
-    // 16-byte units are spread over the banks such that the 16 lanes that LDS serves together find 16 different places
     auto key_swizzle = [](int pos) { return KS == 64 ? (pos >> 2) & 3 : (pos >> 1) & 7; };
     auto value_swizzle = [](int dim) { return (dim >> 1) & 7; };
     const int32_t* table = c.tables + (size_t)max(seq, 0) * c.width;
-    // the pages of a tile's four 16-position blocks (page 0 for one that may not be followed), and which positions count
-    struct TilePages {
-        int page[4];
-        uint64_t live;
+    auto look_up = [&](int tile) NHIP_INLINE {
+        return scalar_load(table, min((64 * tile + 16 * wave) >> c.page_shift, c.width - 1));
     };
-    auto find_pages = [&](int tile) NHIP_INLINE {
-        TilePages r;
-        r.live = 0;
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int t = (64 * tile + 16 * k) >> c.page_shift;
-            const int page = scalar_load(table, min(t, c.width - 1));
-            const bool good = page >= 0 && page < c.pages;
-            r.live |= good ? 0xFFFFull << (16 * k) : 0;
-            r.page[k] = good ? page : 0;
-        }
-        const int lo = from - 64 * tile, hi = last_pos + 1 - 64 * tile;  // [lo, hi) of the tile
-        if (lo > 0) r.live &= ~0ull << lo;
-        if (hi < 64) r.live &= (1ull << hi) - 1;
-        return r;
-    };
-    auto cell = [&](const TilePages& t, int tile, int block) NHIP_INLINE {
-        const int pg = block == 0 ? t.page[0] : block == 1 ? t.page[1] : block == 2 ? t.page[2] : t.page[3];
-        return (((size_t)pg * c.kv_heads + kvh) << c.page_shift) + ((64 * tile + 16 * block) & in_page);
+    auto cell = [&](int tile, int page) NHIP_INLINE {
+        const int pg = page >= 0 && page < c.pages ? page : 0;
+        return (((size_t)pg * c.kv_heads + kvh) << c.page_shift) + ((64 * tile + 16 * wave) & in_page);
     };
     i32x4 kr[KU], vr[VU];
-    float scale_r = 0.0f;
-    auto load_keys = [&](const TilePages& t, int tile) NHIP_INLINE {
+    float scale_r;
+    auto load_keys = [&](int tile, int page) NHIP_INLINE {
+        const size_t at = cell(tile, page);
 #pragma unroll
-        for (int u = 0; u < KU; u++) {
-            const int block = QK <= 64 ? wave : (wave >> 1) + 2 * u;
+        for (int u = 0; u < KU; u++)
             if (k_does)
-                kr[u] = *reinterpret_cast<const i32x4*>(c.keys + cell(t, tile, block) * QK +
-                                                        ((k_pos & 15) * QK + 16 * k_ch));
-        }
+                kr[u] = *reinterpret_cast<const i32x4*>(c.keys + at * QK + ((k_pos + 8 * u) * QK + 16 * k_ch));
+        scale_r = (lane & 16 ? c.vscale : c.kscale)[at + (lane & 15)];
     };
-    auto load_values = [&](const TilePages& t, int tile) NHIP_INLINE {
+    auto load_values = [&](int tile, int page) NHIP_INLINE {
+        const size_t at = cell(tile, page);
 #pragma unroll
         for (int u = 0; u < VU; u++)
-            vr[u] = *reinterpret_cast<const i32x4*>(c.values + cell(t, tile, v_block + 2 * u) * V + 16 * v_dim);
-        const float* s = lane & 16 ? c.vscale : c.kscale;
-        scale_r = s[cell(t, tile, wave) + (lane & 15)];
+            vr[u] = *reinterpret_cast<const i32x4*>(c.values + at * V + 16 * (lane + 64 * u));
     };
-    auto store_keys = [&](int buf) NHIP_INLINE {
+    auto store_keys = [&](int tile, int page) NHIP_INLINE {
 #pragma unroll
         for (int u = 0; u < KU; u++) {
-            const int pos = k_pos + 32 * u;
-            if (k_does) *reinterpret_cast<i32x4*>(lds_k[buf] + pos * KS + 16 * (k_ch ^ key_swizzle(pos))) = kr[u];
+            const int pos = 16 * wave + k_pos + 8 * u;
+            if (k_does)
+                *reinterpret_cast<i32x4*>(lds_k[tile & 1] + pos * KS + 16 * (k_ch ^ key_swizzle(pos))) = kr[u];
         }
-    };
-    auto store_values = [&](int buf, uint64_t live) NHIP_INLINE {
-#pragma unroll
-        for (int u = 0; u < VU; u++) {
-#pragma unroll
-            for (int e = 0; e < 2; e++)
-                *reinterpret_cast<f16x8*>(lds_v[buf] + v_dim * 128 +
-                                          16 * ((2 * (v_block + 2 * u) + e) ^ value_swizzle(v_dim))) =
-                    codes_f16((uint32_t)vr[u][2 * e], (uint32_t)vr[u][2 * e + 1]);
-        }
+        // the positions that count, [lo, hi) of the block
+        const int lo = from - 64 * tile - 16 * wave, hi = last_pos + 1 - 64 * tile - 16 * wave;
+        uint32_t live = page >= 0 && page < c.pages ? 0xFFFFu : 0;
+        live &= lo >= 16 ? 0 : 0xFFFFu << max(lo, 0);
+        live &= hi <= 0 ? 0 : 0xFFFFu >> (16 - min(hi, 16));
         // A value scale that is no finite number spoils the rows that attend
         // its position, and no others: their score becomes NaN, the scale 0.
-        const int pos = 16 * wave + (lane & 15);
         const uint64_t odd = __ballot((__float_as_uint(scale_r) & 0x7F800000u) == 0x7F800000u) >> 16;
-        const bool spoilt = (odd >> (lane & 15)) & 1;
-        float x = spoilt ? (lane & 16 ? 0.0f : NAN) : scale_r;
-        x = (live >> pos) & 1 ? x : 0.0f;
-        if (lane < 32) (lane & 16 ? lds_vs : lds_ks)[buf][pos] = x;
+        float x = (odd >> (lane & 15)) & 1 ? (lane & 16 ? 0.0f : NAN) : scale_r;
+        x = (live >> (lane & 15)) & 1 ? x : 0.0f;
+        if (lane < 32) (lane & 16 ? lds_vs : lds_ks)[tile & 3][16 * wave + (lane & 15)] = x;
+        if (lane == 0) lds_live[tile & 3][wave] = (uint16_t)live;
+    };
+    auto store_values = [&](int tile) NHIP_INLINE {
+#pragma unroll
+        for (int u = 0; u < VU; u++) {
+            const int dim = lane + 64 * u;
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+                *reinterpret_cast<f16x8*>(lds_v[tile & 1] + dim * 128 + 16 * ((2 * wave + e) ^ value_swizzle(dim))) =
+                    codes_f16((uint32_t)vr[u][2 * e], (uint32_t)vr[u][2 * e + 1]);
+        }
     };
 
     f32x16 o[DT];
@@ -693,23 +675,22 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
     const int slot = 16 * ((lane >> 3) & 1) + 8 * g + (lane & 7);  // the position whose scales this lane holds
 
     if (begin < end) {
-        TilePages pages = find_pages(begin);
-        load_keys(pages, begin);
-        load_values(pages, begin);
-        store_keys(0);
-        store_values(0, pages.live);
-        uint64_t live = pages.live;
-        pages = find_pages(min(begin + 1, end - 1));
+        // (past the last tile its own is staged again, and not used)
+        auto clamped = [&](int tile) NHIP_INLINE { return min(tile, end - 1); };
+        int page = look_up(begin);
+        load_keys(begin, page);
+        load_values(begin, page);
+        int page_next = look_up(clamped(begin + 1));
+        store_keys(begin, page);
+        store_values(begin);
         __syncthreads();
         for (int tile = begin; tile < end; tile++) {
-            const int buf = (tile - begin) & 1;
-            // (past the last tile its own are staged again, and not used)
-            load_keys(pages, min(tile + 1, end - 1));
-            load_values(pages, min(tile + 1, end - 1));
-            const uint64_t live_next = pages.live;
-            pages = find_pages(min(tile + 2, end - 1));
-            if (64 * tile <= wave_last && (p.window == 0 || 64 * tile + 63 >= wave_first - p.window + 1)) {
-                const uint8_t* kb = lds_k[buf] + key_row * KS;
+            page = page_next;
+            load_keys(clamped(tile + 1), page);
+            load_values(clamped(tile + 1), page);
+            page_next = look_up(clamped(tile + 2));
+            if ((64 * tile <= wave_last) & (64 * tile + 63 >= wave_first - from_window)) {
+                const uint8_t* kb = lds_k[tile & 1] + key_row * KS;
                 i32x16 s[2];
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
@@ -724,24 +705,10 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
                 float ks[2], vs[2];
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
-                    ks[t] = lds_ks[buf][32 * t + slot];
-                    vs[t] = lds_vs[buf][32 * t + slot];
+                    ks[t] = lds_ks[tile & 3][32 * t + slot];
+                    vs[t] = lds_vs[tile & 3][32 * t + slot];
                 }
-                // the exponent of the value scales follows their largest
-                const int e01 = (int)(__float_as_uint(fmaxf(fabsf(vs[0]), fabsf(vs[1]))) >> 23) - 127;
-                if (__ballot(e01 > exponent)) {
-                    int e = e01;
-                    for (int off = 32; off; off >>= 1) e = max(e, __shfl_xor(e, off));
-                    e = __builtin_amdgcn_readfirstlane(min(e, 100));
-                    if (e > exponent) {
-                        const float keep = __uint_as_float((uint32_t)max(127 + exponent - e, 0) << 23);
-#pragma unroll
-                        for (int d = 0; d < DT; d++) o[d] *= keep;
-                        exponent = e;
-                    }
-                }
-                const float unit = __uint_as_float((uint32_t)(127 - exponent) << 23);
-                const float vn[2] = {vs[0] * unit, vs[1] * unit};
+                const uint2 counted = *reinterpret_cast<const uint2*>(lds_live[tile & 3]);
                 float z[2][16];
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
@@ -751,31 +718,42 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
                     NHIP_DOT(15)
 #undef NHIP_DOT
                 }
-                if (live != ~0ull || 64 * tile + 63 > wave_first ||
-                    (p.window > 0 && 64 * tile < wave_last - p.window + 1)) {
-                    const uint64_t bits = live >> (8 * g);
+                const bool whole = __builtin_amdgcn_readfirstlane(counted.x & counted.y) == ~0u;
+                if (!whole | (64 * tile + 63 > wave_first) | (64 * tile < wave_last - from_window)) {
                     const int last = q_pos - 64 * tile - 8 * g, first = q_first - 64 * tile - 8 * g;
 #pragma unroll
-                    for (int t = 0; t < 2; t++)
+                    for (int t = 0; t < 2; t++) {
+                        const uint32_t bits = (t ? counted.y : counted.x) >> (8 * g);
 #pragma unroll
                         for (int r = 0; r < 16; r++) {
-                            const int at = 32 * t + 16 * (r / 8) + r % 8;
-                            z[t][r] = at <= last && at >= first && ((bits >> at) & 1) ? z[t][r] : -INFINITY;
+                            const int at = 16 * (r / 8) + r % 8;
+                            z[t][r] = (32 * t + at <= last) & (32 * t + at >= first) & ((bits >> at) & 1) ? z[t][r]
+                                                                                                          : -INFINITY;
                         }
+                    }
                 }
                 float up = z[0][0];
 #pragma unroll
                 for (int r = 1; r < 32; r++) up = fmaxf(up, z[r / 16][r % 16]);
                 up = fmaxf(up, lane_xor<32>(up)) * qs;
-                if (__ballot(up - peak > kHeadroom)) {
-                    const float to = fmaxf(peak, up - (kHeadroom - kLag));
-                    const float keep = __builtin_amdgcn_exp2f(peak - to);
+                // the exponent of the value scales follows their largest
+                const int ev = (int)(__float_as_uint(fmaxf(fabsf(vs[0]), fabsf(vs[1]))) >> 23) - 127;
+                if (__ballot((up - peak > kHeadroom) | (ev > exponent))) {
+                    const float to = up - peak > kHeadroom ? up - (kHeadroom - kLag) : peak;
+                    float keep = __builtin_amdgcn_exp2f(peak - to);
                     peak = to;
                     total[0] *= keep;
                     total[1] *= keep;
+                    int e = ev;
+                    for (int off = 32; off; off >>= 1) e = max(e, __shfl_xor(e, off));
+                    e = max(__builtin_amdgcn_readfirstlane(min(e, 100)), exponent);
+                    keep *= __uint_as_float((uint32_t)max(127 + exponent - e, 0) << 23);
+                    exponent = e;
 #pragma unroll
                     for (int d = 0; d < DT; d++) o[d] *= keep;
                 }
+                const float unit = __uint_as_float((uint32_t)(127 - exponent) << 23);
+                const float vn[2] = {vs[0] * unit, vs[1] * unit};
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
                     float w[16];
@@ -799,7 +777,7 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
                             hi.h[k] = to_f16(a, b);
                             lo.h[k] = rest_f16(a, b, hi.h[k], minus_one);
                         }
-                        const uint8_t* vb = lds_v[buf] + (lane & 31) * 128 + 16 * (value_x ^ (4 * t + 2 * u));
+                        const uint8_t* vb = lds_v[tile & 1] + (lane & 31) * 128 + 16 * (value_x ^ (4 * t + 2 * u));
 #pragma unroll
                         for (int d = 0; d < DT; d++) {
                             const f16x8 v = *reinterpret_cast<const f16x8*>(vb + 32 * 128 * d);
@@ -808,11 +786,9 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
                         }
                     }
                 }
-                NHIP_SCHED
             }
-            store_keys(buf ^ 1);
-            store_values(buf ^ 1, live_next);
-            live = live_next;
+            store_keys(tile + 1, page);
+            store_values(tile + 1);
             __syncthreads();
         }
     }
