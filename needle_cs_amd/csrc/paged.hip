@@ -51,7 +51,7 @@ constexpr int kMaxEntries = 1024;
 // ---------------------------------------------------------------- append --
 
 struct AppendParams {
-    PagedLayer layer;
+    PagedLayer c;
     const float* k;
     const float* v;
     const int32_t* row_seq;
@@ -59,51 +59,107 @@ struct AppendParams {
     int32_t ldk, ldv, rows;
 };
 
-// Where row r's position lives: its page's first cell and its place in the
-// page; false when a part of the address is out of range.
-__device__ __forceinline__ bool append_target(const AppendParams& p, int r, int kvh, size_t& cell, int& at)
+// A workgroup takes 16 rows of one kv head; L lanes share a row's key (or
+// value) head, four elements each, so a head's peak is a few DPP steps and 16
+// rows of keys leave as whole dwords.  Values change places through LDS: the
+// cache holds 16 positions of a dimension together, and where the 16 rows are
+// consecutive positions of one sequence (a prompt) a lane writes four of them
+// at once; else each goes by itself.  Bound by the bytes read and written:
+// 8185 rows of 8 kv heads of 128 (84 MB) take APPEND_US us, APPEND_TBS TB/s.
+typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+
+template <int L>
+__device__ __forceinline__ float group_max(float v)
 {
-    const PagedLayer& c = p.layer;
-    const int seq = p.row_seq[r], pos = p.row_pos[r];
-    if (seq < 0 || seq >= c.sequences || pos < 0 || (pos >> c.page_shift) >= c.width) return false;
-    const int page = c.tables[(size_t)seq * c.width + (pos >> c.page_shift)];
-    if (page < 0 || page >= c.pages) return false;
-    cell = ((size_t)page * c.kv_heads + kvh) << c.page_shift;
-    at = pos & ((1 << c.page_shift) - 1);
-    return true;
+    v = fmaxf(v, lane_xor<1>(v));
+    v = fmaxf(v, lane_xor<2>(v));
+    v = fmaxf(v, lane_xor<4>(v));
+    v = fmaxf(v, lane_xor<8>(v));
+    return L == 32 ? fmaxf(v, lane_xor<16>(v)) : v;
 }
 
-// One wave per (row, kv head): lane e takes elements e and e + 64.
+template <int QK, int V>
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p)
 {
-    const int lane = threadIdx.x & 63;
-    const int kvh = blockIdx.y;
-    const int r = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6);
-    if (r >= p.rows) return;
-    const PagedLayer& c = p.layer;
-    size_t cell;
-    int at;
-    if (!append_target(p, r, kvh, cell, at)) return;
+    constexpr int L = V <= 64 ? 16 : 32, PASSES = L / 16, ROWS = 256 / L;  // rows of a pass
+    __shared__ size_t cells[16];
+    __shared__ int places[16], positions[16], sequences[16];
+    __shared__ __align__(16) uint8_t turned[V][20];  // value codes by dimension, then row
+    const PagedLayer& c = p.c;
+    const int kvh = blockIdx.y, row0 = (int)blockIdx.x * 16, n = min(16, p.rows - row0);
+    const int l = threadIdx.x & (L - 1), row_of_pass = threadIdx.x / L;
+    f4 x[PASSES][2];
 #pragma unroll
-    for (int part = 0; part < 2; part++) {
-        const int n = part ? c.v : c.qk;
-        const float* x = part ? p.v + (size_t)r * p.ldv + kvh * n : p.k + (size_t)r * p.ldk + kvh * n;
-        const float x0 = lane < n ? x[lane] : 0.0f;
-        const float x1 = lane + 64 < n ? x[lane + 64] : 0.0f;
-        const float peak = wave_max(fmaxf(fabsf(x0), fabsf(x1)));
-        const float scale = peak > 0.0f ? peak / 127.0f : 1.0f;
-        const float inverse = 1.0f / scale;
+    for (int k = 0; k < PASSES; k++) {
+        const size_t r = row0 + min(row_of_pass + k * ROWS, n - 1);
+        x[k][0] = x[k][1] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (4 * l < QK) x[k][0] = *reinterpret_cast<const f4*>(p.k + r * p.ldk + kvh * QK + 4 * l);
+        if (4 * l < V) x[k][1] = *reinterpret_cast<const f4*>(p.v + r * p.ldv + kvh * V + 4 * l);
+    }
+    // where each row's position lives: its page's first cell (of this kv head) and its place in the page, -1 if nowhere
+    if (threadIdx.x < 16) {
+        const int i = threadIdx.x, r = row0 + min(i, n - 1);
+        const int seq = p.row_seq[r], pos = p.row_pos[r];
+        int page = -1;
+        if (seq >= 0 && seq < c.sequences && pos >= 0 && (pos >> c.page_shift) < c.width)
+            page = c.tables[(size_t)seq * c.width + (pos >> c.page_shift)];
+        const bool ok = i < n && page >= 0 && page < c.pages;
+        cells[i] = ok ? ((size_t)page * c.kv_heads + kvh) << c.page_shift : 0;
+        places[i] = ok ? pos & ((1 << c.page_shift) - 1) : -1;
+        positions[i] = pos;
+        sequences[i] = seq;
+    }
+    __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-            const int d = lane + 64 * e;
-            if (d >= n) continue;
-            const int8_t q = (int8_t)ref_quantize_one(e ? x1 : x0, inverse);
-            if (part == 0)
-                c.keys[(cell + at) * n + d] = q;
-            else
-                c.values[cell * n + (size_t)(at >> 4) * (16 * n) + d * 16 + (at & 15)] = q;
+    for (int k = 0; k < PASSES; k++) {
+        const int i = row_of_pass + k * ROWS;
+        const int at = places[i];
+        const size_t cell = cells[i];
+#pragma unroll
+        for (int part = 0; part < 2; part++) {
+            const f4 y = x[k][part];
+            const float peak =
+                group_max<L>(fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3]))));
+            const float scale = peak > 0.0f ? peak / 127.0f : 1.0f;
+            const uint32_t codes = ref_quantize4(make_float4(y[0], y[1], y[2], y[3]), 1.0f / scale);
+            if (part == 1 && 4 * l < V) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) turned[4 * l + e][i] = (uint8_t)(codes >> (8 * e));
+            }
+            if (at < 0) continue;
+            if (part == 0 && 4 * l < QK) *reinterpret_cast<uint32_t*>(c.keys + (cell + at) * QK + 4 * l) = codes;
+            if (l == 0) (part ? c.vscale : c.kscale)[cell + at] = scale;
         }
-        if (lane == 0) (part ? c.vscale : c.kscale)[cell + at] = scale;
+    }
+    __syncthreads();
+    bool consecutive = true;
+    for (int i = 0; i < n; i++)
+        consecutive &= places[i] >= 0 && positions[i] == positions[0] + i && sequences[i] == sequences[0];
+    if (consecutive) {
+        // five quads of positions cover 16 rows whatever place the first has in its quad
+        const int lead = positions[0] & 3;
+        for (int item = threadIdx.x; item < 5 * V; item += 256) {
+            const int d = item & (V - 1), first = 4 * (item / V) - lead;  // the quad's first row
+            if (first >= n) continue;
+            const int some = max(first, 0), at = places[some] & ~3;
+            uint8_t* to = reinterpret_cast<uint8_t*>(c.values) + cells[some] * V + (size_t)(at >> 4) * (16 * V) +
+                          d * 16 + (at & 15);
+            if (first >= 0 && first + 4 <= n) {
+                uint32_t word = 0;
+#pragma unroll
+                for (int e = 0; e < 4; e++) word |= (uint32_t)turned[d][first + e] << (8 * e);
+                *reinterpret_cast<uint32_t*>(to) = word;
+            } else {
+                for (int e = 0; e < 4; e++)
+                    if (first + e >= 0 && first + e < n) to[e] = turned[d][first + e];
+            }
+        }
+    } else {
+        for (int item = threadIdx.x; item < n * V; item += 256) {
+            const int d = item & (V - 1), i = item / V, at = places[i];
+            if (at >= 0)
+                c.values[cells[i] * V + (size_t)(at >> 4) * (16 * V) + d * 16 + (at & 15)] = (int8_t)turned[d][i];
+        }
     }
 }
 
@@ -511,8 +567,13 @@ int32_t nhip_paged_append_dev(const nhip_paged_cache* c, int32_t layer, const fl
     rc = ensure_device();
     if (rc) return rc;
     const AppendParams p{paged_layer(c, layer), d_k, d_v, d_row_seq, d_row_pos, ldk, ldv, rows};
-    hipLaunchKernelGGL(paged_append_kernel, dim3((unsigned)(rows + 3) / 4, (unsigned)c->kv_heads), dim3(256), 0,
-                       as_stream(stream), p);
+    const dim3 grid((unsigned)(rows + 15) / 16, (unsigned)c->kv_heads);
+    if (c->qk_dim == 48)
+        hipLaunchKernelGGL((paged_append_kernel<48, 64>), grid, dim3(256), 0, as_stream(stream), p);
+    else if (c->qk_dim == 64)
+        hipLaunchKernelGGL((paged_append_kernel<64, 64>), grid, dim3(256), 0, as_stream(stream), p);
+    else
+        hipLaunchKernelGGL((paged_append_kernel<128, 128>), grid, dim3(256), 0, as_stream(stream), p);
     NHIP_CHECK_HIP(hipGetLastError());
     return NHIP_OK;
 }

@@ -469,6 +469,7 @@ struct PromptParams {
     const int32_t* run_pos;
     float* parts;  // as DecodeParams'
     float* stats;
+    int32_t* counts;  // [rows][heads]: the parts of a row
     int32_t rows, heads, group, runs, window, max_count, blocks, max_parts;
     float scale;
 };
@@ -594,6 +595,8 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
     const int from = p.window > 0 ? max(first_pos - p.window + 1, 0) : 0;
     const int from_window = p.window > 0 ? p.window - 1 : 1 << 30;  // positions before its own that a row attends
     const int tile0 = from >> 6, tile1 = last_pos >= 0 ? (last_pos >> 6) + 1 : tile0;
+    const int parts = (tile1 - tile0 + p.blocks - 1) / p.blocks;
+    if (part > 0 && part >= parts) return;
     const int begin = tile0 + part * p.blocks;
     const int end = min(tile1, begin + p.blocks);
 
@@ -807,7 +810,8 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
     const float unit = __uint_as_float((uint32_t)(127 + exponent) << 23);
     float factor;
     float* to;
-    if (p.max_parts == 1) {
+    if (p.max_parts > 1 && part == 0 && g == 0) p.counts[q_at] = parts;
+    if (parts <= 1) {
         factor = all != 0.0f ? unit / all : 0.0f;
         to = p.out + q_at * V;
     } else {
@@ -823,6 +827,51 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
             const f32x4 x = {o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]};
             *reinterpret_cast<f32x4*>(to + 32 * d + 8 * b + 4 * g) = x * factor;
         }
+}
+
+// Joins the parts of rows that were split, a wave per (row, head); rows of no
+// run have no parts.
+template <int V>
+__global__ __launch_bounds__(256) void paged_prompt_join_kernel(PromptParams p)
+{
+    const int row = blockIdx.x, lane = threadIdx.x & 63;
+    const int head = (int)blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (head >= p.heads) return;
+    bool in_run = false;
+    for (int i = lane; i < p.runs; i += 64) {
+        const RunRows r = run_rows(p, i);
+        in_run |= row >= r.row0 && row < r.row1;
+    }
+    if (!__ballot(in_run)) return;
+    const size_t q_at = (size_t)row * p.heads + head;
+    const int parts = p.counts[q_at];
+    if (parts <= 1) return;
+    const size_t first = q_at * p.max_parts;
+    float2 stat = make_float2(kNoScore, 0.0f);
+    if (lane < parts) stat = *reinterpret_cast<const float2*>(p.stats + 2 * (first + lane));
+    const float factor = __builtin_amdgcn_exp2f(stat.x - wave_max(stat.x));
+    float all = factor * stat.y;
+    for (int off = 32; off; off >>= 1) all += __shfl_xor(all, off);
+    constexpr int E = V / 64;
+    float sum[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) sum[e] = 0.0f;
+    const float* from = p.parts + first * V + lane;
+    for (int k = 0; k < parts; k += 4) {
+        float x[4][E];
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+            for (int e = 0; e < E; e++) x[u][e] = from[(size_t)min(k + u, parts - 1) * V + 64 * e];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const float f = k + u < parts ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(factor), k + u)) : 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; e++) sum[e] = k + u < parts ? fmaf(x[u][e], f, sum[e]) : sum[e];
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < E; e++) p.out[q_at * V + lane + 64 * e] = all != 0.0f ? sum[e] / all : 0.0f;
 }
 
 int32_t check_attention(const nhip_paged_cache* c, int32_t rows, int32_t heads, int32_t max_count)
@@ -864,19 +913,40 @@ struct PromptSplit {
     int64_t tiles;
     int blocks, parts;
 };
-PromptSplit prompt_split(const nhip_paged_cache* c, int32_t rows, int32_t heads, int32_t runs, int32_t max_count)
+
+// A block takes 1 to 2.5 us of a workgroup, joining parts about 4 us.  Where
+// the tiles fill the CUs, or have fewer than 6 blocks, they stay whole (16 runs of up to 700 rows, 16 kv
+// heads: 38 us whole, 45 in two parts).  Up to 96 workgroups, or 256 with 32
+// or more blocks each, are split until about 768 are there, in parts of two
+// blocks or more (16 rows after 32,000 positions, 8 kv heads of 128: 798 us
+// whole, 37 in 63 parts; 512 rows after 8,000, 16 kv heads: 182 and 50; 416
+// rows from 0, 112 workgroups of up to 8 blocks: 14.8 whole, 16.7 in parts).
+// A window bounds a tile's blocks; it never makes more parts, as the workspace
+// is sized without it.
+PromptSplit prompt_split(const nhip_paged_cache* c, int32_t rows, int32_t heads, int32_t runs, int32_t max_count,
+                         int32_t window)
 {
-    const int64_t queries = (int64_t)rows * (heads / c->kv_heads);
+    const int group = heads / c->kv_heads;
     PromptSplit s;
-    s.tiles = queries / kTileQueries + std::min(runs, rows);
-    s.blocks = max_count / 64 + 2;
-    s.parts = 1;
+    s.tiles = (int64_t)rows * group / kTileQueries + std::min(runs, rows);
+    const int64_t units = s.tiles * c->kv_heads;
+    int most = max_count / 64 + 2;
+    s.blocks = most;
+    if (most >= 6 && (units <= 96 || (units <= 256 && most >= 32)))
+        s.blocks = (int)std::min<int64_t>(
+            most, std::max<int64_t>({2, (units * most + 767) / 768, (most + kMaxParts - 1) / kMaxParts}));
+    s.parts = (most + s.blocks - 1) / s.blocks;
+    if (window > 0 && window < max_count) {
+        most = std::min<int64_t>(most, ((int64_t)window + kTileQueries / group) / 64 + 2);
+        s.blocks = std::max(2, (most + s.parts - 1) / s.parts);
+        s.parts = (most + s.blocks - 1) / s.blocks;
+    }
     return s;
 }
 
 size_t prompt_workspace(const nhip_paged_cache* c, int32_t rows, int32_t heads, const PromptSplit& s)
 {
-    return s.parts > 1 ? (size_t)rows * heads * s.parts * (c->v_dim + 2) * sizeof(float) : 0;
+    return s.parts > 1 ? (size_t)rows * heads * ((size_t)s.parts * (c->v_dim + 2) + 1) * sizeof(float) : 0;
 }
 
 template <int QK, int V>
@@ -884,6 +954,10 @@ int32_t launch_prompt(const PromptParams& p, const PromptSplit& s, hipStream_t s
 {
     hipLaunchKernelGGL((paged_prompt_kernel<QK, V>), dim3(s.tiles * p.c.kv_heads, s.parts), dim3(256), 0, stream, p);
     NHIP_CHECK_HIP(hipGetLastError());
+    if (s.parts > 1) {
+        hipLaunchKernelGGL((paged_prompt_join_kernel<V>), dim3(p.rows, (p.heads + 3) / 4), dim3(256), 0, stream, p);
+        NHIP_CHECK_HIP(hipGetLastError());
+    }
     return NHIP_OK;
 }
 
@@ -940,7 +1014,7 @@ size_t nhip_paged_prompt_workspace(const nhip_paged_cache* c, int32_t rows, int3
                                    int32_t max_count)
 {
     if (check_attention(c, rows, heads, max_count) || check_runs(runs, 0)) return 0;
-    return prompt_workspace(c, rows, heads, prompt_split(c, rows, heads, runs, max_count));
+    return prompt_workspace(c, rows, heads, prompt_split(c, rows, heads, runs, max_count, 0));
 }
 
 int32_t nhip_paged_prompt_dev(const nhip_paged_cache* c, int32_t layer, const int8_t* d_q, const float* d_q_scales,
@@ -953,7 +1027,7 @@ int32_t nhip_paged_prompt_dev(const nhip_paged_cache* c, int32_t layer, const in
     rc = check_runs(runs, window);
     if (rc) return rc;
     if (rows == 0 || runs == 0) return NHIP_OK;
-    const PromptSplit split = prompt_split(c, rows, heads, runs, max_count);
+    const PromptSplit split = prompt_split(c, rows, heads, runs, max_count, window);
     NHIP_REQUIRE(split.tiles * c->kv_heads <= (1 << 23), "paged prompt: %d rows in %d runs of %d kv heads are too many",
                  rows, runs, c->kv_heads);
     rc = check_call(c, layer, d_q, d_q_scales, d_out, d_workspace, workspace_bytes,
@@ -972,6 +1046,7 @@ int32_t nhip_paged_prompt_dev(const nhip_paged_cache* c, int32_t layer, const in
     p.run_pos = d_run_pos;
     p.parts = static_cast<float*>(d_workspace);
     p.stats = p.parts + (size_t)rows * heads * split.parts * c->v_dim;
+    p.counts = reinterpret_cast<int32_t*>(p.stats + (size_t)2 * rows * heads * split.parts);
     p.rows = rows;
     p.heads = heads;
     p.group = heads / c->kv_heads;

@@ -102,6 +102,27 @@ def test_prompt_refuses_its_own():
             cache().prompt(0, A, A, 3, 12, runs, A, A, A, window, 96, A, BIG, A)
 
 
+def test_workspace_sizes_need_no_device():
+    """They are the same before and after a device is chosen, and a window never needs more."""
+    c = cache(pages=4096, width=4096)
+    assert c.decode_workspace(4, 12, 300) == 0
+    assert c.decode_workspace(1, 12, 60000) >= 4 * 12 * 2 * 66
+    assert c.prompt_workspace(4000, 12, 3, 60000) == 0
+    assert c.prompt_workspace(20, 12, 1, 60000) >= 4 * 20 * 12 * 2 * 66
+
+
+def test_attention_workspaces_are_checked():
+    c = cache(pages=4096, width=4096)
+    need = c.decode_workspace(1, 12, 60000)
+    for ws, size in ((None, need), (A, need - 1), (A + 8, need)):
+        with refused("workspace"):
+            c.decode(0, A, A, 1, 12, A, A, A, 60000, ws, size, A)
+    need = c.prompt_workspace(20, 12, 1, 60000)
+    for ws, size in ((None, need), (A, need - 1), (A + 8, need)):
+        with refused("workspace"):
+            c.prompt(0, A, A, 20, 12, 1, A, A, A, 0, 60000, ws, size, A)
+
+
 def test_workspaces_are_checked():
     c = cache()
     need = c.pages_workspace(4)

@@ -292,6 +292,43 @@ def test_prompt_few_rows_of_a_long_context(hip):
     check_prompt(gpu, 0, q, qs, runs, 1500, 6005)
 
 
+@pytest.mark.parametrize("window", [0, 1, 700, 3000])
+def test_prompt_split_over_the_length(hip, window):
+    """Few tiles of a long context, in parts that are joined: runs shorter and
+    longer than a part, pages outside the pool, rows behind the last run."""
+    rng = np.random.default_rng(20 + window)
+    runs = [(3, 0, 3000), (2, 1, 20), (0, 2, 0), (1, 3, 1500)]
+    pool = Pool(rng, 1, 330, 16, 2, 48, 64, 4, 200)
+    pool.give(rng, [n + p for n, _, p in runs])
+    pool.tables[0, 7:40] = -1
+    gpu = Gpu(hip, pool)
+    assert gpu.cache.prompt_workspace(8, 12, 4, 3200) > 0
+    q, qs = queries(rng, 8, 12, 48)
+    check_prompt(gpu, 0, q, qs, runs, window, 3200, rows_behind=2)
+
+
+def test_prompt_spoilt_positions(hip):
+    """NaN and infinite scales in a row's future do not reach it; they spoil
+    the rows that attend them."""
+    rng = np.random.default_rng(23)
+    pool = Pool(rng, 1, 40, 16, 2, 64, 64, 1, 8)
+    pool.give(rng, [120])
+    keys, values = pool.key_scales.copy(), pool.value_scales.copy()
+    for scales, pos, bad in ((pool.value_scales, 50, np.nan), (pool.value_scales, 90, np.inf),
+                             (pool.key_scales, 70, np.nan)):
+        scales[0, pool.tables[0, pos // 16], :, pos % 16] = bad
+    gpu = Gpu(hip, pool)
+    q, qs = queries(rng, 120, 4, 64)
+    got = gpu.prompt(0, q, qs, [0, 120], [0], [0], 0, 128)
+    assert np.isnan(got[50:]).all() and np.isfinite(got[:50]).all()
+    count = gpu.decode(0, q, qs, [0] * 120, [0] * 120, list(range(1, 121)), 120)
+    assert np.isnan(count[50:]).all() and np.isfinite(count[:50]).all()
+    pool.key_scales, pool.value_scales = keys, values
+    for r in range(50):
+        want, far = pool.attend(0, 0, q[r], qs[r], 0, r + 1, True)
+        assert np.all(np.abs(got[r] - want) <= far) and np.all(np.abs(count[r] - want) <= far)
+
+
 def test_prompt_rows_out_of_range_and_behind(hip):
     """Runs of unknown sequences, before position 0 or past the table give
     zeros where a row is out of range; rows behind the last run stay."""
