@@ -62,10 +62,13 @@ struct AppendParams {
 // A workgroup takes 16 rows of one kv head; L lanes share a row's key (or
 // value) head, four elements each, so a head's peak is a few DPP steps and 16
 // rows of keys leave as whole dwords.  Values change places through LDS: the
-// cache holds 16 positions of a dimension together, and where the 16 rows are
-// consecutive positions of one sequence (a prompt) a lane writes four of them
-// at once; else each goes by itself.  Bound by the bytes read and written:
-// 8185 rows of 8 kv heads of 128 (84 MB) take APPEND_US us, APPEND_TBS TB/s.
+// cache holds 16 positions of a dimension together, and where the rows are
+// consecutive positions of one sequence (a prompt) a lane writes as many of
+// them at once as lie in a block; else each goes by itself.  Bound by the
+// bytes: 8185 rows of 8 kv heads of 128 (84 MB) take 21.2 us, 4.0 TB/s (24.5
+// with 64 rows a workgroup: fewer are in flight); one step's 16 rows 4.4 us,
+// which is the launch.
+constexpr int kAppendRows = 16;
 typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
 
 template <int L>
@@ -81,12 +84,14 @@ __device__ __forceinline__ float group_max(float v)
 template <int QK, int V>
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p)
 {
-    constexpr int L = V <= 64 ? 16 : 32, PASSES = L / 16, ROWS = 256 / L;  // rows of a pass
-    __shared__ size_t cells[16];
-    __shared__ int places[16], positions[16], sequences[16];
-    __shared__ __align__(16) uint8_t turned[V][20];  // value codes by dimension, then row
+    constexpr int N = kAppendRows, L = V <= 64 ? 16 : 32, ROWS = 256 / L, PASSES = N / ROWS;  // rows of a pass
+    __shared__ size_t cells[N];
+    __shared__ int places[N], first_position;
+    // value codes by dimension, then row from 16 on: a block's 16 rows may begin before the first and end behind the last
+    __shared__ __align__(16) uint8_t turned[V][N + 36];
+    __shared__ bool consecutive;
     const PagedLayer& c = p.c;
-    const int kvh = blockIdx.y, row0 = (int)blockIdx.x * 16, n = min(16, p.rows - row0);
+    const int kvh = blockIdx.y, row0 = (int)blockIdx.x * N, n = min(N, p.rows - row0);
     const int l = threadIdx.x & (L - 1), row_of_pass = threadIdx.x / L;
     f4 x[PASSES][2];
 #pragma unroll
@@ -97,7 +102,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p)
         if (4 * l < V) x[k][1] = *reinterpret_cast<const f4*>(p.v + r * p.ldv + kvh * V + 4 * l);
     }
     // where each row's position lives: its page's first cell (of this kv head) and its place in the page, -1 if nowhere
-    if (threadIdx.x < 16) {
+    if (threadIdx.x < N) {
         const int i = threadIdx.x, r = row0 + min(i, n - 1);
         const int seq = p.row_seq[r], pos = p.row_pos[r];
         int page = -1;
@@ -106,8 +111,13 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p)
         const bool ok = i < n && page >= 0 && page < c.pages;
         cells[i] = ok ? ((size_t)page * c.kv_heads + kvh) << c.page_shift : 0;
         places[i] = ok ? pos & ((1 << c.page_shift) - 1) : -1;
-        positions[i] = pos;
-        sequences[i] = seq;
+        // (the first wave's: whether the rows are consecutive positions of one sequence)
+        const int seq0 = __builtin_amdgcn_readfirstlane(seq), pos0 = __builtin_amdgcn_readfirstlane(pos);
+        const uint64_t odd = __ballot(i < n && (!ok || seq != seq0 || pos != pos0 + i));
+        if (i == 0) {
+            consecutive = odd == 0;
+            first_position = pos;
+        }
     }
     __syncthreads();
 #pragma unroll
@@ -124,7 +134,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p)
             const uint32_t codes = ref_quantize4(make_float4(y[0], y[1], y[2], y[3]), 1.0f / scale);
             if (part == 1 && 4 * l < V) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) turned[4 * l + e][i] = (uint8_t)(codes >> (8 * e));
+                for (int e = 0; e < 4; e++) turned[4 * l + e][16 + i] = (uint8_t)(codes >> (8 * e));
             }
             if (at < 0) continue;
             if (part == 0 && 4 * l < QK) *reinterpret_cast<uint32_t*>(c.keys + (cell + at) * QK + 4 * l) = codes;
@@ -132,35 +142,50 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p)
         }
     }
     __syncthreads();
-    bool consecutive = true;
-    for (int i = 0; i < n; i++)
-        consecutive &= places[i] >= 0 && positions[i] == positions[0] + i && sequences[i] == sequences[0];
     if (consecutive) {
-        // five quads of positions cover 16 rows whatever place the first has in its quad
-        const int lead = positions[0] & 3;
-        for (int item = threadIdx.x; item < 5 * V; item += 256) {
-            const int d = item & (V - 1), first = 4 * (item / V) - lead;  // the quad's first row
+        // blocks of 16 positions, whole ones as one store a dimension, the ends in quads where they have them
+        const int lead = first_position & 15;
+        for (int item = threadIdx.x; item < (N / 16 + 1) * V; item += 256) {
+            const int d = item & (V - 1), first = 16 * (item / V) - lead;  // the block's first row
             if (first >= n) continue;
-            const int some = max(first, 0), at = places[some] & ~3;
-            uint8_t* to = reinterpret_cast<uint8_t*>(c.values) + cells[some] * V + (size_t)(at >> 4) * (16 * V) +
-                          d * 16 + (at & 15);
-            if (first >= 0 && first + 4 <= n) {
-                uint32_t word = 0;
+            const int some = max(first, 0), at = places[some] & ~15;
+            uint8_t* to = reinterpret_cast<uint8_t*>(c.values) + cells[some] * V + (size_t)(at >> 4) * (16 * V) + d * 16;
+            const uint32_t* from = reinterpret_cast<const uint32_t*>(turned[d] + ((16 + first) & ~3));
+            uint32_t words[5];
 #pragma unroll
-                for (int e = 0; e < 4; e++) word |= (uint32_t)turned[d][first + e] << (8 * e);
-                *reinterpret_cast<uint32_t*>(to) = word;
-            } else {
-                for (int e = 0; e < 4; e++)
-                    if (first + e >= 0 && first + e < n) to[e] = turned[d][first + e];
+            for (int k = 0; k < 5; k++) words[k] = from[k];
+#pragma unroll
+            for (int k = 0; k < 4; k++) words[k] = __builtin_amdgcn_alignbyte(words[k + 1], words[k], first & 3);
+            if (first >= 0 && first + 16 <= n) {
+                *reinterpret_cast<uint4*>(to) = make_uint4(words[0], words[1], words[2], words[3]);
+                continue;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int row = first + 4 * k;
+                if (row >= 0 && row + 4 <= n) {
+                    *reinterpret_cast<uint32_t*>(to + 4 * k) = words[k];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (row + e >= 0 && row + e < n) to[4 * k + e] = (uint8_t)(words[k] >> (8 * e));
+                }
             }
         }
     } else {
         for (int item = threadIdx.x; item < n * V; item += 256) {
             const int d = item & (V - 1), i = item / V, at = places[i];
             if (at >= 0)
-                c.values[cells[i] * V + (size_t)(at >> 4) * (16 * V) + d * 16 + (at & 15)] = (int8_t)turned[d][i];
+                c.values[cells[i] * V + (size_t)(at >> 4) * (16 * V) + d * 16 + (at & 15)] = (int8_t)turned[d][16 + i];
         }
     }
+}
+
+template <int QK, int V>
+void launch_append(const AppendParams& p, hipStream_t stream)
+{
+    hipLaunchKernelGGL((paged_append_kernel<QK, V>), dim3((unsigned)(p.rows + kAppendRows - 1) / kAppendRows, p.c.kv_heads),
+                       dim3(256), 0, stream, p);
 }
 
 // ----------------------------------------------------------------- pages --
@@ -168,12 +193,12 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p)
 struct Pages {
     nhip_paged_cache c;
     int32_t page_shift;
-    size_t key_units, scale_units, value_units;  // 16-byte units of a page in one layer
+    uint32_t key_units, scale_units, value_units;  // 16-byte units of a page in one layer
 };
 
 Pages pages_of(const nhip_paged_cache* c)
 {
-    const size_t cells = (size_t)c->kv_heads * c->page_size;
+    const uint32_t cells = (uint32_t)c->kv_heads * c->page_size;
     return {*c, __builtin_ctz((unsigned)c->page_size), cells * c->qk_dim / 16, cells * 4 / 16,
             cells * c->v_dim / 16};
 }
@@ -190,34 +215,67 @@ __device__ __forceinline__ int page_count(const Pages& p, int length)
     return (length + (1 << p.page_shift) - 1) >> p.page_shift;
 }
 
-__device__ __forceinline__ void copy_units(uint8_t* pool, size_t units, size_t layer_page, size_t from, size_t to)
+// A page of one layer is copied in slices of kSliceUnits 16-byte units, a
+// workgroup each: eight loads a lane, then eight stores.
+constexpr int kSliceUnits = 2048;
+
+__host__ __device__ inline uint32_t page_units(const Pages& p)
 {
-    const uint4* s = reinterpret_cast<const uint4*>(pool) + (layer_page + from) * units;
-    uint4* d = reinterpret_cast<uint4*>(pool) + (layer_page + to) * units;
-    for (size_t u = threadIdx.x; u < units; u += blockDim.x) d[u] = s[u];
+    return p.key_units + p.value_units + 2 * p.scale_units;
+}
+__host__ __device__ inline uint32_t page_slices(const Pages& p)
+{
+    return (page_units(p) + kSliceUnits - 1) / kSliceUnits;
 }
 
-// One layer of page `from` to page `to`, by a workgroup.
-__device__ __forceinline__ void copy_page_layer(const Pages& p, int layer, int from, int to)
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+// Where unit u of a page's layer lies in the pools, u counting keys, values,
+// key scales, value scales; `cell` is layer * pages + page.
+__device__ __forceinline__ u4* page_unit(const Pages& p, size_t cell, uint32_t u)
+{
+    const uint32_t k = p.key_units, v = p.value_units, s = p.scale_units;
+    const bool keys = u < k, values = u < k + v, key_scales = u < k + v + s;
+    u4* pool = reinterpret_cast<u4*>(keys ? (void*)p.c.keys
+                                     : values ? (void*)p.c.values
+                                     : key_scales ? (void*)p.c.key_scales : (void*)p.c.value_scales);
+    const uint32_t units = keys ? k : values ? v : s;
+    const uint32_t at = keys ? u : values ? u - k : key_scales ? u - k - v : u - k - v - s;
+    return pool + cell * units + at;
+}
+
+__device__ __forceinline__ void copy_slice(const Pages& p, int layer, int from, int to, uint32_t slice)
 {
     const size_t base = (size_t)layer * p.c.pages;
-    copy_units((uint8_t*)p.c.keys, p.key_units, base, from, to);
-    copy_units((uint8_t*)p.c.values, p.value_units, base, from, to);
-    copy_units((uint8_t*)p.c.key_scales, p.scale_units, base, from, to);
-    copy_units((uint8_t*)p.c.value_scales, p.scale_units, base, from, to);
+    const uint32_t first = slice * kSliceUnits + threadIdx.x, last = page_units(p) - 1;
+    u4 x[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) x[k] = *page_unit(p, base + from, min(first + 256 * k, last));
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+        if (first + 256 * k <= last) *page_unit(p, base + to, first + 256 * k) = x[k];
 }
 
-// Pairs of pages; entries out of range (a page that is not to be copied) are
-// skipped.  `total` (may be NULL) holds the number of pairs on the device.
-__global__ __launch_bounds__(256) void paged_copy_kernel(Pages p, const int32_t* src, const int32_t* dst,
-                                                         const int32_t* total, int32_t count)
+// The slices of `n` pairs of pages in every layer, spread over `workers`
+// workgroups; a pair out of range (a page that is not to be copied) is skipped.
+__device__ __forceinline__ void copy_pairs(const Pages& p, const int32_t* src, const int32_t* dst, int n, int worker,
+                                           int workers)
 {
-    const size_t n = (size_t)(total ? *total : count) * p.c.layers;
-    for (size_t i = blockIdx.x; i < n; i += gridDim.x) {
-        const size_t pair = i / p.c.layers;
+    // (a page's layer is at least 1920 bytes, so a pool that fits the device has fewer than 2^32 slices)
+    const uint32_t slices = page_slices(p), layers = p.c.layers;
+    const uint32_t items = (uint32_t)n * layers * slices;
+    for (uint32_t i = worker; i < items; i += workers) {
+        const uint32_t rest = i / slices, pair = rest / layers;
         const int from = src[pair], to = dst[pair];
-        if (is_page(p, from) && is_page(p, to) && from != to) copy_page_layer(p, (int)(i - pair * p.c.layers), from, to);
+        if (is_page(p, from) && is_page(p, to) && from != to)
+            copy_slice(p, (int)(rest - pair * layers), from, to, i - rest * slices);
     }
+}
+
+__global__ __launch_bounds__(256) void paged_copy_kernel(Pages p, const int32_t* src, const int32_t* dst,
+                                                         int32_t count)
+{
+    copy_pairs(p, src, dst, count, blockIdx.x, gridDim.x);
 }
 
 __global__ __launch_bounds__(256) void paged_reset_kernel(Pages p)
@@ -236,6 +294,20 @@ __device__ __forceinline__ bool named_before(const int32_t* seq, int i)
     bool found = false;
     for (int j = threadIdx.x; j < i; j += blockDim.x) found |= seq[j] == s;
     return __syncthreads_or(found) != 0;
+}
+
+// How many of the first n entries of an LDS list equal v (n need not be a
+// multiple of 4; the list is padded to one).
+__device__ __forceinline__ int count_equal(const int* list, int n, int v)
+{
+    int found = 0;
+    const int4* l4 = reinterpret_cast<const int4*>(list);
+#pragma unroll 4
+    for (int j = 0; j < n; j += 4) {
+        const int4 x = l4[j / 4];
+        found += (x.x == v) + (j + 1 < n && x.y == v) + (j + 2 < n && x.z == v) + (j + 3 < n && x.w == v);
+    }
+    return found;
 }
 
 // fork, first half: entry i's new row and length into the workspace, and the
@@ -281,6 +353,50 @@ __global__ __launch_bounds__(256) void paged_fork_write_kernel(Pages p, const in
     if (threadIdx.x == 0) p.c.lengths[d] = keep;
 }
 
+// fork of a few short rows in one launch: one workgroup, the halves on either
+// side of a barrier, a wave per entry.
+constexpr int kForkThreads = 1024;
+__global__ __launch_bounds__(kForkThreads) void paged_fork_kernel(Pages p, const int32_t* dst, const int32_t* src,
+                                                                  const int32_t* length, int32_t count,
+                                                                  int32_t* staged)
+{
+    __shared__ __align__(16) int entry_dst[kMaxEntries];
+    __shared__ int entry_keep[kMaxEntries];
+    const int i = threadIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int d = i < count ? dst[i] : -1, s = i < count ? src[i] : -1;
+    entry_dst[i] = d;
+    __syncthreads();
+    int keep = -1;
+    if (d >= 0 && d < p.c.sequences && s >= 0 && s < p.c.sequences && count_equal(entry_dst, i, d) == 0) {
+        const int has = held_length(p, s);
+        keep = length ? min(max(length[i], 0), has) : has;
+    }
+    entry_keep[i] = keep;
+    __syncthreads();
+    for (int e = wave; e < count; e += kForkThreads / 64) {
+        const int n = page_count(p, max(entry_keep[e], 0));
+        const int32_t* row = p.c.tables + (size_t)(n ? src[e] : 0) * p.c.width;
+        for (int t = lane; t < n; t += 64) {
+            const int page = row[t];
+            staged[(size_t)e * p.c.width + t] = page;
+            if (is_page(p, page)) atomicAdd(&p.c.refs[page], 1);
+        }
+    }
+    __syncthreads();
+    for (int e = wave; e < count; e += kForkThreads / 64) {
+        if (entry_keep[e] < 0) continue;
+        const int to = entry_dst[e];
+        const int n = page_count(p, entry_keep[e]), old = page_count(p, held_length(p, to));
+        int32_t* row = p.c.tables + (size_t)to * p.c.width;
+        for (int t = lane; t < max(old, n); t += 64) {
+            const int page = row[t];
+            if (t < old && is_page(p, page)) atomicAdd(&p.c.refs[page], -1);
+            row[t] = t < n ? staged[(size_t)e * p.c.width + t] : -1;
+        }
+        if (lane == 0) p.c.lengths[to] = entry_keep[e];
+    }
+}
+
 // Exclusive prefix sum over the 1024 threads of a workgroup; *total is the
 // sum.  `waves` is 16 ints of LDS, free again after the call.
 __device__ __forceinline__ int block_scan(int v, int* waves, int* total)
@@ -303,19 +419,30 @@ __device__ __forceinline__ int block_scan(int v, int* waves, int* total)
     return before + sum - v;
 }
 
-constexpr int kPlan = 1024;      // threads of the planning kernels
-constexpr int kPlanPages = 4;    // pages a thread looks at per round
+constexpr int kPlan = 1024;     // threads of the planning kernels
+constexpr int kPlanPages = 16;  // pages a thread looks at per round
 typedef int32_t i4 __attribute__((ext_vector_type(4), aligned(4)));
 
-// The refs of pages [base + 4 tid, base + 4 tid + 4), -1 past the last page.
-__device__ __forceinline__ i4 plan_refs(const Pages& p, int base)
+// The refs of this thread's kPlanPages pages of a round from `base`, -1 past the last page.
+struct PlanRefs {
+    int32_t r[kPlanPages];
+};
+__device__ __forceinline__ PlanRefs plan_refs(const Pages& p, int base)
 {
+    PlanRefs x;
     const int at = base + kPlanPages * (int)threadIdx.x;
-    if (at + 4 <= p.c.pages) return *reinterpret_cast<const i4*>(p.c.refs + at);
-    i4 r = {-1, -1, -1, -1};
-    for (int k = 0; k < 4; k++)
-        if (at + k < p.c.pages) r[k] = p.c.refs[at + k];
-    return r;
+#pragma unroll
+    for (int k = 0; k < kPlanPages; k += 4) {
+        if (at + k + 4 <= p.c.pages) {
+            const i4 v = *reinterpret_cast<const i4*>(p.c.refs + at + k);
+#pragma unroll
+            for (int e = 0; e < 4; e++) x.r[k + e] = v[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) x.r[k + e] = at + k + e < p.c.pages ? p.c.refs[at + k + e] : -1;
+        }
+    }
+    return x;
 }
 
 // resize: one workgroup, a thread per entry.  Every decision first (what an
@@ -327,8 +454,8 @@ __global__ __launch_bounds__(kPlan) void paged_resize_kernel(Pages p, const int3
                                                              int32_t* pair_dst, int32_t* free_list)
 {
     __shared__ int waves[16];
-    __shared__ int entry_seq[kMaxEntries], entry_tail[kMaxEntries], entry_has[kMaxEntries], entry_want[kMaxEntries],
-        entry_start[kMaxEntries];
+    __shared__ __align__(16) int entry_seq[kMaxEntries], entry_tail[kMaxEntries];
+    __shared__ int entry_has[kMaxEntries], entry_want[kMaxEntries], entry_start[kMaxEntries];
     __shared__ uint8_t entry_copies[kMaxEntries];
     const int i = threadIdx.x;
     const int s = i < count ? seq[i] : -1;
@@ -338,8 +465,7 @@ __global__ __launch_bounds__(kPlan) void paged_resize_kernel(Pages p, const int3
     bool ok = i < count && s >= 0 && s < p.c.sequences;
     const bool refused = i < count && (!ok || want_length < 0 || want_length > (p.c.width << p.page_shift));
     ok = ok && !refused;
-    if (ok)
-        for (int j = 0; j < i; j++) ok &= entry_seq[j] != s;
+    ok = ok && count_equal(entry_seq, i, s) == 0;
     int has = 0, want = 0, tail = -1;
     if (ok) {
         const int old = held_length(p, s);
@@ -356,9 +482,8 @@ __global__ __launch_bounds__(kPlan) void paged_resize_kernel(Pages p, const int3
     __syncthreads();
     bool copies = false;
     if (tail >= 0) {
-        int earlier = 0;
-        for (int j = 0; j < i; j++) earlier += entry_tail[j] == tail;
-        copies = earlier < p.c.refs[tail] - 1;
+        const int holders = p.c.refs[tail];
+        copies = holders > 1 && count_equal(entry_tail, i, tail) < holders - 1;
     }
     entry_copies[i] = copies;
     int total, refusals;
@@ -369,12 +494,14 @@ __global__ __launch_bounds__(kPlan) void paged_resize_kernel(Pages p, const int3
     // the `total` lowest free pages
     int found = 0;
     for (int base = 0; base < p.c.pages && found < total; base += kPlan * kPlanPages) {
-        const i4 r = plan_refs(p, base);
+        const PlanRefs x = plan_refs(p, base);
         int here, mine = 0;
-        for (int k = 0; k < 4; k++) mine += r[k] == 0;
+#pragma unroll
+        for (int k = 0; k < kPlanPages; k++) mine += x.r[k] == 0;
         int at = found + block_scan(mine, waves, &here);
-        for (int k = 0; k < 4; k++)
-            if (r[k] == 0) {
+#pragma unroll
+        for (int k = 0; k < kPlanPages; k++)
+            if (x.r[k] == 0) {
                 if (at < total) free_list[at] = base + kPlanPages * i + k;
                 at++;
             }
@@ -414,65 +541,68 @@ __global__ __launch_bounds__(kPlan) void paged_resize_kernel(Pages p, const int3
     }
 }
 
-// compact: one workgroup counts the held pages n, then pairs the free pages
-// below n with the held ones from n on, both in order.
+// compact, first launch: one workgroup counts the held pages n, pairs the
+// free pages below n with the held ones from n on, both in order, and moves
+// their refs.  remap [pages] (written only where something moves) receives the
+// moved pages' new places.
 __global__ __launch_bounds__(kPlan) void paged_compact_plan_kernel(Pages p, int32_t* status, int32_t* total,
-                                                                   int32_t* src, int32_t* dst)
+                                                                   int32_t* src, int32_t* dst, int32_t* remap)
 {
     __shared__ int waves[16];
     int held = 0;
     for (int base = 0; base < p.c.pages; base += kPlan * kPlanPages) {
-        const i4 r = plan_refs(p, base);
-        for (int k = 0; k < 4; k++) held += r[k] > 0;
+        const PlanRefs x = plan_refs(p, base);
+#pragma unroll
+        for (int k = 0; k < kPlanPages; k++) held += x.r[k] > 0;
     }
     int n;
     block_scan(held, waves, &n);
     int holes = 0, movers = 0;
     for (int base = 0; base < p.c.pages; base += kPlan * kPlanPages) {
-        const i4 r = plan_refs(p, base);
+        const PlanRefs x = plan_refs(p, base);
         const int at = base + kPlanPages * (int)threadIdx.x;
-        int hole = 0, mover = 0, sum;
-        for (int k = 0; k < 4; k++) {
-            hole += r[k] == 0 && at + k < n;
-            mover += r[k] > 0 && at + k >= n;
-        }
-        int h = holes + block_scan(hole, waves, &sum);
-        holes += sum;
-        int m = movers + block_scan(mover, waves, &sum);
-        movers += sum;
-        for (int k = 0; k < 4; k++) {
-            if (r[k] == 0 && at + k < n) dst[h++] = at + k;
-            if (r[k] > 0 && at + k >= n) src[m++] = at + k;
+        int both = 0, sum;  // holes in the low half, movers in the high (a round has 2^14 pages)
+#pragma unroll
+        for (int k = 0; k < kPlanPages; k++)
+            both += (x.r[k] == 0 && at + k < n ? 1 : 0) + (x.r[k] > 0 && at + k >= n ? 1 << 16 : 0);
+        const int before = block_scan(both, waves, &sum);
+        int h = holes + (before & 0xFFFF), m = movers + (before >> 16);
+        holes += sum & 0xFFFF;
+        movers += sum >> 16;
+#pragma unroll
+        for (int k = 0; k < kPlanPages; k++) {
+            if (x.r[k] == 0 && at + k < n) dst[h++] = at + k;
+            if (x.r[k] > 0 && at + k >= n) src[m++] = at + k;
         }
     }
+    __syncthreads();
+    const int pairs = min(movers, holes);
+    for (int i = threadIdx.x; i < pairs; i += kPlan) {
+        const int from = src[i], to = dst[i];
+        remap[from] = to;
+        p.c.refs[to] = p.c.refs[from];
+        p.c.refs[from] = 0;
+    }
     if (threadIdx.x == 0) {
-        *total = min(movers, holes);
+        *total = pairs;
         if (status) *status = n;
     }
 }
 
-// The new page of each moved one, over `remap` [pages] (written only where
-// something moves), and the refs that move with them.
-__global__ __launch_bounds__(256) void paged_compact_remap_kernel(Pages p, const int32_t* total, const int32_t* src,
-                                                                  const int32_t* dst, int32_t* remap)
-{
-    const int n = *total;
-    for (int i = (int)blockIdx.x * 256 + (int)threadIdx.x; i < n; i += (int)gridDim.x * 256) {
-        remap[src[i]] = dst[i];
-        p.c.refs[dst[i]] = p.c.refs[src[i]];
-    }
-}
-
-__global__ __launch_bounds__(256) void paged_compact_tables_kernel(Pages p, const int32_t* total, const int32_t* src,
-                                                                   const int32_t* remap)
+// Second launch: the first `table_blocks` workgroups rewrite the tables, the
+// others copy the pages.
+__global__ __launch_bounds__(256) void paged_compact_move_kernel(Pages p, const int32_t* total, const int32_t* src,
+                                                                 const int32_t* dst, const int32_t* remap,
+                                                                 int table_blocks)
 {
     const int n = *total;
     if (n == 0) return;
-    const size_t tid = (size_t)blockIdx.x * 256 + threadIdx.x, stride = (size_t)gridDim.x * 256;
-    for (size_t i = tid; i < (size_t)n; i += stride) p.c.refs[src[i]] = 0;
-    // the movers are the held pages from the first one's index on
-    const int first = src[0];
-    for (int s = blockIdx.x; s < p.c.sequences; s += gridDim.x) {
+    if ((int)blockIdx.x >= table_blocks) {
+        copy_pairs(p, src, dst, n, (int)blockIdx.x - table_blocks, (int)gridDim.x - table_blocks);
+        return;
+    }
+    const int first = src[0];  // every held page from the first moved one on has moved
+    for (int s = blockIdx.x; s < p.c.sequences; s += table_blocks) {
         const int held = page_count(p, held_length(p, s));
         int32_t* row = p.c.tables + (size_t)s * p.c.width;
         for (int t = threadIdx.x; t < held; t += 256)
@@ -503,12 +633,16 @@ int32_t check_workspace(const nhip_paged_cache* c, int32_t count, const void* ws
     return NHIP_OK;
 }
 
-void launch_copy(const Pages& p, const int32_t* src, const int32_t* dst, const int32_t* total, int32_t most,
-                 hipStream_t stream)
+// Workgroups that copy up to `pairs` pages (the pairs in use may be fewer:
+// each worker walks on by the number of workers).
+unsigned copy_workers(const Pages& p, int64_t pairs)
 {
-    const size_t items = (size_t)most * p.c.layers;
-    hipLaunchKernelGGL(paged_copy_kernel, dim3((unsigned)std::min<size_t>(items, 4096)), dim3(256), 0, stream, p, src,
-                       dst, total, most);
+    return (unsigned)std::min<int64_t>(std::max<int64_t>(pairs * p.c.layers * page_slices(p), 1), 8192);
+}
+
+void launch_copy(const Pages& p, const int32_t* src, const int32_t* dst, int32_t count, hipStream_t stream)
+{
+    hipLaunchKernelGGL(paged_copy_kernel, dim3(copy_workers(p, count)), dim3(256), 0, stream, p, src, dst, count);
 }
 
 int32_t resize(const nhip_paged_cache* c, int32_t count, const int32_t* d_seq, const int32_t* d_length, bool grows,
@@ -527,7 +661,7 @@ int32_t resize(const nhip_paged_cache* c, int32_t count, const int32_t* d_seq, c
     hipLaunchKernelGGL(paged_resize_kernel, dim3(1), dim3(kPlan), 0, as_stream(stream), p, d_seq, d_length, count,
                        d_status, w, w + count, w + 2 * count);
     NHIP_CHECK_HIP(hipGetLastError());
-    if (grows && count) launch_copy(p, w, w + count, nullptr, count, as_stream(stream));
+    if (grows && count) launch_copy(p, w, w + count, count, as_stream(stream));
     NHIP_CHECK_HIP(hipGetLastError());
     return NHIP_OK;
 }
@@ -567,13 +701,12 @@ int32_t nhip_paged_append_dev(const nhip_paged_cache* c, int32_t layer, const fl
     rc = ensure_device();
     if (rc) return rc;
     const AppendParams p{paged_layer(c, layer), d_k, d_v, d_row_seq, d_row_pos, ldk, ldv, rows};
-    const dim3 grid((unsigned)(rows + 15) / 16, (unsigned)c->kv_heads);
     if (c->qk_dim == 48)
-        hipLaunchKernelGGL((paged_append_kernel<48, 64>), grid, dim3(256), 0, as_stream(stream), p);
+        launch_append<48, 64>(p, as_stream(stream));
     else if (c->qk_dim == 64)
-        hipLaunchKernelGGL((paged_append_kernel<64, 64>), grid, dim3(256), 0, as_stream(stream), p);
+        launch_append<64, 64>(p, as_stream(stream));
     else
-        hipLaunchKernelGGL((paged_append_kernel<128, 128>), grid, dim3(256), 0, as_stream(stream), p);
+        launch_append<128, 128>(p, as_stream(stream));
     NHIP_CHECK_HIP(hipGetLastError());
     return NHIP_OK;
 }
@@ -592,7 +725,7 @@ int32_t nhip_paged_copy_dev(const nhip_paged_cache* c, int32_t count, const int3
     NHIP_REQUIRE(d_src && d_dst, "paged copy: null pointer");
     rc = ensure_device();
     if (rc) return rc;
-    launch_copy(pages_of(c), d_src, d_dst, nullptr, count, as_stream(stream));
+    launch_copy(pages_of(c), d_src, d_dst, count, as_stream(stream));
     NHIP_CHECK_HIP(hipGetLastError());
     return NHIP_OK;
 }
@@ -610,6 +743,14 @@ int32_t nhip_paged_fork_dev(const nhip_paged_cache* c, int32_t count, const int3
     if (rc) return rc;
     const Pages p = pages_of(c);
     int32_t* w = static_cast<int32_t*>(d_workspace);
+    // 3 rows of 12 pages take 4.1 us in one launch and 6.7 in two, 16 of 63 4.2 and 6.6, but 64 of 19 10.6 and 6.6, 8 of
+    // 1875 31.8 and 11.5: one launch where a wave has one row and few rounds of it.
+    if (count <= kForkThreads / 64 && c->width <= 128) {
+        hipLaunchKernelGGL(paged_fork_kernel, dim3(1), dim3(kForkThreads), 0, as_stream(stream), p, d_dst, d_src,
+                           d_length, count, w);
+        NHIP_CHECK_HIP(hipGetLastError());
+        return NHIP_OK;
+    }
     hipLaunchKernelGGL(paged_fork_stage_kernel, dim3(count), dim3(256), 0, as_stream(stream), p, d_dst, d_src,
                        d_length, w, w + count);
     NHIP_CHECK_HIP(hipGetLastError());
@@ -644,15 +785,11 @@ int32_t nhip_paged_compact_dev(const nhip_paged_cache* c, int32_t* d_status, voi
     int32_t* w = static_cast<int32_t*>(d_workspace);
     int32_t *total = w, *src = w + 16, *dst = src + c->pages, *remap = dst + c->pages;
     hipStream_t s = as_stream(stream);
-    hipLaunchKernelGGL(paged_compact_plan_kernel, dim3(1), dim3(kPlan), 0, s, p, d_status, total, src, dst);
+    hipLaunchKernelGGL(paged_compact_plan_kernel, dim3(1), dim3(kPlan), 0, s, p, d_status, total, src, dst, remap);
     NHIP_CHECK_HIP(hipGetLastError());
-    const unsigned grid = (unsigned)std::min((c->pages + 255) / 256, 1024);
-    hipLaunchKernelGGL(paged_compact_remap_kernel, dim3(grid), dim3(256), 0, s, p, total, src, dst, remap);
-    NHIP_CHECK_HIP(hipGetLastError());
-    launch_copy(p, src, dst, total, (c->pages + 1) / 2, s);
-    NHIP_CHECK_HIP(hipGetLastError());
-    hipLaunchKernelGGL(paged_compact_tables_kernel, dim3((unsigned)std::min(c->sequences, 1024)), dim3(256), 0, s, p,
-                       total, src, remap);
+    const unsigned table_blocks = (unsigned)std::min(c->sequences, 1024);
+    hipLaunchKernelGGL(paged_compact_move_kernel, dim3(table_blocks + copy_workers(p, c->pages / 2)), dim3(256), 0, s, p,
+                       total, src, dst, remap, (int)table_blocks);
     NHIP_CHECK_HIP(hipGetLastError());
     return NHIP_OK;
 }
