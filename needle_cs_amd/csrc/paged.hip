@@ -216,7 +216,8 @@ __device__ __forceinline__ int page_count(const Pages& p, int length)
 }
 
 // A page of one layer is copied in slices of kSliceUnits 16-byte units, a
-// workgroup each: eight loads a lane, then eight stores.
+// workgroup each: eight loads a lane, then eight stores, past the caches (a
+// compaction of 650 MB takes 140 us, 151 through them).
 constexpr int kSliceUnits = 2048;
 
 __host__ __device__ inline uint32_t page_units(const Pages& p)
@@ -250,10 +251,10 @@ __device__ __forceinline__ void copy_slice(const Pages& p, int layer, int from, 
     const uint32_t first = slice * kSliceUnits + threadIdx.x, last = page_units(p) - 1;
     u4 x[8];
 #pragma unroll
-    for (int k = 0; k < 8; k++) x[k] = *page_unit(p, base + from, min(first + 256 * k, last));
+    for (int k = 0; k < 8; k++) x[k] = __builtin_nontemporal_load(page_unit(p, base + from, min(first + 256 * k, last)));
 #pragma unroll
     for (int k = 0; k < 8; k++)
-        if (first + 256 * k <= last) *page_unit(p, base + to, first + 256 * k) = x[k];
+        if (first + 256 * k <= last) __builtin_nontemporal_store(x[k], page_unit(p, base + to, first + 256 * k));
 }
 
 // The slices of `n` pairs of pages in every layer, spread over `workers`
@@ -302,11 +303,14 @@ __device__ __forceinline__ int count_equal(const int* list, int n, int v)
 {
     int found = 0;
     const int4* l4 = reinterpret_cast<const int4*>(list);
-#pragma unroll 4
-    for (int j = 0; j < n; j += 4) {
-        const int4 x = l4[j / 4];
-        found += (x.x == v) + (j + 1 < n && x.y == v) + (j + 2 < n && x.z == v) + (j + 3 < n && x.w == v);
+#pragma unroll 8
+    for (int j = 0; j < n / 4; j++) {
+        const int4 x = l4[j];
+        found += (x.x == v) + (x.y == v) + (x.z == v) + (x.w == v);
     }
+    const int4 x = l4[n / 4];
+    const int rest = n & 3;
+    found += (rest > 0 && x.x == v) + (rest > 1 && x.y == v) + (rest > 2 && x.z == v);
     return found;
 }
 
@@ -458,6 +462,7 @@ __global__ __launch_bounds__(kPlan) void paged_resize_kernel(Pages p, const int3
     __shared__ int entry_has[kMaxEntries], entry_want[kMaxEntries], entry_start[kMaxEntries];
     __shared__ uint8_t entry_copies[kMaxEntries];
     const int i = threadIdx.x;
+    const PlanRefs round0 = plan_refs(p, 0);  // (ahead of the loads that depend on one another)
     const int s = i < count ? seq[i] : -1;
     const int want_length = i < count && length ? length[i] : 0;
     entry_seq[i] = s;
@@ -494,7 +499,7 @@ __global__ __launch_bounds__(kPlan) void paged_resize_kernel(Pages p, const int3
     // the `total` lowest free pages
     int found = 0;
     for (int base = 0; base < p.c.pages && found < total; base += kPlan * kPlanPages) {
-        const PlanRefs x = plan_refs(p, base);
+        const PlanRefs x = base == 0 ? round0 : plan_refs(p, base);
         int here, mine = 0;
 #pragma unroll
         for (int k = 0; k < kPlanPages; k++) mine += x.r[k] == 0;
