@@ -343,6 +343,9 @@ int32_t nhip_attention_decode_noalloc_dev(const int8_t* d_q, const float* d_q_sc
  * (128, 128); kv_heads <= 256; layers <= 4096; pages <= 2^20; sequences <=
  * 65536; width * page_size <= 2^30; a call takes up to 2^20 rows.
  *
+ * Scales are not negative (QuantizeInt8's are positive); a scale that is no
+ * finite number spoils the rows that attend its position, and only those.
+ *
  * The calls below take this struct by pointer (read during the call), are
  * asynchronous on `stream` and may be captured in a graph; calls that write
  * a cache must be ordered with the other calls on it.  A table entry outside

@@ -540,7 +540,7 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
     __shared__ __align__(16) uint8_t lds_k[2][64 * KS];
     __shared__ __align__(16) uint8_t lds_v[2][V * 128];
     __shared__ float lds_ks[4][64], lds_vs[4][64];
-    __shared__ uint16_t lds_live[4][4];
+    __shared__ __align__(8) uint16_t lds_live[4][4];
     const PagedLayer& c = p.c;
     // (a tile's kv heads side by side: with 8 of them each XCD keeps one head's positions in its L2)
     const int tile_of_call = blockIdx.x / c.kv_heads, kvh = blockIdx.x - tile_of_call * c.kv_heads;
@@ -668,7 +668,7 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
     for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
-    float peak = kNoScore, total[2] = {0.0f, 0.0f};
+    float peak = kNoScore, total = 0.0f;
     int exponent = -100;  // of the value scales, the largest so far
     const float minus_one = alone(-1.0f);
     // where this lane reads: the key row of its A row, the value rows of its dimensions
@@ -745,8 +745,7 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
                     const float to = up - peak > kHeadroom ? up - (kHeadroom - kLag) : peak;
                     float keep = __builtin_amdgcn_exp2f(peak - to);
                     peak = to;
-                    total[0] *= keep;
-                    total[1] *= keep;
+                    total *= keep;
                     int e = ev;
                     for (int off = 32; off; off >>= 1) e = max(e, __shfl_xor(e, off));
                     e = max(__builtin_amdgcn_readfirstlane(min(e, 100)), exponent);
@@ -757,12 +756,13 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
                 }
                 const float unit = __uint_as_float((uint32_t)(127 - exponent) << 23);
                 const float vn[2] = {vs[0] * unit, vs[1] * unit};
+                float sum[2] = {0.0f, 0.0f};  // of the tile: a long row's total is a sum of tiles' sums
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
                     float w[16];
 #define NHIP_WEIGHT(r)                                       \
     w[r] = __builtin_amdgcn_exp2f(fmaf(z[t][r], qs, -peak)); \
-    total[r & 1] += w[r];                                    \
+    sum[r & 1] += w[r];                                      \
     w[r] = alone(row_bcast<r>(vn[t]) * w[r]);
                     NHIP_WEIGHT(0) NHIP_WEIGHT(1) NHIP_WEIGHT(2) NHIP_WEIGHT(3) NHIP_WEIGHT(4) NHIP_WEIGHT(5)
                     NHIP_WEIGHT(6) NHIP_WEIGHT(7) NHIP_WEIGHT(8) NHIP_WEIGHT(9) NHIP_WEIGHT(10) NHIP_WEIGHT(11)
@@ -789,6 +789,7 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
                         }
                     }
                 }
+                total += sum[0] + sum[1];
             }
             store_keys(tile + 1, page);
             store_values(tile + 1);
@@ -796,8 +797,7 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
         }
     }
 
-    float all = total[0] + total[1];
-    all += lane_xor<32>(all);
+    float all = total + lane_xor<32>(total);
     if (!mine) return;
     if (q_pos < 0) {  // a row out of range, in a tile of others
         all = 0.0f;

@@ -42,6 +42,7 @@ class PagedCache:
         self.ptr = C.addressof(self.view)
         if self.buffers:
             self.reset()
+            check(lib().nhip_stream_sync(None))  # calls on any stream find it empty
 
     def reset(self, stream=None) -> None:
         check(lib().nhip_paged_reset_dev(self.ptr, stream))

@@ -690,11 +690,12 @@ def test_a_server_s_steps(hip, orc):
 
 
 def test_in_a_graph(hip, orc):
-    """A decode step (branch, grow, append, attend, compact) captured once and
-    replayed: every replay equals the same calls made eagerly on a twin."""
+    """A decode step (branch, grow, append, attend both ways, one of them split
+    over the length, compact) captured once and replayed: every replay equals
+    the same calls made eagerly on a twin."""
     rng = np.random.default_rng(31)
     lengths = [40, 23, 16, 70]
-    pool = Pool(rng, 1, 40, 16, 2, 64, 64, 4, 8)
+    pool = Pool(rng, 1, 40, 16, 2, 64, 64, 4, 64)
     pool.give(rng, lengths)
     twins = [Gpu(hip, pool), Gpu(hip, pool)]
     q, qs = queries(rng, 4, 8, 64)
@@ -705,20 +706,25 @@ def test_in_a_graph(hip, orc):
         out = gpu.dev(np.zeros((4, 8, 64)), np.float32)
         seq, parents, grown, last, first, count = (gpu.dev(a) for a in ([0, 1, 2, 3], [1, 1, 3, 3], [24, 24, 71, 71],
                                                                         [23, 23, 70, 70], [0] * 4, [24, 24, 71, 71]))
+        out2 = gpu.dev(np.zeros((4, 8, 64)), np.float32)
+        runs = gpu.dev([0, 1, 2, 3, 4])
+        parts = gpu.workspace(gpu.cache.prompt_workspace(4, 8, 4, 1024))
         dx, dq, ds = gpu.dev(x, np.float32), gpu.dev(q, np.int8), gpu.dev(qs, np.float32)
         pages, att = (gpu.workspace(n) for n in (gpu.cache.pages_workspace(4),
                                                  gpu.cache.decode_workspace(4, 8, 128)))
         status = gpu.dev([9, 9])
 
         def step(st, gpu=gpu, out=out, seq=seq, parents=parents, grown=grown, last=last, first=first, count=count,
-                 dx=dx, dq=dq, ds=ds, pages=pages, att=att, status=status):
+                 dx=dx, dq=dq, ds=ds, pages=pages, att=att, status=status, out2=out2, runs=runs, parts=parts):
             c = gpu.cache
             c.fork(4, seq.ptr, parents.ptr, last.ptr, *pages, stream=st)
             c.resize(4, seq.ptr, grown.ptr, status.ptr, *pages, stream=st)
             c.append(0, dx.ptr, 256, dx.ptr + 512, 256, seq.ptr, last.ptr, 4, stream=st)
             c.decode(0, dq.ptr, ds.ptr, 4, 8, seq.ptr, first.ptr, count.ptr, 128, *att, out.ptr, stream=st)
+            c.prompt(0, dq.ptr, ds.ptr, 4, 8, 4, runs.ptr, seq.ptr, last.ptr, 0, 1024, *parts, out2.ptr, stream=st)
             c.compact(None, *pages, stream=st)
-        sets.append((gpu, out, step))
+        assert parts[1] > 0
+        sets.append((gpu, out, step, out2))
     with hip.Graph.capture(stream) as graph:
         sets[0][2](stream.ptr)
     check_books(twins[0], Books(pool))  # capturing ran nothing
@@ -730,6 +736,8 @@ def test_in_a_graph(hip, orc):
         other.sync()
         a, b = (s[1].download(np.float32) for s in sets)
         assert np.array_equal(a, b) and np.abs(a).max() > 0
+        a2, b2 = (s[3].download(np.float32) for s in sets)
+        assert np.array_equal(a2, b2) and np.abs(a2 - a).max() <= 1e-4 * np.abs(a).max()
         for name in Pool.NAMES:
             assert np.array_equal(twins[0].get(name), twins[1].get(name), equal_nan=True), name
     graph.close()
