@@ -153,8 +153,17 @@ __device__ __forceinline__ Span decode_span(const DecodeParams& p, int row)
     return s;
 }
 
-template <int QK, int V, int W>
-__global__ __launch_bounds__(64 * W, QK <= 64 ? 4 : 2) void paged_decode_kernel(DecodeParams p)
+// ONE: a kv head per query head, where fifteen of sixteen columns of scores
+// would be spent on no head.  Then S = Q K^T with the positions as columns:
+// product t has block t's positions and the head in row 4 t alone, and the
+// four add up to one result in which lane l holds position l's score, so each
+// is formed and weighted once.  The lanes of a row of 16 then pass their
+// weights (both fp16 parts in a word) to all of them, which is the value
+// product's operand (every column the same head).  16 rows of up to 2048
+// positions, 16 heads of 64: 11.3 us, 12.5 in the general form; the same over
+// two to four heads a kv head was no faster.
+template <int QK, int V, int W, bool ONE>
+__global__ __launch_bounds__(64 * W, QK <= 64 ? 4 : ONE ? 2 : 3) void paged_decode_kernel(DecodeParams p)
 {
     constexpr int KH = (QK + 63) / 64, VT = V / 16;
     extern __shared__ __align__(16) float lds[];  // [W][group][V] sums, then [W][16] M, [W][16] total
@@ -172,8 +181,8 @@ __global__ __launch_bounds__(64 * W, QK <= 64 ? 4 : 2) void paged_decode_kernel(
     float qs = 0.0f;
 #pragma unroll
     for (int k = 0; k < KH; k++) q[k] = i32x4{0, 0, 0, 0};
-    if (h < p.group) {
-        const size_t head = (size_t)row * p.heads + kvh * p.group + h;
+    if (ONE || h < p.group) {
+        const size_t head = (size_t)row * p.heads + kvh * p.group + (ONE ? 0 : h);
 #pragma unroll
         for (int k = 0; k < KH; k++)
             if (64 * k + 16 * g < QK) q[k] = *reinterpret_cast<const i32x4*>(p.q + head * QK + 64 * k + 16 * g);
@@ -193,15 +202,27 @@ __global__ __launch_bounds__(64 * W, QK <= 64 ? 4 : 2) void paged_decode_kernel(
     bool live;
     // (a block's addresses come from its first cell in page 0 where there is none, whose bytes then meet weight 0)
     auto load_keys = [&](int block, int kpage, int vpage) {
-        const int kpos = 64 * block + 16 * (h >> 2);
-        const int8_t* k = c.keys + ((((size_t)max(kpage, 0) * c.kv_heads + kvh) << c.page_shift) +
-                                    (kpos & in_page) + (h & 3)) * QK;
+        if constexpr (ONE) {
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+            for (int t = 0; t < 4; t++) {
+                const int page = max(__builtin_amdgcn_readlane(vpage, 16 * t), 0);  // block t's
+                const int8_t* k = c.keys + ((((size_t)page * c.kv_heads + kvh) << c.page_shift) +
+                                            ((64 * block + 16 * t) & in_page)) * QK;
 #pragma unroll
-            for (int half = 0; half < KH; half++)
-                kr[t][half] =
-                    *reinterpret_cast<const i32x4*>(k + 4 * t * QK + min(64 * half + 16 * g, QK - 16));
+                for (int half = 0; half < KH; half++)
+                    kr[t][half] = *reinterpret_cast<const i32x4*>(k + (h * QK + min(64 * half + 16 * g, QK - 16)));
+            }
+        } else {
+            const int kpos = 64 * block + 16 * (h >> 2);
+            const int8_t* k = c.keys + ((((size_t)max(kpage, 0) * c.kv_heads + kvh) << c.page_shift) +
+                                        (kpos & in_page) + (h & 3)) * QK;
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int half = 0; half < KH; half++)
+                    kr[t][half] =
+                        *reinterpret_cast<const i32x4*>(k + 4 * t * QK + min(64 * half + 16 * g, QK - 16));
+        }
         const int pos = 64 * block + lane;
         const size_t cell = (((size_t)max(vpage, 0) * c.kv_heads + kvh) << c.page_shift) + (pos & in_page);
         ksr = c.kscale[cell];
@@ -232,13 +253,25 @@ __global__ __launch_bounds__(64 * W, QK <= 64 ? 4 : 2) void paged_decode_kernel(
         vpage = page_at(64 * (block + W) + 16 * g);
     }
     for (; block < end_block; block += W) {
-        i32x4 dots[4];
+        i32x4 dots[ONE ? 1 : 4];
+        if constexpr (ONE) {
+            dots[0] = i32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            dots[t] = i32x4{0, 0, 0, 0};
+            for (int t = 0; t < 4; t++)
 #pragma unroll
-            for (int half = 0; half < KH; half++)
-                dots[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kr[t][half], q[half], dots[t], 0, 0, 0);
+                for (int half = 0; half < KH; half++) {
+                    const i32x4 none = {0, 0, 0, 0};
+                    dots[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(h == 4 * t ? q[half] : none, kr[t][half],
+                                                                    dots[0], 0, 0, 0);
+                }
+        } else {
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                dots[t] = i32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int half = 0; half < KH; half++)
+                    dots[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kr[t][half], q[half], dots[t], 0, 0, 0);
+            }
         }
         const Position x = position(ksr, vsr, live);
         const bool more = block + W < end_block;
@@ -248,43 +281,74 @@ __global__ __launch_bounds__(64 * W, QK <= 64 ? 4 : 2) void paged_decode_kernel(
             kpage = page_at(64 * (block + 2 * W) + 16 * (h >> 2));
             vpage = page_at(64 * (block + 2 * W) + 16 * g);
         }
-        float z[16];
+        float w[16];  // the weights of the 16 positions that this lane gives the value product (ONE: as words)
+        if constexpr (ONE) {
+            const float z = ((float)dots[0][0] * x.ks) * qs + x.e;
+            const float up = fmaxf(peak, wave_max(z) - kHeadroom);
+            if (up > peak) {
+                const float keep = __builtin_amdgcn_exp2f(peak - up);
+                peak = up;
+                total *= keep;
+#pragma unroll
+                for (int t = 0; t < VT; t++) o[t] *= keep;
+            }
+            const float e = __builtin_amdgcn_exp2f(z - peak);
+            total = fmaf(e, x.inv, total);
+            const float y = alone(e * x.frac);  // (both conversions below have to see the rounded product)
+            union {
+                f16x2 h2;
+                float word;
+            } both;
+            both.h2 = to_f16(y, fmaf((float)(_Float16)y, minus_one, y));
+#define NHIP_WORD(j) w[j] = row_bcast<j>(both.word);
+            NHIP_WORD(0) NHIP_WORD(1) NHIP_WORD(2) NHIP_WORD(3) NHIP_WORD(4) NHIP_WORD(5) NHIP_WORD(6) NHIP_WORD(7)
+            NHIP_WORD(8) NHIP_WORD(9) NHIP_WORD(10) NHIP_WORD(11) NHIP_WORD(12) NHIP_WORD(13) NHIP_WORD(14)
+            NHIP_WORD(15)
+#undef NHIP_WORD
+        } else {
+            float z[16];
 #define NHIP_SCORE(j) z[j] = ((float)dots[(j) / 4][(j) % 4] * row_bcast<j>(x.ks)) * qs + row_bcast<j>(x.e);
-        NHIP_SCORE(0) NHIP_SCORE(1) NHIP_SCORE(2) NHIP_SCORE(3) NHIP_SCORE(4) NHIP_SCORE(5) NHIP_SCORE(6)
-        NHIP_SCORE(7) NHIP_SCORE(8) NHIP_SCORE(9) NHIP_SCORE(10) NHIP_SCORE(11) NHIP_SCORE(12) NHIP_SCORE(13)
-        NHIP_SCORE(14) NHIP_SCORE(15)
+            NHIP_SCORE(0) NHIP_SCORE(1) NHIP_SCORE(2) NHIP_SCORE(3) NHIP_SCORE(4) NHIP_SCORE(5) NHIP_SCORE(6)
+            NHIP_SCORE(7) NHIP_SCORE(8) NHIP_SCORE(9) NHIP_SCORE(10) NHIP_SCORE(11) NHIP_SCORE(12) NHIP_SCORE(13)
+            NHIP_SCORE(14) NHIP_SCORE(15)
 #undef NHIP_SCORE
-        float up = z[0];
+            float up = z[0];
 #pragma unroll
-        for (int j = 1; j < 16; j++) up = fmaxf(up, z[j]);
-        up = fmaxf(peak, rows_max(up) - kHeadroom);
-        if (__ballot(up > peak)) {
-            const float keep = __builtin_amdgcn_exp2f(peak - up);
-            peak = up;
-            total *= keep;
+            for (int j = 1; j < 16; j++) up = fmaxf(up, z[j]);
+            up = fmaxf(peak, rows_max(up) - kHeadroom);
+            if (__ballot(up > peak)) {
+                const float keep = __builtin_amdgcn_exp2f(peak - up);
+                peak = up;
+                total *= keep;
 #pragma unroll
-            for (int t = 0; t < VT; t++) o[t] *= keep;
-        }
-        float w[16];
+                for (int t = 0; t < VT; t++) o[t] *= keep;
+            }
 #define NHIP_WEIGHT(j)                                  \
     w[j] = __builtin_amdgcn_exp2f(z[j] - peak);         \
     total = fmaf(row_bcast<j>(x.inv), w[j], total);     \
     w[j] = alone(row_bcast<j>(x.frac) * w[j]);
-        NHIP_WEIGHT(0) NHIP_WEIGHT(1) NHIP_WEIGHT(2) NHIP_WEIGHT(3) NHIP_WEIGHT(4) NHIP_WEIGHT(5) NHIP_WEIGHT(6)
-        NHIP_WEIGHT(7) NHIP_WEIGHT(8) NHIP_WEIGHT(9) NHIP_WEIGHT(10) NHIP_WEIGHT(11) NHIP_WEIGHT(12)
-        NHIP_WEIGHT(13) NHIP_WEIGHT(14) NHIP_WEIGHT(15)
+            NHIP_WEIGHT(0) NHIP_WEIGHT(1) NHIP_WEIGHT(2) NHIP_WEIGHT(3) NHIP_WEIGHT(4) NHIP_WEIGHT(5)
+            NHIP_WEIGHT(6) NHIP_WEIGHT(7) NHIP_WEIGHT(8) NHIP_WEIGHT(9) NHIP_WEIGHT(10) NHIP_WEIGHT(11)
+            NHIP_WEIGHT(12) NHIP_WEIGHT(13) NHIP_WEIGHT(14) NHIP_WEIGHT(15)
 #undef NHIP_WEIGHT
+        }
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             union {
                 f16x2 h2[4];
+                uint32_t u[4];
                 f16x8 v;
             } hi, lo;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 const float a = w[8 * u + 2 * k], b = w[8 * u + 2 * k + 1];
-                hi.h2[k] = to_f16(a, b);
-                lo.h2[k] = rest_f16(a, b, hi.h2[k], minus_one);
+                if constexpr (ONE) {
+                    hi.u[k] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x05040100u);
+                    lo.u[k] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+                } else {
+                    hi.h2[k] = to_f16(a, b);
+                    lo.h2[k] = rest_f16(a, b, hi.h2[k], minus_one);
+                }
             }
 #pragma unroll
             for (int t = 0; t < VT; t++) {
@@ -296,6 +360,12 @@ __global__ __launch_bounds__(64 * W, QK <= 64 ? 4 : 2) void paged_decode_kernel(
         if (more) load_values(block + W, vpage_now);
     }
     total = rows_sum(total);
+    if constexpr (ONE) {
+        total += lane_xor<1>(total);
+        total += lane_xor<2>(total);
+        total += lane_xor<4>(total);
+        total += lane_xor<8>(total);
+    }
 
     // the waves' parts joined: every wave scales its sums to the common maximum
     float* peaks = lds + (size_t)W * p.group * V;
@@ -427,10 +497,11 @@ int32_t launch_decode(const DecodeParams& p, const Split& s, int32_t rows, hipSt
 {
     const size_t lds = (size_t)s.waves * (p.group * V + 32) * sizeof(float);
     const dim3 grid(rows, p.c.kv_heads, s.parts);
-    if (s.waves == 4)
-        hipLaunchKernelGGL((paged_decode_kernel<QK, V, 4>), grid, dim3(256), lds, stream, p);
+    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * s.waves), lds, stream, p); };
+    if (p.group == 1)
+        launch(s.waves == 4 ? paged_decode_kernel<QK, V, 4, true> : paged_decode_kernel<QK, V, 8, true>);
     else
-        hipLaunchKernelGGL((paged_decode_kernel<QK, V, 8>), grid, dim3(512), lds, stream, p);
+        launch(s.waves == 4 ? paged_decode_kernel<QK, V, 4, false> : paged_decode_kernel<QK, V, 8, false>);
     NHIP_CHECK_HIP(hipGetLastError());
     if (s.parts > 1) {
         hipLaunchKernelGGL((paged_join_kernel<V>), dim3(rows, p.heads), dim3(256), 0, stream, p);
