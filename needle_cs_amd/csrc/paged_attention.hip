@@ -163,7 +163,7 @@ __device__ __forceinline__ Span decode_span(const DecodeParams& p, int row)
 // positions, 16 heads of 64: 11.3 us, 12.5 in the general form; the same over
 // two to four heads a kv head was no faster.
 template <int QK, int V, int W, bool ONE>
-__global__ __launch_bounds__(64 * W, QK <= 64 ? 4 : ONE ? 2 : 3) void paged_decode_kernel(DecodeParams p)
+__global__ __launch_bounds__(64 * W, QK <= 64 ? 4 : 2) void paged_decode_kernel(DecodeParams p)
 {
     constexpr int KH = (QK + 63) / 64, VT = V / 16;
     extern __shared__ __align__(16) float lds[];  // [W][group][V] sums, then [W][16] M, [W][16] total
