@@ -343,8 +343,9 @@ int32_t nhip_attention_decode_noalloc_dev(const int8_t* d_q, const float* d_q_sc
  * (128, 128); kv_heads <= 256; layers <= 4096; pages <= 2^20; sequences <=
  * 65536; width * page_size <= 2^30; a call takes up to 2^20 rows.
  *
- * Scales are not negative (QuantizeInt8's are positive); a scale that is no
- * finite number spoils the rows that attend its position, and only those.
+ * Scales are not negative (QuantizeInt8's are positive).  A scale that is no
+ * finite number spoils the rows that attend its position, and only those; so
+ * may a value scale of more than 2^60, and outputs under 2^-60 lose digits.
  *
  * The calls below take this struct by pointer (read during the call), are
  * asynchronous on `stream` and may be captured in a graph; calls that write
@@ -401,7 +402,10 @@ int32_t nhip_paged_decode_dev(const nhip_paged_cache* c, int32_t layer, const in
  * ... of sequence run_seq[i].  Their keys and values are in the cache already
  * (nhip_paged_append_dev), as are those of the positions before them.  The row
  * at position p attends [0, p], or with window > 0 [max(0, p-window+1), p].
- * Everything else as nhip_paged_decode_dev; max_count bounds every position
+ * Everything else as nhip_paged_decode_dev; but a
+ * position's weight times its value scale is kept to 2^-30 of the row's largest
+ * weight times the largest value scale that it attends, so where a row's value
+ * scales lie more than 2^14 apart the small ones lose digits.  max_count bounds every position
  * + 1 (rows beyond give zeros), and rows behind the last run are left as they
  * are. */
 size_t nhip_paged_prompt_workspace(const nhip_paged_cache* c, int32_t rows, int32_t heads, int32_t runs,

@@ -42,13 +42,14 @@ __device__ __forceinline__ float row_bcast(float v)
 // 2^-24, which is 2^-39 of the largest weight.  The sum of the softmax takes
 // w 2^-e.  A position that does not count has e = -inf, which makes w 0.
 constexpr float kHeadroom = 14.0f;
+constexpr float kMaxExponent = 60.0f;  // of a value scale, either way
 struct Position {
     float ks, e, frac, inv;
 };
 __device__ __forceinline__ Position position(float ks, float vs, bool live)
 {
     int e = (int)((__float_as_uint(vs) >> 23) & 255) - 127;
-    e = min(max(e, -60), 60);
+    e = min(max(e, -(int)kMaxExponent), (int)kMaxExponent);
     Position r;
     r.inv = live ? __uint_as_float((uint32_t)(127 - e) << 23) : 0.0f;
     r.frac = live ? vs * r.inv : 0.0f;
@@ -651,7 +652,7 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
         if (32 * k + 16 * g < QK) q[k] = *reinterpret_cast<const i32x4*>(p.q + q_at * QK + 32 * k + 16 * g);
     }
     float qs = p.q_scales[q_at] * p.scale;
-    qs = qs == 0.0f ? 1e-30f : qs;  // (a score is then 0, and a position left out still -inf)
+    qs = qs == 0.0f ? 1.2e-38f : qs;  // (a score is then 0, and a position left out still -inf)
 
     // the wave's and the workgroup's positions (the last query's row is the furthest)
     auto pos_of = [&](int at) {
@@ -739,8 +740,10 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
     for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
-    float peak = kNoScore, total = 0.0f;
-    int exponent = -100;  // of the value scales, the largest so far
+    // peak: the reference of the scores; exponent: that of the largest value
+    // scale the query has attended; base = peak + exponent; lowest: the least
+    // exponent of the wave's queries
+    float peak = kNoScore, exponent = -kMaxExponent, base = kNoScore, lowest = -kMaxExponent, total = 0.0f;
     const float minus_one = alone(-1.0f);
     // where this lane reads: the key row of its A row, the value rows of its dimensions
     const int m = lane & 31;
@@ -793,48 +796,57 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
 #undef NHIP_DOT
                 }
                 const bool whole = __builtin_amdgcn_readfirstlane(counted.x & counted.y) == ~0u;
-                if (!whole | (64 * tile + 63 > wave_first) | (64 * tile < wave_last - from_window)) {
+                // the largest value scale, of the lane's two positions or, in a tile
+                // that not every query attends whole, of those that the query attends
+                float largest = fmaxf(vs[0], vs[1]), against = lowest;
+                const bool masked = !whole | (64 * tile + 63 > wave_first) | (64 * tile < wave_last - from_window);
+                if (masked) {
                     const int last = q_pos - 64 * tile - 8 * g, first = q_first - 64 * tile - 8 * g;
+                    largest = 0.0f;
+                    against = exponent;
 #pragma unroll
                     for (int t = 0; t < 2; t++) {
                         const uint32_t bits = (t ? counted.y : counted.x) >> (8 * g);
-#pragma unroll
-                        for (int r = 0; r < 16; r++) {
+                        auto mask = [&](int r, float scale) NHIP_INLINE {
                             const int at = 16 * (r / 8) + r % 8;
-                            z[t][r] = (32 * t + at <= last) & (32 * t + at >= first) & ((bits >> at) & 1) ? z[t][r]
-                                                                                                          : -INFINITY;
-                        }
+                            const bool attends =
+                                (32 * t + at <= last) & (32 * t + at >= first) & ((bits >> at) & 1);
+                            z[t][r] = attends ? z[t][r] : -INFINITY;
+                            largest = fmaxf(largest, attends ? scale : 0.0f);
+                        };
+#define NHIP_MASK(r) mask(r, row_bcast<r>(vs[t]));
+                        NHIP_MASK(0) NHIP_MASK(1) NHIP_MASK(2) NHIP_MASK(3) NHIP_MASK(4) NHIP_MASK(5) NHIP_MASK(6)
+                        NHIP_MASK(7) NHIP_MASK(8) NHIP_MASK(9) NHIP_MASK(10) NHIP_MASK(11) NHIP_MASK(12)
+                        NHIP_MASK(13) NHIP_MASK(14) NHIP_MASK(15)
+#undef NHIP_MASK
                     }
+                    largest = fmaxf(largest, lane_xor<32>(largest));
                 }
                 float up = z[0][0];
 #pragma unroll
                 for (int r = 1; r < 32; r++) up = fmaxf(up, z[r / 16][r % 16]);
                 up = fmaxf(up, lane_xor<32>(up)) * qs;
-                // the exponent of the value scales follows their largest
-                const int ev = (int)(__float_as_uint(fmaxf(fabsf(vs[0]), fabsf(vs[1]))) >> 23) - 127;
-                if (__ballot((up - peak > kHeadroom) | (ev > exponent))) {
-                    const float to = up - peak > kHeadroom ? up - (kHeadroom - kLag) : peak;
-                    float keep = __builtin_amdgcn_exp2f(peak - to);
-                    peak = to;
+                float ev = fminf((float)((int)(__float_as_uint(largest) >> 23) - 127), kMaxExponent);
+                if (__ballot((up - peak > kHeadroom) | (ev > against))) {
+                    if (!masked)
+                        for (int off = 32; off; off >>= 1) ev = fmaxf(ev, __shfl_xor(ev, off));
+                    peak = up - peak > kHeadroom ? up - (kHeadroom - kLag) : peak;
+                    exponent = fmaxf(exponent, ev);
+                    lowest = -wave_max(-exponent);
+                    const float to = peak + exponent, keep = __builtin_amdgcn_exp2f(base - to);
+                    base = to;
                     total *= keep;
-                    int e = ev;
-                    for (int off = 32; off; off >>= 1) e = max(e, __shfl_xor(e, off));
-                    e = max(__builtin_amdgcn_readfirstlane(min(e, 100)), exponent);
-                    keep *= __uint_as_float((uint32_t)max(127 + exponent - e, 0) << 23);
-                    exponent = e;
 #pragma unroll
                     for (int d = 0; d < DT; d++) o[d] *= keep;
                 }
-                const float unit = __uint_as_float((uint32_t)(127 - exponent) << 23);
-                const float vn[2] = {vs[0] * unit, vs[1] * unit};
                 float sum[2] = {0.0f, 0.0f};  // of the tile: a long row's total is a sum of tiles' sums
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
                     float w[16];
 #define NHIP_WEIGHT(r)                                       \
-    w[r] = __builtin_amdgcn_exp2f(fmaf(z[t][r], qs, -peak)); \
+    w[r] = __builtin_amdgcn_exp2f(fmaf(z[t][r], qs, -base)); \
     sum[r & 1] += w[r];                                      \
-    w[r] = alone(row_bcast<r>(vn[t]) * w[r]);
+    w[r] = alone(row_bcast<r>(vs[t]) * w[r]);
                     NHIP_WEIGHT(0) NHIP_WEIGHT(1) NHIP_WEIGHT(2) NHIP_WEIGHT(3) NHIP_WEIGHT(4) NHIP_WEIGHT(5)
                     NHIP_WEIGHT(6) NHIP_WEIGHT(7) NHIP_WEIGHT(8) NHIP_WEIGHT(9) NHIP_WEIGHT(10) NHIP_WEIGHT(11)
                     NHIP_WEIGHT(12) NHIP_WEIGHT(13) NHIP_WEIGHT(14) NHIP_WEIGHT(15)
@@ -872,24 +884,23 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
     if (!mine) return;
     if (q_pos < 0) {  // a row out of range, in a tile of others
         all = 0.0f;
-        peak = kNoScore;
+        base = kNoScore;
 #pragma unroll
         for (int d = 0; d < DT; d++)
 #pragma unroll
             for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
     }
-    const float unit = __uint_as_float((uint32_t)(127 + exponent) << 23);
     float factor;
     float* to;
     if (p.max_parts > 1 && part == 0 && g == 0) p.counts[q_at] = parts;
     if (parts <= 1) {
-        factor = all != 0.0f ? unit / all : 0.0f;
+        factor = all != 0.0f ? 1.0f / all : 0.0f;
         to = p.out + q_at * V;
     } else {
         const size_t at = q_at * p.max_parts + part;
-        factor = unit;
+        factor = 1.0f;
         to = p.parts + at * V;
-        if (g == 0) *reinterpret_cast<float2*>(p.stats + 2 * at) = make_float2(peak, all);
+        if (g == 0) *reinterpret_cast<float2*>(p.stats + 2 * at) = make_float2(base, all);
     }
 #pragma unroll
     for (int d = 0; d < DT; d++)

@@ -63,7 +63,7 @@ class Pool:
             w /= w.sum()
             out[h] = (w * vs) @ v
             far[h] = bound(len(cells), np.abs(z).max(), vs) * ((w * np.abs(vs)) @ np.abs(v))
-            largest = np.nanmax(self.value_scales) * PROMPT_LAG if prompt else (w * np.abs(vs)).max()
+            largest = vs.max() * PROMPT_LAG if prompt else (w * np.abs(vs)).max()
             far[h] += FLOOR * 2 * largest * np.abs(v).sum(0)
         return out, far
 
@@ -75,7 +75,7 @@ class Pool:
 FLOOR = 2.0 ** -39
 
 #: A prompt's weights are scaled by the running maximum that is up to 2^8 behind
-#: and by the largest value scale of the kv head so far, not by the product.
+#: and by the largest value scale that the row attends, not by the product.
 PROMPT_LAG = 2.0 ** 8
 
 

@@ -329,6 +329,44 @@ def test_prompt_spoilt_positions(hip):
         assert np.all(np.abs(got[r] - want) <= far) and np.all(np.abs(count[r] - want) <= far)
 
 
+@pytest.mark.parametrize("kv,group", [(2, 1), (1, 6)])
+@pytest.mark.parametrize("window", [0, 1, 40, 130])
+def test_large_scales_reach_only_the_rows_that_attend_them(hip, window, kv, group):
+    """Value scales 2^40 to 2^58 times the others: a row before such a position,
+    or whose window has left it, is as exact as without it."""
+    rng = np.random.default_rng(29)
+    pool = Pool(rng, 1, 40, 16, kv, 64, 64, 1, 20)
+    pool.give(rng, [310])
+    for pos, e in ((40, 46), (63, 40), (64, 50), (170, 58), (309, 58)):
+        pool.value_scales[0, pool.tables[0, pos // 16], :, pos % 16] = 2.0 ** e
+    gpu = Gpu(hip, pool)
+    q, qs = queries(rng, 310, kv * group, 64)
+    got = gpu.prompt(0, q, qs, [0, 310], [0], [0], window, 310)
+    first = [max(0, p - window + 1) if window else 0 for p in range(310)]
+    count = [p + 1 - f for p, f in enumerate(first)]
+    single = gpu.decode(0, q, qs, [0] * 310, first, count, 310)
+    for p in range(310):
+        want, far = pool.attend(0, 0, q[p], qs[p], first[p], count[p], True)
+        assert np.all(np.abs(got[p] - want) <= far), p
+        want, far = pool.attend(0, 0, q[p], qs[p], first[p], count[p])
+        assert np.all(np.abs(single[p] - want) <= far), p
+
+
+@pytest.mark.parametrize("e", [-58, 58])
+def test_scales_far_from_one(hip, e):
+    """All value scales times 2^e, rows whole and in parts."""
+    rng = np.random.default_rng(31)
+    pool = Pool(rng, 1, 80, 16, 2, 64, 64, 1, 80)
+    pool.give(rng, [1250])
+    pool.value_scales *= np.float32(2.0 ** e)
+    gpu = Gpu(hip, pool)
+    q, qs = queries(rng, 30, 4, 64)
+    check_prompt(gpu, 0, q, qs, [(30, 0, 1220)], 0, 1250)
+    check_prompt(gpu, 0, q, qs, [(30, 0, 100)], 0, 130)
+    check_decode(gpu, 0, q, qs, [(0, 0, 1250 - r) for r in range(30)], 1250)
+    check_decode(gpu, 0, q, qs, [(0, r, 300) for r in range(30)], 300)
+
+
 def test_prompt_rows_out_of_range_and_behind(hip):
     """Runs of unknown sequences, before position 0 or past the table give
     zeros where a row is out of range; rows behind the last run stay."""
