@@ -564,33 +564,50 @@ __device__ __forceinline__ RunRows run_rows(const PromptParams& p, int run)
     return r;
 }
 
-// The run of tile `tile` (the runs' tiles in order) and the tile's place in
-// it, by one wave, a lane a run; run -1 past the last.
-__device__ __forceinline__ int find_tile(const PromptParams& p, int tile, int& in_run, int& of_run)
+// The run whose tile has the place `place` in the call, the tile's number in
+// the run and the run's tiles, by one wave; -1 where the place has no tile.
+//
+// Up to 64 runs, a lane each: their tiles follow one another, and places
+// without a tile come last, which keeps the CUs even.  More: run i's tiles
+// have the places from floor(its first query / 128) + i on, as many as it can
+// need however the runs before it end, so that 64 probes a step find the run
+// without a sum over all.  (16 runs of up to 700 rows, 16 kv heads: 37.6 us,
+// 43.9 by the search; runs of 20 rows, 2 kv heads: 200 of them 18.4 us by the
+// search, 19.3 by sums of 64 at a time, 1000 of them 42.4 and 60.3.)
+__device__ __forceinline__ int find_tile(const PromptParams& p, int place, int& in_run, int& of_run)
 {
     const int lane = threadIdx.x & 63;
-    int before = 0;
-    for (int base = 0; base < p.runs; base += 64) {
-        int n = 0;
-        if (base + lane < p.runs) {
-            const RunRows r = run_rows(p, base + lane);
-            n = (int)(((int64_t)(r.row1 - r.row0) * p.group + kTileQueries - 1) / kTileQueries);
-        }
+    auto tiles = [&](int run) {
+        const RunRows r = run_rows(p, run);
+        return ((r.row1 - r.row0) * p.group + kTileQueries - 1) / kTileQueries;
+    };
+    if (p.runs <= 64) {
+        const int n = lane < p.runs ? tiles(lane) : 0;
         int sum = n;
         for (int off = 1; off < 64; off <<= 1) {
             const int up = __shfl_up(sum, off);
             if (lane >= off) sum += up;
         }
-        const uint64_t hit = __ballot(before + sum > tile);
-        if (hit) {
-            const int l = __builtin_ctzll(hit);
-            of_run = __builtin_amdgcn_readlane(n, l);
-            in_run = tile - before - (__builtin_amdgcn_readlane(sum, l) - of_run);
-            return base + l;
-        }
-        before += __builtin_amdgcn_readlane(sum, 63);
+        const uint64_t hit = __ballot(sum > place);
+        if (hit == 0) return -1;
+        const int run = __builtin_ctzll(hit);
+        of_run = __builtin_amdgcn_readlane(n, run);
+        in_run = place - (__builtin_amdgcn_readlane(sum, run) - of_run);
+        return run;
     }
-    return -1;
+    auto first_place = [&](int run) { return run_rows(p, run).row0 * p.group / kTileQueries + run; };
+    int run = 0, n = p.runs;
+    do {
+        const int step = (n + 63) / 64;
+        const uint64_t before = __ballot(lane * step < n && first_place(run + min(lane * step, n - 1)) <= place);
+        if (before == 0) return -1;
+        const int l = 63 - __builtin_clzll(before);
+        run += l * step;
+        n = min(step, n - l * step);
+    } while (n > 1);
+    of_run = tiles(run);
+    in_run = place - first_place(run);
+    return in_run < of_run ? run : -1;
 }
 
 // An int32 of an array that no kernel of the launch writes, by a scalar load.
@@ -989,7 +1006,7 @@ int32_t check_call(const nhip_paged_cache* c, int32_t layer, const int8_t* q, co
     return NHIP_OK;
 }
 
-// How a prompt call is split: tiles of 128 queries (at most), and where those
+// How a prompt call is split: places of tiles of 128 queries, and where those
 // are few, 64-position blocks of a part and parts of the longest row.
 struct PromptSplit {
     int64_t tiles;
@@ -1010,7 +1027,7 @@ PromptSplit prompt_split(const nhip_paged_cache* c, int32_t rows, int32_t heads,
 {
     const int group = heads / c->kv_heads;
     PromptSplit s;
-    s.tiles = (int64_t)rows * group / kTileQueries + std::min(runs, rows);
+    s.tiles = (int64_t)rows * group / kTileQueries + runs;
     const int64_t units = s.tiles * c->kv_heads;
     int most = max_count / 64 + 2;
     s.blocks = most;
