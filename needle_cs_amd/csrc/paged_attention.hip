@@ -543,6 +543,7 @@ struct PromptParams {
     float* stats;
     int32_t* counts;  // [rows][heads]: the parts of a row
     int32_t rows, heads, group, runs, window, max_count, blocks, max_parts;
+    int32_t tiles_a_round;  // of 256 workgroups, where the tiles are sorted; else 0
     float scale;
 };
 
@@ -565,15 +566,24 @@ __device__ __forceinline__ RunRows run_rows(const PromptParams& p, int run)
 }
 
 // The run whose tile has the place `place` in the call, the tile's number in
-// the run and the run's tiles, by one wave; -1 where the place has no tile.
+// the run (the last, which attends most, first) and the run's tiles, by one
+// wave; -1 where the place has no tile.
 //
-// Up to 64 runs, a lane each: their tiles follow one another, and places
-// without a tile come last, which keeps the CUs even.  More: run i's tiles
-// have the places from floor(its first query / 128) + i on, as many as it can
-// need however the runs before it end, so that 64 probes a step find the run
-// without a sum over all.  (16 runs of up to 700 rows, 16 kv heads: 37.6 us,
-// 43.9 by the search; runs of 20 rows, 2 kv heads: 200 of them 18.4 us by the
-// search, 19.3 by sums of 64 at a time, 1000 of them 42.4 and 60.3.)
+// 2 to 64 runs, a lane each: where the workgroups are more than the CUs, the
+// tiles come in the order of their last blocks, most first (a search for the
+// block count that the place's rank falls into), and every other round of 256
+// workgroups the other way round: a CU takes one of each round, and its heavy
+// tile meets a light one (16 runs of up to 700 rows, 16 kv heads: 34.2 us; in
+// the order of the runs 37.8; sorted, but all rounds alike, 37.1.  40 runs of
+// up to 900, more than are resident at once: 87, 105 and 86).  Fewer
+// workgroups keep the runs' order, and one run's tiles are in order already
+// (4000 rows: 103 us as they come, 104 back and forth).
+//
+// Otherwise run i's tiles have the places from floor(its first query / 128) +
+// i on, as many as it can need however the runs before it end, so that 64
+// probes a step find the run without a sum over all (runs of 20 rows, 2 kv
+// heads: 200 of them 18.3 us, 19.2 by sums of 64 at a time; 1000 of them 42.7
+// and 60.3).
 __device__ __forceinline__ int find_tile(const PromptParams& p, int place, int& in_run, int& of_run)
 {
     const int lane = threadIdx.x & 63;
@@ -581,18 +591,49 @@ __device__ __forceinline__ int find_tile(const PromptParams& p, int place, int& 
         const RunRows r = run_rows(p, run);
         return ((r.row1 - r.row0) * p.group + kTileQueries - 1) / kTileQueries;
     };
-    if (p.runs <= 64) {
-        const int n = lane < p.runs ? tiles(lane) : 0;
+    if (p.runs > 1 && p.runs <= 64) {
+        // lane i: run i's queries, tiles and the position of its first row here
+        const int own = min(lane, p.runs - 1);
+        const RunRows r = run_rows(p, own);
+        const int rows = lane < p.runs ? r.row1 - r.row0 : 0, all = (rows * p.group + kTileQueries - 1) / kTileQueries;
+        const int64_t at = (int64_t)p.run_pos[own] + r.row0 - p.run_rows[own];
+        const int pos = (int)min(max(at, (int64_t)0), (int64_t)1 << 30);
+        // this run's tiles that reach position 64 (blocks - 1)
+        auto reach = [&](int blocks) {
+            const int row = min(max(64 * (blocks - 1) - pos, 0), rows);
+            return row >= rows ? 0 : all - row * p.group / kTileQueries;
+        };
+        int rank = place;
+        if (p.tiles_a_round) {
+            const int in_round = place % p.tiles_a_round;
+            if ((place / p.tiles_a_round) & 1) rank = place - in_round + p.tiles_a_round - 1 - in_round;
+        }
+        if (rank >= wave_sum_i32(all)) return -1;
+        const int most = p.tiles_a_round ? p.max_count / 64 + 1 : 1;
+        // `passed` tiles, at most the rank, have `above` blocks or more; more than the rank have `blocks`
+        int blocks = 1, above = most + 1, passed = 0;
+        while (above - blocks > 1) {
+            const int middle = (blocks + above) / 2, n = __builtin_amdgcn_readfirstlane(wave_sum_i32(reach(middle)));
+            if (n > rank) {
+                blocks = middle;
+            } else {
+                above = middle;
+                passed = n;
+            }
+        }
+        const int n = reach(blocks) - (above > most ? 0 : reach(above));
         int sum = n;
         for (int off = 1; off < 64; off <<= 1) {
             const int up = __shfl_up(sum, off);
             if (lane >= off) sum += up;
         }
-        const uint64_t hit = __ballot(sum > place);
+        const uint64_t hit = __ballot(sum > rank - passed);
         if (hit == 0) return -1;
         const int run = __builtin_ctzll(hit);
-        of_run = __builtin_amdgcn_readlane(n, run);
-        in_run = place - (__builtin_amdgcn_readlane(sum, run) - of_run);
+        of_run = __builtin_amdgcn_readlane(all, run);
+        // the run's tiles of so many blocks are the last but those of more
+        const int more = __builtin_amdgcn_readlane(above > most ? 0 : reach(above), run);
+        in_run = more + (rank - passed) - (__builtin_amdgcn_readlane(sum, run) - __builtin_amdgcn_readlane(n, run));
         return run;
     }
     auto first_place = [&](int run) { return run_rows(p, run).row0 * p.group / kTileQueries + run; };
@@ -1010,7 +1051,7 @@ int32_t check_call(const nhip_paged_cache* c, int32_t layer, const int8_t* q, co
 // are few, 64-position blocks of a part and parts of the longest row.
 struct PromptSplit {
     int64_t tiles;
-    int blocks, parts;
+    int blocks, parts, tiles_a_round;
 };
 
 // A block takes 1 to 2.5 us of a workgroup, joining parts about 4 us.  Where
@@ -1039,6 +1080,11 @@ PromptSplit prompt_split(const nhip_paged_cache* c, int32_t rows, int32_t heads,
         most = std::min<int64_t>(most, ((int64_t)window + kTileQueries / group) / 64 + 2);
         s.blocks = std::max(2, (most + s.parts - 1) / s.parts);
         s.parts = (most + s.blocks - 1) / s.blocks;
+    }
+    s.tiles_a_round = 0;
+    if (runs > 1 && runs <= 64 && s.parts == 1 && s.tiles * c->kv_heads > 256) {
+        s.tiles_a_round = std::max(1, 256 / c->kv_heads);
+        s.tiles = (s.tiles + s.tiles_a_round - 1) / s.tiles_a_round * s.tiles_a_round;
     }
     return s;
 }
@@ -1154,6 +1200,7 @@ int32_t nhip_paged_prompt_dev(const nhip_paged_cache* c, int32_t layer, const in
     p.max_count = max_count;
     p.blocks = split.blocks;
     p.max_parts = split.parts;
+    p.tiles_a_round = split.tiles_a_round;
     p.scale = score_scale(c->qk_dim);
     if (c->qk_dim == 48) return launch_prompt<48, 64>(p, split, as_stream(stream));
     if (c->qk_dim == 64) return launch_prompt<64, 64>(p, split, as_stream(stream));

@@ -382,6 +382,17 @@ def test_prompt_many_runs(hip, runs, rows):
     check_prompt(Gpu(hip, pool), 0, q, qs, spec, 0, 300, rows_behind=5)
 
 
+@pytest.mark.parametrize("kv,window", [(48, 0), (100, 0), (48, 20)])
+def test_prompt_tiles_in_order_of_their_length(hip, kv, window):
+    """More workgroups than CUs, of runs of different ends: each tile is taken once."""
+    rng = np.random.default_rng(37)
+    pool = Pool(rng, 1, 60, 16, kv, 48, 64, 4, 16)
+    pool.give(rng, [200, 150, 40, 10])
+    runs = [(3, 2, 37), (0, 1, 0), (133, 0, 40), (9, 1, 120), (1, 3, 9), (4, 9, 0), (20, 1, 0), (2, 0, 198)]
+    q, qs = queries(rng, sum(n for n, _, _ in runs) + 2, kv, 48)
+    check_prompt(Gpu(hip, pool), 0, q, qs, runs, window, 200, rows_behind=2)
+
+
 def test_prompt_rows_out_of_range_and_behind(hip):
     """Runs of unknown sequences, before position 0 or past the table give
     zeros where a row is out of range; rows behind the last run stay."""
