@@ -120,6 +120,14 @@ __device__ __forceinline__ float rows_sum(float v)
 //            the codes are the 16 bytes that the cache holds of one dimension
 //            and 16 positions, one load.
 // Nothing passes through LDS until the waves' parts are joined.
+//
+// A long call is bound by its bytes: 32 rows of up to 32768 positions, 8 kv
+// heads of 128 under 32 heads (1.38 GB) take 277 us, 5.0 TB/s, which is the
+// rate of a large copy.  A short one is a chain of latencies: table entry,
+// keys, two exchanges of four lanes for the maximum, exponentials, values,
+// join; 3 rows of up to 192 positions take 4.5 us, of which 2.5 are the launch.
+// Measured and not kept: two blocks of loads in flight (360 us in the place
+// of 292, for the registers), 16 waves a workgroup (no gain).
 struct DecodeParams {
     PagedLayer c;
     const int8_t* q;
@@ -459,16 +467,19 @@ struct Split {
     int waves, blocks, parts;
 };
 
-// A wave takes about 1.3 us a block beside 4 us for the launch; joining parts
+// A wave takes about 1 us a block beside 4 us for the launch; joining parts
 // costs 3 us.  So rows of few blocks stay whole: up to 18 (4 rows of 1024
-// positions, 16 kv heads: 7.7 us whole, 8.0 in parts; 2 rows of 1556, 4 kv
-// heads of 128: 15.5 whole, 10.9 in parts), or up to 40 where the workgroups
-// fill half the CUs anyway (16 rows of up to 2048, 16 kv heads: 13.4 us
-// whole, 15.7 in parts).  Longer ones are cut into parts of at least 8 blocks
-// such that the longest rows give 2048 workgroups (32 rows of up to 32768 on 8
-// kv heads of 128: 292 us in parts of 65 blocks, 372 in parts of 8), at most
-// kMaxParts.  Four waves a workgroup where one round of them reaches the end
-// or the workgroups are many, else eight (the 16 rows above: 13.4 and 17.1).
+// positions, 16 kv heads: 6.0 us whole, 7.6 in parts; 2 rows of 1556, 4 kv
+// heads of 128: 14.9 whole, 10.6 in parts), or up to 40 where the workgroups
+// fill half the CUs anyway (16 rows of up to 2048, 16 kv heads: 10.9 us whole,
+// 13.4 in parts).  Longer ones are cut into parts of at least 8 blocks such
+// that the longest rows give 2048 workgroups (32 rows of up to 32768 on 8 kv
+// heads of 128: 277 us, 294 with 1024 workgroups; 4 rows of up to 8000: 17.8,
+// 49.9 whole), at most kMaxParts.  Eight waves a workgroup, which a row's
+// blocks are dealt to in turn (the 16 rows above: 10.9 us, 15.1 with four); but
+// four where there are 512 workgroups or more (the 32 rows: 277 and 307), or
+// rows of up to 10 blocks, where it makes no difference (16 rows of 256, 8 kv
+// heads: 4.9 both ways).
 Split decode_split(const nhip_paged_cache* c, int32_t rows, int32_t max_count)
 {
     const int64_t units = (int64_t)rows * c->kv_heads;
@@ -529,8 +540,24 @@ int32_t launch_decode(const DecodeParams& p, const Split& s, int32_t rows, hipSt
 //            multiplication), and a query's maximum and total are its lane's.
 //   values   O^T = V^T P^T by v_mfma_f32_32x32x16_f16: registers 8 u .. 8 u + 7
 //            are the eight weights that product u wants of this lane.
-// The weights are 2^(z - M) with M within 2^8 of the running maximum: the sums
-// are rescaled only when a maximum moves further, a few times a row.
+// The weights are 2^(z - M), M the running maximum less up to 2^8 plus the
+// exponent of the largest value scale that the row has attended, so that a
+// weight times its value scale fits fp16, and its two fp16 parts keep 2^-30 of
+// the largest; the sums are rescaled only when M has to move, a few times a row.
+//
+// Bound by the issue of instructions: a position and query costs about 10
+// vector operations of 4 cycles a wave (conversion, two scalings, maximum,
+// exponential, sum, two conversions and the rest between them) beside its
+// share of the products, and vector and matrix instructions of a SIMD's two
+// waves overlap in part only.  One run of 8192 rows, 32 heads on 8 of 128
+// takes 732 us (719 to 760 from one card to the next), 550 Gflop: 750 TFLOP/s.
+// Its products, the values' made twice for the weights' two parts, would take
+// 633 us at the rates of a large int8 and a large fp16 product (one part: 394,
+// but weights of 11 bits are off by 2^-12 each).  Measured and not kept there: eight waves
+// in two phases (893 us), a tile's scores ahead of the last one's values (776
+// to 857, for the registers), operands read from LDS a phase ahead (788),
+// 16-query waves, four a SIMD (783), set instruction orders (733 to 769), a
+// raised wave priority in the products (767).
 struct PromptParams {
     PagedLayer c;
     const int8_t* q;
@@ -1056,7 +1083,7 @@ struct PromptSplit {
 
 // A block takes 1 to 2.5 us of a workgroup, joining parts about 4 us.  Where
 // the tiles fill the CUs, or have fewer than 6 blocks, they stay whole (16 runs of up to 700 rows, 16 kv
-// heads: 38 us whole, 45 in two parts).  Up to 96 workgroups, or 256 with 32
+// heads: 34 us whole, 45 in two parts).  Up to 96 workgroups, or 256 with 32
 // or more blocks each, are split until about 768 are there, in parts of two
 // blocks or more (16 rows after 32,000 positions, 8 kv heads of 128: 798 us
 // whole, 37 in 63 parts; 512 rows after 8,000, 16 kv heads: 182 and 50; 416
