@@ -5,6 +5,7 @@
 // e^(z_s - m), in one pass with a running maximum m and fp32 sums.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "paged.hpp"
 
@@ -139,6 +140,7 @@ struct DecodeParams {
     float* parts;  // [rows][heads][max_parts][V]: a part's sums
     float* stats;  // [rows][heads][max_parts][2]: its maximum and total
     int32_t heads, group, max_count, blocks, max_parts;  // blocks: 64-position blocks of a part
+    int32_t rows, rows_a_round;  // rows_a_round: of 256 workgroups, where the rows are sorted; else 0
     float scale;
 };
 
@@ -162,6 +164,36 @@ __device__ __forceinline__ Span decode_span(const DecodeParams& p, int row)
     return s;
 }
 
+// The row of rank `place` by blocks, most first, every other round of 256
+// workgroups the other way round, and its span; -1 past the last.  By one
+// wave, a lane a row.
+__device__ __forceinline__ int ordered_row(const DecodeParams& p, int place, Span& s)
+{
+    const int lane = threadIdx.x & 63, in_round = place % p.rows_a_round;
+    const int rank = (place / p.rows_a_round) & 1 ? place - in_round + p.rows_a_round - 1 - in_round : place;
+    if (rank >= p.rows) return -1;
+    const Span own = decode_span(p, min(lane, p.rows - 1));
+    const int blocks = lane < p.rows ? own.block1 - own.block0 : -1;
+    int least = 0, above = p.blocks + 1;  // at most `rank` rows have `above` blocks or more, more than that have `least`
+    while (above - least > 1) {
+        const int middle = (least + above) / 2;
+        if (__popcll(__ballot(blocks >= middle)) > rank)
+            least = middle;
+        else
+            above = middle;
+    }
+    const uint64_t equal = __ballot(blocks == least);
+    const int before = rank - __popcll(__ballot(blocks > least));
+    const uint64_t hit = __ballot(blocks == least && __popcll(equal & (((uint64_t)1 << lane) - 1)) == before);
+    const int row = __builtin_ctzll(hit);
+    s.seq = __builtin_amdgcn_readlane(own.seq, row);
+    s.first = __builtin_amdgcn_readlane(own.first, row);
+    s.end = __builtin_amdgcn_readlane(own.end, row);
+    s.block0 = __builtin_amdgcn_readlane(own.block0, row);
+    s.block1 = __builtin_amdgcn_readlane(own.block1, row);
+    return row;
+}
+
 // ONE: a kv head per query head, where fifteen of sixteen columns of scores
 // would be spent on no head.  Then S = Q K^T with the positions as columns:
 // product t has block t's positions and the head in row 4 t alone, and the
@@ -171,16 +203,32 @@ __device__ __forceinline__ Span decode_span(const DecodeParams& p, int row)
 // product's operand (every column the same head).  16 rows of up to 2048
 // positions, 16 heads of 64: 11.3 us, 12.5 in the general form; the same over
 // two to four heads a kv head was no faster.
-template <int QK, int V, int W, bool ONE>
+//
+// SORTED: calls of up to 64 whole rows and more workgroups than CUs deal the
+// rows to the CUs by their length (ordered_row), so that the longest do not
+// meet: 64 rows of up to 2048 positions, 8 kv heads: 18.7 us, 20.9 in the
+// order of the call; 16 kv heads 27.5 and 33.0; 48 rows, 8 heads of 128 25.9
+// and 33.3; but rows of 1040 each 16.5 and 15.9.  (Its own variant: the
+// registers of the choice cost the others up to 0.5 us.)
+template <int QK, int V, int W, bool ONE, bool SORTED>
 __global__ __launch_bounds__(64 * W, QK <= 64 ? 4 : 2) void paged_decode_kernel(DecodeParams p)
 {
     constexpr int KH = (QK + 63) / 64, VT = V / 16;
     extern __shared__ __align__(16) float lds[];  // [W][group][V] sums, then [W][16] M, [W][16] total
     const PagedLayer& c = p.c;
-    const int row = blockIdx.x, kvh = blockIdx.y, part = blockIdx.z;
+    int row = blockIdx.x, kvh = blockIdx.y, part = blockIdx.z;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = lane & 15, g = lane >> 4;
-    const Span s = decode_span(p, row);
+    Span s;
+    if constexpr (SORTED) {
+        const int place = blockIdx.x / c.kv_heads;
+        kvh = blockIdx.x - place * c.kv_heads;
+        part = 0;
+        row = ordered_row(p, place, s);
+        if (row < 0) return;
+    } else {
+        s = decode_span(p, row);
+    }
     const int total_blocks = s.block1 - s.block0;
     const int parts = (total_blocks + p.blocks - 1) / p.blocks;
     if (part > 0 && part >= parts) return;
@@ -464,7 +512,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(DecodeParams p)
 // How a decode call is split: waves of a workgroup, 64-position blocks of a
 // part, parts of the longest row.
 struct Split {
-    int waves, blocks, parts;
+    int waves, blocks, parts, rows_a_round;
 };
 
 // A wave takes about 1 us a block beside 4 us for the launch; joining parts
@@ -493,6 +541,7 @@ Split decode_split(const nhip_paged_cache* c, int32_t rows, int32_t max_count)
     }
     s.parts = (most + s.blocks - 1) / s.blocks;
     s.waves = most <= 10 || units * s.parts >= 512 ? 4 : 8;
+    s.rows_a_round = s.parts == 1 && rows <= 64 && units > 256 ? std::max(1, 256 / c->kv_heads) : 0;
     return s;
 }
 
@@ -508,12 +557,19 @@ template <int QK, int V>
 int32_t launch_decode(const DecodeParams& p, const Split& s, int32_t rows, hipStream_t stream)
 {
     const size_t lds = (size_t)s.waves * (p.group * V + 32) * sizeof(float);
-    const dim3 grid(rows, p.c.kv_heads, s.parts);
+    const int rounds = s.rows_a_round ? (rows + s.rows_a_round - 1) / s.rows_a_round : 0;
+    const dim3 grid = rounds ? dim3(rounds * s.rows_a_round * p.c.kv_heads) : dim3(rows, p.c.kv_heads, s.parts);
     auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * s.waves), lds, stream, p); };
+    auto choose = [&](auto one, auto sorted) {
+        launch(s.waves == 4 ? paged_decode_kernel<QK, V, 4, one(), sorted()>
+                            : paged_decode_kernel<QK, V, 8, one(), sorted()>);
+    };
+    const std::true_type yes;
+    const std::false_type no;
     if (p.group == 1)
-        launch(s.waves == 4 ? paged_decode_kernel<QK, V, 4, true> : paged_decode_kernel<QK, V, 8, true>);
+        rounds ? choose(yes, yes) : choose(yes, no);
     else
-        launch(s.waves == 4 ? paged_decode_kernel<QK, V, 4, false> : paged_decode_kernel<QK, V, 8, false>);
+        rounds ? choose(no, yes) : choose(no, no);
     NHIP_CHECK_HIP(hipGetLastError());
     if (s.parts > 1) {
         hipLaunchKernelGGL((paged_join_kernel<V>), dim3(rows, p.heads), dim3(256), 0, stream, p);
@@ -1176,6 +1232,8 @@ int32_t nhip_paged_decode_dev(const nhip_paged_cache* c, int32_t layer, const in
     p.max_count = max_count;
     p.blocks = split.blocks;
     p.max_parts = split.parts;
+    p.rows = rows;
+    p.rows_a_round = split.rows_a_round;
     p.scale = score_scale(c->qk_dim);
     if (c->qk_dim == 48) return launch_decode<48, 64>(p, split, rows, as_stream(stream));
     if (c->qk_dim == 64) return launch_decode<64, 64>(p, split, rows, as_stream(stream));

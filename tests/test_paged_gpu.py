@@ -139,6 +139,23 @@ def test_decode_many_rows(hip):
     check_decode(Gpu(hip, pool), 0, q, qs, spec, 90)
 
 
+@pytest.mark.parametrize("kv,group,rows", [(48, 1, 11), (100, 1, 64), (8, 2, 64), (8, 1, 63), (256, 1, 2)])
+def test_decode_rows_in_order_of_their_length(hip, kv, group, rows):
+    """More workgroups than CUs, rows of many lengths, equal ones and none."""
+    rng = np.random.default_rng(39)
+    pool = Pool(rng, 1, 80, 16, kv, 48, 64, 4, 20)
+    pool.give(rng, [300, 150, 64, 10])
+    q, qs = queries(rng, rows, kv * group, 48)
+    spec = []
+    for _ in range(rows):
+        s = int(rng.integers(0, 4))
+        n = int(rng.integers(0, pool.lengths[s] + 1) // (1 + 3 * rng.integers(0, 2)))
+        spec.append((s, int(rng.integers(0, pool.lengths[s] - n + 1)), n))
+    spec[rows // 2], spec[rows // 3] = (0, 0, 0), (5, 0, 9)
+    spec[-1] = (0, 0, 300)
+    check_decode(Gpu(hip, pool), 0, q, qs, spec, 300)
+
+
 def test_decode_rows_out_of_range_give_zeros(hip):
     rng = np.random.default_rng(7)
     pool = Pool(rng, 1, 40, 16, 2, 64, 64, 3, 8)
