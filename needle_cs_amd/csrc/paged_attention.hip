@@ -559,7 +559,13 @@ int32_t launch_decode(const DecodeParams& p, const Split& s, int32_t rows, hipSt
     const size_t lds = (size_t)s.waves * (p.group * V + 32) * sizeof(float);
     const int rounds = s.rows_a_round ? (rows + s.rows_a_round - 1) / s.rows_a_round : 0;
     const dim3 grid = rounds ? dim3(rounds * s.rows_a_round * p.c.kv_heads) : dim3(rows, p.c.kv_heads, s.parts);
-    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * s.waves), lds, stream, p); };
+    hipError_t set = hipSuccess;
+    auto launch = [&](auto kernel) {
+        if (lds > 65536)  // (eight waves of 16 heads of 128)
+            set = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (set == hipSuccess) hipLaunchKernelGGL(kernel, grid, dim3(64 * s.waves), lds, stream, p);
+    };
     auto choose = [&](auto one, auto sorted) {
         launch(s.waves == 4 ? paged_decode_kernel<QK, V, 4, one(), sorted()>
                             : paged_decode_kernel<QK, V, 8, one(), sorted()>);
@@ -570,6 +576,7 @@ int32_t launch_decode(const DecodeParams& p, const Split& s, int32_t rows, hipSt
         rounds ? choose(yes, yes) : choose(yes, no);
     else
         rounds ? choose(no, yes) : choose(no, no);
+    NHIP_CHECK_HIP(set);
     NHIP_CHECK_HIP(hipGetLastError());
     if (s.parts > 1) {
         hipLaunchKernelGGL((paged_join_kernel<V>), dim3(rows, p.heads), dim3(256), 0, stream, p);

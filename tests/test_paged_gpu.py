@@ -129,6 +129,16 @@ def test_decode_long_and_split(hip):
     assert np.allclose(a, b, rtol=1e-4, atol=1e-4)
 
 
+@pytest.mark.parametrize("rows,kv,lo,hi", [(2, 1, 1000, 1300), (1, 2, 700, 900), (9, 64, 700, 730)])
+def test_decode_sixteen_heads_of_128(hip, rows, kv, lo, hi):
+    """The largest joins: eight waves and four, of 16 heads of 128."""
+    rng = np.random.default_rng(8)
+    pool = Pool(rng, 1, 50, 64, kv, 128, 128, 2, 21)
+    pool.give(rng, [hi, lo])
+    q, qs = queries(rng, rows, 16 * kv, 128)
+    check_decode(Gpu(hip, pool), 0, q, qs, [(i % 2, 3 * i, lo - 3 * i) for i in range(rows)], hi)
+
+
 def test_decode_many_rows(hip):
     rng = np.random.default_rng(6)
     lengths = rng.integers(1, 90, 300)
