@@ -68,8 +68,9 @@ struct AppendParams {
 // cache holds 16 positions of a dimension together, and where the rows are
 // consecutive positions of one sequence (a prompt) a lane writes as many of
 // them at once as lie in a block; else each goes by itself.  Bound by the
-// bytes: 8185 rows of 8 kv heads of 128 (84 MB) take 21.0 us, 4.0 TB/s (24.5
-// with 64 rows a workgroup: fewer are in flight); one step's 16 rows 4.4 us,
+// bytes: 8185 rows of 8 kv heads of 128 (84 MB) take 19.6 us, 4.3 TB/s (20.8
+// with the groups dealt to the XCDs one by one: 26 MB were written for 17; and
+// then 24.5 with 64 rows a workgroup: fewer are in flight); one step's 16 rows 4.4 us,
 // which is the launch.
 constexpr int kAppendRows = 16;
 typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
@@ -94,7 +95,11 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p)
     __shared__ __align__(16) uint8_t turned[V][N + 36];
     __shared__ bool consecutive;
     const PagedLayer& c = p.c;
-    const int kvh = blockIdx.y, row0 = (int)blockIdx.x * N, n = min(N, p.rows - row0);
+    // an XCD takes neighbouring groups of rows, so that the pieces of a block that two workgroups write meet in its L2
+    const uint32_t id = blockIdx.y * gridDim.x + blockIdx.x, group = (id & 7) * (gridDim.x * gridDim.y / 8) + id / 8;
+    const uint32_t groups = (p.rows + N - 1) / N;
+    if (group >= groups * c.kv_heads) return;
+    const int kvh = group / groups, row0 = (int)(group - kvh * groups) * N, n = min(N, p.rows - row0);
     const int l = threadIdx.x & (L - 1), row_of_pass = threadIdx.x / L;
     f4 x[PASSES][2];
 #pragma unroll
@@ -187,8 +192,9 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p)
 template <int QK, int V>
 void launch_append(const AppendParams& p, hipStream_t stream)
 {
-    hipLaunchKernelGGL((paged_append_kernel<QK, V>), dim3((unsigned)(p.rows + kAppendRows - 1) / kAppendRows, p.c.kv_heads),
-                       dim3(256), 0, stream, p);
+    const unsigned groups = (unsigned)(p.rows + kAppendRows - 1) / kAppendRows * p.c.kv_heads;
+    const unsigned x = std::min((groups + 7) / 8 * 8, 1u << 20);  // (a multiple of 8)
+    hipLaunchKernelGGL((paged_append_kernel<QK, V>), dim3(x, (groups + x - 1) / x), dim3(256), 0, stream, p);
 }
 
 // ----------------------------------------------------------------- pages --

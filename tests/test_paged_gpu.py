@@ -510,6 +510,28 @@ def test_append(hip, orc, qk, v, page, kv):
         assert np.array_equal(gpu.get(name), getattr(pool, name), equal_nan=name.endswith("scales")), name
 
 
+def test_append_of_over_a_million_workgroups(hip, orc):
+    """70,000 rows of 256 kv heads, four of which go somewhere."""
+    rng = np.random.default_rng(43)
+    rows, kv, at = 70000, 256, [0, 17, 40000, 69999]
+    pool = Pool(rng, 1, 6, 16, kv, 48, 64, 1, 6)
+    pool.give(rng, [90])
+    k = rng.standard_normal((4, kv, 48)).astype(np.float32)
+    v = rng.standard_normal((4, kv, 64)).astype(np.float32)
+    bufs = [hip.DeviceBuffer(4 * rows * kv * d) for d in (48, 64)]
+    for b, x in zip(bufs, (k, v)):
+        b.zero()
+        for i, r in enumerate(at):
+            b.upload(x[i], offset=r * x[i].nbytes)
+    seq, pos = np.full(rows, -1, dtype=np.int32), np.arange(rows, dtype=np.int32)
+    seq[at], pos[at] = 0, [3, 88, 50, 51]
+    gpu = Gpu(hip, pool)
+    gpu.cache.append(0, bufs[0].ptr, kv * 48, bufs[1].ptr, kv * 64, gpu.dev(seq).ptr, gpu.dev(pos).ptr, rows)
+    expected_append(orc, pool, 0, k, v, seq[at], pos[at])
+    for name in Pool.NAMES:
+        assert np.array_equal(gpu.get(name), getattr(pool, name), equal_nan=name.endswith("scales")), name
+
+
 # ----------------------------------------------------------------- pages --
 
 def check_books(gpu, books, pool_before=None):
