@@ -406,7 +406,8 @@ int32_t nhip_paged_decode_dev(const nhip_paged_cache* c, int32_t layer, const in
  * value scale is kept to 2^-30 of the row's largest weight times the largest
  * value scale that the row attends, so where these scales lie more than 2^14
  * apart the small ones lose digits.  max_count bounds every position + 1 (rows
- * beyond give zeros), and rows behind the last run are left as they are. */
+ * beyond give zeros), and rows behind the last run are left as they are.
+ * (rows * heads / kv_heads / 128 + runs) * kv_heads <= 2^23. */
 size_t nhip_paged_prompt_workspace(const nhip_paged_cache* c, int32_t rows, int32_t heads, int32_t runs,
                                    int32_t max_count);
 int32_t nhip_paged_prompt_dev(const nhip_paged_cache* c, int32_t layer, const int8_t* d_q, const float* d_q_scales,

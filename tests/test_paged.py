@@ -102,6 +102,13 @@ def test_prompt_refuses_its_own():
             cache().prompt(0, A, A, 3, 12, runs, A, A, A, window, 96, A, BIG, A)
 
 
+def test_prompt_refuses_more_tiles_than_a_grid_holds():
+    with refused("too many"):
+        cache(kv_heads=16).prompt(0, A, A, 3, 16, 1 << 20, A, A, A, 0, 96, A, BIG, A)
+    with refused("too many"):
+        cache(kv_heads=256).prompt(0, A, A, 1 << 20, 4096, 1, A, A, A, 0, 96, A, BIG, A)
+
+
 def test_workspace_sizes_need_no_device():
     """They are the same before and after a device is chosen, and a window never needs more."""
     c = cache(pages=4096, width=4096)
