@@ -659,73 +659,103 @@ __device__ __forceinline__ RunRows run_rows(const PromptParams& p, int run)
 // the run (the last, which attends most, first) and the run's tiles, by one
 // wave; -1 where the place has no tile.
 //
-// 2 to 64 runs, a lane each: where the workgroups are more than the CUs, the
-// tiles come in the order of their last blocks, most first (a search for the
-// block count that the place's rank falls into), and every other round of 256
-// workgroups the other way round: a CU takes one of each round, and its heavy
-// tile meets a light one (16 runs of up to 700 rows, 16 kv heads: 34.2 us; in
-// the order of the runs 37.8; sorted, but all rounds alike, 37.1.  40 runs of
-// up to 900, more than are resident at once: 87, 105 and 86).  Fewer
-// workgroups keep the runs' order, and one run's tiles are in order already
-// (4000 rows: 103 us as they come, 104 back and forth).
-//
-// Otherwise run i's tiles have the places from floor(its first query / 128) +
-// i on, as many as it can need however the runs before it end, so that 64
-// probes a step find the run without a sum over all (runs of 20 rows, 2 kv
-// heads: 200 of them 18.3 us, 19.2 by sums of 64 at a time; 1000 of them 42.7
-// and 60.3).
-__device__ __forceinline__ int find_tile(const PromptParams& p, int place, int& in_run, int& of_run)
+// In the order of length: R runs a lane.  Where the workgroups are more than
+// the CUs, the tiles come in the order of their last blocks, most first (a
+// search for the block count that the place's rank falls into), and every
+// other round of 256 workgroups the other way round: a CU takes one of each
+// round, and its heavy tile meets a light one (16 runs of up to 700 rows, 16 kv
+// heads: 34.2 us; in the order of the runs 37.8; sorted, but all rounds alike,
+// 37.1.  40 runs of up to 900, more than are resident at once: 87, 105 and
+// 86).  Fewer workgroups keep the runs' order, and so do more than 6144, which
+// even out by themselves and gain by a run's tiles side by side (32 heads on 8,
+// runs of up to 500: 80 of them, 5640 workgroups, 155 us sorted and 158 in the
+// runs' order; 120, 8460 workgroups, 244 and 240).
+constexpr int kSortedGroups = 6144;
+template <int R>
+__device__ __forceinline__ int find_tile_by_length(const PromptParams& p, int place, int& in_run, int& of_run)
 {
     const int lane = threadIdx.x & 63;
-    auto tiles = [&](int run) {
+    int rows[R], all[R], pos[R];  // a run's rows, tiles, and the position of its first row here
+    int mine = 0;
+#pragma unroll
+    for (int k = 0; k < R; k++) {
+        const int run = min(R * lane + k, p.runs - 1);
         const RunRows r = run_rows(p, run);
-        return ((r.row1 - r.row0) * p.group + kTileQueries - 1) / kTileQueries;
-    };
-    if (p.runs > 1 && p.runs <= 64) {
-        // lane i: run i's queries, tiles and the position of its first row here
-        const int own = min(lane, p.runs - 1);
-        const RunRows r = run_rows(p, own);
-        const int rows = lane < p.runs ? r.row1 - r.row0 : 0, all = (rows * p.group + kTileQueries - 1) / kTileQueries;
-        const int64_t at = (int64_t)p.run_pos[own] + r.row0 - p.run_rows[own];
-        const int pos = (int)min(max(at, (int64_t)0), (int64_t)1 << 30);
-        // this run's tiles that reach position 64 (blocks - 1)
-        auto reach = [&](int blocks) {
-            const int row = min(max(64 * (blocks - 1) - pos, 0), rows);
-            return row >= rows ? 0 : all - row * p.group / kTileQueries;
-        };
-        int rank = place;
-        if (p.tiles_a_round) {
-            const int in_round = place % p.tiles_a_round;
-            if ((place / p.tiles_a_round) & 1) rank = place - in_round + p.tiles_a_round - 1 - in_round;
-        }
-        if (rank >= wave_sum_i32(all)) return -1;
-        const int most = p.tiles_a_round ? p.max_count / 64 + 1 : 1;
-        // `passed` tiles, at most the rank, have `above` blocks or more; more than the rank have `blocks`
-        int blocks = 1, above = most + 1, passed = 0;
-        while (above - blocks > 1) {
-            const int middle = (blocks + above) / 2, n = __builtin_amdgcn_readfirstlane(wave_sum_i32(reach(middle)));
-            if (n > rank) {
-                blocks = middle;
-            } else {
-                above = middle;
-                passed = n;
-            }
-        }
-        const int n = reach(blocks) - (above > most ? 0 : reach(above));
-        int sum = n;
-        for (int off = 1; off < 64; off <<= 1) {
-            const int up = __shfl_up(sum, off);
-            if (lane >= off) sum += up;
-        }
-        const uint64_t hit = __ballot(sum > rank - passed);
-        if (hit == 0) return -1;
-        const int run = __builtin_ctzll(hit);
-        of_run = __builtin_amdgcn_readlane(all, run);
-        // the run's tiles of so many blocks are the last but those of more
-        const int more = __builtin_amdgcn_readlane(above > most ? 0 : reach(above), run);
-        in_run = more + (rank - passed) - (__builtin_amdgcn_readlane(sum, run) - __builtin_amdgcn_readlane(n, run));
-        return run;
+        rows[k] = R * lane + k < p.runs ? r.row1 - r.row0 : 0;
+        all[k] = (rows[k] * p.group + kTileQueries - 1) / kTileQueries;
+        const int64_t at = (int64_t)p.run_pos[run] + r.row0 - p.run_rows[run];
+        pos[k] = (int)min(max(at, (int64_t)0), (int64_t)1 << 30);
+        mine += all[k];
     }
+    // a run's tiles that reach position 64 (blocks - 1)
+    auto reach = [&](int k, int blocks) {
+        const int row = min(max(64 * (blocks - 1) - pos[k], 0), rows[k]);
+        return row >= rows[k] ? 0 : all[k] - row * p.group / kTileQueries;
+    };
+    int rank = place;
+    if (p.tiles_a_round) {
+        const int in_round = place % p.tiles_a_round;
+        if ((place / p.tiles_a_round) & 1) rank = place - in_round + p.tiles_a_round - 1 - in_round;
+    }
+    if (rank >= __builtin_amdgcn_readfirstlane(wave_sum_i32(mine))) return -1;
+    const int most = p.tiles_a_round ? p.max_count / 64 + 1 : 1;
+    // `passed` tiles, at most the rank, have `above` blocks or more; more than the rank have `blocks`
+    int blocks = 1, above = most + 1, passed = 0;
+    while (above - blocks > 1) {
+        const int middle = (blocks + above) / 2;
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < R; k++) n += reach(k, middle);
+        n = __builtin_amdgcn_readfirstlane(wave_sum_i32(n));
+        if (n > rank) {
+            blocks = middle;
+        } else {
+            above = middle;
+            passed = n;
+        }
+    }
+    int more[R], n[R], sum = 0;  // a run's tiles of more blocks, and of as many
+#pragma unroll
+    for (int k = 0; k < R; k++) {
+        more[k] = above > most ? 0 : reach(k, above);
+        n[k] = reach(k, blocks) - more[k];
+        sum += n[k];
+    }
+    const int own = sum;
+    for (int off = 1; off < 64; off <<= 1) {
+        const int up = __shfl_up(sum, off);
+        if (lane >= off) sum += up;
+    }
+    const uint64_t hit = __ballot(sum > rank - passed);
+    if (hit == 0) return -1;
+    const int l = __builtin_ctzll(hit);
+    int at = rank - passed - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(own, l)), run = -1;
+#pragma unroll
+    for (int k = 0; k < R; k++) {
+        const int here = __builtin_amdgcn_readlane(n[k], l);
+        if (run < 0 && at < here) {
+            run = R * l + k;
+            of_run = __builtin_amdgcn_readlane(all[k], l);
+            in_run = __builtin_amdgcn_readlane(more[k], l) + at;
+        }
+        at -= here;
+    }
+    return run;
+}
+
+// Up to 64 runs go by length, a lane each; up to 256 four a lane (80 of up to
+// 300 rows, 8 kv heads: 34.9 us, 45.0 by the search below).  Otherwise, and for
+// one run, whose tiles are in order already (4000 rows: 103 us as they come,
+// 104 back and forth), run i's tiles have the places from floor(its first
+// query / 128) + i on, as many as it can need however the runs before it end,
+// so that 64 probes a step find the run without a sum over all (runs of 20
+// rows, 2 kv heads: 1000 of them 42.7 us, 60.3 by sums of 64 at a time).
+constexpr int kSortedRuns = 256;
+__device__ __forceinline__ int find_tile(const PromptParams& p, int place, int& in_run, int& of_run)
+{
+    if (p.runs > 1 && p.runs <= 64) return find_tile_by_length<1>(p, place, in_run, of_run);
+    if (p.runs > 1 && p.runs <= kSortedRuns) return find_tile_by_length<kSortedRuns / 64>(p, place, in_run, of_run);
+    const int lane = threadIdx.x & 63;
     auto first_place = [&](int run) { return run_rows(p, run).row0 * p.group / kTileQueries + run; };
     int run = 0, n = p.runs;
     do {
@@ -736,7 +766,8 @@ __device__ __forceinline__ int find_tile(const PromptParams& p, int place, int& 
         run += l * step;
         n = min(step, n - l * step);
     } while (n > 1);
-    of_run = tiles(run);
+    const RunRows r = run_rows(p, run);
+    of_run = ((r.row1 - r.row0) * p.group + kTileQueries - 1) / kTileQueries;
     in_run = place - first_place(run);
     return in_run < of_run ? run : -1;
 }
@@ -1172,7 +1203,8 @@ PromptSplit prompt_split(const nhip_paged_cache* c, int32_t rows, int32_t heads,
         s.parts = (most + s.blocks - 1) / s.blocks;
     }
     s.tiles_a_round = 0;
-    if (runs > 1 && runs <= 64 && s.parts == 1 && s.tiles * c->kv_heads > 256) {
+    const int64_t groups = s.tiles * c->kv_heads;
+    if (runs > 1 && runs <= kSortedRuns && s.parts == 1 && groups > 256 && groups <= kSortedGroups) {
         s.tiles_a_round = std::max(1, 256 / c->kv_heads);
         s.tiles = (s.tiles + s.tiles_a_round - 1) / s.tiles_a_round * s.tiles_a_round;
     }

@@ -394,18 +394,19 @@ def test_scales_far_from_one(hip, e):
     check_decode(gpu, 0, q, qs, [(0, r, 300) for r in range(30)], 300)
 
 
-@pytest.mark.parametrize("runs,rows", [(63, 40), (65, 9), (700, 3), (4200, 2)])
-def test_prompt_many_runs(hip, runs, rows):
+@pytest.mark.parametrize("runs,rows,kv", [(63, 40, 1), (65, 9, 1), (700, 3, 1), (4200, 2, 1), (255, 6, 3), (100, 4, 64),
+                                          (256, 2, 1), (257, 2, 1)])
+def test_prompt_many_runs(hip, runs, rows, kv):
     """Runs of 0 to `rows` rows, many of them empty, some longer than a tile."""
     rng = np.random.default_rng(33)
-    pool = Pool(rng, 1, 60, 16, 1, 64, 64, 3, 20)
+    pool = Pool(rng, 1, 60, 16, kv, 64, 64, 3, 20)
     pool.give(rng, [300, 150, 64])  # (every run lies in its sequence)
     spec = [(int(n), int(s), int(rng.integers(0, 8))) for n, s in zip(rng.integers(0, rows + 1, runs),
                                                                      rng.integers(0, 3, runs))]
     spec[runs // 3] = (131, 0, 100)
     spec[-1] = (70, 1, 3)
     spec[-2] = spec[0] = (0, 0, 0)
-    q, qs = queries(rng, sum(n for n, _, _ in spec) + 5, 2, 64)
+    q, qs = queries(rng, sum(n for n, _, _ in spec) + 5, 2 * kv if kv < 9 else kv, 64)
     check_prompt(Gpu(hip, pool), 0, q, qs, spec, 0, 300, rows_behind=5)
 
 
