@@ -613,7 +613,7 @@ int32_t launch_decode(const DecodeParams& p, const Split& s, int32_t rows, hipSt
 // exponential, sum, two conversions and the rest between them) beside its
 // share of the products, and vector and matrix instructions of a SIMD's two
 // waves overlap in part only.  One run of 8192 rows, 32 heads on 8 of 128
-// takes 732 us (719 to 760 from one card to the next), 550 Gflop: 750 TFLOP/s.
+// takes 732 us (709 to 770 from one card to the next), 550 Gflop: 750 TFLOP/s.
 // Its products, the values' made twice for the weights' two parts, would take
 // 633 us at the rates of a large int8 and a large fp16 product (one part: 394,
 // but weights of 11 bits are off by 2^-12 each).  Measured and not kept there: eight waves
