@@ -370,9 +370,11 @@ int32_t nhip_paged_reset_dev(const nhip_paged_cache* c, void* stream);
  * keys d_k[r*ldk + kvh*qk_dim ..], values d_v[r*ldv + kvh*v_dim ..] (fp32;
  * columns of a wider matrix such as a fused Q/K/V projection's output;
  * ldk >= kv_heads*qk_dim, ldv >= kv_heads*v_dim).  The position's page must
- * be held already (nhip_paged_resize_dev) and by this sequence alone; rows
- * whose sequence, position or page is out of range write nothing.  Two rows
- * of a call at one position leave it unspecified.  lengths are not read. */
+ * be held already (nhip_paged_resize_dev) and by this sequence alone: rows
+ * whose sequence, position or page is out of range write nothing, nor do rows
+ * whose page has more than one holder (refs), so that after a resize that
+ * found too few pages no other sequence's positions are written.  Two rows of
+ * a call at one position leave it unspecified.  lengths are not read. */
 int32_t nhip_paged_append_dev(const nhip_paged_cache* c, int32_t layer, const float* d_k, int32_t ldk,
                               const float* d_v, int32_t ldv, const int32_t* d_row_seq, const int32_t* d_row_pos,
                               int32_t rows, void* stream);

@@ -59,19 +59,24 @@ struct AppendParams {
     const float* v;
     const int32_t* row_seq;
     const int32_t* row_pos;
+    const int32_t* refs;
     int32_t ldk, ldv, rows;
 };
 
+// A row whose page other sequences hold too writes nothing: a resize that found
+// too few pages has not made the row's copy of it, and only the device knows.
+//
 // A workgroup takes 16 rows of one kv head; L lanes share a row's key (or
 // value) head, four elements each, so a head's peak is a few DPP steps and 16
 // rows of keys leave as whole dwords.  Values change places through LDS: the
 // cache holds 16 positions of a dimension together, and where the rows are
 // consecutive positions of one sequence (a prompt) a lane writes as many of
 // them at once as lie in a block; else each goes by itself.  Bound by the
-// bytes: 8185 rows of 8 kv heads of 128 (84 MB) take 19.6 us, 4.3 TB/s (20.8
-// with the groups dealt to the XCDs one by one: 26 MB were written for 17; and
-// then 24.5 with 64 rows a workgroup: fewer are in flight); one step's 16 rows 4.4 us,
-// which is the launch.
+// bytes: 8185 rows of 8 kv heads of 128 (84 MB) take 18.2 us, 4.6 TB/s (with
+// the groups dealt to the XCDs one by one 26 MB were written for 17, 1.2 us
+// more; with 64 rows a workgroup, fewer of which are in flight, 3.7 us more).
+// One step's 16 rows take 4.5 us: a launch (2.5) and the chain sequence, page,
+// holders, store, which the codes are formed beside.
 constexpr int kAppendRows = 16;
 typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
 
@@ -110,13 +115,34 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p)
         if (4 * l < V) x[k][1] = *reinterpret_cast<const f4*>(p.v + r * p.ldv + kvh * V + 4 * l);
     }
     // where each row's position lives: its page's first cell (of this kv head) and its place in the page, -1 if nowhere
+    int seq = -1, pos = 0, page = -1;
     if (threadIdx.x < N) {
-        const int i = threadIdx.x, r = row0 + min(i, n - 1);
-        const int seq = p.row_seq[r], pos = p.row_pos[r];
-        int page = -1;
+        const int r = row0 + min((int)threadIdx.x, n - 1);
+        seq = p.row_seq[r], pos = p.row_pos[r];
         if (seq >= 0 && seq < c.sequences && pos >= 0 && (pos >> c.page_shift) < c.width)
             page = c.tables[(size_t)seq * c.width + (pos >> c.page_shift)];
-        const bool ok = i < n && page >= 0 && page < c.pages;
+    }
+    float scales[PASSES][2];
+    uint32_t codes[PASSES][2];
+#pragma unroll
+    for (int k = 0; k < PASSES; k++) {
+        const int i = row_of_pass + k * ROWS;
+#pragma unroll
+        for (int part = 0; part < 2; part++) {
+            const f4 y = x[k][part];
+            const float peak =
+                group_max<L>(fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3]))));
+            scales[k][part] = peak > 0.0f ? peak / 127.0f : 1.0f;
+            codes[k][part] = ref_quantize4(make_float4(y[0], y[1], y[2], y[3]), 1.0f / scales[k][part]);
+            if (part == 1 && 4 * l < V) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) turned[4 * l + e][16 + i] = (uint8_t)(codes[k][part] >> (8 * e));
+            }
+        }
+    }
+    if (threadIdx.x < N) {
+        const int i = threadIdx.x;
+        const bool ok = i < n && page >= 0 && page < c.pages && p.refs[page] <= 1;
         cells[i] = ok ? ((size_t)page * c.kv_heads + kvh) << c.page_shift : 0;
         places[i] = ok ? pos & ((1 << c.page_shift) - 1) : -1;
         // (the first wave's: whether the rows are consecutive positions of one sequence)
@@ -130,26 +156,15 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p)
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < PASSES; k++) {
-        const int i = row_of_pass + k * ROWS;
-        const int at = places[i];
-        const size_t cell = cells[i];
-#pragma unroll
-        for (int part = 0; part < 2; part++) {
-            const f4 y = x[k][part];
-            const float peak =
-                group_max<L>(fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3]))));
-            const float scale = peak > 0.0f ? peak / 127.0f : 1.0f;
-            const uint32_t codes = ref_quantize4(make_float4(y[0], y[1], y[2], y[3]), 1.0f / scale);
-            if (part == 1 && 4 * l < V) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) turned[4 * l + e][16 + i] = (uint8_t)(codes >> (8 * e));
-            }
-            if (at < 0) continue;
-            if (part == 0 && 4 * l < QK) *reinterpret_cast<uint32_t*>(c.keys + (cell + at) * QK + 4 * l) = codes;
-            if (l == 0) (part ? c.vscale : c.kscale)[cell + at] = scale;
+        const int at = places[row_of_pass + k * ROWS];
+        const size_t cell = cells[row_of_pass + k * ROWS];
+        if (at < 0) continue;
+        if (4 * l < QK) *reinterpret_cast<uint32_t*>(c.keys + (cell + at) * QK + 4 * l) = codes[k][0];
+        if (l == 0) {
+            c.kscale[cell + at] = scales[k][0];
+            c.vscale[cell + at] = scales[k][1];
         }
     }
-    __syncthreads();
     if (consecutive) {
         // blocks of 16 positions, whole ones as one store a dimension, the ends in quads where they have them
         const int lead = first_position & 15;
@@ -714,7 +729,7 @@ int32_t nhip_paged_append_dev(const nhip_paged_cache* c, int32_t layer, const fl
                  "paged append: row strides %d, %d below a row's columns", ldk, ldv);
     rc = ensure_device();
     if (rc) return rc;
-    const AppendParams p{paged_layer(c, layer), d_k, d_v, d_row_seq, d_row_pos, ldk, ldv, rows};
+    const AppendParams p{paged_layer(c, layer), d_k, d_v, d_row_seq, d_row_pos, c->refs, ldk, ldv, rows};
     if (c->qk_dim == 48)
         launch_append<48, 64>(p, as_stream(stream));
     else if (c->qk_dim == 64)

@@ -511,6 +511,57 @@ def test_append(hip, orc, qk, v, page, kv):
         assert np.array_equal(gpu.get(name), getattr(pool, name), equal_nan=name.endswith("scales")), name
 
 
+@pytest.mark.parametrize("qk,v", DIMS)
+def test_append_writes_no_page_that_others_hold(hip, orc, qk, v):
+    """A step whose resize finds too few pages appends all the same (a graph
+    does): no byte of a shared page changes, rows on pages of their own are
+    written, and the step goes through once pages are free."""
+    rng = np.random.default_rng(qk)
+    pool = Pool(rng, 2, 5, 16, 2, qk, v, 4, 6)
+    pool.give(rng, [40, 0, 0, 5])
+    gpu, books = Gpu(hip, pool), Books(pool)
+    ws = gpu.workspace(gpu.cache.pages_workspace(4))
+    gpu.cache.fork(2, gpu.dev([1, 2]).ptr, gpu.dev([0, 0]).ptr, gpu.dev([20, 40]).ptr, *ws)
+    books.fork([1, 2], [0, 0], [20, 40])
+    before = pools(gpu)
+    status = gpu.dev([9, 9])
+    seq, length = [0, 1, 2, 3], [41, 21, 41, 6]
+    gpu.cache.resize(4, gpu.dev(seq).ptr, gpu.dev(length).ptr, status.ptr, *ws)
+    assert tuple(status.download(np.int32)) == books.resize(seq, length) == (1, 0)
+    pos = [40, 20, 40, 5]
+    x = rng.standard_normal((4, 2 * (qk + v))).astype(np.float32)
+    dx, dseq, dpos = gpu.dev(x, np.float32), gpu.dev(seq), gpu.dev(pos)
+
+    def append():
+        gpu.cache.append(1, dx.ptr, x.shape[1], dx.ptr + 8 * qk, x.shape[1], dseq.ptr, dpos.ptr, 4)
+
+    def expect(rows):
+        for name in ("keys", "key_scales", "values", "value_scales"):
+            setattr(pool, name, before[name].copy())
+        pool.tables = books.tables
+        for a, b in books.moved:
+            for name in ("keys", "key_scales", "values", "value_scales"):
+                getattr(pool, name)[:, b] = before[name][:, a]
+        expected_append(orc, pool, 1, x[rows, :2 * qk].reshape(-1, 2, qk), x[rows, 2 * qk:].reshape(-1, 2, v),
+                        [seq[r] for r in rows], [pos[r] for r in rows])
+        for name in ("keys", "key_scales", "values", "value_scales"):
+            assert np.array_equal(gpu.get(name), getattr(pool, name), equal_nan=True), name
+        check_books(gpu, books)
+
+    append()
+    expect([3])
+    gpu.cache.free(1, dseq.ptr + 8, *ws)  # sequence 2 ends: the last page of sequence 0 is its own
+    books.resize([2], [0])
+    append()
+    expect([0, 3])
+    before = pools(gpu)
+    gpu.cache.resize(2, dseq.ptr, gpu.dev(length).ptr, status.ptr, *ws)
+    assert tuple(status.download(np.int32)) == books.resize(seq[:2], length[:2]) == (0, 0)
+    assert len(books.moved) == 1
+    append()
+    expect([0, 1, 3])
+
+
 def test_append_of_over_a_million_workgroups(hip, orc):
     """70,000 rows of 256 kv heads, four of which go somewhere."""
     rng = np.random.default_rng(43)
