@@ -631,8 +631,9 @@ struct PromptParams {
     const int32_t* run_pos;
     float* parts;  // as DecodeParams'
     float* stats;
-    int32_t* counts;  // [rows][heads]: the parts of a row
     int32_t rows, heads, group, runs, window, max_count, blocks, max_parts;
+    int32_t places;  // of tiles that the grid holds
+    uint32_t group_part;  // 2^31 / group, rounded up
     int32_t tiles_a_round;  // of 256 workgroups, where the tiles are sorted; else 0
     float scale;
 };
@@ -653,6 +654,52 @@ __device__ __forceinline__ RunRows run_rows(const PromptParams& p, int run)
     r.row0 = min(max(p.run_rows[run], 0), p.rows);
     r.row1 = max(r.row0, min(p.run_rows[run + 1], p.rows));
     return r;
+}
+
+// x / group for a query or head x < 2^24 (group <= 16, so the quotient is exact).
+__device__ __forceinline__ int over_group(const PromptParams& p, int x)
+{
+    return (int)(((uint64_t)(uint32_t)x * p.group_part) >> 31);
+}
+
+__device__ __forceinline__ int run_tiles(const PromptParams& p, const RunRows& r)
+{
+    return ((r.row1 - r.row0) * p.group + kTileQueries - 1) / kTileQueries;
+}
+
+// The position that query `at` (row-major over the group's heads) of a run
+// sits at, cut to the call's limit; -1 where the run has no positions.  run_pos
+// belongs to the run's first row as the caller counts them, which may lie
+// before row 0.
+struct RunPositions {
+    int64_t pos0;  // of its first row here
+    int limit;
+    bool known;
+    __device__ __forceinline__ int at(const PromptParams& p, int query) const
+    {
+        const int64_t x = pos0 + over_group(p, query);
+        return known ? (int)(x < limit ? x : limit - 1) : -1;
+    }
+};
+__device__ __forceinline__ RunPositions run_positions(const PromptParams& p, int row0, int first_row, int seq, int pos)
+{
+    return {(int64_t)pos + row0 - first_row, min(p.c.width << p.c.page_shift, p.max_count),
+            seq >= 0 && seq < p.c.sequences && pos >= 0};
+}
+
+// The 64-position tiles [begin, end) that a tile of queries at positions
+// first .. last attends, and the parts that they are cut into.
+struct TileSpan {
+    int from, begin, end, parts;
+};
+__device__ __forceinline__ TileSpan tile_span(const PromptParams& p, int first, int last)
+{
+    TileSpan s;
+    s.from = p.window > 0 ? max(first - p.window + 1, 0) : 0;
+    s.begin = s.from >> 6;
+    s.end = last >= 0 ? (last >> 6) + 1 : s.begin;
+    s.parts = (s.end - s.begin + p.blocks - 1) / p.blocks;
+    return s;
 }
 
 // The run whose tile has the place `place` in the call, the tile's number in
@@ -767,7 +814,7 @@ __device__ __forceinline__ int find_tile(const PromptParams& p, int place, int& 
         n = min(step, n - l * step);
     } while (n > 1);
     const RunRows r = run_rows(p, run);
-    of_run = ((r.row1 - r.row0) * p.group + kTileQueries - 1) / kTileQueries;
+    of_run = run_tiles(p, r);
     in_run = place - first_place(run);
     return in_run < of_run ? run : -1;
 }
@@ -808,20 +855,16 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
     // the last tiles of a run attend most: they go first
     const int q0 = __builtin_amdgcn_readfirstlane((of_run - 1 - in_run) * kTileQueries);
     const int qn = min(kTileQueries, queries - q0);
-    // positions: run_pos belongs to the run's first row as the caller counts
-    // them, which may lie before row 0
-    const int seq = scalar_load(p.run_seq, run), pos_of_run = scalar_load(p.run_pos, run);
-    const int64_t pos0 = (int64_t)pos_of_run + row0 - scalar_load(p.run_rows, run);
-    const int limit = min(c.width << c.page_shift, p.max_count);
-    const bool known = seq >= 0 && seq < c.sequences && pos_of_run >= 0;
+    const int seq = scalar_load(p.run_seq, run);
+    const RunPositions at = run_positions(p, row0, scalar_load(p.run_rows, run), seq, scalar_load(p.run_pos, run));
 
     // this lane's query
     const int query = q0 + 32 * wave + (lane & 31);
     const bool mine = query < q0 + qn;
     const int q_row = min(query, queries - 1) / p.group;
     const int head = kvh * p.group + min(query, queries - 1) - q_row * p.group;
-    const int64_t far_pos = pos0 + q_row;
-    const int q_pos = known && far_pos < limit ? (int)far_pos : -1;  // -1 attends nothing
+    const int64_t far_pos = at.pos0 + q_row;
+    const int q_pos = at.known && far_pos < at.limit ? (int)far_pos : -1;  // -1 attends nothing
     const int q_first = p.window > 0 ? max(q_pos - p.window + 1, 0) : 0;
     const size_t q_at = (size_t)(row0 + q_row) * p.heads + head;
     i32x4 q[KK];
@@ -834,22 +877,17 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
     qs = qs == 0.0f ? 1.2e-38f : qs;  // (a score is then 0, and a position left out still -inf)
 
     // the wave's and the workgroup's positions (the last query's row is the furthest)
-    auto pos_of = [&](int at) {
-        const int64_t x = pos0 + at / p.group;
-        return known ? (int)(x < limit ? x : limit - 1) : -1;
-    };
-    const int wave_first = __builtin_amdgcn_readfirstlane(pos_of(min(q0 + 32 * wave, queries - 1)));
-    const int wave_last = 32 * wave < qn ? __builtin_amdgcn_readfirstlane(pos_of(min(q0 + 32 * wave + 31, queries - 1)))
+    const int wave_first = __builtin_amdgcn_readfirstlane(at.at(p, min(q0 + 32 * wave, queries - 1)));
+    const int wave_last = 32 * wave < qn ? __builtin_amdgcn_readfirstlane(at.at(p, min(q0 + 32 * wave + 31, queries - 1)))
                                          : -1;
-    const int first_pos = __builtin_amdgcn_readfirstlane(pos_of(q0));
-    const int last_pos = __builtin_amdgcn_readfirstlane(pos_of(q0 + qn - 1));
-    const int from = p.window > 0 ? max(first_pos - p.window + 1, 0) : 0;
+    const int first_pos = __builtin_amdgcn_readfirstlane(at.at(p, q0));
+    const int last_pos = __builtin_amdgcn_readfirstlane(at.at(p, q0 + qn - 1));
+    const TileSpan span = tile_span(p, first_pos, last_pos);
+    const int from = span.from, parts = span.parts;
     const int from_window = p.window > 0 ? p.window - 1 : 1 << 30;  // positions before its own that a row attends
-    const int tile0 = from >> 6, tile1 = last_pos >= 0 ? (last_pos >> 6) + 1 : tile0;
-    const int parts = (tile1 - tile0 + p.blocks - 1) / p.blocks;
     if (part > 0 && part >= parts) return;
-    const int begin = tile0 + part * p.blocks;
-    const int end = min(tile1, begin + p.blocks);
+    const int begin = span.begin + part * p.blocks;
+    const int end = min(span.end, begin + p.blocks);
 
     // Staging: a wave brings one 16-position block of a tile, so its page is a
     // scalar, looked up a tile ahead.  Units are spread over the banks such
@@ -1071,7 +1109,6 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
     }
     float factor;
     float* to;
-    if (p.max_parts > 1 && part == 0 && g == 0) p.counts[q_at] = parts;
     if (parts <= 1) {
         factor = all != 0.0f ? 1.0f / all : 0.0f;
         to = p.out + q_at * V;
@@ -1091,28 +1128,53 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
 }
 
 // Joins the parts of rows that were split, a wave per (row, head); rows of no
-// run have no parts.
+// run have no parts.  A row's parts follow from its run, as its tile counted
+// them: nothing is read of a workspace that no tile has written, also where
+// the runs overlap (run_rows that do not ascend) and not every tile finds a
+// place in the grid.  (Split calls have few tiles, so few runs, whose tiles
+// are placed in the runs' order.)
 template <int V>
 __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PromptParams p)
 {
     const int row = blockIdx.x, lane = threadIdx.x & 63;
     const int head = (int)blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (head >= p.heads) return;
-    bool in_run = false;
-    for (int i = lane; i < p.runs; i += 64) {
-        const RunRows r = run_rows(p, i);
-        in_run |= row >= r.row0 && row < r.row1;
+    int tiles_before = 0;
+    RunRows r = {0, 0};
+    RunPositions at = {};
+    uint64_t hit = 0;
+    for (int i0 = 0; i0 < p.runs && hit == 0; i0 += 64) {
+        // (a run's four words at once: the join is a chain of latencies)
+        const int i = min(i0 + lane, p.runs - 1);
+        const int first_row = p.run_rows[i], seq = p.run_seq[i], pos = p.run_pos[i];
+        RunRows own = run_rows(p, i);
+        if (i0 + lane > i) own = {0, 0};
+        hit = __ballot(row >= own.row0 && row < own.row1);
+        const int l = hit ? __builtin_ctzll(hit) : 63;
+        r = {__builtin_amdgcn_readlane(own.row0, l), __builtin_amdgcn_readlane(own.row1, l)};
+        at = run_positions(p, r.row0, __builtin_amdgcn_readlane(first_row, l), __builtin_amdgcn_readlane(seq, l),
+                           __builtin_amdgcn_readlane(pos, l));
+        if (l > 0) tiles_before += wave_sum_i32(hit == 0 || lane < l ? run_tiles(p, own) : 0);
     }
-    if (!__ballot(in_run)) return;
-    const size_t q_at = (size_t)row * p.heads + head;
-    const int parts = p.counts[q_at];
+    if (hit == 0) return;
+    const int queries = (r.row1 - r.row0) * p.group, tiles = run_tiles(p, r);
+    const int of_group = head - over_group(p, head) * p.group;
+    const int tile = ((row - r.row0) * p.group + of_group) / kTileQueries;
+    if (__builtin_amdgcn_readfirstlane(tiles_before) + tiles - 1 - tile >= p.places) return;
+    const int q0 = tile * kTileQueries;
+    const int parts = tile_span(p, at.at(p, q0), at.at(p, min(q0 + kTileQueries, queries) - 1)).parts;
     if (parts <= 1) return;
+    const size_t q_at = (size_t)row * p.heads + head;
     const size_t first = q_at * p.max_parts;
     float2 stat = make_float2(kNoScore, 0.0f);
     if (lane < parts) stat = *reinterpret_cast<const float2*>(p.stats + 2 * (first + lane));
     const float factor = __builtin_amdgcn_exp2f(stat.x - wave_max(stat.x));
     float all = factor * stat.y;
-    for (int off = 32; off; off >>= 1) all += __shfl_xor(all, off);
+    all = rows_sum(all);
+    all += lane_xor<8>(all);
+    all += lane_xor<4>(all);
+    all += lane_xor<2>(all);
+    all += lane_xor<1>(all);
     constexpr int E = V / 64;
     float sum[E];
 #pragma unroll
@@ -1213,7 +1275,7 @@ PromptSplit prompt_split(const nhip_paged_cache* c, int32_t rows, int32_t heads,
 
 size_t prompt_workspace(const nhip_paged_cache* c, int32_t rows, int32_t heads, const PromptSplit& s)
 {
-    return s.parts > 1 ? (size_t)rows * heads * ((size_t)s.parts * (c->v_dim + 2) + 1) * sizeof(float) : 0;
+    return s.parts > 1 ? (size_t)rows * heads * s.parts * (c->v_dim + 2) * sizeof(float) : 0;
 }
 
 template <int QK, int V>
@@ -1315,7 +1377,6 @@ int32_t nhip_paged_prompt_dev(const nhip_paged_cache* c, int32_t layer, const in
     p.run_pos = d_run_pos;
     p.parts = static_cast<float*>(d_workspace);
     p.stats = p.parts + (size_t)rows * heads * split.parts * c->v_dim;
-    p.counts = reinterpret_cast<int32_t*>(p.stats + (size_t)2 * rows * heads * split.parts);
     p.rows = rows;
     p.heads = heads;
     p.group = heads / c->kv_heads;
@@ -1324,6 +1385,8 @@ int32_t nhip_paged_prompt_dev(const nhip_paged_cache* c, int32_t layer, const in
     p.max_count = max_count;
     p.blocks = split.blocks;
     p.max_parts = split.parts;
+    p.places = (int32_t)split.tiles;
+    p.group_part = (uint32_t)(((1u << 31) + p.group - 1) / p.group);
     p.tiles_a_round = split.tiles_a_round;
     p.scale = score_scale(c->qk_dim);
     if (c->qk_dim == 48) return launch_prompt<48, 64>(p, split, as_stream(stream));

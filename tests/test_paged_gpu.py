@@ -451,6 +451,33 @@ def test_prompt_ignores_what_run_rows_may_not_say(hip):
         assert np.all(ok[1] if r >= 4 else ok[0] | ok[1])
 
 
+@pytest.mark.parametrize("left", [0xA5, 0x3F])
+@pytest.mark.parametrize("group,window", [(1, 0), (1, 900), (3, 0)])
+def test_prompt_split_of_runs_that_overlap(hip, left, group, window):
+    """Ends that do not ascend, in a call that is split: the tiles of the last
+    run find no place, so its own rows stay as they were whatever the workspace
+    held; the other runs say the same of their rows, which are right."""
+    rng = np.random.default_rng(17)
+    heads, rows, ends = group, 300, [0, 260, 0, 260, 0, 260, 0, 260, 0, 260, 0, 260, 0, 300]
+    pool = Pool(rng, 1, 45, 32, 1, 64, 64, 1, 48)
+    pool.give(rng, [1400])
+    gpu = Gpu(hip, pool)
+    need = gpu.cache.prompt_workspace(rows, heads, 13, 1500)
+    assert need > 0
+    q, qs = queries(rng, rows, heads, 64)
+    out = gpu.dev(np.full((rows, heads, 64), -77.0), np.float32)
+    ws = gpu.dev(np.full(need, left), np.uint8)
+    ends, zeros, pos = gpu.dev(ends), gpu.dev([0] * 13), gpu.dev([1100] * 13)
+    gpu.cache.prompt(0, gpu.dev(q, np.int8).ptr, gpu.dev(qs, np.float32).ptr, rows, heads, 13, ends.ptr, zeros.ptr,
+                     pos.ptr, window, 1500, ws.ptr, need, out.ptr)
+    got = out.download(np.float32).reshape(rows, heads, 64)
+    assert (got[260:] == -77.0).all()
+    for r in range(0, 260, 7):
+        first = max(0, 1100 + r - window + 1) if window else 0
+        want, far = pool.attend(0, 0, q[r], qs[r], first, 1100 + r + 1 - first, True)
+        assert np.all(np.abs(got[r] - want) <= far), r
+
+
 def test_prompt_leaves_out_pages_outside_the_pool(hip):
     rng = np.random.default_rng(18)
     pool = Pool(rng, 1, 40, 16, 2, 64, 64, 2, 8)
