@@ -404,10 +404,8 @@ int32_t nhip_paged_decode_dev(const nhip_paged_cache* c, int32_t layer, const in
  * ... of sequence run_seq[i].  Their keys and values are in the cache already
  * (nhip_paged_append_dev), as are those of the positions before them.  The row
  * at position p attends [0, p], or with window > 0 [max(0, p-window+1), p].
- * Everything else as nhip_paged_decode_dev; but a position's weight times its
- * value scale is kept to 2^-30 of the row's largest weight times the largest
- * value scale that the row attends, so where these scales lie more than 2^14
- * apart the small ones lose digits.  max_count bounds every position + 1 (rows
+ * Everything else as nhip_paged_decode_dev; a position's weight times its value
+ * scale is kept to 2^-30 of the row's largest such product.  max_count bounds every position + 1 (rows
  * beyond give zeros), and rows behind the last run are left as they are.
  * (rows * heads / kv_heads / 128 + runs) * kv_heads <= 2^23. */
 size_t nhip_paged_prompt_workspace(const nhip_paged_cache* c, int32_t rows, int32_t heads, int32_t runs,

@@ -44,6 +44,7 @@ __device__ __forceinline__ float row_bcast(float v)
 // w 2^-e.  A position that does not count has e = -inf, which makes w 0.
 constexpr float kHeadroom = 14.0f;
 constexpr float kMaxExponent = 60.0f;  // of a value scale, either way
+constexpr float kLeastScale = 1.4e-45f;
 struct Position {
     float ks, e, frac, inv;
 };
@@ -57,6 +58,12 @@ __device__ __forceinline__ Position position(float ks, float vs, bool live)
     r.ks = live ? ks : 0.0f;
     r.e = live ? (float)e : -INFINITY;
     return r;
+}
+
+__device__ __forceinline__ float scale_exponent(float vs)
+{
+    const int e = (int)((__float_as_uint(vs) >> 23) & 255) - 127;
+    return (float)min(max(e, -(int)kMaxExponent), (int)kMaxExponent);
 }
 
 // Eight int8 codes (two words) as fp16, exactly: the byte c + 128 in the low
@@ -603,10 +610,13 @@ int32_t launch_decode(const DecodeParams& p, const Split& s, int32_t rows, hipSt
 //            multiplication), and a query's maximum and total are its lane's.
 //   values   O^T = V^T P^T by v_mfma_f32_32x32x16_f16: registers 8 u .. 8 u + 7
 //            are the eight weights that product u wants of this lane.
-// The weights are 2^(z - M), M the running maximum less up to 2^8 plus the
-// exponent of the largest value scale that the row has attended, so that a
-// weight times its value scale fits fp16, and its two fp16 parts keep 2^-30 of
-// the largest; the sums are rescaled only when M has to move, a few times a row.
+// The weights are 2^(z - M), with M such that a weight times its value scale
+// stays below 2^15, which fits fp16, while the row's largest such product is at
+// least 2^5: its two fp16 parts, to a step of 2^-24, keep 2^-30 of it.  M thus
+// follows the maximum of z + e (e the scale's exponent), and a scale that is
+// large where the weight is small does not move it.  Whether it has to move is
+// asked with a bound, the tile's largest score and largest exponent; only where
+// that is too large, a few times a row, is the maximum formed.
 //
 // Bound by the issue of instructions: a position and query costs about 10
 // vector operations of 4 cycles a wave (conversion, two scalings, maximum,
@@ -639,7 +649,7 @@ struct PromptParams {
 };
 
 constexpr int kTileQueries = 128;
-constexpr float kLag = 8.0f;  // log2 of how far a weight may grow past the reference before the sums are rescaled
+constexpr float kLag = 8.0f;  // log2 of how far a product may grow before the sums are rescaled
 
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -937,7 +947,8 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
         // its position, and no others: their score becomes NaN, the scale 0.
         const uint64_t odd = __ballot((__float_as_uint(scale_r) & 0x7F800000u) == 0x7F800000u) >> 16;
         float x = (odd >> (lane & 15)) & 1 ? (lane & 16 ? 0.0f : NAN) : scale_r;
-        x = (live >> (lane & 15)) & 1 ? x : 0.0f;
+        // (a position that counts has a scale above 0: the least there is makes its products 0)
+        x = (live >> (lane & 15)) & 1 ? (lane & 16 ? fmaxf(x, kLeastScale) : x) : 0.0f;
         if (lane < 32) (lane & 16 ? lds_vs : lds_ks)[tile & 3][16 * wave + (lane & 15)] = x;
         if (lane == 0) lds_live[tile & 3][wave] = (uint16_t)live;
     };
@@ -957,10 +968,10 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
     for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
-    // peak: the reference of the scores; exponent: that of the largest value
-    // scale the query has attended; base = peak + exponent; lowest: the least
-    // exponent of the wave's queries
-    float peak = kNoScore, exponent = -kMaxExponent, base = kNoScore, lowest = -kMaxExponent, total = 0.0f;
+    // base: M; bound: an exponent that no value scale of a tile may pass (ceiling:
+    // 2^(bound + 1)) and limit: base + 14 - bound, which no score may pass,
+    // without M being looked at again
+    float base = kNoScore, bound = 0.0f, ceiling = 0.0f, limit = kNoScore, total = 0.0f;
     const float minus_one = alone(-1.0f);
     // where this lane reads: the key row of its A row, the value rows of its dimensions
     const int m = lane & 31;
@@ -1013,44 +1024,79 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
 #undef NHIP_DOT
                 }
                 const bool whole = __builtin_amdgcn_readfirstlane(counted.x & counted.y) == ~0u;
-                // the largest value scale, of the lane's two positions or, in a tile
-                // that not every query attends whole, of those that the query attends
-                float largest = fmaxf(vs[0], vs[1]), against = lowest;
+                const float largest = fmaxf(vs[0], vs[1]);  // of the lane's two positions
                 const bool masked = !whole | (64 * tile + 63 > wave_first) | (64 * tile < wave_last - from_window);
                 if (masked) {
                     const int last = q_pos - 64 * tile - 8 * g, first = q_first - 64 * tile - 8 * g;
-                    largest = 0.0f;
-                    against = exponent;
 #pragma unroll
                     for (int t = 0; t < 2; t++) {
                         const uint32_t bits = (t ? counted.y : counted.x) >> (8 * g);
-                        auto mask = [&](int r, float scale) NHIP_INLINE {
+#pragma unroll
+                        for (int r = 0; r < 16; r++) {
                             const int at = 16 * (r / 8) + r % 8;
                             const bool attends =
                                 (32 * t + at <= last) & (32 * t + at >= first) & ((bits >> at) & 1);
                             z[t][r] = attends ? z[t][r] : -INFINITY;
-                            largest = fmaxf(largest, attends ? scale : 0.0f);
-                        };
-#define NHIP_MASK(r) mask(r, row_bcast<r>(vs[t]));
-                        NHIP_MASK(0) NHIP_MASK(1) NHIP_MASK(2) NHIP_MASK(3) NHIP_MASK(4) NHIP_MASK(5) NHIP_MASK(6)
-                        NHIP_MASK(7) NHIP_MASK(8) NHIP_MASK(9) NHIP_MASK(10) NHIP_MASK(11) NHIP_MASK(12)
-                        NHIP_MASK(13) NHIP_MASK(14) NHIP_MASK(15)
-#undef NHIP_MASK
+                        }
                     }
-                    largest = fmaxf(largest, lane_xor<32>(largest));
                 }
                 float up = z[0][0];
 #pragma unroll
                 for (int r = 1; r < 32; r++) up = fmaxf(up, z[r / 16][r % 16]);
                 up = fmaxf(up, lane_xor<32>(up)) * qs;
-                float ev = fminf((float)((int)(__float_as_uint(largest) >> 23) - 127), kMaxExponent);
-                if (__ballot((up - peak > kHeadroom) | (ev > against))) {
-                    if (!masked)
-                        for (int off = 32; off; off >>= 1) ev = fmaxf(ev, __shfl_xor(ev, off));
-                    peak = up - peak > kHeadroom ? up - (kHeadroom - kLag) : peak;
-                    exponent = fmaxf(exponent, ev);
-                    lowest = -wave_max(-exponent);
-                    const float to = peak + exponent, keep = __builtin_amdgcn_exp2f(base - to);
+                float to = base;
+                if (__ballot((up > limit) | (largest >= ceiling))) {
+                    // Values that are all 0 have scale 1 (QuantizeInt8), which says nothing
+                    // of their size: the least in its place, so that the others keep their digits.
+                    if (__ballot((vs[0] == 1.0f) | (vs[1] == 1.0f))) {
+                        uint32_t any[4] = {0, 0, 0, 0};  // of 8 positions, lanes 8 o .. 8 o + 7 those of octet o
+#pragma unroll
+                        for (int k = 0; k < V / 8; k++) {
+                            const int dim = 8 * k + (lane & 7);
+                            const uint4 x = *reinterpret_cast<const uint4*>(lds_v[tile & 1] + dim * 128 +
+                                                                            16 * ((lane >> 3) ^ value_swizzle(dim)));
+                            any[0] |= x.x, any[1] |= x.y, any[2] |= x.z, any[3] |= x.w;
+                        }
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            any[k] |= lane_xor<1>(any[k]);
+                            any[k] |= lane_xor<2>(any[k]);
+                            any[k] |= lane_xor<4>(any[k]);
+                        }
+#pragma unroll
+                        for (int t = 0; t < 2; t++) {
+                            uint32_t pair = 0;  // this lane's position and its neighbour
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                const uint32_t x = (uint32_t)__shfl((int)any[k], (32 * t + slot) & ~7);
+                                pair = ((lane >> 1) & 3) == k ? x : pair;
+                            }
+                            if (vs[t] == 1.0f && ((lane & 1 ? pair >> 16 : pair) & 0xFFFF) == 0) vs[t] = kLeastScale;
+                        }
+                    }
+                    const float e[2] = {scale_exponent(vs[0]), scale_exponent(vs[1])};
+                    bound = wave_max(fmaxf(e[0], e[1]));
+                    // the scales within a factor of four: one exponent stands for all
+                    float most = up + bound;
+                    const float least = fminf(vs[0] > 0.0f ? e[0] : bound, vs[1] > 0.0f ? e[1] : bound);
+                    if (wave_max(bound - least) > 1.0f) {
+                        most = -INFINITY;
+#pragma unroll
+                        for (int t = 0; t < 2; t++) {
+#define NHIP_MOST(r) most = fmaxf(most, z[t][r] * qs + row_bcast<r>(e[t]));
+                            NHIP_MOST(0) NHIP_MOST(1) NHIP_MOST(2) NHIP_MOST(3) NHIP_MOST(4) NHIP_MOST(5) NHIP_MOST(6)
+                            NHIP_MOST(7) NHIP_MOST(8) NHIP_MOST(9) NHIP_MOST(10) NHIP_MOST(11) NHIP_MOST(12)
+                            NHIP_MOST(13) NHIP_MOST(14) NHIP_MOST(15)
+#undef NHIP_MOST
+                        }
+                        most = fmaxf(most, lane_xor<32>(most));
+                    }
+                    to = most > base + kHeadroom ? most - (kHeadroom - kLag) : base;
+                    ceiling = __uint_as_float((uint32_t)(128 + (int)bound) << 23);
+                    limit = to + (kHeadroom - bound);
+                }
+                if (__ballot(to > base)) {
+                    const float keep = __builtin_amdgcn_exp2f(base - to);
                     base = to;
                     total *= keep;
 #pragma unroll

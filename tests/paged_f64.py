@@ -67,6 +67,27 @@ class Pool:
             far[h] += FLOOR * 2 * largest * np.abs(v).sum(0)
         return out, far
 
+    def attend_products(self, layer, seq, q, q_scales, first, count, prompt=False):
+        """As attend, with the bound that holds whatever the scales are: the
+        floor is that of the largest weight times scale (PROMPT_LAG behind it in
+        a prompt), and values whose codes are all 0 have no part in it."""
+        heads = q.shape[0]
+        out, far = np.zeros((heads, self.v)), np.zeros((heads, self.v))
+        at = np.arange(first, first + count)
+        t, at = self.tables[seq, at // self.page], at % self.page
+        for h in range(heads):
+            j = h // (heads // self.kv)
+            k, ks = self.keys[layer, t, j, at].astype(np.float64), self.key_scales[layer, t, j, at].astype(np.float64)
+            v = self.values[layer, t, j, at // 16, :, at % 16].astype(np.float64)
+            vs = np.where(v.any(1), self.value_scales[layer, t, j, at].astype(np.float64), 0.0)
+            z = (k @ q[h].astype(np.float64)) * ks * float(q_scales[h]) / np.sqrt(self.qk)
+            w = np.exp(z - z.max())
+            w /= w.sum()
+            out[h] = (w * vs) @ v
+            far[h] = bound(count, np.abs(z).max(), vs[vs > 0] if vs.any() else np.ones(1)) * ((w * vs) @ np.abs(v))
+            far[h] += FLOOR * 2 * (w * vs).max() * (PROMPT_LAG if prompt else 1.0) * np.abs(v).sum(0)
+        return out, far
+
 
 #: The weights w vs enter the value product as two fp16 numbers.  Below 2^-14
 #: fp16 has a step of 2^-24, so a weight is off by up to 2^-25 besides its

@@ -379,6 +379,87 @@ def test_large_scales_reach_only_the_rows_that_attend_them(hip, window, kv, grou
         assert np.all(np.abs(single[p] - want) <= far), p
 
 
+def zero_values_among_small_ones(rng, peak, qk, v, kv, lengths):
+    """A cache whose values have peaks up to `peak`, every seventh of them all 0
+    with the scale 1 that QuantizeInt8 gives it."""
+    pool = Pool(rng, 1, sum(-(-n // 16) for n in lengths) + 1, 16, kv, qk, v, len(lengths), 40)
+    pool.give(rng, lengths)
+    pool.value_scales *= np.float32(peak / 127 / 0.03)
+    for s, n in enumerate(lengths):
+        for pos in range(s % 3, n, 7):
+            p, at = pool.tables[s, pos // 16], pos % 16
+            pool.values[0, p, :, at // 16, :, at % 16] = 0
+            pool.value_scales[0, p, :, at] = 1.0
+    return pool
+
+
+@pytest.mark.parametrize("qk,v", DIMS)
+@pytest.mark.parametrize("peak", [100.0, 1e-2, 1e-4, 1e-9])
+def test_prompt_zero_values_among_small_ones(hip, qk, v, peak):
+    """Values that are all 0 cost the others no digits (the first tile has some,
+    with an attended whole tile after it; a run of zeros alone gives zeros)."""
+    rng = np.random.default_rng(61)
+    pool = zero_values_among_small_ones(rng, peak, qk, v, 2, [200, 90, 20])
+    for p in pool.tables[2, :2]:
+        pool.values[0, p], pool.value_scales[0, p] = 0, 1.0
+    runs = [(60, 0, 140), (90, 1, 0), (20, 2, 0)]
+    q, qs = queries(rng, 170, 4, qk)
+    got = Gpu(hip, pool).prompt(0, q, qs, [0, 60, 150, 170], [0, 1, 2], [140, 0, 0], 0, 200)
+    assert not got[150:].any()
+    off = rms = 0.0
+    for r, (s, p) in enumerate([(s, pos + j) for n, s, pos in runs[:2] for j in range(n)]):
+        want, far = pool.attend_products(0, s, q[r], qs[r], 0, p + 1, True)
+        assert np.all(np.abs(got[r] - want) <= far), r
+        off, rms = off + np.sum((got[r] - want) ** 2), rms + np.sum(want ** 2)
+    assert np.sqrt(off) <= 1e-5 * np.sqrt(rms)
+
+
+@pytest.mark.parametrize("far_apart", [13, 40])
+@pytest.mark.parametrize("window", [0, 300])
+def test_prompt_large_scales_of_small_weight(hip, far_apart, window):
+    """Value scales 2^13 and 2^40 times the others where the weight is about
+    e^-30: the row is exact to its largest product of the two."""
+    rng = np.random.default_rng(67)
+    pool = Pool(rng, 1, 45, 16, 2, 64, 64, 1, 45)
+    pool.give(rng, [700])
+    pool.keys = rng.integers(-20, 21, pool.keys.shape, dtype=np.int8)
+    for pos in (5, 64, 200, 207, 480):
+        p, at = pool.tables[0, pos // 16], pos % 16
+        pool.keys[0, p, :, at] = -120
+        pool.key_scales[0, p, :, at] = 0.02
+        pool.value_scales[0, p, :, at] *= np.float32(2.0 ** far_apart)
+    gpu = Gpu(hip, pool)
+    rows = 690
+    q = rng.integers(60, 128, (rows, 4, 64), dtype=np.int8)
+    qs = rng.uniform(0.015, 0.02, (rows, 4)).astype(np.float32)
+    got = gpu.prompt(0, q, qs, [0, rows], [0], [10], window, 700)
+    off, rms = 0.0, 0.0
+    for r in range(0, rows, 3):
+        first = max(0, 10 + r - window + 1) if window else 0
+        want, far = pool.attend_products(0, 0, q[r], qs[r], first, 10 + r + 1 - first, True)
+        assert np.all(np.abs(got[r] - want) <= far), r
+        off, rms = off + np.sum((got[r] - want) ** 2), rms + np.sum(want ** 2)
+    assert np.sqrt(off) <= 1e-5 * np.sqrt(rms)
+
+
+@pytest.mark.parametrize("scale", [0.0, 1e-44, 1e-30])
+def test_prompt_scales_of_nothing(hip, scale):
+    """Value scales of 0 or next to it, some of a sequence's and all of one's:
+    what they hide is 0, the rest as exact as without it."""
+    rng = np.random.default_rng(71)
+    pool = Pool(rng, 1, 30, 16, 2, 64, 64, 2, 12)
+    pool.give(rng, [170, 75])
+    for pos in list(range(30, 90)) + [3, 100, 131]:
+        pool.value_scales[0, pool.tables[0, pos // 16], :, pos % 16] = scale
+    pool.value_scales[0, pool.tables[1, :5]] = scale
+    q, qs = queries(rng, 245, 4, 64, 0.1)
+    got = Gpu(hip, pool).prompt(0, q, qs, [0, 170, 245], [0, 1], [0, 0], 0, 170)
+    assert np.abs(got[170:]).max() <= 128 * scale
+    for r in range(0, 170, 3):
+        want, far = pool.attend_products(0, 0, q[r], qs[r], 0, r + 1, True)
+        assert np.all(np.abs(got[r] - want) <= far), r
+
+
 @pytest.mark.parametrize("e", [-58, 58])
 def test_scales_far_from_one(hip, e):
     """All value scales times 2^e, rows whole and in parts."""
