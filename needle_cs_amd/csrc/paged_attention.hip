@@ -217,8 +217,11 @@ __device__ __forceinline__ int ordered_row(const DecodeParams& p, int place, Spa
 // order of the call; 16 kv heads 27.5 and 33.0; 48 rows, 8 heads of 128 25.9
 // and 33.3; but rows of 1040 each 16.5 and 15.9.  (Its own variant: the
 // registers of the choice cost the others up to 0.5 us.)
+//
+// Registers: the general form for dims of 128 has to stay within 168, which
+// three waves a SIMD share (32 rows of up to 32768: 276 us, 289 with 169).
 template <int QK, int V, int W, bool ONE, bool SORTED>
-__global__ __launch_bounds__(64 * W, QK <= 64 ? 4 : 2) void paged_decode_kernel(DecodeParams p)
+__global__ __launch_bounds__(64 * W, QK <= 64 ? 4 : ONE || SORTED ? 2 : 3) void paged_decode_kernel(DecodeParams p)
 {
     constexpr int KH = (QK + 63) / 64, VT = V / 16;
     extern __shared__ __align__(16) float lds[];  // [W][group][V] sums, then [W][16] M, [W][16] total
@@ -337,13 +340,30 @@ __global__ __launch_bounds__(64 * W, QK <= 64 ? 4 : 2) void paged_decode_kernel(
                     dots[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kr[t][half], q[half], dots[t], 0, 0, 0);
             }
         }
-        const Position x = position(ksr, vsr, live);
+        Position x = position(ksr, vsr, live);
         const bool more = block + W < end_block;
         if (more) load_keys(block + W, kpage, vpage);
         vpage_now = vpage;
         if (block + 2 * W < end_block) {
             kpage = page_at(64 * (block + 2 * W) + 16 * (h >> 2));
             vpage = page_at(64 * (block + 2 * W) + 16 * g);
+        }
+        // Values that are all 0 have scale 1 (QuantizeInt8), which says nothing of
+        // their size: 0 in its place, so that the others keep their digits.
+        if (__ballot(x.frac == 1.0f && x.e == 0.0f)) {
+            uint32_t word = 0;  // the codes of this lane's position and three beside it, of any dimension
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                uint32_t any = 0;
+#pragma unroll
+                for (int t = 0; t < VT; t++) any |= (uint32_t)vr[t][k];
+                any |= lane_xor<1>(any);
+                any |= lane_xor<2>(any);
+                any |= lane_xor<4>(any);
+                any |= lane_xor<8>(any);
+                word = ((lane >> 2) & 3) == k ? any : word;
+            }
+            if (x.frac == 1.0f && x.e == 0.0f && ((word >> (8 * (lane & 3))) & 255) == 0) x = position(x.ks, 0.0f, true);
         }
         float w[16];  // the weights of the 16 positions that this lane gives the value product (ONE: as words)
         if constexpr (ONE) {

@@ -414,6 +414,26 @@ def test_prompt_zero_values_among_small_ones(hip, qk, v, peak):
     assert np.sqrt(off) <= 1e-5 * np.sqrt(rms)
 
 
+@pytest.mark.parametrize("qk,v", DIMS)
+@pytest.mark.parametrize("kv,group", [(2, 2), (2, 1)])
+@pytest.mark.parametrize("peak", [100.0, 1e-4, 1e-9])
+def test_decode_zero_values_among_small_ones(hip, peak, qk, v, kv, group):
+    """As above, whole and in parts; a row of zeros alone gives zeros."""
+    rng = np.random.default_rng(63)
+    pool = zero_values_among_small_ones(rng, peak, qk, v, kv, [600, 90, 20])
+    for p in pool.tables[2, :2]:
+        pool.values[0, p], pool.value_scales[0, p] = 0, 1.0
+    spec = [(0, 0, 600), (1, 0, 90), (0, 130, 77), (0, 599, 1), (1, 1, 1), (2, 0, 20)]
+    q, qs = queries(rng, 6, kv * group, qk)
+    gpu = Gpu(hip, pool)
+    for max_count in (600, 640):
+        got = gpu.decode(0, q, qs, *zip(*spec), max_count)
+        assert not got[5].any()
+        want, far = (np.stack(x) for x in zip(*[pool.attend_products(0, s, q[r], qs[r], f, n)
+                                                for r, (s, f, n) in enumerate(spec)]))
+        close(got, want, far)
+
+
 @pytest.mark.parametrize("far_apart", [13, 40])
 @pytest.mark.parametrize("window", [0, 300])
 def test_prompt_large_scales_of_small_weight(hip, far_apart, window):
