@@ -384,9 +384,11 @@ int32_t nhip_paged_append_dev(const nhip_paged_cache* c, int32_t layer, const fl
  * attend positions row_first[r] .. row_first[r]+row_count[r]-1 of sequence
  * row_seq[r]; query head h reads kv head h / (heads/kv_heads) and scores are
  * scaled by 1/sqrt(qk_dim), as in nhip_attention_decode_dev.  out fp32
- * [rows][heads][v_dim].  Softmax statistics and sums are fp32 and the result
- * is within 1e-5 of RMS(out) of exact arithmetic; it is the same for the same
- * call, but not the bits of the reference's order.  max_count bounds every
+ * [rows][heads][v_dim].  Scores, softmax statistics and sums are fp32 and the
+ * result is within 1e-5 of RMS(out) of exact arithmetic, or within 1e-7 of it
+ * times the row's largest |score| where that is above 100 (up to 1e6: a score
+ * is rounded to 2^-24 of itself); it is the same for the same call, but not
+ * the bits of the reference's order.  max_count bounds every
  * row_count (it decides how the work is split).  Rows of count 0, and rows
  * whose sequence or span is out of range or whose count exceeds max_count,
  * give zeros; positions on pages outside [0, pages) are left out.

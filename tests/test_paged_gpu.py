@@ -462,6 +462,36 @@ def test_prompt_large_scales_of_small_weight(hip, far_apart, window):
     assert np.sqrt(off) <= 1e-5 * np.sqrt(rms)
 
 
+@pytest.mark.parametrize("score", [30.0, 100.0, 1000.0, -1000.0, 1e5])
+@pytest.mark.parametrize("qk,v", DIMS)
+@pytest.mark.parametrize("group", [1, 4])
+def test_large_scores_that_nearly_tie(hip, score, qk, v, group):
+    """Every position has the score up to its key scale's rounding.  In fp32 a
+    score is off by three roundings of its own (those that a row's scores share
+    move all its weights alike), each at most 2^-24 of it: 2^-24 |score| in the
+    mean square, under 1e-7 |score|; 1e-5 where that is less."""
+    rng = np.random.default_rng(83)
+    pool = Pool(rng, 1, 20, 16, 2, qk, v, 1, 20)
+    pool.give(rng, [300])
+    base = rng.integers(60, 120, qk)
+    pool.keys = (base + rng.integers(-7, 8, pool.keys.shape)).astype(np.int8)
+    q = np.broadcast_to(rng.integers(60, 128, qk), (300, 2 * group, qk)).astype(np.int8)
+    qs = rng.uniform(0.7, 1.0, (300, 2 * group)).astype(np.float32)
+    dots = pool.keys.astype(np.float64) @ q[0, 0].astype(np.float64)
+    live = ~np.isnan(pool.key_scales)
+    pool.key_scales[live] = (score * np.sqrt(qk) / dots)[live]
+    gpu, rows = Gpu(hip, pool), np.arange(0, 300, 5)
+    both = {True: gpu.prompt(0, q, qs, [0, 300], [0], [0], 0, 300),
+            False: gpu.decode(0, q, qs, [0] * 300, [0] * 300, np.arange(1, 301), 300)}
+    for prompt, got in both.items():
+        off = rms = 0.0
+        for r in rows:
+            want, far = pool.attend_products(0, 0, q[r], qs[r], 0, r + 1, prompt)
+            assert np.all(np.abs(got[r] - want) <= far), (prompt, r)
+            off, rms = off + np.sum((got[r] - want) ** 2), rms + np.sum(want ** 2)
+        assert np.sqrt(off / rms) <= max(1e-5, 1e-7 * abs(score)), prompt
+
+
 @pytest.mark.parametrize("scale", [0.0, 1e-44, 1e-30])
 def test_prompt_scales_of_nothing(hip, scale):
     """Value scales of 0 or next to it, some of a sequence's and all of one's:
