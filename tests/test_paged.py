@@ -1,6 +1,7 @@
 """The paged cache's entry points refuse what they cannot do, before any
 device work (no GPU here), and their struct has its declared layout."""
 import ctypes as C
+import random
 
 import pytest
 
@@ -116,6 +117,45 @@ def test_workspace_sizes_need_no_device():
     assert c.decode_workspace(1, 12, 60000) >= 4 * 12 * 2 * 66
     assert c.prompt_workspace(4000, 12, 3, 60000) == 0
     assert c.prompt_workspace(20, 12, 1, 60000) >= 4 * 20 * 12 * 2 * 66
+
+
+#: (pages of 16, kv heads, query heads, rows, runs, max_count) -> decode's and a prompt's workspace for dims of 48 / 64:
+#: rows * heads * parts * (64 + 2) * 4 bytes, with the parts that the rules make of max_count // 64 + 2 blocks
+WORKSPACES = [
+    ((4096, 2, 12, 4, 1, 300), (0, 4 * 12 * 3 * 264)),
+    ((4096, 2, 12, 1, 1, 60000), (1 * 12 * 63 * 264, 1 * 12 * 63 * 264)),
+    ((4096, 2, 12, 20, 1, 60000), (20 * 12 * 50 * 264, 20 * 12 * 63 * 264)),
+    ((4096, 16, 16, 300, 3, 8000), (0, 300 * 16 * 10 * 264)),  # 80 workgroups of 127 blocks: 14 a part
+    ((4096, 16, 16, 300, 3, 1500), (0, 300 * 16 * 9 * 264)),  # of 25: 3 a part
+    ((4096, 16, 16, 4000, 3, 60000), (0, 0)),
+]
+
+
+@pytest.mark.parametrize("call,want", WORKSPACES)
+def test_workspace_sizes(call, want):
+    """Here without a device; tests/test_paged_gpu.py asks for the same with one."""
+    width, kv, heads, rows, runs, max_count = call
+    c = cache(pages=width, width=width, kv_heads=kv)
+    assert (c.decode_workspace(rows, heads, max_count), c.prompt_workspace(rows, heads, runs, max_count)) == want
+
+
+def test_a_window_never_needs_more_workspace():
+    """A prompt call whose workspace is as large as the query says is refused for
+    its missing arrays, never for the workspace, whatever its window."""
+    rng = random.Random(5)
+    split = 0
+    for _ in range(400):
+        kv, group = rng.choice([1, 2, 3, 8, 16, 48]), rng.choice([1, 2, 3, 5, 6, 16])
+        width = int(2 ** rng.uniform(0, 13))
+        max_count = rng.randint(0, 16 * width)
+        rows, runs = int(2 ** rng.uniform(0, 12)), int(2 ** rng.uniform(0, 8))
+        c = cache(pages=width, width=width, kv_heads=kv)
+        need = c.prompt_workspace(rows, kv * group, runs, max_count)
+        split += need > 0
+        for window in [0, 1, max_count, max_count + 1, 2 ** 31 - 1] + [int(2 ** rng.uniform(0, 17)) for _ in range(6)]:
+            with refused("prompt: null pointer"):
+                c.prompt(0, A, A, rows, kv * group, runs, None, None, None, window, max_count, A, need, A)
+    assert split > 100
 
 
 def test_attention_workspaces_are_checked():
