@@ -8,6 +8,7 @@ import numpy as np
 import pytest
 
 from paged_f64 import Books, Pool
+from test_paged import WORKSPACES
 
 pytestmark = pytest.mark.gpu
 
@@ -166,6 +167,33 @@ def test_decode_rows_in_order_of_their_length(hip, kv, group, rows):
     check_decode(Gpu(hip, pool), 0, q, qs, spec, 300)
 
 
+@pytest.mark.parametrize("kv,group,rows,qk,v", [(5, 1, 60, 48, 64), (5, 3, 60, 48, 64), (8, 1, 40, 64, 64),
+                                                (8, 2, 63, 64, 64), (8, 1, 48, 128, 128), (16, 2, 17, 128, 128)])
+def test_decode_rows_in_order_of_their_length_by_eight_waves(hip, kv, group, rows, qk, v):
+    """257 to 511 workgroups of rows of 11 to 40 blocks: whole rows, sorted, eight waves each."""
+    rng = np.random.default_rng(47)
+    assert 256 < kv * rows < 512
+    pool = Pool(rng, 1, 60, 64, kv, qk, v, 5, 30)
+    pool.give(rng, [1900, 1100, 300, 64, 5])
+    q, qs = queries(rng, rows, kv * group, qk)
+    spec = []
+    for _ in range(rows):
+        s = int(rng.integers(0, 5))
+        n = int(rng.integers(0, pool.lengths[s] + 1) // (1 + 5 * rng.integers(0, 2)))
+        spec.append((s, int(rng.integers(0, pool.lengths[s] - n + 1)), n))
+    spec[rows // 2], spec[rows // 3] = (0, 0, 0), (9, 0, 9)
+    spec[-1] = (0, 0, 1900)
+    gpu = Gpu(hip, pool)
+    assert gpu.cache.decode_workspace(rows, kv * group, 1900) == 0
+    seq, first, count = (np.array(x) for x in zip(*spec))
+    got = gpu.decode(0, q, qs, seq, first, count, 1900)
+    want, far = np.zeros(got.shape), np.zeros(got.shape)
+    for r, (s, f, n) in enumerate(spec):
+        if s < 5 and n:
+            want[r], far[r] = pool.attend_products(0, s, q[r], qs[r], f, n)
+    close(got, want, far)
+
+
 def test_decode_rows_out_of_range_give_zeros(hip):
     rng = np.random.default_rng(7)
     pool = Pool(rng, 1, 40, 16, 2, 64, 64, 3, 8)
@@ -254,6 +282,15 @@ def test_decode_offsets_past_32_bits(hip):
     p = int(tables[0, 600 // page])
     scales = bufs["key_scales"].download(np.float32, kv * page, offset=4 * (pages + p) * kv * page).reshape(kv, page)
     assert np.array_equal(scales[:, 600 % page], np.abs(x[0, :kv * d].reshape(kv, d)).max(1) / np.float32(127))
+
+
+def test_workspace_sizes_with_a_device(hip):
+    """The same as without one (tests/test_paged.py)."""
+    from needle_cs_amd.paged import PagedCache
+    names = ("keys", "key_scales", "values", "value_scales", "tables", "lengths", "refs")
+    for (width, kv, heads, rows, runs, max_count), want in WORKSPACES:
+        c = PagedCache(2, width, 16, kv, 48, 64, 4, width, buffers={n: 0x10000 for n in names})
+        assert (c.decode_workspace(rows, heads, max_count), c.prompt_workspace(rows, heads, runs, max_count)) == want
 
 
 # ---------------------------------------------------------------- prompt --
