@@ -499,6 +499,32 @@ def test_prompt_large_scales_of_small_weight(hip, far_apart, window):
     assert np.sqrt(off) <= 1e-5 * np.sqrt(rms)
 
 
+@pytest.mark.parametrize("codes,scale", [(0, 1.0), (0, 0.0), (100, 0.0), (100, 1e-44)])
+@pytest.mark.parametrize("kv,group", [(2, 2), (4, 1)])
+def test_values_of_nothing_that_take_the_weight(hip, codes, scale, kv, group):
+    """Every twentieth position has about e^14 times the others' weight and a
+    value of 0, by its codes or by its scale: the others' digits stay."""
+    rng = np.random.default_rng(73)
+    pool = Pool(rng, 1, 45, 16, kv, 128, 128, 1, 45)
+    pool.give(rng, [700])
+    pool.keys = rng.integers(-20, 21, pool.keys.shape, dtype=np.int8)
+    for pos in range(7, 700, 20):
+        p, at = pool.tables[0, pos // 16], pos % 16
+        pool.keys[0, p, :, at] = 100
+        pool.key_scales[0, p, :, at] = 0.008
+        pool.values[0, p, :, at // 16, :, at % 16] = codes
+        pool.value_scales[0, p, :, at] = scale
+    gpu = Gpu(hip, pool)
+    q = rng.integers(90, 128, (700, kv * group, 128), dtype=np.int8)
+    qs = rng.uniform(0.015, 0.016, (700, kv * group)).astype(np.float32)
+    both = {True: gpu.prompt(0, q, qs, [0, 700], [0], [0], 0, 700),
+            False: gpu.decode(0, q, qs, [0] * 700, [0] * 700, np.arange(1, 701), 700)}
+    for prompt, got in both.items():
+        for r in range(0, 700, 9):
+            want, far = pool.attend_products(0, 0, q[r], qs[r], 0, r + 1, prompt)
+            assert np.all(np.abs(got[r] - want) <= far), (prompt, r)
+
+
 @pytest.mark.parametrize("score", [30.0, 100.0, 1000.0, -1000.0, 1e5])
 @pytest.mark.parametrize("qk,v", DIMS)
 @pytest.mark.parametrize("group", [1, 4])
