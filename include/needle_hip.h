@@ -343,9 +343,10 @@ int32_t nhip_attention_decode_noalloc_dev(const int8_t* d_q, const float* d_q_sc
  * (128, 128); kv_heads <= 256; layers <= 4096; pages <= 2^20; sequences <=
  * 65536; width * page_size <= 2^30; a call takes up to 2^20 rows.
  *
- * Scales are not negative (QuantizeInt8's are positive).  A scale that is no
- * finite number spoils the rows that attend its position, and only those; so
- * may a value scale of more than 2^60, and outputs under 2^-60 lose digits.
+ * Scales, the queries' among them, are not negative (QuantizeInt8's are
+ * positive).  A scale that is no finite number may spoil the rows that attend
+ * its position, and only those; so may a value scale of more than 2^60, and
+ * outputs under 2^-60 lose digits.
  *
  * The calls below take this struct by pointer (read during the call), are
  * asynchronous on `stream` and may be captured in a graph; calls that write
@@ -368,8 +369,9 @@ int32_t nhip_paged_reset_dev(const nhip_paged_cache* c, void* stream);
 /* Row r's new key and value, QuantizeInt8 (src/Needle/Scalar.cs:67-74) per kv
  * head, into layer `layer` at position row_pos[r] of sequence row_seq[r]:
  * keys d_k[r*ldk + kvh*qk_dim ..], values d_v[r*ldv + kvh*v_dim ..] (fp32;
- * columns of a wider matrix such as a fused Q/K/V projection's output;
- * ldk >= kv_heads*qk_dim, ldv >= kv_heads*v_dim).  The position's page must
+ * columns of a wider matrix; ldk >= kv_heads*qk_dim, ldv >= kv_heads*v_dim).
+ * They are cached as they are: what a model does to its keys before attention
+ * (rotation by position, normalization) is done before this call.  The position's page must
  * be held already (nhip_paged_resize_dev) and by this sequence alone: rows
  * whose sequence, position or page is out of range write nothing, nor do rows
  * whose page has more than one holder (refs), so that after a resize that
@@ -407,7 +409,8 @@ int32_t nhip_paged_decode_dev(const nhip_paged_cache* c, int32_t layer, const in
  * (nhip_paged_append_dev), as are those of the positions before them.  The row
  * at position p attends [0, p], or with window > 0 [max(0, p-window+1), p].
  * Everything else as nhip_paged_decode_dev; a position's weight times its value
- * scale is kept to 2^-30 of the row's largest such product.  max_count bounds every position + 1 (rows
+ * scale is kept to 2^-30 of the row's largest such product (values whose codes
+ * are all 0, with QuantizeInt8's scale of 1, count as none).  max_count bounds every position + 1 (rows
  * beyond give zeros), and rows behind the last run are left as they are.
  * (rows * heads / kv_heads / 128 + runs) * kv_heads <= 2^23. */
 size_t nhip_paged_prompt_workspace(const nhip_paged_cache* c, int32_t rows, int32_t heads, int32_t runs,

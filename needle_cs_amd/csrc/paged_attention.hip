@@ -129,13 +129,15 @@ __device__ __forceinline__ float rows_sum(float v)
 //            and 16 positions, one load.
 // Nothing passes through LDS until the waves' parts are joined.
 //
-// A long call is bound by its bytes: 32 rows of up to 32768 positions, 8 kv
-// heads of 128 under 32 heads (1.38 GB) take 277 us, 5.0 TB/s, which is the
-// rate of a large copy.  A short one is a chain of latencies: table entry,
+// A long call is bound by what its loads in flight bring: 32 rows of up to 32768
+// positions, 8 kv heads of 128 under 32 heads (1.38 GB) take 276 us, 5.0 TB/s,
+// where a reduction over 4 GiB reads 6.4.  A short one is a chain of latencies: table entry,
 // keys, two exchanges of four lanes for the maximum, exponentials, values,
-// join; 3 rows of up to 192 positions take 4.5 us, of which 2.5 are the launch.
+// join; 3 rows of up to 192 positions take 4.3 us, of which 2.5 are the launch.
 // Measured and not kept: two blocks of loads in flight (360 us in the place
-// of 292, for the registers), 16 waves a workgroup (no gain).
+// of 292, for the registers); 16 waves a workgroup for dims of 64 (16 rows of up
+// to 2048, 16 kv heads: 10.7 us, 10.9 with eight; but 16 rows of up to 1024, 2
+// kv heads: 7.2 and 6.9).
 struct DecodeParams {
     PagedLayer c;
     const int8_t* q;
@@ -208,14 +210,14 @@ __device__ __forceinline__ int ordered_row(const DecodeParams& p, int place, Spa
 // is formed and weighted once.  The lanes of a row of 16 then pass their
 // weights (both fp16 parts in a word) to all of them, which is the value
 // product's operand (every column the same head).  16 rows of up to 2048
-// positions, 16 heads of 64: 11.3 us, 12.5 in the general form; the same over
-// two to four heads a kv head was no faster.
+// positions, 16 heads of 64: 10.9 us (compared when it came: 11.3, 12.5 in the
+// general form); the same over two to four heads a kv head was no faster.
 //
 // SORTED: calls of up to 64 whole rows and more workgroups than CUs deal the
 // rows to the CUs by their length (ordered_row), so that the longest do not
 // meet: 64 rows of up to 2048 positions, 8 kv heads: 18.7 us, 20.9 in the
 // order of the call; 16 kv heads 27.5 and 33.0; 48 rows, 8 heads of 128 25.9
-// and 33.3; but rows of 1040 each 16.5 and 15.9.  (Its own variant: the
+// (now 24) and 33.3; but rows of 1040 each 16.5 and 15.9.  (Its own variant: the
 // registers of the choice cost the others up to 0.5 us.)
 //
 // Registers: the general form for dims of 128 has to stay within 168, which
@@ -542,19 +544,26 @@ struct Split {
     int waves, blocks, parts, rows_a_round;
 };
 
-// A wave takes about 1 us a block beside 4 us for the launch; joining parts
-// costs 3 us.  So rows of few blocks stay whole: up to 18 (4 rows of 1024
-// positions, 16 kv heads: 6.0 us whole, 7.6 in parts; 2 rows of 1556, 4 kv
-// heads of 128: 14.9 whole, 10.6 in parts), or up to 40 where the workgroups
-// fill half the CUs anyway (16 rows of up to 2048, 16 kv heads: 10.9 us whole,
-// 13.4 in parts).  Longer ones are cut into parts of at least 8 blocks such
-// that the longest rows give 2048 workgroups (32 rows of up to 32768 on 8 kv
-// heads of 128: 277 us, 294 with 1024 workgroups; 4 rows of up to 8000: 17.8,
-// 49.9 whole), at most kMaxParts.  Eight waves a workgroup, which a row's
-// blocks are dealt to in turn (the 16 rows above: 10.9 us, 15.1 with four); but
-// four where there are 512 workgroups or more (the 32 rows: 277 and 307), or
-// rows of up to 10 blocks, where it makes no difference (16 rows of 256, 8 kv
-// heads: 4.9 both ways).
+// Parts cost a second launch and even out the rows.  Measured whole and in
+// parts, at rows of 700, 1100, 1600 and 2400 positions (12 to 39 blocks):
+//   8 or 32 workgroups, dims of 64    5.9  7.6  9.0 12.5 us   parts  8.2  8.2  8.2  8.4
+//                       dims of 128   8.5 11.5 15.4 20.6             10.1 10.3 10.5 10.9
+//   128 workgroups,     dims of 64    6.3  8.5 10.8 14.0              8.6 10.5 12.2 15.4
+//                       dims of 128   9.5 12.6 16.7 21.8             11.9 17.3 17.2 21.3
+//   256 workgroups,     dims of 64    8.2 10.4 12.8 17.4             11.3 13.9 16.8 21.3
+//                       dims of 128  12.0 15.9 20.9 31.3             15.7 19.8 24.4 37.3
+// So rows stay whole up to 18 blocks (for few workgroups the two meet a little
+// above for dims of 64, a little below for 128), or up to 40 where the
+// workgroups fill half the CUs (where 128 of them meet at 40 for dims of 128;
+// rows of very different lengths gain there by parts: 16 of 32 to 2400, 8 kv
+// heads of 128: 21.1 whole, 18.0 in parts).  Longer ones are cut into parts of
+// at least 8 blocks such that the longest rows give 2048 workgroups (32 rows of
+// up to 32768 on 8 kv heads of 128: 276 us, 294 with 1024 workgroups; 4 rows of
+// up to 8000: 17.5, 49.9 whole), at most kMaxParts.  Eight waves a workgroup,
+// which a row's blocks are dealt to in turn (16 rows of up to 2048, 16 kv heads:
+// 10.9 us, 15.1 with four); but four where there are 512 workgroups or more (the
+// 32 rows: 276 and 307), or rows of up to 10 blocks, where it makes no
+// difference (16 rows of 256, 8 kv heads: 4.9 both ways).
 Split decode_split(const nhip_paged_cache* c, int32_t rows, int32_t max_count)
 {
     const int64_t units = (int64_t)rows * c->kv_heads;
@@ -636,14 +645,17 @@ int32_t launch_decode(const DecodeParams& p, const Split& s, int32_t rows, hipSt
 // follows the maximum of z + e (e the scale's exponent), and a scale that is
 // large where the weight is small does not move it.  Whether it has to move is
 // asked with a bound, the tile's largest score and largest exponent; only where
-// that is too large, a few times a row, is the maximum formed.
+// that is too large, a few times a row, is the maximum formed (in every tile
+// where one position in 32 is a value of zeros the call below takes 925 us, and
+// where the scales lie e^3 apart 814).
 //
 // Bound by the issue of instructions: a position and query costs about 10
 // vector operations of 4 cycles a wave (conversion, two scalings, maximum,
 // exponential, sum, two conversions and the rest between them) beside its
 // share of the products, and vector and matrix instructions of a SIMD's two
 // waves overlap in part only.  One run of 8192 rows, 32 heads on 8 of 128
-// takes 732 us (709 to 770 from one card to the next), 550 Gflop: 750 TFLOP/s.
+// takes 742 us (726 to 757 from one card to the next; up to 1000 in the first
+// 40 passes, until the card's clock has settled), 550 Gflop: 741 TFLOP/s.
 // Its products, the values' made twice for the weights' two parts, would take
 // 633 us at the rates of a large int8 and a large fp16 product (one part: 394,
 // but weights of 11 bits are off by 2^-12 each).  Measured and not kept there: eight waves
@@ -1308,7 +1320,7 @@ struct PromptSplit {
 // heads: 34 us whole, 45 in two parts).  Up to 96 workgroups, or 256 with 32
 // or more blocks each, are split until about 768 are there, in parts of two
 // blocks or more (16 rows after 32,000 positions, 8 kv heads of 128: 798 us
-// whole, 37 in 63 parts; 512 rows after 8,000, 16 kv heads: 182 and 50; 416
+// whole, 37 in 63 parts; 512 rows after 8,000, 16 kv heads: 182 and 56; 416
 // rows from 0, 112 workgroups of up to 8 blocks: 14.8 whole, 16.7 in parts).
 // A window bounds a tile's blocks; it never makes more parts, as the workspace
 // is sized without it.
