@@ -198,6 +198,31 @@ int32_t nhip_weights_info(const nhip_weights* w, int32_t* rows, int32_t* cols, i
 int32_t nhip_quantize_rows_dev(const float* d_x, int32_t tokens, int32_t cols, int8_t* d_q,
                                float* d_scales, void* stream);
 
+/* x fp32 rows of codes back to numbers, the inverse of nhip_quantize_rows_dev:
+ * d_x[r*ldx + i] = d_q[r*cols + i] * d_scales[r].  rows <= 2^26, cols <= 2^20,
+ * ldx >= cols. */
+int32_t nhip_dequantize_rows_dev(const int8_t* d_q, const float* d_scales, int32_t rows, int32_t cols, float* d_x,
+                                 int32_t ldx, void* stream);
+
+/* A layer's residual addition, root-mean-square norm and quantization, the
+ * rows of the next int8 product in one launch (no counterpart in the
+ * reference, whose engine runs them one after the other).  For row r:
+ *   s = x + delta                    (d_delta NULL: s = x), to d_sum if given
+ *   h = (s * (1 / sqrt(mean(s^2) + eps))) * g
+ *   d_q[r][..], d_scales[r] = QuantizeInt8(h), as nhip_quantize_rows_dev's
+ * with g = d_gain[i] (d_gain NULL: 1), or 1 + d_gain[i] with zero_centered
+ * (Ops.ZeroCenteredRms's gains).  The mean and the square root are formed in
+ * 64 bits and the inverse rounded to fp32 once; every other operation is one
+ * fp32 operation, so that the result does not depend on how a row is summed
+ * (but for one rounding of the inverse in some 10^8 rows).  d_x, d_delta and
+ * d_sum have row strides ldx, ldd and ld_sum >= cols (columns of wider
+ * matrices); d_sum may be d_x or d_delta (with its stride), and overlaps
+ * nothing else.  A row with a NaN or an infinity has codes of no meaning, and
+ * no effect on the others.  rows <= 2^26, cols <= 2^20. */
+int32_t nhip_add_rms_quantize_dev(const float* d_x, int32_t ldx, const float* d_delta, int32_t ldd,
+                                  const float* d_gain, int32_t zero_centered, float eps, int32_t rows, int32_t cols,
+                                  float* d_sum, int32_t ld_sum, int8_t* d_q, float* d_scales, void* stream);
+
 /* Quant.Prepare on device (Quant.cs:473-488): x fp32 [tokens][cols] ->
  * values int8 [tokens][cols] (planes order), scales/offsets fp32
  * [tokens][stride]. */
@@ -317,6 +342,66 @@ int32_t nhip_attention_decode_noalloc_dev(const int8_t* d_q, const float* d_q_sc
                                           const int32_t* d_row_first, const int32_t* d_row_count,
                                           int32_t max_chunks, float* d_out, void* stream);
 
+/* --------------------------------------------------- rotary positions ---- */
+
+/* Rotation of query and key heads by position.  A head's first `dim`
+ * dimensions are pairs (x0, x1): dimensions i and i + dim/2 (Scalar.Rope,
+ * src/Needle/Scalar.cs:233-248), or with `interleaved` dimensions 2i and
+ * 2i + 1, i < dim/2.  At position p
+ *   x0' = x0 * cos[p][i] - x1 * sin[p][i],  x1' = x1 * cos[p][i] + x0 * sin[p][i]
+ * (every operation rounded to fp32, as the decoder engine rotates); the head's
+ * other dimensions stay as they are.  cos and sin are device tables
+ * [positions][dim/2], made by nhip_rotary_table_dev or by the caller.  dim is
+ * even and at most 512.  The struct is read during the call. */
+typedef struct nhip_rotary {
+    const float* cos;
+    const float* sin;
+    int32_t positions, dim, interleaved;
+} nhip_rotary;
+
+/* How a table's frequencies follow from theta, f_i = theta^(-2i/dim), for
+ * contexts longer than a model was made for (factor >= 1):
+ *   NHIP_ROTARY_PLAIN   f_i
+ *   NHIP_ROTARY_LINEAR  f_i / factor (positions packed closer)
+ *   NHIP_ROTARY_BASE    theta times factor^(dim/(dim-2)): the slowest pair is
+ *                       slowed by factor, the fastest not (dim > 2)
+ *   NHIP_ROTARY_PARTS   a ramp over the pairs: those that turn more than `high`
+ *                       times over `original` positions keep f_i, those of less
+ *                       than `low` turns take f_i / factor.  With b(t) = dim *
+ *                       ln(original / (2 pi t)) / (2 ln theta), lo =
+ *                       max(floor(b(high)), 0), hi = min(ceil(b(low)), dim - 1) (lo +
+ *                       0.001 where they are equal): r = clamp((i - lo) / (hi -
+ *                       lo), 0, 1), f_i / factor * r + f_i * (1 - r)
+ *   NHIP_ROTARY_BANDS   the same by the turns themselves: r = clamp((original *
+ *                       f_i / (2 pi) - low) / (high - low), 0, 1),
+ *                       f_i / factor * (1 - r) + f_i * r
+ * cos and sin are multiplied by magnitude (1 for none).  low, high and
+ * original are used by the last two (0 < low < high, original > 0). */
+enum {
+    NHIP_ROTARY_PLAIN = 0,
+    NHIP_ROTARY_LINEAR = 1,
+    NHIP_ROTARY_BASE = 2,
+    NHIP_ROTARY_PARTS = 3,
+    NHIP_ROTARY_BANDS = 4
+};
+typedef struct nhip_rotary_scaling {
+    double theta, factor, low, high, original, magnitude;
+    int32_t kind;
+} nhip_rotary_scaling;
+
+/* cos and sin of positions first .. first+count-1 (0 <= first, first + count <=
+ * 2^30) into d_cos, d_sin [count][dim/2]: angles and their cos and sin in 64
+ * bits, rounded to fp32 at the end.  A table grows by calls on its next rows. */
+int32_t nhip_rotary_table_dev(float* d_cos, float* d_sin, int32_t first, int32_t count, int32_t dim,
+                              const nhip_rotary_scaling* scaling, void* stream);
+/* The heads of every row, d_x[r*ldx + h*head_dim ..], rotated by position
+ * d_row_pos[r] into d_y[r*ldy + h*head_dim ..].  d_y may be d_x (with ldy =
+ * ldx), and overlaps it in no other way.  Rows whose position is outside
+ * [0, positions) write nothing.  rows <= 2^20, head_dim >= dim, head_dim <=
+ * 4096, heads * head_dim <= ldx, ldy and 2^24. */
+int32_t nhip_rotary_dev(const nhip_rotary* r, const float* d_x, int32_t ldx, int32_t heads, int32_t head_dim,
+                        const int32_t* d_row_pos, int32_t rows, float* d_y, int32_t ldy, void* stream);
+
 /* --------------------------------------------- paged KV cache (serving) -- */
 
 /* No counterpart in the reference: an int8 KV cache in pages, for servers
@@ -381,6 +466,30 @@ int32_t nhip_paged_append_dev(const nhip_paged_cache* c, int32_t layer, const fl
                               const float* d_v, int32_t ldv, const int32_t* d_row_seq, const int32_t* d_row_pos,
                               int32_t rows, void* stream);
 
+/* nhip_rotary_dev on the rows' query and key heads, nhip_quantize_rows_dev on
+ * the queries and nhip_paged_append_dev, in one launch and with their bits:
+ * row r's query heads d_q[r*ldq + h*qk_dim ..] and keys d_k[r*ldk + ..] rotated
+ * by row_pos[r], the queries' codes and scales to d_codes int8
+ * [rows][heads][qk_dim] and d_q_scales [rows][heads], ready for the attention
+ * calls, keys and values to position row_pos[r] of sequence row_seq[r].  Rows
+ * that nhip_paged_append_dev would not write write nothing to the cache; rows
+ * whose position is outside the table write nothing to it either, and have
+ * queries of codes 0 and scale 1.  r->dim <= qk_dim; heads <= 4096 (a multiple
+ * of kv_heads); d_codes 4-byte aligned. */
+int32_t nhip_paged_rotary_append_dev(const nhip_paged_cache* c, int32_t layer, const nhip_rotary* r, const float* d_q,
+                                     int32_t ldq, int32_t heads, const float* d_k, int32_t ldk, const float* d_v,
+                                     int32_t ldv, const int32_t* d_row_seq, const int32_t* d_row_pos, int32_t rows,
+                                     int8_t* d_codes, float* d_q_scales, void* stream);
+
+/* Cached positions back to numbers: the keys and values that layer `layer`
+ * holds at position row_pos[r] of sequence row_seq[r], code * scale, to
+ * d_k[r*ldk + kvh*qk_dim ..] and d_v[r*ldv + kvh*v_dim ..] (fp32; either may be
+ * NULL; strides as nhip_paged_append_dev's).  Rows whose sequence, position or
+ * page is out of range give zeros.  lengths are not read. */
+int32_t nhip_paged_read_dev(const nhip_paged_cache* c, int32_t layer, const int32_t* d_row_seq,
+                            const int32_t* d_row_pos, int32_t rows, float* d_k, int32_t ldk, float* d_v, int32_t ldv,
+                            void* stream);
+
 /* Attention of one new token per row: row r's query heads (q int8
  * [rows][heads][qk_dim] with q_scales [rows][heads], QuantizeInt8 per head)
  * attend positions row_first[r] .. row_first[r]+row_count[r]-1 of sequence
@@ -419,6 +528,29 @@ int32_t nhip_paged_prompt_dev(const nhip_paged_cache* c, int32_t layer, const in
                               int32_t rows, int32_t heads, int32_t runs, const int32_t* d_run_rows,
                               const int32_t* d_run_seq, const int32_t* d_run_pos, int32_t window, int32_t max_count,
                               void* d_workspace, size_t workspace_bytes, float* d_out, void* stream);
+
+/* Attention over a window and a sequence's first positions ("sinks"), which
+ * stay visible however far the window has moved.  decode: row r attends the
+ * first min(sinks, row_first[r]) positions of its sequence beside [row_first[r],
+ * row_first[r] + row_count[r]) (a row of count 0 attends nothing); prompt: the
+ * row at position p attends the positions up to p that lie in [max(0, p-window+1), p]
+ * or in [0, sinks).  Everything else as the calls without sinks, which these are for sinks =
+ * 0 (and for window = 0); positions between sinks and window are not read, and
+ * their pages' table entries may be anything.  sinks >= 0. */
+size_t nhip_paged_decode_sinks_workspace(const nhip_paged_cache* c, int32_t rows, int32_t heads, int32_t sinks,
+                                         int32_t max_count);
+int32_t nhip_paged_decode_sinks_dev(const nhip_paged_cache* c, int32_t layer, const int8_t* d_q,
+                                    const float* d_q_scales, int32_t rows, int32_t heads, const int32_t* d_row_seq,
+                                    const int32_t* d_row_first, const int32_t* d_row_count, int32_t sinks,
+                                    int32_t max_count, void* d_workspace, size_t workspace_bytes, float* d_out,
+                                    void* stream);
+size_t nhip_paged_prompt_sinks_workspace(const nhip_paged_cache* c, int32_t rows, int32_t heads, int32_t runs,
+                                         int32_t sinks, int32_t max_count);
+int32_t nhip_paged_prompt_sinks_dev(const nhip_paged_cache* c, int32_t layer, const int8_t* d_q,
+                                    const float* d_q_scales, int32_t rows, int32_t heads, int32_t runs,
+                                    const int32_t* d_run_rows, const int32_t* d_run_seq, const int32_t* d_run_pos,
+                                    int32_t window, int32_t sinks, int32_t max_count, void* d_workspace,
+                                    size_t workspace_bytes, float* d_out, void* stream);
 
 /* Pages.  All of a call's entries act together (as if every entry read the
  * cache as it was before the call); of entries that name the same sequence
@@ -579,6 +711,38 @@ int32_t nhip_topk_lse_dev(const float* d_logits, int32_t rows, int32_t n, int32_
  * d_value[r] (optional) = that value.  Asynchronous on `stream`. */
 int32_t nhip_argmax_dev(const float* d_x, int32_t ldx, int32_t n, int32_t rows, int32_t* d_index, float* d_value,
                         void* stream);
+/* One id per row of logits, drawn with a given number (no counterpart in the
+ * reference, which takes the largest).  Row r's ids are those with a finite or +inf
+ * logit d_logits[r*ldx + i], i < n, and a set bit in the row's mask
+ * (as nhip_argmax_masked_dev's; d_mask NULL: every id; ids past `words` * 32
+ * have none), in the order of their logits, the largest first, ties to the lower
+ * id.  Weights are e^((logit - largest) / temperature), as whole multiples of
+ * 2^-42 (of the largest logit's weight, 1).  Kept are, one rule behind the other,
+ *   top_k  the first top_k ids (<= 0: all);
+ *   top_p  of those, an id as long as the ones before it weigh less than top_p
+ *          times all of them; always the first (>= 1 or NaN: all);
+ *   min_p  of those, ids of weight >= min_p (at most 1; NaN: all).
+ * With t = floor(random * total weight of the kept ids), d_ids[r] is the lowest
+ * kept id for which the weights of the kept ids up to it exceed t.  A
+ * temperature <= 0 or NaN takes the first id; where the largest logit is +inf,
+ * the ids that have it weigh 1 and the others 0.  random counts as
+ * clamped to [0, 1) (NaN: 0).  d_logprobs (may be NULL) is ln(weight / total
+ * weight of the kept ids).  A row without ids gives -1 and -inf.
+ * Every sum is one of whole numbers: the same call gives the same ids.
+ * The parameters are device arrays of `rows` entries each; NULL for
+ * temperature (1), top_k, top_p, min_p (all ids).  n <= 2^19, rows <= 2^16. */
+typedef struct nhip_sampling {
+    const float* random;
+    const float* temperature;
+    const int32_t* top_k;
+    const float* top_p;
+    const float* min_p;
+} nhip_sampling;
+/* The workspace needs no initialisation; calls that may overlap need one each. */
+size_t nhip_sample_workspace(int32_t rows, int32_t n);
+int32_t nhip_sample_dev(const float* d_logits, int32_t ldx, int32_t n, int32_t rows, const nhip_sampling* s,
+                        const uint32_t* d_mask, int32_t mask_ld, int32_t words, void* d_workspace,
+                        size_t workspace_bytes, int32_t* d_ids, float* d_logprobs, void* stream);
 /* Engine.CopyFrom (src/Needle/Engine.cs:367-379): positions [0, length) of
  * slot src into slot dst, whose length (for nhip_decoder_step) becomes
  * `length`. */

@@ -136,6 +136,22 @@ _PROTOS = {
     "nhip_paged_resize_dev": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
     "nhip_paged_free_dev": (_i32, [_vp, _i32, _vp, _vp, _sz, _vp]),
     "nhip_paged_compact_dev": (_i32, [_vp, _vp, _vp, _sz, _vp]),
+    "nhip_paged_rotary_append_dev": (_i32, [_vp, _i32, _vp, _vp, _i32, _i32, _vp, _i32, _vp, _i32, _vp, _vp, _i32, _vp,
+                                            _vp, _vp]),
+    "nhip_paged_read_dev": (_i32, [_vp, _i32, _vp, _vp, _i32, _vp, _i32, _vp, _i32, _vp]),
+    "nhip_paged_decode_sinks_workspace": (_sz, [_vp, _i32, _i32, _i32, _i32]),
+    "nhip_paged_decode_sinks_dev": (_i32, [_vp, _i32, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _i32, _i32, _vp, _sz, _vp,
+                                           _vp]),
+    "nhip_paged_prompt_sinks_workspace": (_sz, [_vp, _i32, _i32, _i32, _i32, _i32]),
+    "nhip_paged_prompt_sinks_dev": (_i32, [_vp, _i32, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _vp,
+                                           _sz, _vp, _vp]),
+    "nhip_rotary_table_dev": (_i32, [_vp, _vp, _i32, _i32, _i32, _vp, _vp]),
+    "nhip_rotary_dev": (_i32, [_vp, _vp, _i32, _i32, _i32, _vp, _i32, _vp, _i32, _vp]),
+    "nhip_add_rms_quantize_dev": (_i32, [_vp, _i32, _vp, _i32, _vp, _i32, C.c_float, _i32, _i32, _vp, _i32, _vp, _vp,
+                                         _vp]),
+    "nhip_dequantize_rows_dev": (_i32, [_vp, _vp, _i32, _i32, _vp, _i32, _vp]),
+    "nhip_sample_workspace": (_sz, [_i32, _i32]),
+    "nhip_sample_dev": (_i32, [_vp, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _vp, _sz, _vp, _vp, _vp]),
     "nhip_table_release": (_i32, [_vp, _sz, _vp]),
     "nhip_table_cached": (_i32, [_vp, _vp]),
     "nhip_matmul_batch_dev": (_i32, [_vp, _i32, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp]),

@@ -15,8 +15,10 @@
 // one workgroup: a fork of 3 rows 2.6 us, a resize 5 to 10 (entries, tables,
 // refs, then the free pages by prefix sums), a compaction's plan 6.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.hpp"
+#include "rotary.hpp"
 
 namespace nhip {
 
@@ -63,6 +65,15 @@ struct AppendParams {
     int32_t ldk, ldv, rows;
 };
 
+// The same with the rows' queries and keys rotated by position first.
+struct RotaryAppendParams : AppendParams {
+    RotaryTable r;
+    const float* q;
+    int8_t* codes;
+    float* q_scales;
+    int32_t ldq, heads;
+};
+
 // A row whose page other sequences hold too writes nothing: a resize that found
 // too few pages has not made the row's copy of it, and only the device knows.
 //
@@ -90,9 +101,36 @@ __device__ __forceinline__ float group_max(float v)
     return L == 32 ? fmaxf(v, lane_xor<16>(v)) : v;
 }
 
-template <int QK, int V>
-__global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p)
+// 16 rows of one query head, rotated and quantized, by the lanes of the append.
+template <int QK, int L>
+__device__ __forceinline__ void append_queries(const RotaryAppendParams& p, int head, int row0)
 {
+    constexpr int ROWS = 256 / L, PASSES = kAppendRows / ROWS;
+    const int l = threadIdx.x & (L - 1);
+#pragma unroll
+    for (int k = 0; k < PASSES; k++) {
+        const int row = row0 + (int)threadIdx.x / L + k * ROWS;
+        const int at = min(row, p.rows - 1), pos = p.row_pos[at];
+        const float* from = p.q + (size_t)at * p.ldq + head * QK;
+        f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (4 * l < QK && pos >= 0 && pos < p.r.positions) {
+            const size_t table = (size_t)pos * (p.r.dim / 2);
+            y = rotated4(from, l, *reinterpret_cast<const f4*>(from + 4 * l), p.r, p.r.cos + table, p.r.sin + table);
+        }
+        const float peak = group_max<L>(fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3]))));
+        const float scale = peak > 0.0f ? peak / 127.0f : 1.0f;
+        const uint32_t codes = ref_quantize4(make_float4(y[0], y[1], y[2], y[3]), 1.0f / scale);
+        if (row >= p.rows) continue;
+        const size_t to = (size_t)row * p.heads + head;
+        if (4 * l < QK) *reinterpret_cast<uint32_t*>(p.codes + to * QK + 4 * l) = codes;
+        if (l == 0) p.q_scales[to] = scale;
+    }
+}
+
+template <int QK, int V, typename Params>
+__global__ __launch_bounds__(256) void paged_append_kernel(Params p)
+{
+    constexpr bool ROTARY = std::is_same<Params, RotaryAppendParams>::value;
     constexpr int N = kAppendRows, L = V <= 64 ? 16 : 32, ROWS = 256 / L, PASSES = N / ROWS;  // rows of a pass
     __shared__ size_t cells[N];
     __shared__ int places[N], first_position;
@@ -103,6 +141,13 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p)
     // an XCD takes neighbouring groups of rows, so that the pieces of a block that two workgroups write meet in its L2
     const uint32_t id = blockIdx.y * gridDim.x + blockIdx.x, group = (id & 7) * (gridDim.x * gridDim.y / 8) + id / 8;
     const uint32_t groups = (p.rows + N - 1) / N;
+    if constexpr (ROTARY) {
+        if (group >= groups * c.kv_heads) {
+            const uint32_t head = group / groups - c.kv_heads;
+            if ((int)head < p.heads) append_queries<QK, L>(p, head, (int)(group % groups) * N);
+            return;
+        }
+    }
     if (group >= groups * c.kv_heads) return;
     const int kvh = group / groups, row0 = (int)(group - kvh * groups) * N, n = min(N, p.rows - row0);
     const int l = threadIdx.x & (L - 1), row_of_pass = threadIdx.x / L;
@@ -113,13 +158,22 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p)
         x[k][0] = x[k][1] = f4{0.0f, 0.0f, 0.0f, 0.0f};
         if (4 * l < QK) x[k][0] = *reinterpret_cast<const f4*>(p.k + r * p.ldk + kvh * QK + 4 * l);
         if (4 * l < V) x[k][1] = *reinterpret_cast<const f4*>(p.v + r * p.ldv + kvh * V + 4 * l);
+        if constexpr (ROTARY) {
+            const int pos = p.row_pos[r];
+            if (4 * l < QK && pos >= 0 && pos < p.r.positions) {
+                const size_t table = (size_t)pos * (p.r.dim / 2);
+                x[k][0] = rotated4(p.k + r * p.ldk + kvh * QK, l, x[k][0], p.r, p.r.cos + table, p.r.sin + table);
+            }
+        }
     }
     // where each row's position lives: its page's first cell (of this kv head) and its place in the page, -1 if nowhere
     int seq = -1, pos = 0, page = -1;
     if (threadIdx.x < N) {
         const int r = row0 + min((int)threadIdx.x, n - 1);
         seq = p.row_seq[r], pos = p.row_pos[r];
-        if (seq >= 0 && seq < c.sequences && pos >= 0 && (pos >> c.page_shift) < c.width)
+        bool known = pos >= 0;
+        if constexpr (ROTARY) known = known && pos < p.r.positions;
+        if (seq >= 0 && seq < c.sequences && known && (pos >> c.page_shift) < c.width)
             page = c.tables[(size_t)seq * c.width + (pos >> c.page_shift)];
     }
     float scales[PASSES][2];
@@ -204,12 +258,83 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p)
     }
 }
 
-template <int QK, int V>
-void launch_append(const AppendParams& p, hipStream_t stream)
+template <int QK, int V, typename Params>
+void launch_append(const Params& p, int heads, hipStream_t stream)
 {
-    const unsigned groups = (unsigned)(p.rows + kAppendRows - 1) / kAppendRows * p.c.kv_heads;
+    const unsigned groups = (unsigned)(p.rows + kAppendRows - 1) / kAppendRows * heads;
     const unsigned x = std::min((groups + 7) / 8 * 8, 1u << 20);  // (a multiple of 8)
-    hipLaunchKernelGGL((paged_append_kernel<QK, V>), dim3(x, (groups + x - 1) / x), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((paged_append_kernel<QK, V, Params>), dim3(x, (groups + x - 1) / x), dim3(256), 0, stream, p);
+}
+
+template <typename Params>
+int32_t launch_append(const nhip_paged_cache* c, const Params& p, int heads, hipStream_t stream)
+{
+    if (c->qk_dim == 48)
+        launch_append<48, 64>(p, heads, stream);
+    else if (c->qk_dim == 64)
+        launch_append<64, 64>(p, heads, stream);
+    else
+        launch_append<128, 128>(p, heads, stream);
+    NHIP_CHECK_HIP(hipGetLastError());
+    return NHIP_OK;
+}
+
+int32_t check_append(const nhip_paged_cache* c, const char* what, int32_t layer, int32_t rows)
+{
+    int32_t rc = paged_check(c);
+    if (rc) return rc;
+    NHIP_REQUIRE(layer >= 0 && layer < c->layers, "paged %s: layer %d of %d", what, layer, c->layers);
+    NHIP_REQUIRE(rows >= 0 && rows <= kPagedMaxRows, "paged %s: %d rows", what, rows);
+    return NHIP_OK;
+}
+
+// ------------------------------------------------------------------ read --
+
+struct ReadParams {
+    PagedLayer c;
+    const int32_t* row_seq;
+    const int32_t* row_pos;
+    float* k;
+    float* v;
+    int32_t ldk, ldv, rows;
+};
+
+// A workgroup takes 16 rows of one kv head, L lanes a row, as the append.
+template <int QK, int V>
+__global__ __launch_bounds__(256) void paged_read_kernel(ReadParams p)
+{
+    constexpr int N = kAppendRows, L = V <= 64 ? 16 : 32, ROWS = 256 / L;
+    const PagedLayer& c = p.c;
+    const int row0 = blockIdx.x * N, kvh = blockIdx.y, l = threadIdx.x & (L - 1);
+    for (int row = row0 + (int)threadIdx.x / L; row < min(row0 + N, p.rows); row += ROWS) {
+        const int seq = p.row_seq[row], pos = p.row_pos[row];
+        int page = -1;
+        if (seq >= 0 && seq < c.sequences && pos >= 0 && (pos >> c.page_shift) < c.width)
+            page = c.tables[(size_t)seq * c.width + (pos >> c.page_shift)];
+        const bool ok = page >= 0 && page < c.pages;
+        const int at = pos & ((1 << c.page_shift) - 1);
+        const size_t cell = ok ? ((size_t)page * c.kv_heads + kvh) << c.page_shift : 0;
+        if (p.k && 4 * l < QK) {
+            f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (ok) {
+                const uint32_t codes = *reinterpret_cast<const uint32_t*>(c.keys + (cell + at) * QK + 4 * l);
+                const float scale = c.kscale[cell + at];
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e] = (float)(int8_t)(codes >> (8 * e)) * scale;
+            }
+            *reinterpret_cast<f4*>(p.k + (size_t)row * p.ldk + kvh * QK + 4 * l) = y;
+        }
+        if (p.v) {
+            f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (ok) {
+                const int8_t* from = c.values + cell * V + (size_t)(at >> 4) * (16 * V) + 64 * l + (at & 15);
+                const float scale = c.vscale[cell + at];
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e] = (float)from[16 * e] * scale;
+            }
+            *reinterpret_cast<f4*>(p.v + (size_t)row * p.ldv + kvh * V + 4 * l) = y;
+        }
+    }
 }
 
 // ----------------------------------------------------------------- pages --
@@ -719,10 +844,8 @@ int32_t nhip_paged_append_dev(const nhip_paged_cache* c, int32_t layer, const fl
                               const float* d_v, int32_t ldv, const int32_t* d_row_seq, const int32_t* d_row_pos,
                               int32_t rows, void* stream)
 {
-    int32_t rc = paged_check(c);
+    int32_t rc = check_append(c, "append", layer, rows);
     if (rc) return rc;
-    NHIP_REQUIRE(layer >= 0 && layer < c->layers, "paged append: layer %d of %d", layer, c->layers);
-    NHIP_REQUIRE(rows >= 0 && rows <= kPagedMaxRows, "paged append: %d rows", rows);
     if (rows == 0) return NHIP_OK;
     NHIP_REQUIRE(d_k && d_v && d_row_seq && d_row_pos, "paged append: null pointer");
     NHIP_REQUIRE(ldk >= c->kv_heads * c->qk_dim && ldv >= c->kv_heads * c->v_dim,
@@ -730,12 +853,54 @@ int32_t nhip_paged_append_dev(const nhip_paged_cache* c, int32_t layer, const fl
     rc = ensure_device();
     if (rc) return rc;
     const AppendParams p{paged_layer(c, layer), d_k, d_v, d_row_seq, d_row_pos, c->refs, ldk, ldv, rows};
+    return launch_append(c, p, c->kv_heads, as_stream(stream));
+}
+
+int32_t nhip_paged_rotary_append_dev(const nhip_paged_cache* c, int32_t layer, const nhip_rotary* r, const float* d_q,
+                                     int32_t ldq, int32_t heads, const float* d_k, int32_t ldk, const float* d_v,
+                                     int32_t ldv, const int32_t* d_row_seq, const int32_t* d_row_pos, int32_t rows,
+                                     int8_t* d_codes, float* d_q_scales, void* stream)
+{
+    int32_t rc = check_append(c, "rotary append", layer, rows);
+    if (rc) return rc;
+    rc = rotary_check(r);
+    if (rc) return rc;
+    NHIP_REQUIRE(r->dim <= c->qk_dim, "paged rotary append: %d of %d dimensions rotated", r->dim, c->qk_dim);
+    NHIP_REQUIRE(heads >= 1 && heads <= 4096 && heads % c->kv_heads == 0,
+                 "paged rotary append: %d heads on %d kv heads (a multiple, at most 4096)", heads, c->kv_heads);
+    NHIP_REQUIRE(ldq >= heads * c->qk_dim && ldk >= c->kv_heads * c->qk_dim && ldv >= c->kv_heads * c->v_dim,
+                 "paged rotary append: row strides %d, %d, %d below a row's columns", ldq, ldk, ldv);
+    if (rows == 0) return NHIP_OK;
+    NHIP_REQUIRE(d_q && d_k && d_v && d_row_seq && d_row_pos && d_codes && d_q_scales,
+                 "paged rotary append: null pointer");
+    NHIP_REQUIRE((reinterpret_cast<uintptr_t>(d_codes) & 3) == 0, "paged rotary append: the codes are not 4-byte aligned");
+    rc = ensure_device();
+    if (rc) return rc;
+    const RotaryAppendParams p{{paged_layer(c, layer), d_k, d_v, d_row_seq, d_row_pos, c->refs, ldk, ldv, rows},
+                               rotary_table(r), d_q, d_codes, d_q_scales, ldq, heads};
+    return launch_append(c, p, c->kv_heads + heads, as_stream(stream));
+}
+
+int32_t nhip_paged_read_dev(const nhip_paged_cache* c, int32_t layer, const int32_t* d_row_seq,
+                            const int32_t* d_row_pos, int32_t rows, float* d_k, int32_t ldk, float* d_v, int32_t ldv,
+                            void* stream)
+{
+    int32_t rc = check_append(c, "read", layer, rows);
+    if (rc) return rc;
+    if (rows == 0) return NHIP_OK;
+    NHIP_REQUIRE(d_row_seq && d_row_pos && (d_k || d_v), "paged read: null pointer");
+    NHIP_REQUIRE((!d_k || ldk >= c->kv_heads * c->qk_dim) && (!d_v || ldv >= c->kv_heads * c->v_dim),
+                 "paged read: row strides %d, %d below a row's columns", ldk, ldv);
+    rc = ensure_device();
+    if (rc) return rc;
+    const ReadParams p{paged_layer(c, layer), d_row_seq, d_row_pos, d_k, d_v, ldk, ldv, rows};
+    const dim3 grid((rows + kAppendRows - 1) / kAppendRows, c->kv_heads);
     if (c->qk_dim == 48)
-        launch_append<48, 64>(p, as_stream(stream));
+        hipLaunchKernelGGL((paged_read_kernel<48, 64>), grid, dim3(256), 0, as_stream(stream), p);
     else if (c->qk_dim == 64)
-        launch_append<64, 64>(p, as_stream(stream));
+        hipLaunchKernelGGL((paged_read_kernel<64, 64>), grid, dim3(256), 0, as_stream(stream), p);
     else
-        launch_append<128, 128>(p, as_stream(stream));
+        hipLaunchKernelGGL((paged_read_kernel<128, 128>), grid, dim3(256), 0, as_stream(stream), p);
     NHIP_CHECK_HIP(hipGetLastError());
     return NHIP_OK;
 }

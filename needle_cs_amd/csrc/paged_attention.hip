@@ -150,13 +150,19 @@ struct DecodeParams {
     float* stats;  // [rows][heads][max_parts][2]: its maximum and total
     int32_t heads, group, max_count, blocks, max_parts;  // blocks: 64-position blocks of a part
     int32_t rows, rows_a_round;  // rows_a_round: of 256 workgroups, where the rows are sorted; else 0
+    int32_t sinks;
     float scale;
 };
 
-// A row's span in 64-position blocks (none when it is out of range).
+// A row's span in 64-position blocks (none when it is out of range).  With
+// sinks the blocks [block0, block1) are numbered over both parts: the first
+// `sink_blocks` hold positions below `sinks` (of this row: those before first),
+// and `skip` is what lies between them and the others.
 struct Span {
     int seq, first, end, block0, block1;
+    int sinks, sink_blocks, skip;
 };
+template <bool SINKS>
 __device__ __forceinline__ Span decode_span(const DecodeParams& p, int row)
 {
     Span s;
@@ -170,18 +176,27 @@ __device__ __forceinline__ Span decode_span(const DecodeParams& p, int row)
     s.end = s.first + count;
     s.block0 = s.first >> 6;
     s.block1 = count > 0 ? (s.end + 63) >> 6 : s.block0;
+    s.sinks = s.sink_blocks = s.skip = 0;
+    if (SINKS && count > 0) {
+        s.sinks = min(p.sinks, s.first);
+        s.sink_blocks = min((s.sinks + 63) >> 6, s.block0);
+        s.skip = s.block0 - s.sink_blocks;
+        s.block0 = 0;
+        s.block1 -= s.skip;
+    }
     return s;
 }
 
 // The row of rank `place` by blocks, most first, every other round of 256
 // workgroups the other way round, and its span; -1 past the last.  By one
 // wave, a lane a row.
+template <bool SINKS>
 __device__ __forceinline__ int ordered_row(const DecodeParams& p, int place, Span& s)
 {
     const int lane = threadIdx.x & 63, in_round = place % p.rows_a_round;
     const int rank = (place / p.rows_a_round) & 1 ? place - in_round + p.rows_a_round - 1 - in_round : place;
     if (rank >= p.rows) return -1;
-    const Span own = decode_span(p, min(lane, p.rows - 1));
+    const Span own = decode_span<SINKS>(p, min(lane, p.rows - 1));
     const int blocks = lane < p.rows ? own.block1 - own.block0 : -1;
     int least = 0, above = p.blocks + 1;  // at most `rank` rows have `above` blocks or more, more than that have `least`
     while (above - least > 1) {
@@ -200,6 +215,9 @@ __device__ __forceinline__ int ordered_row(const DecodeParams& p, int place, Spa
     s.end = __builtin_amdgcn_readlane(own.end, row);
     s.block0 = __builtin_amdgcn_readlane(own.block0, row);
     s.block1 = __builtin_amdgcn_readlane(own.block1, row);
+    s.sinks = __builtin_amdgcn_readlane(own.sinks, row);
+    s.sink_blocks = __builtin_amdgcn_readlane(own.sink_blocks, row);
+    s.skip = __builtin_amdgcn_readlane(own.skip, row);
     return row;
 }
 
@@ -222,7 +240,10 @@ __device__ __forceinline__ int ordered_row(const DecodeParams& p, int place, Spa
 //
 // Registers: the general form for dims of 128 has to stay within 168, which
 // three waves a SIMD share (32 rows of up to 32768: 276 us, 289 with 169).
-template <int QK, int V, int W, bool ONE, bool SORTED>
+//
+// SINKS: the row's blocks are its first positions' and its window's, one behind
+// the other; its own variant, so that the others keep their registers.
+template <int QK, int V, int W, bool ONE, bool SORTED, bool SINKS>
 __global__ __launch_bounds__(64 * W, QK <= 64 ? 4 : ONE || SORTED ? 2 : 3) void paged_decode_kernel(DecodeParams p)
 {
     constexpr int KH = (QK + 63) / 64, VT = V / 16;
@@ -233,13 +254,13 @@ __global__ __launch_bounds__(64 * W, QK <= 64 ? 4 : ONE || SORTED ? 2 : 3) void 
     const int h = lane & 15, g = lane >> 4;
     Span s;
     if constexpr (SORTED) {
-        const int place = blockIdx.x / c.kv_heads;
-        kvh = blockIdx.x - place * c.kv_heads;
+        const int rank = blockIdx.x / c.kv_heads;
+        kvh = blockIdx.x - rank * c.kv_heads;
         part = 0;
-        row = ordered_row(p, place, s);
+        row = ordered_row<SINKS>(p, rank, s);
         if (row < 0) return;
     } else {
-        s = decode_span(p, row);
+        s = decode_span<SINKS>(p, row);
     }
     const int total_blocks = s.block1 - s.block0;
     const int parts = (total_blocks + p.blocks - 1) / p.blocks;
@@ -260,6 +281,8 @@ __global__ __launch_bounds__(64 * W, QK <= 64 ? 4 : ONE || SORTED ? 2 : 3) void 
 
     const int32_t* table = c.tables + (size_t)s.seq * c.width;
     const int in_page = (1 << c.page_shift) - 1;
+    // block `block` of the row's numbering as a block of its positions
+    auto place = [&](int block) { return SINKS && block >= s.sink_blocks ? block + s.skip : block; };
     // the page of position `pos` of a 64-position block: -1 where it may not be followed
     auto page_at = [&](int pos) {
         const int t = pos >> c.page_shift;
@@ -296,7 +319,7 @@ __global__ __launch_bounds__(64 * W, QK <= 64 ? 4 : ONE || SORTED ? 2 : 3) void 
         const size_t cell = (((size_t)max(vpage, 0) * c.kv_heads + kvh) << c.page_shift) + (pos & in_page);
         ksr = c.kscale[cell];
         vsr = c.vscale[cell];
-        live = vpage >= 0 && pos >= s.first && pos < s.end;
+        live = vpage >= 0 && (pos >= s.first || (SINKS && pos < s.sinks)) && pos < s.end;
     };
     auto load_values = [&](int block, int vpage) {
         const int pos = 64 * block + 16 * g;
@@ -314,12 +337,12 @@ __global__ __launch_bounds__(64 * W, QK <= 64 ? 4 : ONE || SORTED ? 2 : 3) void 
     int block = s.block0 + part * p.blocks + wave;
     int kpage = -1, vpage = -1, vpage_now = -1;
     if (block < end_block) {
-        kpage = page_at(64 * block + 16 * (h >> 2));
-        vpage = page_at(64 * block + 16 * g);
-        load_keys(block, kpage, vpage);
-        load_values(block, vpage);
-        kpage = page_at(64 * (block + W) + 16 * (h >> 2));
-        vpage = page_at(64 * (block + W) + 16 * g);
+        kpage = page_at(64 * place(block) + 16 * (h >> 2));
+        vpage = page_at(64 * place(block) + 16 * g);
+        load_keys(place(block), kpage, vpage);
+        load_values(place(block), vpage);
+        kpage = page_at(64 * place(block + W) + 16 * (h >> 2));
+        vpage = page_at(64 * place(block + W) + 16 * g);
     }
     for (; block < end_block; block += W) {
         i32x4 dots[ONE ? 1 : 4];
@@ -344,11 +367,11 @@ __global__ __launch_bounds__(64 * W, QK <= 64 ? 4 : ONE || SORTED ? 2 : 3) void 
         }
         Position x = position(ksr, vsr, live);
         const bool more = block + W < end_block;
-        if (more) load_keys(block + W, kpage, vpage);
+        if (more) load_keys(place(block + W), kpage, vpage);
         vpage_now = vpage;
         if (block + 2 * W < end_block) {
-            kpage = page_at(64 * (block + 2 * W) + 16 * (h >> 2));
-            vpage = page_at(64 * (block + 2 * W) + 16 * g);
+            kpage = page_at(64 * place(block + 2 * W) + 16 * (h >> 2));
+            vpage = page_at(64 * place(block + 2 * W) + 16 * g);
         }
         // Values that are all 0 have scale 1 (QuantizeInt8), which says nothing of
         // their size: 0 in its place, so that the others keep their digits.
@@ -443,7 +466,7 @@ __global__ __launch_bounds__(64 * W, QK <= 64 ? 4 : ONE || SORTED ? 2 : 3) void 
                 o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo.v, o[t], 0, 0, 0);
             }
         }
-        if (more) load_values(block + W, vpage_now);
+        if (more) load_values(place(block + W), vpage_now);
     }
     total = rows_sum(total);
     if constexpr (ONE) {
@@ -501,7 +524,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(DecodeParams p)
 {
     __shared__ float factors[kMaxParts], quarters[4][V];
     const int row = blockIdx.x, head = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const Span s = decode_span(p, row);
+    const Span s = decode_span<true>(p, row);
     const int parts = (s.block1 - s.block0 + p.blocks - 1) / p.blocks;
     if (parts <= 1) return;
     const size_t first = ((size_t)row * p.heads + head) * p.max_parts;
@@ -564,10 +587,11 @@ struct Split {
 // 10.9 us, 15.1 with four); but four where there are 512 workgroups or more (the
 // 32 rows: 276 and 307), or rows of up to 10 blocks, where it makes no
 // difference (16 rows of 256, 8 kv heads: 4.9 both ways).
-Split decode_split(const nhip_paged_cache* c, int32_t rows, int32_t max_count)
+Split decode_split(const nhip_paged_cache* c, int32_t rows, int32_t max_count, int32_t sinks)
 {
     const int64_t units = (int64_t)rows * c->kv_heads;
-    const int most = max_count / 64 + 2;  // blocks of a row: its ends need not be a block's
+    // blocks of a row: its ends need not be a block's, and its sinks have some of their own
+    const int most = max_count / 64 + 2 + (std::min(sinks, c->width * c->page_size) + 63) / 64;
     Split s;
     if (most <= 18 || (most <= 40 && units >= 128)) {
         s.blocks = most;
@@ -603,8 +627,12 @@ int32_t launch_decode(const DecodeParams& p, const Split& s, int32_t rows, hipSt
         if (set == hipSuccess) hipLaunchKernelGGL(kernel, grid, dim3(64 * s.waves), lds, stream, p);
     };
     auto choose = [&](auto one, auto sorted) {
-        launch(s.waves == 4 ? paged_decode_kernel<QK, V, 4, one(), sorted()>
-                            : paged_decode_kernel<QK, V, 8, one(), sorted()>);
+        if (p.sinks)
+            launch(s.waves == 4 ? paged_decode_kernel<QK, V, 4, one(), sorted(), true>
+                                : paged_decode_kernel<QK, V, 8, one(), sorted(), true>);
+        else
+            launch(s.waves == 4 ? paged_decode_kernel<QK, V, 4, one(), sorted(), false>
+                                : paged_decode_kernel<QK, V, 8, one(), sorted(), false>);
     };
     const std::true_type yes;
     const std::false_type no;
@@ -677,6 +705,7 @@ struct PromptParams {
     int32_t places;  // of tiles that the grid holds
     uint32_t group_part;  // 2^31 / group, rounded up
     int32_t tiles_a_round;  // of 256 workgroups, where the tiles are sorted; else 0
+    int32_t sinks;  // with a window
     float scale;
 };
 
@@ -730,16 +759,26 @@ __device__ __forceinline__ RunPositions run_positions(const PromptParams& p, int
 }
 
 // The 64-position tiles [begin, end) that a tile of queries at positions
-// first .. last attends, and the parts that they are cut into.
+// first .. last attends, and the parts that they are cut into.  With sinks they
+// are numbered from 0 over both parts of what it attends, as a decode row's
+// blocks: sink_tiles of them, then those from sink_tiles + skip on.
 struct TileSpan {
-    int from, begin, end, parts;
+    int from, begin, end, parts, sink_tiles, skip;
 };
+template <bool SINKS>
 __device__ __forceinline__ TileSpan tile_span(const PromptParams& p, int first, int last)
 {
     TileSpan s;
     s.from = p.window > 0 ? max(first - p.window + 1, 0) : 0;
     s.begin = s.from >> 6;
     s.end = last >= 0 ? (last >> 6) + 1 : s.begin;
+    s.sink_tiles = s.skip = 0;
+    if (SINKS && p.sinks > 0 && last >= 0) {
+        s.sink_tiles = min((min(p.sinks, s.from) + 63) >> 6, s.begin);
+        s.skip = s.begin - s.sink_tiles;
+        s.begin = 0;
+        s.end -= s.skip;
+    }
     s.parts = (s.end - s.begin + p.blocks - 1) / p.blocks;
     return s;
 }
@@ -869,7 +908,9 @@ __device__ __forceinline__ int32_t scalar_load(const int32_t* a, int64_t i)
 
 #define NHIP_INLINE __attribute__((always_inline))
 
-template <int QK, int V>
+// SINKS: as the decode kernel's.  A tile's rows begin to attend at different
+// positions, and every one of them attends the sinks.
+template <int QK, int V, bool SINKS>
 __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(PromptParams p)
 {
     constexpr int KS = QK <= 64 ? 64 : 128;  // bytes of a key row in LDS
@@ -924,7 +965,7 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
                                          : -1;
     const int first_pos = __builtin_amdgcn_readfirstlane(at.at(p, q0));
     const int last_pos = __builtin_amdgcn_readfirstlane(at.at(p, q0 + qn - 1));
-    const TileSpan span = tile_span(p, first_pos, last_pos);
+    const TileSpan span = tile_span<SINKS>(p, first_pos, last_pos);
     const int from = span.from, parts = span.parts;
     const int from_window = p.window > 0 ? p.window - 1 : 1 << 30;  // positions before its own that a row attends
     if (part > 0 && part >= parts) return;
@@ -940,12 +981,16 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
     auto key_swizzle = [](int pos) { return KS == 64 ? (pos >> 2) & 3 : (pos >> 1) & 7; };
     auto value_swizzle = [](int dim) { return (dim >> 1) & 7; };
     const int32_t* table = c.tables + (size_t)max(seq, 0) * c.width;
+    // the first position of tile `tile` of the span's numbering
+    auto start = [&](int tile) NHIP_INLINE {
+        return 64 * (SINKS && tile >= span.sink_tiles ? tile + span.skip : tile);
+    };
     auto look_up = [&](int tile) NHIP_INLINE {
-        return scalar_load(table, min((64 * tile + 16 * wave) >> c.page_shift, c.width - 1));
+        return scalar_load(table, min((start(tile) + 16 * wave) >> c.page_shift, c.width - 1));
     };
     auto cell = [&](int tile, int page) NHIP_INLINE {
         const int pg = page >= 0 && page < c.pages ? page : 0;
-        return (((size_t)pg * c.kv_heads + kvh) << c.page_shift) + ((64 * tile + 16 * wave) & in_page);
+        return (((size_t)pg * c.kv_heads + kvh) << c.page_shift) + ((start(tile) + 16 * wave) & in_page);
     };
     i32x4 kr[KU], vr[VU];
     float scale_r;
@@ -970,10 +1015,15 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
             if (k_does)
                 *reinterpret_cast<i32x4*>(lds_k[tile & 1] + pos * KS + 16 * (k_ch ^ key_swizzle(pos))) = kr[u];
         }
-        // the positions that count, [lo, hi) of the block
-        const int lo = from - 64 * tile - 16 * wave, hi = last_pos + 1 - 64 * tile - 16 * wave;
+        // the positions that count, [lo, hi) of the block and with sinks those before `sunk`
+        const int lo = from - start(tile) - 16 * wave, hi = last_pos + 1 - start(tile) - 16 * wave;
         uint32_t live = page >= 0 && page < c.pages ? 0xFFFFu : 0;
-        live &= lo >= 16 ? 0 : 0xFFFFu << max(lo, 0);
+        uint32_t counts = lo >= 16 ? 0 : 0xFFFFu << max(lo, 0);
+        if constexpr (SINKS) {
+            const int sunk = p.sinks - start(tile) - 16 * wave;
+            counts |= sunk <= 0 ? 0 : 0xFFFFu >> (16 - min(sunk, 16));
+        }
+        live &= counts;
         live &= hi <= 0 ? 0 : 0xFFFFu >> (16 - min(hi, 16));
         // A value scale that is no finite number spoils the rows that attend
         // its position, and no others: their score becomes NaN, the scale 0.
@@ -1026,7 +1076,9 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
             load_keys(clamped(tile + 1), page);
             load_values(clamped(tile + 1), page);
             page_next = look_up(clamped(tile + 2));
-            if ((64 * tile <= wave_last) & (64 * tile + 63 >= wave_first - from_window)) {
+            const int tile_pos = start(tile);
+            if ((tile_pos <= wave_last) &
+                ((tile_pos + 63 >= wave_first - from_window) | (SINKS && tile_pos < p.sinks))) {
                 const uint8_t* kb = lds_k[tile & 1] + key_row * KS;
                 i32x16 s[2];
 #pragma unroll
@@ -1057,17 +1109,19 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
                 }
                 const bool whole = __builtin_amdgcn_readfirstlane(counted.x & counted.y) == ~0u;
                 const float largest = fmaxf(vs[0], vs[1]);  // of the lane's two positions
-                const bool masked = !whole | (64 * tile + 63 > wave_first) | (64 * tile < wave_last - from_window);
+                const bool masked = !whole | (tile_pos + 63 > wave_first) | (tile_pos < wave_last - from_window);
                 if (masked) {
-                    const int last = q_pos - 64 * tile - 8 * g, first = q_first - 64 * tile - 8 * g;
+                    const int last = q_pos - tile_pos - 8 * g, first = q_first - tile_pos - 8 * g;
+                    const int sunk = SINKS ? p.sinks - tile_pos - 8 * g : 0;
 #pragma unroll
                     for (int t = 0; t < 2; t++) {
                         const uint32_t bits = (t ? counted.y : counted.x) >> (8 * g);
 #pragma unroll
                         for (int r = 0; r < 16; r++) {
                             const int at = 16 * (r / 8) + r % 8;
-                            const bool attends =
-                                (32 * t + at <= last) & (32 * t + at >= first) & ((bits >> at) & 1);
+                            const bool attends = (32 * t + at <= last) &
+                                                 ((32 * t + at >= first) | (SINKS && 32 * t + at < sunk)) &
+                                                 ((bits >> at) & 1);
                             z[t][r] = attends ? z[t][r] : -INFINITY;
                         }
                     }
@@ -1240,7 +1294,7 @@ __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PromptParams p)
     const int tile = ((row - r.row0) * p.group + of_group) / kTileQueries;
     if (__builtin_amdgcn_readfirstlane(tiles_before) + tiles - 1 - tile >= p.places) return;
     const int q0 = tile * kTileQueries;
-    const int parts = tile_span(p, at.at(p, q0), at.at(p, min(q0 + kTileQueries, queries) - 1)).parts;
+    const int parts = tile_span<true>(p, at.at(p, q0), at.at(p, min(q0 + kTileQueries, queries) - 1)).parts;
     if (parts <= 1) return;
     const size_t q_at = (size_t)row * p.heads + head;
     const size_t first = q_at * p.max_parts;
@@ -1325,7 +1379,7 @@ struct PromptSplit {
 // A window bounds a tile's blocks; it never makes more parts, as the workspace
 // is sized without it.
 PromptSplit prompt_split(const nhip_paged_cache* c, int32_t rows, int32_t heads, int32_t runs, int32_t max_count,
-                         int32_t window)
+                         int32_t window, int32_t sinks)
 {
     const int group = heads / c->kv_heads;
     PromptSplit s;
@@ -1338,7 +1392,7 @@ PromptSplit prompt_split(const nhip_paged_cache* c, int32_t rows, int32_t heads,
             most, std::max<int64_t>({2, (units * most + 767) / 768, (most + kMaxParts - 1) / kMaxParts}));
     s.parts = (most + s.blocks - 1) / s.blocks;
     if (window > 0 && window < max_count) {
-        most = std::min<int64_t>(most, ((int64_t)window + kTileQueries / group) / 64 + 2);
+        most = std::min<int64_t>(most, ((int64_t)window + kTileQueries / group) / 64 + 2 + ((int64_t)sinks + 63) / 64);
         s.blocks = std::max(2, (most + s.parts - 1) / s.parts);
         s.parts = (most + s.blocks - 1) / s.blocks;
     }
@@ -1359,7 +1413,8 @@ size_t prompt_workspace(const nhip_paged_cache* c, int32_t rows, int32_t heads, 
 template <int QK, int V>
 int32_t launch_prompt(const PromptParams& p, const PromptSplit& s, hipStream_t stream)
 {
-    hipLaunchKernelGGL((paged_prompt_kernel<QK, V>), dim3(s.tiles * p.c.kv_heads, s.parts), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((p.sinks ? paged_prompt_kernel<QK, V, true> : paged_prompt_kernel<QK, V, false>),
+                       dim3(s.tiles * p.c.kv_heads, s.parts), dim3(256), 0, stream, p);
     NHIP_CHECK_HIP(hipGetLastError());
     if (s.parts > 1) {
         hipLaunchKernelGGL((paged_prompt_join_kernel<V>), dim3(p.rows, (p.heads + 3) / 4), dim3(256), 0, stream, p);
@@ -1373,23 +1428,24 @@ int32_t launch_prompt(const PromptParams& p, const PromptSplit& s, hipStream_t s
 
 using namespace nhip;
 
-extern "C" {
+namespace {
 
-size_t nhip_paged_decode_workspace(const nhip_paged_cache* c, int32_t rows, int32_t heads, int32_t max_count)
+int32_t check_sinks(int32_t sinks)
 {
-    if (check_attention(c, rows, heads, max_count)) return 0;
-    return decode_workspace(c, rows, heads, decode_split(c, rows, max_count));
+    NHIP_REQUIRE(sinks >= 0, "paged attention: %d sinks", sinks);
+    return NHIP_OK;
 }
 
-int32_t nhip_paged_decode_dev(const nhip_paged_cache* c, int32_t layer, const int8_t* d_q, const float* d_q_scales,
-                              int32_t rows, int32_t heads, const int32_t* d_row_seq, const int32_t* d_row_first,
-                              const int32_t* d_row_count, int32_t max_count, void* d_workspace,
-                              size_t workspace_bytes, float* d_out, void* stream)
+int32_t decode(const nhip_paged_cache* c, int32_t layer, const int8_t* d_q, const float* d_q_scales, int32_t rows,
+               int32_t heads, const int32_t* d_row_seq, const int32_t* d_row_first, const int32_t* d_row_count,
+               int32_t sinks, int32_t max_count, void* d_workspace, size_t workspace_bytes, float* d_out, void* stream)
 {
     int32_t rc = check_attention(c, rows, heads, max_count);
     if (rc) return rc;
+    rc = check_sinks(sinks);
+    if (rc) return rc;
     if (rows == 0) return NHIP_OK;
-    const Split split = decode_split(c, rows, max_count);
+    const Split split = decode_split(c, rows, max_count, sinks);
     rc = check_call(c, layer, d_q, d_q_scales, d_out, d_workspace, workspace_bytes,
                     decode_workspace(c, rows, heads, split));
     if (rc) return rc;
@@ -1413,30 +1469,26 @@ int32_t nhip_paged_decode_dev(const nhip_paged_cache* c, int32_t layer, const in
     p.max_parts = split.parts;
     p.rows = rows;
     p.rows_a_round = split.rows_a_round;
+    p.sinks = sinks;
     p.scale = score_scale(c->qk_dim);
     if (c->qk_dim == 48) return launch_decode<48, 64>(p, split, rows, as_stream(stream));
     if (c->qk_dim == 64) return launch_decode<64, 64>(p, split, rows, as_stream(stream));
     return launch_decode<128, 128>(p, split, rows, as_stream(stream));
 }
 
-size_t nhip_paged_prompt_workspace(const nhip_paged_cache* c, int32_t rows, int32_t heads, int32_t runs,
-                                   int32_t max_count)
-{
-    if (check_attention(c, rows, heads, max_count) || check_runs(runs, 0)) return 0;
-    return prompt_workspace(c, rows, heads, prompt_split(c, rows, heads, runs, max_count, 0));
-}
-
-int32_t nhip_paged_prompt_dev(const nhip_paged_cache* c, int32_t layer, const int8_t* d_q, const float* d_q_scales,
-                              int32_t rows, int32_t heads, int32_t runs, const int32_t* d_run_rows,
-                              const int32_t* d_run_seq, const int32_t* d_run_pos, int32_t window, int32_t max_count,
-                              void* d_workspace, size_t workspace_bytes, float* d_out, void* stream)
+int32_t prompt(const nhip_paged_cache* c, int32_t layer, const int8_t* d_q, const float* d_q_scales, int32_t rows,
+               int32_t heads, int32_t runs, const int32_t* d_run_rows, const int32_t* d_run_seq,
+               const int32_t* d_run_pos, int32_t window, int32_t sinks, int32_t max_count, void* d_workspace,
+               size_t workspace_bytes, float* d_out, void* stream)
 {
     int32_t rc = check_attention(c, rows, heads, max_count);
     if (rc) return rc;
     rc = check_runs(runs, window);
     if (rc) return rc;
+    rc = check_sinks(sinks);
+    if (rc) return rc;
     if (rows == 0 || runs == 0) return NHIP_OK;
-    const PromptSplit split = prompt_split(c, rows, heads, runs, max_count, window);
+    const PromptSplit split = prompt_split(c, rows, heads, runs, max_count, window, sinks);
     NHIP_REQUIRE(split.tiles * c->kv_heads <= (1 << 23), "paged prompt: %d rows in %d runs of %d kv heads are too many",
                  rows, runs, c->kv_heads);
     rc = check_call(c, layer, d_q, d_q_scales, d_out, d_workspace, workspace_bytes,
@@ -1466,10 +1518,79 @@ int32_t nhip_paged_prompt_dev(const nhip_paged_cache* c, int32_t layer, const in
     p.places = (int32_t)split.tiles;
     p.group_part = (uint32_t)(((1u << 31) + p.group - 1) / p.group);
     p.tiles_a_round = split.tiles_a_round;
+    p.sinks = window > 0 ? sinks : 0;
     p.scale = score_scale(c->qk_dim);
     if (c->qk_dim == 48) return launch_prompt<48, 64>(p, split, as_stream(stream));
     if (c->qk_dim == 64) return launch_prompt<64, 64>(p, split, as_stream(stream));
     return launch_prompt<128, 128>(p, split, as_stream(stream));
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t nhip_paged_decode_workspace(const nhip_paged_cache* c, int32_t rows, int32_t heads, int32_t max_count)
+{
+    return nhip_paged_decode_sinks_workspace(c, rows, heads, 0, max_count);
+}
+
+int32_t nhip_paged_decode_dev(const nhip_paged_cache* c, int32_t layer, const int8_t* d_q, const float* d_q_scales,
+                              int32_t rows, int32_t heads, const int32_t* d_row_seq, const int32_t* d_row_first,
+                              const int32_t* d_row_count, int32_t max_count, void* d_workspace,
+                              size_t workspace_bytes, float* d_out, void* stream)
+{
+    return decode(c, layer, d_q, d_q_scales, rows, heads, d_row_seq, d_row_first, d_row_count, 0, max_count,
+                  d_workspace, workspace_bytes, d_out, stream);
+}
+
+size_t nhip_paged_decode_sinks_workspace(const nhip_paged_cache* c, int32_t rows, int32_t heads, int32_t sinks,
+                                         int32_t max_count)
+{
+    if (check_attention(c, rows, heads, max_count) || check_sinks(sinks)) return 0;
+    return decode_workspace(c, rows, heads, decode_split(c, rows, max_count, sinks));
+}
+
+int32_t nhip_paged_decode_sinks_dev(const nhip_paged_cache* c, int32_t layer, const int8_t* d_q,
+                                    const float* d_q_scales, int32_t rows, int32_t heads, const int32_t* d_row_seq,
+                                    const int32_t* d_row_first, const int32_t* d_row_count, int32_t sinks,
+                                    int32_t max_count, void* d_workspace, size_t workspace_bytes, float* d_out,
+                                    void* stream)
+{
+    return decode(c, layer, d_q, d_q_scales, rows, heads, d_row_seq, d_row_first, d_row_count, sinks, max_count,
+                  d_workspace, workspace_bytes, d_out, stream);
+}
+
+size_t nhip_paged_prompt_workspace(const nhip_paged_cache* c, int32_t rows, int32_t heads, int32_t runs,
+                                   int32_t max_count)
+{
+    return nhip_paged_prompt_sinks_workspace(c, rows, heads, runs, 0, max_count);
+}
+
+int32_t nhip_paged_prompt_dev(const nhip_paged_cache* c, int32_t layer, const int8_t* d_q, const float* d_q_scales,
+                              int32_t rows, int32_t heads, int32_t runs, const int32_t* d_run_rows,
+                              const int32_t* d_run_seq, const int32_t* d_run_pos, int32_t window, int32_t max_count,
+                              void* d_workspace, size_t workspace_bytes, float* d_out, void* stream)
+{
+    return prompt(c, layer, d_q, d_q_scales, rows, heads, runs, d_run_rows, d_run_seq, d_run_pos, window, 0, max_count,
+                  d_workspace, workspace_bytes, d_out, stream);
+}
+
+// (A call's parts are counted as if nothing bounded its rows' positions, so neither window nor sinks need more.)
+size_t nhip_paged_prompt_sinks_workspace(const nhip_paged_cache* c, int32_t rows, int32_t heads, int32_t runs,
+                                         int32_t sinks, int32_t max_count)
+{
+    if (check_attention(c, rows, heads, max_count) || check_runs(runs, 0) || check_sinks(sinks)) return 0;
+    return prompt_workspace(c, rows, heads, prompt_split(c, rows, heads, runs, max_count, 0, 0));
+}
+
+int32_t nhip_paged_prompt_sinks_dev(const nhip_paged_cache* c, int32_t layer, const int8_t* d_q,
+                                    const float* d_q_scales, int32_t rows, int32_t heads, int32_t runs,
+                                    const int32_t* d_run_rows, const int32_t* d_run_seq, const int32_t* d_run_pos,
+                                    int32_t window, int32_t sinks, int32_t max_count, void* d_workspace,
+                                    size_t workspace_bytes, float* d_out, void* stream)
+{
+    return prompt(c, layer, d_q, d_q_scales, rows, heads, runs, d_run_rows, d_run_seq, d_run_pos, window, sinks,
+                  max_count, d_workspace, workspace_bytes, d_out, stream);
 }
 
 }  // extern "C"

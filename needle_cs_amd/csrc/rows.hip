@@ -1,0 +1,296 @@
+// rows.hip -- row operations between a layer's int8 products on gfx950: the
+// residual's addition with the root-mean-square norm and QuantizeInt8, and
+// rows of codes back to numbers.
+#include <algorithm>
+
+#include "common.hpp"
+
+namespace nhip {
+namespace {
+
+constexpr int32_t kMaxRows = 1 << 26, kMaxCols = 1 << 20;
+constexpr int kMaxGroups = 1 << 20;  // workgroups of a launch; they take the further rows in turn
+
+typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32_bytes __attribute__((aligned(1)));
+
+// Elements i .. i + 3 of a row of n, 0 past its end.
+__device__ __forceinline__ float4 load4(const float* row, int i, int n)
+{
+    if (i + 4 <= n) {
+        const f4 v = *reinterpret_cast<const f4*>(row + i);
+        return make_float4(v[0], v[1], v[2], v[3]);
+    }
+    return make_float4(i < n ? row[i] : 0.0f, i + 1 < n ? row[i + 1] : 0.0f, i + 2 < n ? row[i + 2] : 0.0f, 0.0f);
+}
+__device__ __forceinline__ void store4(float* row, int i, int n, float4 v)
+{
+    if (i + 4 <= n) {
+        *reinterpret_cast<f4*>(row + i) = f4{v.x, v.y, v.z, v.w};
+        return;
+    }
+    if (i < n) row[i] = v.x;
+    if (i + 1 < n) row[i + 1] = v.y;
+    if (i + 2 < n) row[i + 2] = v.z;
+}
+__device__ __forceinline__ void store_codes4(int8_t* row, int i, int n, uint32_t codes)
+{
+    if (i + 4 <= n) {
+        *reinterpret_cast<u32_bytes*>(row + i) = codes;
+        return;
+    }
+    for (int e = 0; e < 3 && i + e < n; e++) row[i + e] = (int8_t)(codes >> (8 * e));
+}
+
+struct NormParams {
+    const float* x;
+    const float* delta;
+    const float* gain;
+    float* sum;
+    int8_t* q;
+    float* scales;
+    int32_t ldx, ldd, lds, rows, cols, zero_centered;
+    float eps;
+};
+
+__device__ __forceinline__ float4 gain4(const NormParams& p, int i)
+{
+    if (!p.gain) return make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+    float4 g = load4(p.gain, i, p.cols);
+    if (p.zero_centered) g = make_float4(1.0f + g.x, 1.0f + g.y, 1.0f + g.z, 1.0f + g.w);
+    return g;
+}
+
+__device__ __forceinline__ float4 sum4(const NormParams& p, size_t row, int i)
+{
+    float4 v = load4(p.x + row * p.ldx, i, p.cols);
+    if (p.delta) {
+        const float4 d = load4(p.delta + row * p.ldd, i, p.cols);
+        v = make_float4(v.x + d.x, v.y + d.y, v.z + d.z, v.w + d.w);
+    }
+    return v;
+}
+
+__device__ __forceinline__ double squares4(float4 v, double s)
+{
+    s = fma((double)v.x, (double)v.x, s);
+    s = fma((double)v.y, (double)v.y, s);
+    s = fma((double)v.z, (double)v.z, s);
+    return fma((double)v.w, (double)v.w, s);
+}
+
+__device__ __forceinline__ float4 normed4(float4 v, float r, float4 g)
+{
+    return make_float4((v.x * r) * g.x, (v.y * r) * g.y, (v.z * r) * g.z, (v.w * r) * g.w);
+}
+
+__device__ __forceinline__ float peak4(float m, float4 v)
+{
+    return fmaxf(fmaxf(m, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+}
+
+// The sum and the maximum over the T threads of a row, in every thread.  (A
+// row's two uses alternate, each behind a barrier of its own.)
+template <int T>
+__device__ __forceinline__ double row_sum(double v, double* lds)
+{
+    for (int off = 32; off; off >>= 1) v += __shfl_xor(v, off);
+    if constexpr (T > 64) {
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0.0;
+        for (int w = 0; w < T / 64; w++) v += lds[w];
+    }
+    return v;
+}
+template <int T>
+__device__ __forceinline__ float row_max(float v, float* lds)
+{
+    v = wave_max(v);
+    if constexpr (T > 64) {
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = lds[0];
+        for (int w = 1; w < T / 64; w++) v = fmaxf(v, lds[w]);
+    }
+    return v;
+}
+
+__device__ __forceinline__ float inverse_rms(const NormParams& p, double squares)
+{
+    return (float)(1.0 / sqrt(squares / (double)p.cols + (double)p.eps));
+}
+
+// T threads a row, which they hold in registers, G groups of four elements
+// each (HELD), or read again for each of the three passes.  A held row is
+// read once and written once.
+template <int T, int G, bool HELD>
+__global__ __launch_bounds__(T < 256 ? 256 : T) void add_rms_quantize_kernel(NormParams p)
+{
+    constexpr int WG = T < 256 ? 256 : T;
+    __shared__ double sums[WG / 64];
+    __shared__ float peaks[WG / 64];
+    const int t = threadIdx.x % T;
+    for (size_t row = (size_t)blockIdx.x * (WG / T) + threadIdx.x / T; row < (size_t)p.rows;
+         row += (size_t)gridDim.x * (WG / T)) {
+        float4 v[G];
+        double squares = 0.0;
+        const int passes = HELD ? G : (p.cols + 4 * T - 1) / (4 * T);
+        if constexpr (HELD) {
+#pragma unroll
+            for (int j = 0; j < G; j++) v[j] = sum4(p, row, 4 * (t + T * j));
+#pragma unroll
+            for (int j = 0; j < G; j++) squares = squares4(v[j], squares);
+        }
+        if (p.sum || !HELD) {
+#pragma unroll
+            for (int j = 0; j < passes; j++) {
+                const int i = 4 * (t + T * j);
+                float4 s;
+                if constexpr (HELD) {
+                    s = v[j];
+                } else {
+                    s = sum4(p, row, i);
+                    squares = squares4(s, squares);
+                }
+                if (p.sum) store4(p.sum + row * p.lds, i, p.cols, s);
+            }
+        }
+        const float r = inverse_rms(p, row_sum<T>(squares, sums));
+        // (a row that is not held comes back from the sums, where they are kept: x may be the same memory)
+        auto again = [&](int i) {
+            return normed4(p.sum ? load4(p.sum + row * p.lds, i, p.cols) : sum4(p, row, i), r, gain4(p, i));
+        };
+        float peak = 0.0f;
+#pragma unroll
+        for (int j = 0; j < passes; j++) {
+            const int i = 4 * (t + T * j);
+            if constexpr (HELD) {
+                v[j] = normed4(v[j], r, gain4(p, i));
+                peak = peak4(peak, v[j]);
+            } else {
+                peak = peak4(peak, again(i));
+            }
+        }
+        peak = row_max<T>(peak, peaks);
+        const float scale = peak > 0.0f ? peak / 127.0f : 1.0f;
+        const float inverse = 1.0f / scale;
+#pragma unroll
+        for (int j = 0; j < passes; j++) {
+            const int i = 4 * (t + T * j);
+            float4 h;
+            if constexpr (HELD)
+                h = v[j];
+            else
+                h = again(i);
+            store_codes4(p.q + row * p.cols, i, p.cols, ref_quantize4(h, inverse));
+        }
+        if (t == 0) p.scales[row] = scale;
+    }
+}
+
+template <int T, int G, bool HELD>
+void launch_norm(const NormParams& p, hipStream_t stream)
+{
+    constexpr int WG = T < 256 ? 256 : T, ROWS = WG / T;
+    hipLaunchKernelGGL((add_rms_quantize_kernel<T, G, HELD>), dim3(std::min((p.rows + ROWS - 1) / ROWS, kMaxGroups)),
+                       dim3(WG), 0, stream, p);
+}
+
+// L lanes a row.
+template <int L>
+__global__ __launch_bounds__(256) void dequantize_rows_kernel(const int8_t* q, const float* scales, int rows, int cols,
+                                                             float* x, int ldx)
+{
+    const int l = threadIdx.x % L;
+    for (size_t row = (size_t)blockIdx.x * (256 / L) + threadIdx.x / L; row < (size_t)rows;
+         row += (size_t)gridDim.x * (256 / L)) {
+        const float scale = scales[row];
+        const int8_t* from = q + row * cols;
+        for (int i = 4 * l; i < cols; i += 4 * L) {
+            uint32_t c = 0;
+            if (i + 4 <= cols)
+                c = *reinterpret_cast<const u32_bytes*>(from + i);
+            else
+                for (int e = 0; i + e < cols; e++) c |= (uint32_t)(uint8_t)from[i + e] << (8 * e);
+            store4(x + row * ldx, i, cols,
+                   make_float4((float)(int8_t)c * scale, (float)(int8_t)(c >> 8) * scale,
+                               (float)(int8_t)(c >> 16) * scale, (float)(int8_t)(c >> 24) * scale));
+        }
+    }
+}
+
+template <int L>
+void launch_dequantize(const int8_t* q, const float* scales, int rows, int cols, float* x, int ldx, hipStream_t stream)
+{
+    hipLaunchKernelGGL((dequantize_rows_kernel<L>), dim3(std::min((rows + 256 / L - 1) / (256 / L), kMaxGroups)),
+                       dim3(256), 0, stream, q, scales, rows, cols, x, ldx);
+}
+
+int32_t check_rows(const char* what, int32_t rows, int32_t cols)
+{
+    NHIP_REQUIRE(rows >= 0 && rows <= kMaxRows && cols >= 1 && cols <= kMaxCols, "%s: %d rows of %d out of range", what,
+                 rows, cols);
+    return NHIP_OK;
+}
+
+}  // namespace
+}  // namespace nhip
+
+using namespace nhip;
+
+extern "C" {
+
+int32_t nhip_add_rms_quantize_dev(const float* d_x, int32_t ldx, const float* d_delta, int32_t ldd,
+                                  const float* d_gain, int32_t zero_centered, float eps, int32_t rows, int32_t cols,
+                                  float* d_sum, int32_t ld_sum, int8_t* d_q, float* d_scales, void* stream)
+{
+    int32_t rc = check_rows("add_rms_quantize", rows, cols);
+    if (rc) return rc;
+    NHIP_REQUIRE(ldx >= cols && (!d_delta || ldd >= cols) && (!d_sum || ld_sum >= cols),
+                 "add_rms_quantize: strides %d, %d, %d are less than %d columns", ldx, ldd, ld_sum, cols);
+    NHIP_REQUIRE(eps > 0.0f && eps <= 1.0f, "add_rms_quantize: eps %g is not in (0, 1]", (double)eps);
+    NHIP_REQUIRE(zero_centered == 0 || zero_centered == 1, "add_rms_quantize: zero_centered %d", zero_centered);
+    if (rows == 0) return NHIP_OK;
+    NHIP_REQUIRE(d_x && d_q && d_scales, "add_rms_quantize: null pointer");
+    NHIP_REQUIRE((d_sum != d_x || ld_sum == ldx) && (!d_sum || d_sum != d_delta || ld_sum == ldd),
+                 "add_rms_quantize: sums in place have their rows' stride");
+    rc = ensure_device();
+    if (rc) return rc;
+    const NormParams p = {d_x,      d_delta, d_gain, d_sum, d_q,  d_scales, ldx,
+                          ldd, ld_sum,  rows,   cols,  zero_centered, eps};
+    hipStream_t s = as_stream(stream);
+    if (cols <= 1024)
+        launch_norm<64, 4, true>(p, s);
+    else if (cols <= 4096)
+        launch_norm<256, 4, true>(p, s);
+    else if (cols <= 16384)
+        launch_norm<1024, 4, true>(p, s);
+    else
+        launch_norm<1024, 1, false>(p, s);
+    NHIP_CHECK_HIP(hipGetLastError());
+    return NHIP_OK;
+}
+
+int32_t nhip_dequantize_rows_dev(const int8_t* d_q, const float* d_scales, int32_t rows, int32_t cols, float* d_x,
+                                 int32_t ldx, void* stream)
+{
+    int32_t rc = check_rows("dequantize_rows", rows, cols);
+    if (rc) return rc;
+    NHIP_REQUIRE(ldx >= cols, "dequantize_rows: stride %d is less than %d columns", ldx, cols);
+    if (rows == 0) return NHIP_OK;
+    NHIP_REQUIRE(d_q && d_scales && d_x, "dequantize_rows: null pointer");
+    rc = ensure_device();
+    if (rc) return rc;
+    hipStream_t s = as_stream(stream);
+    if (cols <= 64)
+        launch_dequantize<16>(d_q, d_scales, rows, cols, d_x, ldx, s);
+    else if (cols <= 128)
+        launch_dequantize<32>(d_q, d_scales, rows, cols, d_x, ldx, s);
+    else
+        launch_dequantize<256>(d_q, d_scales, rows, cols, d_x, ldx, s);
+    NHIP_CHECK_HIP(hipGetLastError());
+    return NHIP_OK;
+}
+
+}  // extern "C"

@@ -50,6 +50,15 @@ class PagedCache:
     def append(self, layer: int, k, ldk: int, v, ldv: int, row_seq, row_pos, rows: int, stream=None) -> None:
         check(lib().nhip_paged_append_dev(self.ptr, layer, k, ldk, v, ldv, row_seq, row_pos, rows, stream))
 
+    def rotary_append(self, layer: int, rotary, q, ldq: int, heads: int, k, ldk: int, v, ldv: int, row_seq, row_pos,
+                      rows: int, codes, q_scales, stream=None) -> None:
+        """`rotary`: a ``needle_cs_amd.rotary.Rotary``."""
+        check(lib().nhip_paged_rotary_append_dev(self.ptr, layer, rotary.ptr, q, ldq, heads, k, ldk, v, ldv, row_seq,
+                                                 row_pos, rows, codes, q_scales, stream))
+
+    def read(self, layer: int, row_seq, row_pos, rows: int, k, ldk: int, v, ldv: int, stream=None) -> None:
+        check(lib().nhip_paged_read_dev(self.ptr, layer, row_seq, row_pos, rows, k, ldk, v, ldv, stream))
+
     def decode_workspace(self, rows: int, heads: int, max_count: int) -> int:
         return lib().nhip_paged_decode_workspace(self.ptr, rows, heads, max_count)
 
@@ -65,6 +74,24 @@ class PagedCache:
                window: int, max_count: int, workspace, workspace_bytes: int, out, stream=None) -> None:
         check(lib().nhip_paged_prompt_dev(self.ptr, layer, q, q_scales, rows, heads, runs, run_rows, run_seq, run_pos,
                                           window, max_count, workspace, workspace_bytes, out, stream))
+
+    def decode_sinks_workspace(self, rows: int, heads: int, sinks: int, max_count: int) -> int:
+        return lib().nhip_paged_decode_sinks_workspace(self.ptr, rows, heads, sinks, max_count)
+
+    def decode_sinks(self, layer: int, q, q_scales, rows: int, heads: int, row_seq, row_first, row_count, sinks: int,
+                     max_count: int, workspace, workspace_bytes: int, out, stream=None) -> None:
+        check(lib().nhip_paged_decode_sinks_dev(self.ptr, layer, q, q_scales, rows, heads, row_seq, row_first,
+                                                row_count, sinks, max_count, workspace, workspace_bytes, out, stream))
+
+    def prompt_sinks_workspace(self, rows: int, heads: int, runs: int, sinks: int, max_count: int) -> int:
+        return lib().nhip_paged_prompt_sinks_workspace(self.ptr, rows, heads, runs, sinks, max_count)
+
+    def prompt_sinks(self, layer: int, q, q_scales, rows: int, heads: int, runs: int, run_rows, run_seq, run_pos,
+                     window: int, sinks: int, max_count: int, workspace, workspace_bytes: int, out,
+                     stream=None) -> None:
+        check(lib().nhip_paged_prompt_sinks_dev(self.ptr, layer, q, q_scales, rows, heads, runs, run_rows, run_seq,
+                                                run_pos, window, sinks, max_count, workspace, workspace_bytes, out,
+                                                stream))
 
     def pages_workspace(self, count: int) -> int:
         return lib().nhip_paged_pages_workspace(self.ptr, count)
