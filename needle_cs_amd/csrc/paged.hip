@@ -101,33 +101,93 @@ __device__ __forceinline__ float group_max(float v)
     return L == 32 ? fmaxf(v, lane_xor<16>(v)) : v;
 }
 
-// 16 rows of one query head, rotated and quantized, by the lanes of the append.
-template <int QK, int L>
-__device__ __forceinline__ void append_queries(const RotaryAppendParams& p, int head, int row0)
+// A position's page and its place there, for a row to be written: page -1 where
+// it may not be.
+struct Place {
+    int page, at;
+};
+// Heads that one workgroup rotates.
+template <int QK, int H>
+__host__ __device__ constexpr int rotated_heads()
 {
-    constexpr int ROWS = 256 / L, PASSES = kAppendRows / ROWS;
-    const int l = threadIdx.x & (L - 1);
+    return H * (256 / (QK <= 64 ? 8 : 16) / kAppendRows);
+}
+__device__ __forceinline__ Place place_of(const PagedLayer& c, const int32_t* refs, int seq, int pos)
+{
+    int page = -1;
+    if (seq >= 0 && seq < c.sequences && pos >= 0 && (pos >> c.page_shift) < c.width)
+        page = c.tables[(size_t)seq * c.width + (pos >> c.page_shift)];
+    if (page < 0 || page >= c.pages || refs[page] > 1) page = -1;
+    return {page, pos & ((1 << c.page_shift) - 1)};
+}
+
+// Query and key heads rotated and quantized: 16 rows, L lanes a head, a unit of
+// eight elements each, and H x 16 / L heads in turn, so that a unit's cos and
+// sin are read once a row.  Heads from p.heads on are the keys'.
+template <int QK, int H>
+__device__ __forceinline__ void append_rotated(const RotaryAppendParams& p, int first_head, int row0)
+{
+    constexpr int L = QK <= 64 ? 8 : 16, SIDE = 256 / L / kAppendRows;  // heads side by side
+    const PagedLayer& c = p.c;
+    const int l = threadIdx.x % L, slot = threadIdx.x / L, side = slot / kAppendRows;
+    const int row = row0 + slot % kAppendRows, at = min(row, p.rows - 1);
+    const int heads = p.heads + c.kv_heads;
+    const int pos = p.row_pos[at];
+    const bool known = pos >= 0 && pos < p.r.positions, mine = 8 * l < QK;
+    const RotaryUnit unit = rotary_unit(p.r, mine ? l : 0, known ? pos : 0);
+    auto from = [&](int head) {
+        return head < p.heads ? p.q + (size_t)at * p.ldq + head * QK
+                              : p.k + (size_t)at * p.ldk + (head - p.heads) * QK;
+    };
+    f4 a[H], b[H];
 #pragma unroll
-    for (int k = 0; k < PASSES; k++) {
-        const int row = row0 + (int)threadIdx.x / L + k * ROWS;
-        const int at = min(row, p.rows - 1), pos = p.row_pos[at];
-        const float* from = p.q + (size_t)at * p.ldq + head * QK;
-        f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (4 * l < QK && pos >= 0 && pos < p.r.positions) {
-            const size_t table = (size_t)pos * (p.r.dim / 2);
-            y = rotated4(from, l, *reinterpret_cast<const f4*>(from + 4 * l), p.r, p.r.cos + table, p.r.sin + table);
+    for (int k = 0; k < H; k++) {
+        const float* head = from(min(first_head + side + SIDE * k, heads - 1));
+        a[k] = *reinterpret_cast<const f4*>(head + unit.a);
+        b[k] = *reinterpret_cast<const f4*>(head + unit.b);
+    }
+    Place place = {-1, 0};
+    if (first_head + SIDE * H > p.heads && known) place = place_of(c, p.refs, p.row_seq[at], pos);
+#pragma unroll
+    for (int k = 0; k < H; k++) {
+        const int head = first_head + side + SIDE * k;
+        if (head >= heads) continue;
+        rotate_unit(p.r, unit, from(head), a[k], b[k]);
+        if (!known || !mine) a[k] = b[k] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        float peak = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) peak = fmaxf(peak, fmaxf(fabsf(a[k][e]), fabsf(b[k][e])));
+        peak = fmaxf(peak, lane_xor<1>(peak));
+        peak = fmaxf(peak, lane_xor<2>(peak));
+        peak = fmaxf(peak, lane_xor<4>(peak));
+        if (L == 16) peak = fmaxf(peak, lane_xor<8>(peak));
+        const float scale = peak > 0.0f ? peak / 127.0f : 1.0f, inverse = 1.0f / scale;
+        int8_t* codes;
+        float* scales;
+        if (head < p.heads) {
+            const size_t to = (size_t)row * p.heads + head;
+            codes = p.codes + to * QK;
+            scales = p.q_scales + to;
+        } else {
+            const size_t cell = (((size_t)place.page * c.kv_heads + head - p.heads) << c.page_shift) + place.at;
+            codes = c.keys + cell * QK;
+            scales = c.kscale + cell;
+            if (place.page < 0) continue;
         }
-        const float peak = group_max<L>(fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3]))));
-        const float scale = peak > 0.0f ? peak / 127.0f : 1.0f;
-        const uint32_t codes = ref_quantize4(make_float4(y[0], y[1], y[2], y[3]), 1.0f / scale);
         if (row >= p.rows) continue;
-        const size_t to = (size_t)row * p.heads + head;
-        if (4 * l < QK) *reinterpret_cast<uint32_t*>(p.codes + to * QK + 4 * l) = codes;
-        if (l == 0) p.q_scales[to] = scale;
+        if (mine) {
+            *reinterpret_cast<uint32_t*>(codes + unit.a) =
+                ref_quantize4(make_float4(a[k][0], a[k][1], a[k][2], a[k][3]), inverse);
+            *reinterpret_cast<uint32_t*>(codes + unit.b) =
+                ref_quantize4(make_float4(b[k][0], b[k][1], b[k][2], b[k][3]), inverse);
+        }
+        if (l == 0) *scales = scale;
     }
 }
 
-template <int QK, int V, typename Params>
+// ROTARY: the keys go with the queries, H heads to a lane, in workgroups behind
+// those of the values.
+template <int QK, int V, int H, typename Params>
 __global__ __launch_bounds__(256) void paged_append_kernel(Params p)
 {
     constexpr bool ROTARY = std::is_same<Params, RotaryAppendParams>::value;
@@ -143,8 +203,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(Params p)
     const uint32_t groups = (p.rows + N - 1) / N;
     if constexpr (ROTARY) {
         if (group >= groups * c.kv_heads) {
-            const uint32_t head = group / groups - c.kv_heads;
-            if ((int)head < p.heads) append_queries<QK, L>(p, head, (int)(group % groups) * N);
+            const uint32_t first = (group / groups - c.kv_heads) * rotated_heads<QK, H>();
+            if ((int)first < p.heads + c.kv_heads) append_rotated<QK, H>(p, first, (int)(group % groups) * N);
             return;
         }
     }
@@ -156,15 +216,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(Params p)
     for (int k = 0; k < PASSES; k++) {
         const size_t r = row0 + min(row_of_pass + k * ROWS, n - 1);
         x[k][0] = x[k][1] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (4 * l < QK) x[k][0] = *reinterpret_cast<const f4*>(p.k + r * p.ldk + kvh * QK + 4 * l);
+        if (!ROTARY && 4 * l < QK) x[k][0] = *reinterpret_cast<const f4*>(p.k + r * p.ldk + kvh * QK + 4 * l);
         if (4 * l < V) x[k][1] = *reinterpret_cast<const f4*>(p.v + r * p.ldv + kvh * V + 4 * l);
-        if constexpr (ROTARY) {
-            const int pos = p.row_pos[r];
-            if (4 * l < QK && pos >= 0 && pos < p.r.positions) {
-                const size_t table = (size_t)pos * (p.r.dim / 2);
-                x[k][0] = rotated4(p.k + r * p.ldk + kvh * QK, l, x[k][0], p.r, p.r.cos + table, p.r.sin + table);
-            }
-        }
     }
     // where each row's position lives: its page's first cell (of this kv head) and its place in the page, -1 if nowhere
     int seq = -1, pos = 0, page = -1;
@@ -182,7 +235,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(Params p)
     for (int k = 0; k < PASSES; k++) {
         const int i = row_of_pass + k * ROWS;
 #pragma unroll
-        for (int part = 0; part < 2; part++) {
+        for (int part = ROTARY ? 1 : 0; part < 2; part++) {
             const f4 y = x[k][part];
             const float peak =
                 group_max<L>(fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3]))));
@@ -213,9 +266,9 @@ __global__ __launch_bounds__(256) void paged_append_kernel(Params p)
         const int at = places[row_of_pass + k * ROWS];
         const size_t cell = cells[row_of_pass + k * ROWS];
         if (at < 0) continue;
-        if (4 * l < QK) *reinterpret_cast<uint32_t*>(c.keys + (cell + at) * QK + 4 * l) = codes[k][0];
+        if (!ROTARY && 4 * l < QK) *reinterpret_cast<uint32_t*>(c.keys + (cell + at) * QK + 4 * l) = codes[k][0];
         if (l == 0) {
-            c.kscale[cell + at] = scales[k][0];
+            if (!ROTARY) c.kscale[cell + at] = scales[k][0];
             c.vscale[cell + at] = scales[k][1];
         }
     }
@@ -258,23 +311,38 @@ __global__ __launch_bounds__(256) void paged_append_kernel(Params p)
     }
 }
 
-template <int QK, int V, typename Params>
+template <int QK, int V, int H, typename Params>
 void launch_append(const Params& p, int heads, hipStream_t stream)
 {
     const unsigned groups = (unsigned)(p.rows + kAppendRows - 1) / kAppendRows * heads;
     const unsigned x = std::min((groups + 7) / 8 * 8, 1u << 20);  // (a multiple of 8)
-    hipLaunchKernelGGL((paged_append_kernel<QK, V, Params>), dim3(x, (groups + x - 1) / x), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((paged_append_kernel<QK, V, H, Params>), dim3(x, (groups + x - 1) / x), dim3(256), 0, stream, p);
+}
+template <int QK, int V>
+void launch_append(const AppendParams& p, hipStream_t stream)
+{
+    launch_append<QK, V, 1>(p, p.c.kv_heads, stream);
+}
+template <int QK, int V>
+void launch_append(const RotaryAppendParams& p, hipStream_t stream)
+{
+    const int heads = p.heads + p.c.kv_heads;
+    auto workgroups = [&](int side) { return p.c.kv_heads + (heads + side - 1) / side; };
+    if ((int64_t)p.rows * heads >= 1 << 14)
+        launch_append<QK, V, 4>(p, workgroups(rotated_heads<QK, 4>()), stream);
+    else
+        launch_append<QK, V, 1>(p, workgroups(rotated_heads<QK, 1>()), stream);
 }
 
 template <typename Params>
-int32_t launch_append(const nhip_paged_cache* c, const Params& p, int heads, hipStream_t stream)
+int32_t launch_append(const nhip_paged_cache* c, const Params& p, hipStream_t stream)
 {
     if (c->qk_dim == 48)
-        launch_append<48, 64>(p, heads, stream);
+        launch_append<48, 64>(p, stream);
     else if (c->qk_dim == 64)
-        launch_append<64, 64>(p, heads, stream);
+        launch_append<64, 64>(p, stream);
     else
-        launch_append<128, 128>(p, heads, stream);
+        launch_append<128, 128>(p, stream);
     NHIP_CHECK_HIP(hipGetLastError());
     return NHIP_OK;
 }
@@ -299,41 +367,83 @@ struct ReadParams {
     int32_t ldk, ldv, rows;
 };
 
-// A workgroup takes 16 rows of one kv head, L lanes a row, as the append.
+// L lanes take 16 rows of one kv head.  Where those are consecutive positions of
+// one sequence a lane reads four dimensions of a block of 16 positions, 64 bytes,
+// and has a row's four values for each of them; else a value is four bytes of
+// four units.
 template <int QK, int V>
 __global__ __launch_bounds__(256) void paged_read_kernel(ReadParams p)
 {
-    constexpr int N = kAppendRows, L = V <= 64 ? 16 : 32, ROWS = 256 / L;
+    constexpr int N = kAppendRows, L = V <= 64 ? 16 : 32;
     const PagedLayer& c = p.c;
-    const int row0 = blockIdx.x * N, kvh = blockIdx.y, l = threadIdx.x & (L - 1);
-    for (int row = row0 + (int)threadIdx.x / L; row < min(row0 + N, p.rows); row += ROWS) {
-        const int seq = p.row_seq[row], pos = p.row_pos[row];
-        int page = -1;
-        if (seq >= 0 && seq < c.sequences && pos >= 0 && (pos >> c.page_shift) < c.width)
-            page = c.tables[(size_t)seq * c.width + (pos >> c.page_shift)];
-        const bool ok = page >= 0 && page < c.pages;
-        const int at = pos & ((1 << c.page_shift) - 1);
-        const size_t cell = ok ? ((size_t)page * c.kv_heads + kvh) << c.page_shift : 0;
-        if (p.k && 4 * l < QK) {
+    const int l = threadIdx.x & (L - 1), kvh = blockIdx.y;
+    const int row0 = (int)(blockIdx.x * (256 / L) + threadIdx.x / L) * N, n = min(N, p.rows - row0);
+    if (n <= 0) return;
+    // lane i of the 16 holds row i's page and place
+    const int own = row0 + min(l & 15, n - 1), seq = p.row_seq[own], pos = p.row_pos[own];
+    int page = -1;
+    if (seq >= 0 && seq < c.sequences && pos >= 0 && (pos >> c.page_shift) < c.width)
+        page = c.tables[(size_t)seq * c.width + (pos >> c.page_shift)];
+    if (page >= c.pages) page = -1;
+    const int place = pos & ((1 << c.page_shift) - 1);
+    const int first_lane = (threadIdx.x & 63) & ~(L - 1);
+    const int seq0 = __shfl(seq, first_lane), pos0 = __shfl(pos, first_lane);
+    const uint64_t odd = __ballot(page < 0 || seq != seq0 || (int64_t)pos != (int64_t)pos0 + min(l & 15, n - 1));
+    const bool consecutive = ((odd >> first_lane) & (L == 32 ? 0xFFFFFFFFull : 0xFFFFull)) == 0;
+    auto cell_of = [&](int i) {  // row i's cell
+        const int pg = __shfl(page, first_lane + i), at = __shfl(place, first_lane + i);
+        return pg < 0 ? (size_t)-1 : (((size_t)pg * c.kv_heads + kvh) << c.page_shift) + at;
+    };
+    if (p.k) {
+#pragma unroll 4
+        for (int i = 0; i < n; i++) {
+            const size_t cell = cell_of(i);
             f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (ok) {
-                const uint32_t codes = *reinterpret_cast<const uint32_t*>(c.keys + (cell + at) * QK + 4 * l);
-                const float scale = c.kscale[cell + at];
+            if (4 * l < QK && cell != (size_t)-1) {
+                const uint32_t codes = *reinterpret_cast<const uint32_t*>(c.keys + cell * QK + 4 * l);
+                const float scale = c.kscale[cell];
 #pragma unroll
                 for (int e = 0; e < 4; e++) y[e] = (float)(int8_t)(codes >> (8 * e)) * scale;
             }
-            *reinterpret_cast<f4*>(p.k + (size_t)row * p.ldk + kvh * QK + 4 * l) = y;
+            if (4 * l < QK) *reinterpret_cast<f4*>(p.k + (size_t)(row0 + i) * p.ldk + kvh * QK + 4 * l) = y;
         }
-        if (p.v) {
-            f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (ok) {
-                const int8_t* from = c.values + cell * V + (size_t)(at >> 4) * (16 * V) + 64 * l + (at & 15);
-                const float scale = c.vscale[cell + at];
+    }
+    if (!p.v) return;
+    if (consecutive) {
+        const int lead = pos0 & 15;
+        for (int block = 0; 16 * block - lead < n; block++) {
+            const int some = max(16 * block - lead, 0);  // a row of the block
+            const size_t cell = cell_of(some) & ~(size_t)15;
+            uint4 codes[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) y[e] = (float)from[16 * e] * scale;
+            for (int e = 0; e < 4; e++)
+                codes[e] = *reinterpret_cast<const uint4*>(c.values + cell * V + 16 * (4 * l + e));
+#pragma unroll
+            for (int at = 0; at < 16; at++) {
+                const int i = 16 * block + at - lead;
+                if (i < 0 || i >= n) continue;
+                const float scale = c.vscale[cell + at];
+                f4 y;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t word = at < 4 ? codes[e].x : at < 8 ? codes[e].y : at < 12 ? codes[e].z : codes[e].w;
+                    y[e] = (float)(int8_t)(word >> (8 * (at & 3))) * scale;
+                }
+                *reinterpret_cast<f4*>(p.v + (size_t)(row0 + i) * p.ldv + kvh * V + 4 * l) = y;
             }
-            *reinterpret_cast<f4*>(p.v + (size_t)row * p.ldv + kvh * V + 4 * l) = y;
         }
+        return;
+    }
+    for (int i = 0; i < n; i++) {
+        const size_t cell = cell_of(i);
+        f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (cell != (size_t)-1) {
+            const int8_t* from = c.values + (cell & ~(size_t)15) * V + 64 * l + (cell & 15);
+            const float scale = c.vscale[cell];
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = (float)from[16 * e] * scale;
+        }
+        *reinterpret_cast<f4*>(p.v + (size_t)(row0 + i) * p.ldv + kvh * V + 4 * l) = y;
     }
 }
 
@@ -853,7 +963,7 @@ int32_t nhip_paged_append_dev(const nhip_paged_cache* c, int32_t layer, const fl
     rc = ensure_device();
     if (rc) return rc;
     const AppendParams p{paged_layer(c, layer), d_k, d_v, d_row_seq, d_row_pos, c->refs, ldk, ldv, rows};
-    return launch_append(c, p, c->kv_heads, as_stream(stream));
+    return launch_append(c, p, as_stream(stream));
 }
 
 int32_t nhip_paged_rotary_append_dev(const nhip_paged_cache* c, int32_t layer, const nhip_rotary* r, const float* d_q,
@@ -878,7 +988,7 @@ int32_t nhip_paged_rotary_append_dev(const nhip_paged_cache* c, int32_t layer, c
     if (rc) return rc;
     const RotaryAppendParams p{{paged_layer(c, layer), d_k, d_v, d_row_seq, d_row_pos, c->refs, ldk, ldv, rows},
                                rotary_table(r), d_q, d_codes, d_q_scales, ldq, heads};
-    return launch_append(c, p, c->kv_heads + heads, as_stream(stream));
+    return launch_append(c, p, as_stream(stream));
 }
 
 int32_t nhip_paged_read_dev(const nhip_paged_cache* c, int32_t layer, const int32_t* d_row_seq,
@@ -894,7 +1004,8 @@ int32_t nhip_paged_read_dev(const nhip_paged_cache* c, int32_t layer, const int3
     rc = ensure_device();
     if (rc) return rc;
     const ReadParams p{paged_layer(c, layer), d_row_seq, d_row_pos, d_k, d_v, ldk, ldv, rows};
-    const dim3 grid((rows + kAppendRows - 1) / kAppendRows, c->kv_heads);
+    const int a_group = kAppendRows * 256 / (c->v_dim <= 64 ? 16 : 32);  // rows of a workgroup
+    const dim3 grid((rows + a_group - 1) / a_group, c->kv_heads);
     if (c->qk_dim == 48)
         hipLaunchKernelGGL((paged_read_kernel<48, 64>), grid, dim3(256), 0, as_stream(stream), p);
     else if (c->qk_dim == 64)

@@ -1,5 +1,6 @@
 // rotary.hpp -- what the kernels that rotate heads by position share: the
-// checks of a caller's nhip_rotary, and the table as kernels see it.
+// checks of a caller's nhip_rotary, the table as kernels see it, and eight
+// elements of a head rotated in registers.
 #pragma once
 
 #include "common.hpp"
@@ -21,33 +22,75 @@ inline RotaryTable rotary_table(const nhip_rotary* r) { return {r->cos, r->sin, 
 
 typedef float rotary_f4 __attribute__((ext_vector_type(4), aligned(4)));
 
-// Elements 4l .. 4l + 3 of a head rotated by the table rows c and s, a partner
-// outside them from memory (the lane beside it has just read it).
-__device__ __forceinline__ rotary_f4 rotated4(const float* head, int l, rotary_f4 x, const RotaryTable& r,
-                                              const float* c, const float* s)
+// Unit u of a head: eight of its elements, a .. a + 3 and b .. b + 3, with the
+// cos and sin of its pairs.  Where dim is a multiple of 8 a unit is four whole
+// pairs (or elements that stay), so that it is rotated in registers, and its
+// cos and sin, read once, serve every head of the row; else (MIXED) the
+// partners and the table come from memory, element by element.
+struct RotaryUnit {
+    int a, b;
+    enum Kind { STAYS, HALVES, NEIGHBOURS, MIXED } kind;
+    rotary_f4 c, s;
+    const float *cos_row, *sin_row;
+};
+
+__device__ __forceinline__ RotaryUnit rotary_unit(const RotaryTable& r, int u, int pos)
 {
-    const int half = r.dim / 2;
-    rotary_f4 y = x;
-    if (r.interleaved) {
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const int i = 2 * l + k;
-            if (i < half) {
-                y[2 * k] = x[2 * k] * c[i] - x[2 * k + 1] * s[i];
-                y[2 * k + 1] = x[2 * k + 1] * c[i] + x[2 * k] * s[i];
+    const size_t row = (size_t)pos * (r.dim / 2);
+    RotaryUnit x = {8 * u, 8 * u + 4, RotaryUnit::STAYS, {}, {}, r.cos + row, r.sin + row};
+    if (8 * u < r.dim) {
+        if (r.dim & 7) {
+            x.kind = RotaryUnit::MIXED;
+        } else {
+            x.kind = r.interleaved ? RotaryUnit::NEIGHBOURS : RotaryUnit::HALVES;
+            x.c = *reinterpret_cast<const rotary_f4*>(x.cos_row + 4 * u);
+            x.s = *reinterpret_cast<const rotary_f4*>(x.sin_row + 4 * u);
+            if (!r.interleaved) {
+                x.a = 4 * u;
+                x.b = 4 * u + r.dim / 2;
             }
         }
-    } else {
+    }
+    return x;
+}
+
+// The unit's elements xa, xb of the head at `head`, rotated.
+__device__ __forceinline__ void rotate_unit(const RotaryTable& r, const RotaryUnit& u, const float* head, rotary_f4& xa,
+                                            rotary_f4& xb)
+{
+    const rotary_f4 p = xa, q = xb;
+    if (u.kind == RotaryUnit::HALVES) {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const int i = 4 * l + e;
-            if (i < half)
-                y[e] = x[e] * c[i] - head[i + half] * s[i];
-            else if (i < r.dim)
-                y[e] = x[e] * c[i - half] + head[i - half] * s[i - half];
+            xa[e] = p[e] * u.c[e] - q[e] * u.s[e];
+            xb[e] = q[e] * u.c[e] + p[e] * u.s[e];
+        }
+    } else if (u.kind == RotaryUnit::NEIGHBOURS) {
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            xa[2 * e] = p[2 * e] * u.c[e] - p[2 * e + 1] * u.s[e];
+            xa[2 * e + 1] = p[2 * e + 1] * u.c[e] + p[2 * e] * u.s[e];
+            xb[2 * e] = q[2 * e] * u.c[2 + e] - q[2 * e + 1] * u.s[2 + e];
+            xb[2 * e + 1] = q[2 * e + 1] * u.c[2 + e] + q[2 * e] * u.s[2 + e];
+        }
+    } else if (u.kind == RotaryUnit::MIXED) {
+        const int half = r.dim / 2;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int i = u.a + e;
+            if (i >= r.dim) break;
+            const bool second = r.interleaved ? i & 1 : i >= half;
+            const int pair = r.interleaved ? i >> 1 : second ? i - half : i;
+            const float own = e < 4 ? p[e & 3] : q[e & 3];
+            const float other = head[r.interleaved ? i ^ 1 : second ? i - half : i + half];
+            const float c = u.cos_row[pair], s = u.sin_row[pair];
+            const float y = second ? own * c + other * s : own * c - other * s;
+            if (e < 4)
+                xa[e & 3] = y;
+            else
+                xb[e & 3] = y;
         }
     }
-    return y;
 }
 
 }  // namespace nhip
