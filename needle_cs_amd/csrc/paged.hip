@@ -124,7 +124,7 @@ __device__ __forceinline__ Place place_of(const PagedLayer& c, const int32_t* re
 // Query and key heads rotated and quantized: 16 rows, L lanes a head, a unit of
 // eight elements each, and H x 16 / L heads in turn, so that a unit's cos and
 // sin are read once a row.  Heads from p.heads on are the keys'.
-template <int QK, int H>
+template <int QK, int H, bool MIXED>
 __device__ __forceinline__ void append_rotated(const RotaryAppendParams& p, int first_head, int row0)
 {
     constexpr int L = QK <= 64 ? 8 : 16, SIDE = 256 / L / kAppendRows;  // heads side by side
@@ -134,7 +134,7 @@ __device__ __forceinline__ void append_rotated(const RotaryAppendParams& p, int 
     const int heads = p.heads + c.kv_heads;
     const int pos = p.row_pos[at];
     const bool known = pos >= 0 && pos < p.r.positions, mine = 8 * l < QK;
-    const RotaryUnit unit = rotary_unit(p.r, mine ? l : 0, known ? pos : 0);
+    const RotaryUnit unit = rotary_unit<MIXED>(p.r, mine ? l : 0, known ? pos : 0);
     auto from = [&](int head) {
         return head < p.heads ? p.q + (size_t)at * p.ldq + head * QK
                               : p.k + (size_t)at * p.ldk + (head - p.heads) * QK;
@@ -152,7 +152,7 @@ __device__ __forceinline__ void append_rotated(const RotaryAppendParams& p, int 
     for (int k = 0; k < H; k++) {
         const int head = first_head + side + SIDE * k;
         if (head >= heads) continue;
-        rotate_unit(p.r, unit, from(head), a[k], b[k]);
+        rotate_unit<MIXED>(p.r, unit, from(head), a[k], b[k]);
         if (!known || !mine) a[k] = b[k] = f4{0.0f, 0.0f, 0.0f, 0.0f};
         float peak = 0.0f;
 #pragma unroll
@@ -185,9 +185,9 @@ __device__ __forceinline__ void append_rotated(const RotaryAppendParams& p, int 
     }
 }
 
-// ROTARY: the keys go with the queries, H heads to a lane, in workgroups behind
-// those of the values.
-template <int QK, int V, int H, typename Params>
+// ROTARY: the keys go with the queries, H heads to a lane, in workgroups of
+// their own.
+template <int QK, int V, int H, bool MIXED, typename Params>
 __global__ __launch_bounds__(256) void paged_append_kernel(Params p)
 {
     constexpr bool ROTARY = std::is_same<Params, RotaryAppendParams>::value;
@@ -199,16 +199,22 @@ __global__ __launch_bounds__(256) void paged_append_kernel(Params p)
     __shared__ bool consecutive;
     const PagedLayer& c = p.c;
     // an XCD takes neighbouring groups of rows, so that the pieces of a block that two workgroups write meet in its L2
-    const uint32_t id = blockIdx.y * gridDim.x + blockIdx.x, group = (id & 7) * (gridDim.x * gridDim.y / 8) + id / 8;
-    const uint32_t groups = (p.rows + N - 1) / N;
+    // (and, where keys go apart, as much of either kind of workgroup as the others)
+    const uint32_t id = blockIdx.y * gridDim.x + blockIdx.x;
+    const uint32_t groups = (p.rows + N - 1) / N, all = groups * c.kv_heads;
+    const uint32_t share = ROTARY ? (all + 7) / 8 : gridDim.x * gridDim.y / 8;
     if constexpr (ROTARY) {
-        if (group >= groups * c.kv_heads) {
-            const uint32_t first = (group / groups - c.kv_heads) * rotated_heads<QK, H>();
-            if ((int)first < p.heads + c.kv_heads) append_rotated<QK, H>(p, first, (int)(group % groups) * N);
+        if (id / 8 >= share) {
+            constexpr int heads = rotated_heads<QK, H>();
+            const uint32_t rotated = groups * ((p.heads + c.kv_heads + heads - 1) / heads);
+            const uint32_t part = (id & 7) * ((rotated + 7) / 8) + id / 8 - share;
+            if (id / 8 - share < (rotated + 7) / 8 && part < rotated)
+                append_rotated<QK, H, MIXED>(p, part / groups * heads, (int)(part % groups) * N);
             return;
         }
     }
-    if (group >= groups * c.kv_heads) return;
+    const uint32_t group = (id & 7) * share + id / 8;
+    if (group >= all) return;
     const int kvh = group / groups, row0 = (int)(group - kvh * groups) * N, n = min(N, p.rows - row0);
     const int l = threadIdx.x & (L - 1), row_of_pass = threadIdx.x / L;
     f4 x[PASSES][2];
@@ -311,27 +317,33 @@ __global__ __launch_bounds__(256) void paged_append_kernel(Params p)
     }
 }
 
-template <int QK, int V, int H, typename Params>
-void launch_append(const Params& p, int heads, hipStream_t stream)
+template <int QK, int V, int H, bool MIXED, typename Params>
+void launch_append(const Params& p, unsigned groups, hipStream_t stream)
 {
-    const unsigned groups = (unsigned)(p.rows + kAppendRows - 1) / kAppendRows * heads;
     const unsigned x = std::min((groups + 7) / 8 * 8, 1u << 20);  // (a multiple of 8)
-    hipLaunchKernelGGL((paged_append_kernel<QK, V, H, Params>), dim3(x, (groups + x - 1) / x), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((paged_append_kernel<QK, V, H, MIXED, Params>), dim3(x, (groups + x - 1) / x), dim3(256), 0,
+                       stream, p);
 }
+unsigned row_groups(int rows) { return (unsigned)(rows + kAppendRows - 1) / kAppendRows; }
 template <int QK, int V>
 void launch_append(const AppendParams& p, hipStream_t stream)
 {
-    launch_append<QK, V, 1>(p, p.c.kv_heads, stream);
+    launch_append<QK, V, 1, false>(p, row_groups(p.rows) * p.c.kv_heads, stream);
 }
 template <int QK, int V>
 void launch_append(const RotaryAppendParams& p, hipStream_t stream)
 {
-    const int heads = p.heads + p.c.kv_heads;
-    auto workgroups = [&](int side) { return p.c.kv_heads + (heads + side - 1) / side; };
-    if ((int64_t)p.rows * heads >= 1 << 14)
-        launch_append<QK, V, 4>(p, workgroups(rotated_heads<QK, 4>()), stream);
+    const unsigned heads = p.heads + p.c.kv_heads, groups = row_groups(p.rows);
+    // (each XCD's share of either kind of workgroup, rounded up)
+    auto workgroups = [&](unsigned side) {
+        return (groups * p.c.kv_heads + 7) / 8 * 8 + (groups * ((heads + side - 1) / side) + 7) / 8 * 8;
+    };
+    if (p.r.dim % 8)
+        launch_append<QK, V, 1, true>(p, workgroups(rotated_heads<QK, 1>()), stream);
+    else if ((int64_t)p.rows * heads >= 1 << 14)
+        launch_append<QK, V, 4, false>(p, workgroups(rotated_heads<QK, 4>()), stream);
     else
-        launch_append<QK, V, 1>(p, workgroups(rotated_heads<QK, 1>()), stream);
+        launch_append<QK, V, 1, false>(p, workgroups(rotated_heads<QK, 1>()), stream);
 }
 
 template <typename Params>
@@ -367,83 +379,94 @@ struct ReadParams {
     int32_t ldk, ldv, rows;
 };
 
-// L lanes take 16 rows of one kv head.  Where those are consecutive positions of
-// one sequence a lane reads four dimensions of a block of 16 positions, 64 bytes,
-// and has a row's four values for each of them; else a value is four bytes of
-// four units.
+// 4 L threads take the keys or the values (blockIdx.y) of 16 rows of one kv head,
+// L lanes a row.  Where a value's rows are consecutive positions of one sequence a thread reads, for each block of 16
+// positions, the four bytes that four positions have in each of four
+// dimensions, and has four rows' values; else a value is a byte by itself.
 template <int QK, int V>
 __global__ __launch_bounds__(256) void paged_read_kernel(ReadParams p)
 {
-    constexpr int N = kAppendRows, L = V <= 64 ? 16 : 32;
+    constexpr int N = kAppendRows, L = V <= 64 ? 16 : 32, UNITS = 256 / (4 * L);
+    __shared__ size_t cells[UNITS][N];
+    __shared__ bool consecutive[UNITS];
     const PagedLayer& c = p.c;
-    const int l = threadIdx.x & (L - 1), kvh = blockIdx.y;
-    const int row0 = (int)(blockIdx.x * (256 / L) + threadIdx.x / L) * N, n = min(N, p.rows - row0);
-    if (n <= 0) return;
-    // lane i of the 16 holds row i's page and place
-    const int own = row0 + min(l & 15, n - 1), seq = p.row_seq[own], pos = p.row_pos[own];
-    int page = -1;
-    if (seq >= 0 && seq < c.sequences && pos >= 0 && (pos >> c.page_shift) < c.width)
-        page = c.tables[(size_t)seq * c.width + (pos >> c.page_shift)];
-    if (page >= c.pages) page = -1;
-    const int place = pos & ((1 << c.page_shift) - 1);
-    const int first_lane = (threadIdx.x & 63) & ~(L - 1);
-    const int seq0 = __shfl(seq, first_lane), pos0 = __shfl(pos, first_lane);
-    const uint64_t odd = __ballot(page < 0 || seq != seq0 || (int64_t)pos != (int64_t)pos0 + min(l & 15, n - 1));
-    const bool consecutive = ((odd >> first_lane) & (L == 32 ? 0xFFFFFFFFull : 0xFFFFull)) == 0;
-    auto cell_of = [&](int i) {  // row i's cell
-        const int pg = __shfl(page, first_lane + i), at = __shfl(place, first_lane + i);
-        return pg < 0 ? (size_t)-1 : (((size_t)pg * c.kv_heads + kvh) << c.page_shift) + at;
-    };
-    if (p.k) {
-#pragma unroll 4
-        for (int i = 0; i < n; i++) {
-            const size_t cell = cell_of(i);
-            f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (4 * l < QK && cell != (size_t)-1) {
-                const uint32_t codes = *reinterpret_cast<const uint32_t*>(c.keys + cell * QK + 4 * l);
-                const float scale = c.kscale[cell];
-#pragma unroll
-                for (int e = 0; e < 4; e++) y[e] = (float)(int8_t)(codes >> (8 * e)) * scale;
-            }
-            if (4 * l < QK) *reinterpret_cast<f4*>(p.k + (size_t)(row0 + i) * p.ldk + kvh * QK + 4 * l) = y;
-        }
+    const int l = threadIdx.x & (L - 1), sub = (threadIdx.x / L) & 3, u = threadIdx.x / (4 * L);
+    const uint32_t unit = blockIdx.x * UNITS + u, group = unit / c.kv_heads;
+    const int kvh = unit - group * c.kv_heads, row0 = (int)group * N, n = min(N, p.rows - row0);
+    if (threadIdx.x % (4 * L) < N && n > 0) {
+        const int i = threadIdx.x % (4 * L), row = row0 + min(i, n - 1), seq = p.row_seq[row], pos = p.row_pos[row];
+        int page = -1;
+        if (seq >= 0 && seq < c.sequences && pos >= 0 && (pos >> c.page_shift) < c.width)
+            page = c.tables[(size_t)seq * c.width + (pos >> c.page_shift)];
+        if (page >= c.pages) page = -1;
+        cells[u][i] = page < 0 ? (size_t)-1
+                               : (((size_t)page * c.kv_heads + kvh) << c.page_shift) + (pos & ((1 << c.page_shift) - 1));
+        const int lane0 = (threadIdx.x & 63) & ~15;
+        const int seq0 = __shfl(seq, lane0), pos0 = __shfl(pos, lane0);
+        const uint64_t odd = __ballot(page < 0 || seq != seq0 || (int64_t)pos != (int64_t)pos0 + min(i, n - 1));
+        if (i == 0) consecutive[u] = ((odd >> lane0) & 0xFFFF) == 0;
     }
-    if (!p.v) return;
-    if (consecutive) {
-        const int lead = pos0 & 15;
-        for (int block = 0; 16 * block - lead < n; block++) {
-            const int some = max(16 * block - lead, 0);  // a row of the block
-            const size_t cell = cell_of(some) & ~(size_t)15;
-            uint4 codes[4];
+    __syncthreads();
+    if (n <= 0) return;
+    const f4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (blockIdx.y == (p.k ? 0 : 2)) {
+        if (4 * l >= QK) return;
+        uint32_t codes[4];
+        float scale[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const size_t cell = cells[u][min(sub + 4 * k, n - 1)], at = cell == (size_t)-1 ? 0 : cell;
+            codes[k] = *reinterpret_cast<const uint32_t*>(c.keys + at * QK + 4 * l);
+            scale[k] = c.kscale[at];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int i = sub + 4 * k;
+            if (i >= n) break;
+            f4 y;
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = (float)(int8_t)(codes[k] >> (8 * e)) * scale[k];
+            *reinterpret_cast<f4*>(p.k + (size_t)(row0 + i) * p.ldk + kvh * QK + 4 * l) =
+                cells[u][i] == (size_t)-1 ? none : y;
+        }
+        return;
+    }
+    float* to = p.v + (size_t)row0 * p.ldv + kvh * V + 4 * l;
+    if (consecutive[u]) {
+        const int lead = (int)(cells[u][0] & 15);
+#pragma unroll
+        for (int block = 0; block < 2; block++) {
+            const int first = 16 * block + 4 * sub - lead;  // row of the thread's first position
+            if (first + 3 < 0 || first >= n) continue;
+            // (its positions lie in one quad, so in one page)
+            const size_t cell = (cells[u][max(first, 0)] & ~(size_t)15) + 4 * sub;
+            uint32_t codes[4];
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                codes[e] = *reinterpret_cast<const uint4*>(c.values + cell * V + 16 * (4 * l + e));
+                codes[e] = *reinterpret_cast<const uint32_t*>(c.values + (cell - 4 * sub) * V + 16 * (4 * l + e) + 4 * sub);
+            const f4 scale = *reinterpret_cast<const f4*>(c.vscale + cell);
 #pragma unroll
-            for (int at = 0; at < 16; at++) {
-                const int i = 16 * block + at - lead;
-                if (i < 0 || i >= n) continue;
-                const float scale = c.vscale[cell + at];
+            for (int k = 0; k < 4; k++) {
+                if (first + k < 0 || first + k >= n) continue;
                 f4 y;
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const uint32_t word = at < 4 ? codes[e].x : at < 8 ? codes[e].y : at < 12 ? codes[e].z : codes[e].w;
-                    y[e] = (float)(int8_t)(word >> (8 * (at & 3))) * scale;
-                }
-                *reinterpret_cast<f4*>(p.v + (size_t)(row0 + i) * p.ldv + kvh * V + 4 * l) = y;
+                for (int e = 0; e < 4; e++) y[e] = (float)(int8_t)(codes[e] >> (8 * k)) * scale[k];
+                *reinterpret_cast<f4*>(to + (size_t)(first + k) * p.ldv) = y;
             }
         }
         return;
     }
-    for (int i = 0; i < n; i++) {
-        const size_t cell = cell_of(i);
-        f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (cell != (size_t)-1) {
-            const int8_t* from = c.values + (cell & ~(size_t)15) * V + 64 * l + (cell & 15);
-            const float scale = c.vscale[cell];
 #pragma unroll
-            for (int e = 0; e < 4; e++) y[e] = (float)from[16 * e] * scale;
-        }
-        *reinterpret_cast<f4*>(p.v + (size_t)(row0 + i) * p.ldv + kvh * V + 4 * l) = y;
+    for (int k = 0; k < 4; k++) {
+        const int i = sub + 4 * k;
+        if (i >= n) break;
+        const size_t cell = cells[u][i], at = cell == (size_t)-1 ? 0 : cell;
+        const int8_t* from = c.values + (at & ~(size_t)15) * V + 64 * l + (at & 15);
+        const float scale = c.vscale[at];
+        f4 y;
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = (float)from[16 * e] * scale;
+        *reinterpret_cast<f4*>(to + (size_t)i * p.ldv) = cell == (size_t)-1 ? none : y;
     }
 }
 
@@ -1004,8 +1027,8 @@ int32_t nhip_paged_read_dev(const nhip_paged_cache* c, int32_t layer, const int3
     rc = ensure_device();
     if (rc) return rc;
     const ReadParams p{paged_layer(c, layer), d_row_seq, d_row_pos, d_k, d_v, ldk, ldv, rows};
-    const int a_group = kAppendRows * 256 / (c->v_dim <= 64 ? 16 : 32);  // rows of a workgroup
-    const dim3 grid((rows + a_group - 1) / a_group, c->kv_heads);
+    const unsigned units = row_groups(rows) * c->kv_heads, of_one = c->v_dim <= 64 ? 4 : 2;
+    const dim3 grid((units + of_one - 1) / of_one, d_k && d_v ? 2 : 1);
     if (c->qk_dim == 48)
         hipLaunchKernelGGL((paged_read_kernel<48, 64>), grid, dim3(256), 0, as_stream(stream), p);
     else if (c->qk_dim == 64)

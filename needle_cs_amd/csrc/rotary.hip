@@ -125,7 +125,7 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateParams p)
         const float* from = p.x + (size_t)row * p.ldx;
         float* to = p.y + (size_t)row * p.ldy;
         for (int u = threadIdx.x % L; u < units; u += L) {
-            const RotaryUnit unit = rotary_unit(p.r, u, pos);
+            const RotaryUnit unit = rotary_unit<false>(p.r, u, pos);
             for (int h0 = slot; h0 < p.heads; h0 += kHeadsAhead * (256 / L)) {
                 rotary_f4 a[kHeadsAhead], b[kHeadsAhead];
 #pragma unroll
@@ -138,7 +138,7 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateParams p)
                 for (int k = 0; k < kHeadsAhead; k++) {
                     const int h = h0 + k * (256 / L);
                     if (h >= p.heads) break;
-                    rotate_unit(p.r, unit, nullptr, a[k], b[k]);
+                    rotate_unit<false>(p.r, unit, nullptr, a[k], b[k]);
                     *reinterpret_cast<rotary_f4*>(to + h * p.head_dim + unit.a) = a[k];
                     *reinterpret_cast<rotary_f4*>(to + h * p.head_dim + unit.b) = b[k];
                 }

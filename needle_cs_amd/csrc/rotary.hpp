@@ -25,22 +25,24 @@ typedef float rotary_f4 __attribute__((ext_vector_type(4), aligned(4)));
 // Unit u of a head: eight of its elements, a .. a + 3 and b .. b + 3, with the
 // cos and sin of its pairs.  Where dim is a multiple of 8 a unit is four whole
 // pairs (or elements that stay), so that it is rotated in registers, and its
-// cos and sin, read once, serve every head of the row; else (MIXED) the
-// partners and the table come from memory, element by element.
+// cos and sin, read once, serve every head of the row; else (MIXED, a variant
+// of its own for the registers) the partners and the table come from memory,
+// element by element.
 struct RotaryUnit {
     int a, b;
-    enum Kind { STAYS, HALVES, NEIGHBOURS, MIXED } kind;
+    enum Kind { STAYS, HALVES, NEIGHBOURS, ANY } kind;
     rotary_f4 c, s;
     const float *cos_row, *sin_row;
 };
 
+template <bool MIXED>
 __device__ __forceinline__ RotaryUnit rotary_unit(const RotaryTable& r, int u, int pos)
 {
     const size_t row = (size_t)pos * (r.dim / 2);
     RotaryUnit x = {8 * u, 8 * u + 4, RotaryUnit::STAYS, {}, {}, r.cos + row, r.sin + row};
     if (8 * u < r.dim) {
-        if (r.dim & 7) {
-            x.kind = RotaryUnit::MIXED;
+        if (MIXED) {
+            x.kind = RotaryUnit::ANY;
         } else {
             x.kind = r.interleaved ? RotaryUnit::NEIGHBOURS : RotaryUnit::HALVES;
             x.c = *reinterpret_cast<const rotary_f4*>(x.cos_row + 4 * u);
@@ -55,17 +57,18 @@ __device__ __forceinline__ RotaryUnit rotary_unit(const RotaryTable& r, int u, i
 }
 
 // The unit's elements xa, xb of the head at `head`, rotated.
+template <bool MIXED>
 __device__ __forceinline__ void rotate_unit(const RotaryTable& r, const RotaryUnit& u, const float* head, rotary_f4& xa,
                                             rotary_f4& xb)
 {
     const rotary_f4 p = xa, q = xb;
-    if (u.kind == RotaryUnit::HALVES) {
+    if (!MIXED && u.kind == RotaryUnit::HALVES) {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             xa[e] = p[e] * u.c[e] - q[e] * u.s[e];
             xb[e] = q[e] * u.c[e] + p[e] * u.s[e];
         }
-    } else if (u.kind == RotaryUnit::NEIGHBOURS) {
+    } else if (!MIXED && u.kind == RotaryUnit::NEIGHBOURS) {
 #pragma unroll
         for (int e = 0; e < 2; e++) {
             xa[2 * e] = p[2 * e] * u.c[e] - p[2 * e + 1] * u.s[e];
@@ -73,7 +76,7 @@ __device__ __forceinline__ void rotate_unit(const RotaryTable& r, const RotaryUn
             xb[2 * e] = q[2 * e] * u.c[2 + e] - q[2 * e + 1] * u.s[2 + e];
             xb[2 * e + 1] = q[2 * e + 1] * u.c[2 + e] + q[2 * e] * u.s[2 + e];
         }
-    } else if (u.kind == RotaryUnit::MIXED) {
+    } else if (MIXED && u.kind == RotaryUnit::ANY) {
         const int half = r.dim / 2;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
