@@ -2,11 +2,17 @@
 // top-p, min-p and a draw with a given number.
 //
 // The order of a row's ids is that of composites (key(logit), ~id), 64-bit
-// whole numbers: larger comes first, and no two are equal.  Whatever top-k and
-// top-p keep is a prefix of that order, so it is "composite >= cut".  Weights
-// are whole multiples of 2^-42, so that every sum of them is exact and no
-// order of summation shows, those by atomics into LDS among them; a sum of
-// 2^19 weights stays below 2^62.
+// whole numbers: larger comes first, and no two are equal.  Whatever a rule
+// keeps is a prefix of that order, so it is "composite >= cut".  Weights are
+// whole multiples of 2^-42, so that every sum of them is exact and no order of
+// summation shows, those by atomics into LDS among them; a sum of 2^19 weights
+// stays below 2^62.
+//
+// A workgroup takes a row.  It finds the largest logit, from its threads' own
+// largest a logit that what is kept will hardly fall below, and gathers the ids
+// above that into LDS, where the rules and the draw are ranks of few ids or
+// histograms of many.  Rows that keep more than the list holds or than the
+// guess allowed, and rows without rules, are walked instead.
 #include <algorithm>
 #include <cmath>
 
@@ -15,17 +21,22 @@
 namespace nhip {
 namespace {
 
-constexpr int kBins = 1024;      // of a histogram; in the first the last one holds what weighs nothing
-constexpr int kList = 512;       // ids that are ranked against one another
-constexpr int kFew = 256;        // a top-k of no more is found without a histogram
-constexpr int kSegment = 256;    // ids of a wave's step, four a lane
+constexpr int kBins = 1024;    // of a histogram; in the first the last one holds what weighs nothing
+constexpr int kFew = 512;      // ids that are ranked against one another
+constexpr int kSegment = 256;  // ids of a wave's step, four a lane
 constexpr int kMaxIds = 1 << 19;
-constexpr int kTerms = 12;
+constexpr int kTerms = 10;
 constexpr double kOne = 4398046511104.0;  // 2^42, the weight of the largest logit
-constexpr double kLeastScore = -30.0;     // e^-30 2^42 < 1/2: no weight
+constexpr float kLeastScore = -30.0f;     // e^-30 2^42 < 1/2: no weight
 
 typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned long long u64;
+
+// 2^f for |f| <= 1/2, interpolated at Chebyshev's points: within 2^-45.
+constexpr double kPower[kTerms] = {1.0000000000000135,     0.6931471805599462,     0.2402265069564034,
+                                   0.05550410866465167,    0.009618129193934313,   0.0013333558200794592,
+                                   0.0001540343375125101,  1.5252672924850737e-05, 1.325964524488711e-06,
+                                   1.0205905413765595e-07};
 
 struct SampleParams {
     const float* logits;
@@ -34,7 +45,7 @@ struct SampleParams {
     int32_t* ids;
     float* logprobs;
     int32_t ldx, n, mask_ld, words;
-    double taylor[kTerms];  // ln(2)^k / k!: arguments, so that they stay in scalar registers
+    double power[kTerms];  // kPower, as arguments: they stay in scalar registers
 };
 
 // A larger key for a larger logit; +0 and -0 alike.
@@ -48,91 +59,102 @@ __device__ __forceinline__ float logit_of(uint32_t key)
     return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
 __device__ __forceinline__ u64 composite(float l, int id) { return (u64)key_of(l) << 32 | (uint32_t)~id; }
+__device__ __forceinline__ float logit_in(u64 c) { return logit_of((uint32_t)(c >> 32)); }
+__device__ __forceinline__ int id_in(u64 c) { return ~(int)(uint32_t)c; }
 
+// A row's logits as they count: -inf where an id may not be drawn (by the mask,
+// or a NaN); in a row with +inf that is 0 and the others -inf.
 struct Row {
     const float* x;
     const uint32_t* mask;
     int n;
+    bool infinite;
 };
-struct Scale {
-    float peak;
-    double inverse;   // of the temperature
-    double log2e;     // log2(e) times that
-    float bin_scale;  // of half a difference, which does not overflow
-};
-
-// round(2^42 e^((l - peak) / temperature)): 2^t with t = n + f, |f| <= 1/2, by
-// the Taylor polynomial of 2^f (the terms left out are below 2^-47 of it).
-__device__ __forceinline__ u64 weight(const double (&taylor)[kTerms], Scale r, float l)
+__device__ __forceinline__ f4 counted4(const Row& r, f4 v, uint32_t bits)
 {
-    const double t = ((double)l - (double)r.peak) * r.log2e;
-    const double n = rint(fmax(t, -64.0)), f = t - n;
-    double y = taylor[kTerms - 1];
 #pragma unroll
-    for (int k = kTerms - 2; k >= 0; k--) y = fma(y, f, taylor[k]);
-    // (a whole number below 2^51 plus 2^52 is itself in the low bits)
-    const double x = ldexp(y, (int)n + 42) + 4503599627370496.0;
-    const u64 w = (u64)__double_as_longlong(x) & 0xFFFFFFFFFFFFFull;
-    // (-inf, as under a peak of +inf, and NaN weigh nothing)
-    return l == r.peak ? (u64)kOne : t > kLeastScore * 1.4426950408889634 ? w : 0;
-}
-
-// The bin of the first histogram, which descends with the logit: kBins - 1 for what weighs nothing.
-__device__ __forceinline__ int first_bin(Scale r, float l)
-{
-    return l == r.peak ? 0 : (int)fminf((0.5f * r.peak - 0.5f * l) * r.bin_scale, (float)(kBins - 1));
-}
-
-// Four of the row's logits from id i on, -inf where an id may not be drawn
-// (by the mask, past the end, or a NaN).
-__device__ __forceinline__ f4 load4(Row r, int i)
-{
-    f4 v = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-    if (i + 4 <= r.n) {
-        v = *reinterpret_cast<const f4*>(r.x + i);
-    } else {
+    for (int e = 0; e < 4; e++) v[e] = v[e] > -INFINITY ? v[e] : -INFINITY;
+    if (r.mask) {
 #pragma unroll
-        for (int e = 0; e < 3; e++)
-            if (i + e < r.n) v[e] = r.x[i + e];
+        for (int e = 0; e < 4; e++) v[e] = (bits >> e) & 1 ? v[e] : -INFINITY;
+    }
+    if (r.infinite) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = v[e] == INFINITY ? 0.0f : -INFINITY;
     }
     return v;
 }
-__device__ __forceinline__ f4 allowed4(f4 v, uint32_t bits)
+
+// How logits become weights, by the largest of them and a temperature.
+struct Scale {
+    double peak, log2e;      // log2e: log2(e) / temperature
+    float half_peak, bins;   // a bin is (half_peak - logit / 2) * bins, which does not overflow
+    const double* power;
+};
+__device__ __forceinline__ Scale scale_of(float peak, float temperature, const double* power)
 {
-#pragma unroll
-    for (int e = 0; e < 4; e++) v[e] = v[e] > -INFINITY && ((bits >> e) & 1) ? v[e] : -INFINITY;
-    return v;
-}
-__device__ __forceinline__ uint32_t mask4(Row r, int i)
-{
-    return r.mask && i < r.n ? r.mask[i >> 5] >> (i & 31) : 15u;
+    const double inverse = 1.0 / (double)temperature;
+    // (bins is never 0, so that -inf comes last under an infinite temperature too)
+    const double bins = fmin(fmax(2.0 * (kBins - 1) / -kLeastScore * inverse, 1.2e-38), 3e38);
+    return {(double)peak, 1.4426950408889634 * inverse, 0.5f * peak, (float)bins, power};
 }
 
-// f(first id, logits) for every four ids of the row, by the T threads of the
-// workgroup: a wave's 64 fours are one segment, U of its segments are at work
-// and the next U's loads in flight.
-template <int T, int U, typename F>
-__device__ __forceinline__ void each4(Row r, F f)
+// round(2^42 e^((l - peak) / temperature)): 2^t, t = n + f with a whole n and
+// |f| <= 1/2; at t = -22, which takes the place of all below it and of -inf, it is 0.
+__device__ __forceinline__ u64 weight(const Scale& z, float l)
 {
-    constexpr int W = T / 64;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int whole = r.n / kSegment;
+    const double t = fmax(fma((double)l - z.peak, z.log2e, 42.0), -22.0), n = rint(t), f = t - n;
+    double y = z.power[kTerms - 1];
+#pragma unroll
+    for (int k = kTerms - 2; k >= 0; k--) y = fma(y, f, z.power[k]);
+    // (a whole number below 2^51 plus 2^52 is itself in the low bits)
+    const double x = ldexp(y, (int)n) + 4503599627370496.0;
+    return (u64)__double_as_longlong(x) & 0xFFFFFFFFFFFFFull;
+}
+
+// The bin of the first histogram, which descends with the logit: kBins - 1 for what weighs nothing.
+__device__ __forceinline__ int first_bin(const Scale& z, float l)
+{
+    return (int)fminf((z.half_peak - 0.5f * l) * z.bins, (float)(kBins - 1));
+}
+
+__device__ __forceinline__ uint32_t mask_bits(const Row& r, int i)
+{
+    return r.mask ? r.mask[i >> 5] >> (i & 31) : 15u;
+}
+
+// Four logits from id i of a segment, -inf past the row's end.
+__device__ __forceinline__ f4 segment4(const Row& r, int i)
+{
+    f4 v;
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = i + e < r.n ? r.x[i + e] : -INFINITY;
+    return counted4(r, v, i < r.n ? mask_bits(r, i) : 0u);
+}
+
+// f(first id, logits) for every four ids of the segments `segment`, + step, ... below
+// `end`, by one wave: a wave's 64 fours are one segment; U of its segments are at
+// work and the next U's loads in flight.
+template <int U, typename F>
+__device__ __forceinline__ void walk(const Row& r, int segment, int end, int step, F f)
+{
+    const int lane = threadIdx.x & 63, whole = min(r.n / kSegment, end);
     f4 v[U], next[U];
     uint32_t bits[U], next_bits[U];
-    auto load = [&](int segment, f4 (&x)[U], uint32_t (&m)[U]) {
+    auto load = [&](int first, f4 (&x)[U], uint32_t (&m)[U]) {
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int i = kSegment * min(segment + W * u, whole - 1) + 4 * lane;
+            const int i = kSegment * min(first + step * u, whole - 1) + 4 * lane;
             x[u] = *reinterpret_cast<const f4*>(r.x + i);
-            m[u] = r.mask ? r.mask[i >> 5] >> (i & 31) : 15u;
+            m[u] = mask_bits(r, i);
         }
     };
-    if (wave < whole) load(wave, v, bits);
-    for (int segment = wave; segment < whole; segment += W * U) {
-        if (segment + W * U < whole) load(segment + W * U, next, next_bits);
+    if (segment < whole) load(segment, v, bits);
+    for (; segment < whole; segment += step * U) {
+        if (segment + step * U < whole) load(segment + step * U, next, next_bits);
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            if (segment + W * u < whole) f(kSegment * (segment + W * u) + 4 * lane, allowed4(v[u], bits[u]));
+            if (segment + step * u < whole) f(kSegment * (segment + step * u) + 4 * lane, counted4(r, v[u], bits[u]));
             __builtin_amdgcn_sched_barrier(0);  // (one four at a time in the registers)
         }
 #pragma unroll
@@ -141,9 +163,20 @@ __device__ __forceinline__ void each4(Row r, F f)
             bits[u] = next_bits[u];
         }
     }
-    if (whole * kSegment < r.n && wave == whole % W) {
-        const int i = kSegment * whole + 4 * lane;
-        f(i, allowed4(load4(r, i), mask4(r, i)));
+}
+
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
+// f as above for all of the row, by the T threads of the workgroup.
+template <int T, int U, typename F>
+__device__ __forceinline__ void each4(const Row& r, F f)
+{
+    constexpr int W = T / 64;
+    const int whole = r.n / kSegment;
+    walk<U>(r, wave_id(), whole, W, f);
+    if (whole * kSegment < r.n && wave_id() == whole % W) {
+        const int i = kSegment * whole + 4 * (int)(threadIdx.x & 63);
+        f(i, segment4(r, i));
     }
 }
 
@@ -157,51 +190,53 @@ __device__ __forceinline__ u64 wave_sum_u64(u64 v)
 {
     return add_lane_xor<32>(add_lane_xor<16>(add_lane_xor<8>(add_lane_xor<4>(add_lane_xor<2>(add_lane_xor<1>(v))))));
 }
-
-// COPIES of a histogram side by side, a lane's own: lanes of a wave that meet
-// in a bin would wait for one another.
-template <int T>
-struct Shared {
-    static constexpr int COPIES = T == 1024 ? 16 : 4;
-    union {
-        u64 bins[kBins][COPIES];
-        struct {
-            u64 list[kList], weights[kList];
-        };
-    };
-    u64 segments[T == 1024 ? kMaxIds / kSegment : kList];
-    u64 waves[T / 64];
-    uint32_t listed, key_lo, key_hi, bin;
-    u64 cut, before;
-    int id;
-};
-
-// The sum of the values of the threads before this one, and of all.
-template <int T>
-__device__ __forceinline__ u64 block_before(u64 v, u64* waves, u64* all)
+// Sum of the lanes up to this one.
+__device__ __forceinline__ u64 wave_upto(u64 v)
 {
-    u64 upto = v;
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
-        const u64 other = __shfl_up(upto, off);
-        if (lane >= off) upto += other;
+        const u64 other = __shfl_up(v, off);
+        if (lane >= off) v += other;
     }
+    return v;
+}
+
+// COPIES of a histogram of the row side by side, a lane's own: lanes of a wave
+// that meet in a bin would wait for one another.  Where ids are listed the list
+// has their place, and its histograms are short.
+template <int T>
+struct Shared {
+    static constexpr int COPIES = T == 1024 ? 16 : 4, LIST = kBins * COPIES / 2;
+    union {
+        u64 bins[kBins * COPIES];
+        struct {
+            u64 list[LIST], weights[LIST];
+        };
+    };
+    u64 counts[kBins];
+    u64 few[kFew], few_weights[kFew];
+    u64 waves[T / 64];
+    uint32_t listed, few_listed, bin, key;
+    u64 cut, before, mass, total, least, most;
+};
+
+// The sum over the workgroup, in every thread.
+template <int T>
+__device__ __forceinline__ u64 block_sum(Shared<T>& sh, u64 v)
+{
+    v = wave_sum_u64(v);
     __syncthreads();
-    if (lane == 63) waves[threadIdx.x >> 6] = upto;
+    if ((threadIdx.x & 63) == 0) sh.waves[threadIdx.x >> 6] = v;
     __syncthreads();
-    u64 before = 0, sum = 0;
+    u64 sum = 0;
 #pragma unroll
-    for (int w = 0; w < T / 64; w++) {
-        if (w < (int)(threadIdx.x >> 6)) before += waves[w];
-        sum += waves[w];
-    }
-    *all = sum;
-    return before + upto - v;
+    for (int w = 0; w < T / 64; w++) sum += sh.waves[w];
+    return sum;
 }
 
 // What a rule keeps, by the sum of what stands before an id: of ones (top_k) or
-// of weights (top_p).
+// of weights (top_p: those before the mass, and always the first).
 struct Limit {
     u64 count;
     double mass;
@@ -210,26 +245,47 @@ struct Limit {
         return count ? before < count : (double)before < mass;
     }
 };
-
-// The histogram's bin in which a rule ends, and the sum before it, in sh; kBins
-// where it does not end in it.  limit_of(total): the rule.
-template <int T, typename F>
-__device__ __forceinline__ Limit find_bin(Shared<T>& sh, u64 before0, F limit_of)
+__device__ __forceinline__ Limit mass_limit(float top_p, u64 total)
 {
-    constexpr int B = kBins / T, C = Shared<T>::COPIES;
-    u64 q[B], sum = 0, all;
+    return {0, fmax((double)top_p * (double)total, 0.5)};
+}
+
+// One row's settings.
+struct Rules {
+    int top_k;  // 0: all
+    bool by_mass;
+    float top_p, random;
+    double least;  // min_p's weight
+};
+
+// The bin of a histogram (copies of it side by side) in which a rule ends, and
+// the sum before it, in sh.bin and sh.before; kBins where it does not end.
+// SHARE: the rule is the share top_p of all bins.  The sum of all bins.
+template <int T, bool SHARE>
+__device__ __forceinline__ u64 find_bin(Shared<T>& sh, const u64* bins, int copies, u64 before, Limit limit, float top_p)
+{
+    constexpr int B = kBins / T;
+    u64 q[B], own = 0;
 #pragma unroll
     for (int k = 0; k < B; k++) {
         const int b = B * threadIdx.x + k;
         q[k] = 0;
-#pragma unroll
-        for (int c = 0; c < C; c++) q[k] += sh.bins[b][(c + b) % C];
-        sum += q[k];
+        for (int c = 0; c < copies; c++) q[k] += bins[b * copies + ((c + b) & (copies - 1))];
+        own += q[k];
     }
-    u64 before = before0 + block_before<T>(sum, sh.waves, &all);
-    const Limit limit = limit_of(all);
+    const u64 upto = wave_upto(own);
+    if ((threadIdx.x & 63) == 63) sh.waves[threadIdx.x >> 6] = upto;
     if (threadIdx.x == 0) sh.bin = kBins;
     __syncthreads();
+    u64 all = 0;
+    before += upto - own;
+#pragma unroll
+    for (int w = 0; w < T / 64; w++) {
+        const u64 x = sh.waves[w];
+        if (w < (int)(threadIdx.x >> 6)) before += x;
+        all += x;
+    }
+    if (SHARE) limit = mass_limit(top_p, all);
 #pragma unroll
     for (int k = 0; k < B; k++) {
         if (limit.inside(before) && !limit.inside(before + q[k])) {
@@ -239,190 +295,154 @@ __device__ __forceinline__ Limit find_bin(Shared<T>& sh, u64 before0, F limit_of
         before += q[k];
     }
     __syncthreads();
-    return limit;
+    return all;
 }
 
 template <int T>
-__device__ __forceinline__ void clear_bins(Shared<T>& sh)
+__device__ __forceinline__ void clear_bins(u64* bins, int n)
 {
-    u64* all = &sh.bins[0][0];
-    for (int b = threadIdx.x; b < kBins * Shared<T>::COPIES; b += T) all[b] = 0;
+    for (int b = threadIdx.x; b < n; b += T) bins[b] = 0;
     __syncthreads();
 }
 
-// The weights of the list's ids.
+// The ids in order, as the rules below take them: f(composite, logit, place).
 template <int T>
-__device__ __forceinline__ void weigh_list(Shared<T>& sh, const double (&taylor)[kTerms], Scale z, int listed)
-{
-    for (int e = threadIdx.x; e < listed; e += T) sh.weights[e] = weight(taylor, z, logit_of((uint32_t)(sh.list[e] >> 32)));
-    __syncthreads();
-}
-
-// f(place, composite, quantity, quantity of the larger ones) for each of the
-// `listed` composites of sh.list, by as many threads each as the workgroup has:
-// quantities are ones (top_k) or sh.weights.
-template <int T, typename F>
-__device__ __forceinline__ void rank_list(Shared<T>& sh, int listed, bool ones, F f)
-{
-    const int most = listed <= 16 ? 16 : listed <= 64 ? 64 : listed <= 256 ? 256 : 512;
-    const int threads = max(1, min(64, T / most));  // for an id, side by side in a wave
-    for (int e = threadIdx.x / threads; e - (int)(threadIdx.x / threads) < listed; e += T / threads) {
-        const u64 own = e < listed ? sh.list[e] : 0;
-        u64 larger = 0;
-        if (e < listed)
-            for (int k = threadIdx.x % threads; k < listed; k += threads)
-                larger += sh.list[k] > own ? (ones ? 1 : sh.weights[k]) : 0;
-        for (int off = 1; off < threads; off <<= 1) larger += __shfl_xor(larger, off);
-        if (e < listed && threadIdx.x % threads == 0) f(e, own, ones ? 1 : sh.weights[e], larger);
-    }
-}
-
-// Moves sh.cut up to the last id that a rule keeps of those from sh.cut on:
-// the first `count` of them, or (count 0) those of the share top_p.
-template <int T>
-__device__ __forceinline__ void keep(Shared<T>& sh, const double (&taylor)[kTerms], Row r, Scale z, int count, float top_p)
-{
-    const bool masses = count == 0;
-    const u64 cut = sh.cut;
-    const int copy = threadIdx.x % Shared<T>::COPIES;
-    clear_bins(sh);
-    auto add = [&](int bin, float l) { atomicAdd(&sh.bins[bin][copy], masses ? weight(taylor, z, l) : (u64)1); };
-    each4<T, 2>(r, [&](int id, f4 l) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int bin = first_bin(z, l[e]);
-            if (bin < kBins - 1 && composite(l[e], id + e) >= cut) add(bin, l[e]);
-        }
-    });
-    __syncthreads();
-    const Limit limit = find_bin(sh, 0, [&](u64 total) {
-        return Limit{(u64)count, fmax((double)top_p * (double)total, 0.5)};
-    });
-    const int bin = sh.bin;
-    if (bin == kBins) return;
-    uint32_t lo = 0, hi = ~0u;
-    u64 before = sh.before;
-    auto inside = [&](float l, int id) {
-        const uint32_t key = key_of(l);
-        return key >= lo && key <= hi && first_bin(z, l) == bin && composite(l, id) >= cut;
-    };
-    int listed;
-    while (true) {
-        // the bin's ids, as many as the list takes, and their keys
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            sh.listed = 0;
-            sh.key_lo = ~0u;
-            sh.key_hi = 0;
-        }
-        __syncthreads();
-        uint32_t least = ~0u, most = 0;
-        each4<T, 4>(r, [&](int id, f4 l) {
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (inside(l[e], id + e)) {
-                    least = min(least, key_of(l[e]));
-                    most = max(most, key_of(l[e]));
-                    const uint32_t at = atomicAdd(&sh.listed, 1u);
-                    if (at < kList) sh.list[at] = composite(l[e], id + e);
-                }
-        });
-        if (most) {
-            atomicMin(&sh.key_lo, least);
-            atomicMax(&sh.key_hi, most);
-        }
-        __syncthreads();
-        listed = sh.listed;
-        lo = sh.key_lo;
-        hi = sh.key_hi;
-        __syncthreads();
-        if (listed <= kList || lo == hi) break;
-        // a finer histogram over the keys
-        const int shift = max(0, 32 - __builtin_clz(hi - lo) - 10);
-        clear_bins(sh);
+struct RowIds {  // of the row itself
+    static constexpr int COPIES = Shared<T>::COPIES;
+    const Row& r;
+    template <typename F>
+    __device__ __forceinline__ void each(const Shared<T>&, F f) const
+    {
         each4<T, 2>(r, [&](int id, f4 l) {
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                if (inside(l[e], id + e)) add((hi - key_of(l[e])) >> shift, l[e]);
+                if (l[e] > -INFINITY) f(composite(l[e], id + e), l[e], 0);
         });
-        __syncthreads();
-        find_bin(sh, before, [&](u64) { return limit; });
-        before = sh.before;
-        hi -= sh.bin << shift;
-        lo = max(lo, hi - ((1u << shift) - 1));
     }
-    if (listed > kList) {
-        // more ids than that of one logit: the rule keeps the first `ties` of them by id
-        const u64 w = masses ? weight(taylor, z, logit_of(lo)) : 1;
-        u64 ties;
-        if (limit.count) {
-            ties = limit.count - before;
-        } else {
-            ties = (u64)fmin((limit.mass - (double)before) / (double)w, (double)listed);
-            while (ties > 1 && !limit.inside(before + (ties - 1) * w)) ties--;
-            while (ties < (u64)listed && limit.inside(before + ties * w)) ties++;
-            ties = max(ties, (u64)1);
-        }
-        const int segments = (r.n + kSegment - 1) / kSegment, lane = threadIdx.x & 63;
-        constexpr int S = sizeof(sh.segments) / sizeof(u64) / T > 1 ? sizeof(sh.segments) / sizeof(u64) / T : 1;
-        auto equal = [&](int segment) {  // of the lane's four ids
-            const int id = segment * kSegment + 4 * lane;
-            const f4 l = allowed4(load4(r, id), mask4(r, id));
-            uint32_t same = 0;
-#pragma unroll
-            for (int e = 0; e < 4; e++) same |= (inside(l[e], id + e) ? 1u : 0u) << e;
-            return same;
-        };
-        for (int g = threadIdx.x >> 6; g < segments; g += T / 64) {
-            const int n = wave_sum_i32(__builtin_popcount(equal(g)));
-            if (lane == 0) sh.segments[g] = n;
-        }
-        __syncthreads();
-        u64 c[S], sum = 0, all;
-#pragma unroll
-        for (int k = 0; k < S; k++) {
-            const int g = S * threadIdx.x + k;
-            c[k] = g < segments ? sh.segments[g] : 0;
-            sum += c[k];
-        }
-        u64 upto = block_before<T>(sum, sh.waves, &all);
-#pragma unroll
-        for (int k = 0; k < S; k++) {
-            if (upto < ties && upto + c[k] >= ties) {
-                sh.bin = S * threadIdx.x + k;
-                sh.before = upto;
-            }
-            upto += c[k];
-        }
-        __syncthreads();
-        if (threadIdx.x < 64) {
-            const uint32_t same = equal(sh.bin);
-            int to = __builtin_popcount(same);
-            const int own = to;
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {
-                const int other = __shfl_up(to, off);
-                if (lane >= off) to += other;
-            }
-            int at = (int)sh.before + to - own;
-            for (int e = 0; e < 4; e++)
-                if ((same >> e) & 1 && ++at == (int)ties)
-                    sh.cut = (u64)lo << 32 | (uint32_t)~(int)(sh.bin * kSegment + 4 * lane + e);
-        }
-        __syncthreads();
-        return;
+    __device__ __forceinline__ u64* bins(Shared<T>& sh) const { return sh.bins; }
+    __device__ __forceinline__ u64 weight_of(const Shared<T>&, const Scale& z, float l, int) const { return weight(z, l); }
+};
+template <int T>
+struct ListIds {  // of sh.list, with their weights
+    static constexpr int COPIES = 1;
+    int listed;
+    template <typename F>
+    __device__ __forceinline__ void each(const Shared<T>& sh, F f) const
+    {
+        for (int e = threadIdx.x; e < listed; e += T) f(sh.list[e], logit_in(sh.list[e]), e);
     }
-    if (masses) weigh_list(sh, taylor, z, listed);
-    rank_list(sh, listed, !masses, [&](int, u64 own, u64 q, u64 larger) {
-        if (limit.inside(before + larger) && !limit.inside(before + larger + q)) sh.cut = own;
-    });
-    __syncthreads();
+    __device__ __forceinline__ u64* bins(Shared<T>& sh) const { return sh.counts; }
+    __device__ __forceinline__ u64 weight_of(const Shared<T>& sh, const Scale&, float, int e) const { return sh.weights[e]; }
+};
+
+// The place of a thread among those that share the ids of a short list, `threads` to one.
+struct Shares {
+    int threads, place, step, first;
+};
+template <int T>
+__device__ __forceinline__ Shares shares(int listed)
+{
+    Shares s;
+    s.threads = listed <= 64 ? min(16, T / 64) : listed <= 256 ? T / 256 : max(1, T / 512);
+    s.place = threadIdx.x & (s.threads - 1);
+    s.step = T / s.threads;
+    s.first = threadIdx.x / s.threads;
+    return s;
 }
 
-__device__ __forceinline__ float log_probability(Scale r, float l, u64 total)
+// The composite of the last id that a rule keeps of `ids` from `cut` on: the first
+// `count` (0: the share top_p of them, or with total0 the ids that weigh less than that
+// share of it before them).  0 where it keeps all.  A histogram by logit, finer ones by
+// composites where a bin has many ids, and ranks within the last.
+template <int T, typename Ids>
+__device__ __forceinline__ u64 last_kept(Shared<T>& sh, const Scale& z, const Ids& ids, u64 cut, int count, float top_p,
+                                         u64 total0)
 {
-    const double z = l == r.peak ? 0.0 : ((double)l - (double)r.peak) * r.inverse;
-    return (float)(z - log((double)total / kOne));
+    const bool masses = count == 0;
+    constexpr int C = Ids::COPIES;
+    u64* bins = ids.bins(sh);
+    const int copy = threadIdx.x & (C - 1);
+    auto quantity = [&](float l, int place) { return masses ? ids.weight_of(sh, z, l, place) : (u64)1; };
+    clear_bins<T>(bins, kBins * C);
+    ids.each(sh, [&](u64 c, float l, int place) {
+        const int b = first_bin(z, l);
+        if (b < kBins - 1 && c >= cut) atomicAdd(&bins[b * C + copy], quantity(l, place));
+    });
+    __syncthreads();
+    Limit limit = masses ? mass_limit(top_p, total0) : Limit{(u64)count, 0.0};
+    if (masses && total0 == 0)
+        limit = mass_limit(top_p, find_bin<T, true>(sh, bins, C, 0, limit, top_p));
+    else
+        find_bin<T, false>(sh, bins, C, 0, limit, 0.0f);
+    const int bin = sh.bin;
+    if (bin == kBins) return 0;
+    u64 lo = 0, hi = ~(u64)0, before = sh.before;
+    auto inside = [&](u64 c, float l) { return first_bin(z, l) == bin && c >= cut && c >= lo && c <= hi; };
+    int listed = 0;
+    // (64 bits, ten at a time: seven rounds end it, whatever a second look at the logits says)
+    for (int round = 0; round < 8; round++) {
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            sh.few_listed = 0;
+            sh.least = ~(u64)0;
+            sh.most = 0;
+        }
+        __syncthreads();
+        u64 least = ~(u64)0, most = 0;
+        ids.each(sh, [&](u64 c, float l, int place) {
+            if (inside(c, l)) {
+                least = min(least, c);
+                most = max(most, c);
+                const uint32_t at = atomicAdd(&sh.few_listed, 1u);
+                if (at < (uint32_t)kFew) {
+                    sh.few[at] = c;
+                    sh.few_weights[at] = quantity(l, place);
+                }
+            }
+        });
+        if (most) {
+            atomicMin(&sh.least, least);
+            atomicMax(&sh.most, most);
+        }
+        __syncthreads();
+        listed = sh.few_listed;
+        if (listed <= kFew) break;
+        lo = sh.least;
+        hi = sh.most;
+        const int shift = hi > lo ? max(0, 64 - __builtin_clzll(hi - lo) - 10) : 0;
+        clear_bins<T>(bins, kBins * C);
+        ids.each(sh, [&](u64 c, float l, int place) {
+            if (inside(c, l)) atomicAdd(&bins[(int)((hi - c) >> shift) * C + copy], quantity(l, place));
+        });
+        __syncthreads();
+        find_bin<T, false>(sh, bins, C, before, limit, 0.0f);
+        before = sh.before;
+        hi -= (u64)min(sh.bin, (uint32_t)kBins - 1) << shift;
+        lo = max(lo, hi - (((u64)1 << shift) - 1));
+    }
+    listed = min(listed, kFew);
+    if (threadIdx.x == 0) sh.cut = cut;
+    __syncthreads();
+    const Shares s = shares<T>(listed);
+    for (int e0 = 0; e0 < listed; e0 += s.step) {
+        const int e = e0 + s.first;
+        const u64 own = e < listed ? sh.few[e] : 0;
+        u64 larger = 0;
+        for (int i = s.place; i < listed; i += s.threads) {
+            const u64 q = sh.few_weights[i];
+            larger += sh.few[i] > own ? q : 0;
+        }
+        for (int off = 1; off < s.threads; off <<= 1) larger += __shfl_xor(larger, off);
+        larger += before;
+        if (e < listed && s.place == 0 && limit.inside(larger) && !limit.inside(larger + sh.few_weights[e])) sh.cut = own;
+    }
+    __syncthreads();
+    return sh.cut;
+}
+
+__device__ __forceinline__ float log_probability(const Scale& z, float l, u64 total)
+{
+    return (float)(((double)l - z.peak) * z.log2e * 0.6931471805599453 - log((double)total / kOne));
 }
 
 // The t of the draw.
@@ -432,19 +452,227 @@ __device__ __forceinline__ u64 drawn(float random, u64 total)
     return min((u64)fmin(u * (double)total, kOne * kMaxIds), total - 1);
 }
 
+// What a draw found: a thread that has the id has it, the others have -1; all have
+// `missed` where the list did not hold enough.
+struct Chosen {
+    int id;
+    float logprob;
+    bool missed;
+};
+
+// The rules and the draw over sh.list of up to kFew ids, by ranks.  total0: the
+// weight of all ids, for top_p without top_k.  open: ids below the list may be
+// kept too.
+template <int T>
+__device__ __forceinline__ Chosen draw_of_few(Shared<T>& sh, const Scale& z, const Rules& rules, int listed, u64 total0,
+                                              bool open)
+{
+    const Shares s = shares<T>(listed);
+    for (int e = threadIdx.x; e < listed; e += T) sh.weights[e] = weight(z, logit_in(sh.list[e]));
+    if (threadIdx.x == 0) sh.mass = sh.total = 0;
+    __syncthreads();
+    constexpr int K = T == 1024 ? 1 : 2;  // ids of a thread
+    u64 own[K], w[K], before[K];
+    bool kept[K];
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        const int e = s.first + s.step * k;
+        own[k] = e < listed ? sh.list[e] : 0;
+        w[k] = e < listed ? sh.weights[e] : 0;
+        u64 larger = 0;
+        uint32_t rank = 0;
+        for (int i = s.place; i < listed; i += s.threads) {
+            const u64 c = sh.list[i], x = sh.weights[i];
+            larger += c > own[k] ? x : 0;
+            rank += c > own[k] ? 1 : 0;
+        }
+        for (int off = 1; off < s.threads; off <<= 1) {
+            larger += __shfl_xor(larger, off);
+            rank += __shfl_xor(rank, off);
+        }
+        before[k] = larger;
+        kept[k] = e < listed && s.place == 0 && (rules.top_k == 0 || rank < (uint32_t)rules.top_k);
+        if (kept[k]) atomicMax(&sh.mass, larger + w[k]);  // (the last one has all)
+    }
+    __syncthreads();
+    const u64 mass = sh.mass;
+    const Limit limit = mass_limit(rules.top_p, rules.top_k ? mass : total0);
+    if (open && rules.by_mass && rules.top_k == 0 && limit.inside(mass)) return {-1, 0.0f, true};
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        kept[k] = kept[k] && (!rules.by_mass || limit.inside(before[k])) && (double)w[k] >= rules.least;
+        if (kept[k]) atomicMax(&sh.total, before[k] + w[k]);
+        const int e = s.first + s.step * k;
+        if (e < listed && s.place == 0) sh.weights[e] = kept[k] ? w[k] : 0;
+    }
+    __syncthreads();
+    const u64 total = sh.total, at = drawn(rules.random, total);
+    Chosen found = {-1, 0.0f, false};
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        u64 lower = 0;  // the kept weight of lower ids
+        for (int i = s.place; i < listed; i += s.threads) {
+            const u64 x = sh.weights[i];
+            lower += (uint32_t)sh.list[i] > (uint32_t)own[k] ? x : 0;
+        }
+        for (int off = 1; off < s.threads; off <<= 1) lower += __shfl_xor(lower, off);
+        if (kept[k] && lower <= at && at < lower + w[k])
+            found = {id_in(own[k]), log_probability(z, logit_in(own[k]), total), false};
+    }
+    return found;
+}
+
+// The same of more ids, by histograms.
+template <int T>
+__device__ __forceinline__ Chosen draw_of_many(Shared<T>& sh, const Scale& z, const Rules& rules, int listed, u64 total0,
+                                               bool open)
+{
+    u64 sum = 0;
+#pragma unroll 1
+    for (int e = threadIdx.x; e < listed; e += T) sum += sh.weights[e] = weight(z, logit_in(sh.list[e]));
+    const ListIds<T> ids = {listed};
+    u64 cut = 0;
+    if (open && rules.by_mass && rules.top_k == 0 && mass_limit(rules.top_p, total0).inside(block_sum(sh, sum)))
+        return {-1, 0.0f, true};
+#pragma unroll 1
+    for (int rule = rules.top_k ? 0 : 1; rule < (rules.by_mass ? 2 : 1); rule++)
+        cut = max(cut, last_kept(sh, z, ids, cut, rule == 0 ? rules.top_k : 0, rules.top_p, rules.top_k ? 0 : total0));
+    sum = 0;
+    for (int e = threadIdx.x; e < listed; e += T) {
+        const u64 w = sh.list[e] >= cut && (double)sh.weights[e] >= rules.least ? sh.weights[e] : 0;
+        sh.weights[e] = w;
+        sum += w;
+    }
+    const u64 total = block_sum(sh, sum), at = drawn(rules.random, total);
+    // in the order of the ids: the 512 ids, then the id
+    constexpr int SPAN = kMaxIds / kBins;
+    static_assert(SPAN <= kFew, "a bin's ids are few");  // (the list has an id once)
+    clear_bins<T>(sh.counts, kBins);
+    for (int e = threadIdx.x; e < listed; e += T) atomicAdd(&sh.counts[id_in(sh.list[e]) / SPAN], sh.weights[e]);
+    if (threadIdx.x == 0) sh.few_listed = 0;
+    __syncthreads();
+    find_bin<T, false>(sh, sh.counts, 1, 0, Limit{at + 1, 0.0}, 0.0f);
+    const int bin = sh.bin;
+    const u64 before = sh.before;
+    for (int e = threadIdx.x; e < listed; e += T)
+        if (id_in(sh.list[e]) / SPAN == bin && sh.weights[e]) {
+            const uint32_t to = atomicAdd(&sh.few_listed, 1u);
+            sh.few[to] = sh.list[e];
+            sh.few_weights[to] = sh.weights[e];
+        }
+    __syncthreads();
+    const int few = sh.few_listed;
+    const Shares s = shares<T>(few);
+    Chosen found = {-1, 0.0f, false};
+    for (int e0 = 0; e0 < few; e0 += s.step) {
+        const int e = e0 + s.first;
+        const u64 own = e < few ? sh.few[e] : 0;
+        u64 lower = 0;
+        for (int i = s.place; i < few; i += s.threads) {
+            const u64 x = sh.few_weights[i];
+            lower += (uint32_t)sh.few[i] > (uint32_t)own ? x : 0;
+        }
+        for (int off = 1; off < s.threads; off <<= 1) lower += __shfl_xor(lower, off);
+        lower += before;
+        if (e < few && s.place == 0 && lower <= at && at < lower + sh.few_weights[e])
+            found = {id_in(own), log_probability(z, logit_in(own), total), false};
+    }
+    return found;
+}
+
+// The draw over the row itself, of what `cut` and min_p leave: its waves' parts, then
+// the parts of the one that the draw falls into, down to a segment.
+template <int T>
+__device__ __forceinline__ Chosen draw_of_row(Shared<T>& sh, const Row& r, const Scale& z, const Rules& rules, u64 cut)
+{
+    constexpr int W = T / 64;
+    const int lane = threadIdx.x & 63, wave = wave_id(), segments = (r.n + kSegment - 1) / kSegment;
+    auto kept = [&](float l, int id) {
+        const u64 w = weight(z, l);
+        return (cut == 0 || composite(l, id) >= cut) && (double)w >= rules.least ? w : (u64)0;
+    };
+    u64 total = 0, at = 0, before = 0;
+    int first = 0, end = segments;
+    while (true) {
+        const int each = (end - first + W - 1) / W, from = first + wave * each, to = min(end, from + each);
+        u64 sum = 0;
+        auto add = [&](int id, f4 l) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) sum += kept(l[e], id + e);
+        };
+        walk<2>(r, from, min(to, r.n / kSegment), 1, add);
+        if (to == segments && from < to && r.n % kSegment) {
+            const int i = kSegment * (segments - 1) + 4 * lane;
+            add(i, segment4(r, i));
+        }
+        sum = wave_sum_u64(sum);
+        __syncthreads();
+        if (lane == 0) sh.waves[wave] = sum;
+        __syncthreads();
+        if (end - first == segments) {
+#pragma unroll
+            for (int w = 0; w < W; w++) total += sh.waves[w];
+            at = drawn(rules.random, total);
+        }
+        // (the last part at most, whatever a second look at the logits says: another stream may be writing them)
+        int part = 0;
+        for (int w = 0; w + 1 < W && first + (part + 1) * each < end; w++) {
+            if (before + sh.waves[w] > at) break;
+            before += sh.waves[w];
+            part++;
+        }
+        end = min(end, first + (part + 1) * each);
+        first += part * each;
+        if (each == 1) break;
+    }
+    Chosen found = {-1, 0.0f, false};
+    if (threadIdx.x < 64) {
+        const int id = first * kSegment + 4 * lane;
+        const f4 l = segment4(r, id);
+        u64 w[4], own = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            w[e] = kept(l[e], id + e);
+            own += w[e];
+        }
+        u64 from = before + wave_upto(own) - own;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (from <= at && at < from + w[e]) found = {id + e, log_probability(z, l[e], total), false};
+            from += w[e];
+        }
+    }
+    return found;
+}
+
+// A logit that at least `want` of the threads' largest are not below.
+template <int T>
+__device__ __forceinline__ float bound_of(Shared<T>& sh, const Scale& z, float most, int want)
+{
+    if (threadIdx.x == 0) sh.key = ~0u;
+    clear_bins<T>(sh.counts, kBins);
+    const int b = first_bin(z, most);
+    if (b < kBins - 1) atomicAdd(&sh.counts[b], (u64)1);
+    __syncthreads();
+    find_bin<T, false>(sh, sh.counts, 1, 0, Limit{(u64)want, 0.0}, 0.0f);
+    if (sh.bin == kBins) return -INFINITY;
+    if (b == (int)sh.bin) atomicMin(&sh.key, key_of(most));
+    __syncthreads();
+    return logit_of(sh.key);
+}
+
 template <int T>
 __global__ __launch_bounds__(T) void sample_kernel(SampleParams p)
 {
     __shared__ Shared<T> sh;
-    const int row = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const Row r = {p.logits + (size_t)row * p.ldx, p.mask ? p.mask + (size_t)row * p.mask_ld : nullptr,
-                   p.mask ? min(p.n, 32 * min(p.words, kMaxIds / 32)) : p.n};
+    const int row = blockIdx.x;
+    Row r = {p.logits + (size_t)row * p.ldx, p.mask ? p.mask + (size_t)row * p.mask_ld : nullptr,
+             p.mask ? min(p.n, 32 * min(p.words, kMaxIds / 32)) : p.n, false};
     const float t = p.s.temperature ? p.s.temperature[row] : 1.0f;
     const int top_k = p.s.top_k ? p.s.top_k[row] : 0;
     const float top_p = p.s.top_p ? p.s.top_p[row] : 1.0f;
     const float min_p = p.s.min_p ? p.s.min_p[row] : 0.0f;
     const float random = p.s.random[row];
-    const double(&taylor)[kTerms] = p.taylor;
 
     // the thread's first id, then the row's
     float most = -INFINITY;
@@ -460,171 +688,97 @@ __global__ __launch_bounds__(T) void sample_kernel(SampleParams p)
     u64 best = most > -INFINITY ? composite(most, most_id) : 0;
 #pragma unroll
     for (int off = 32; off; off >>= 1) best = max(best, (u64)__shfl_xor(best, off));
-    if (lane == 0) sh.waves[wave] = best;
+    if ((threadIdx.x & 63) == 0) sh.waves[threadIdx.x >> 6] = best;
+    if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < T / 64; w++) best = max(best, sh.waves[w]);
-    const bool first_only = !(t > 0.0f) || top_k == 1 || top_p <= 0.0f;
-    if (best == 0 || first_only) {
+    __syncthreads();
+    if (best == 0 || !(t > 0.0f) || top_k == 1 || top_p <= 0.0f) {
         if (threadIdx.x == 0) {
-            p.ids[row] = best ? ~(int)(uint32_t)best : -1;
+            p.ids[row] = best ? id_in(best) : -1;
             if (p.logprobs) p.logprobs[row] = best ? 0.0f : -INFINITY;
         }
         return;
     }
-    const double inverse = 1.0 / (double)t;
-    const Scale z = {logit_of((uint32_t)(best >> 32)), inverse, 1.4426950408889634 * inverse,
-                     fminf((float)(2 * (kBins - 1) * inverse / -kLeastScore), 3e38f)};
-    const bool by_mass = top_p < 1.0f;
-    const double least = min_p > 0.0f ? (double)fminf(min_p, 1.0f) * kOne : 0.0;
+    r.infinite = logit_in(best) == INFINITY;
+    if (r.infinite) most = most == INFINITY ? 0.0f : -INFINITY;
+    const float peak = r.infinite ? 0.0f : logit_in(best);
+    const Scale z = scale_of(peak, t, p.power);
+    const Rules rules = {top_k > 0 && top_k < r.n ? top_k : 0, top_p < 1.0f, top_p, random,
+                         min_p > 0.0f ? (double)fminf(min_p, 1.0f) * kOne : 0.0};
 
-    if (top_k > 0 && top_k <= kFew) {
-        // At least top_k ids are as large as the top_k-th largest of the threads'
-        // first ones, and not many more: all from its bin on, in a list.
-        uint32_t* counts = reinterpret_cast<uint32_t*>(sh.segments);
-        constexpr int B = kBins / T;
-        for (int b = threadIdx.x; b < kBins; b += T) counts[b] = 0;
-        if (threadIdx.x == 0) {
-            sh.listed = 0;
-            sh.bin = kBins - 2;
+    // A logit that nothing kept is below, or that hardly anything will be (open): as
+    // many of the threads' largest are not below it as top_k keeps, or some more ids in
+    // all, as far as ids fall to the threads by chance (that many of T threads: T ln(T / (T - many)) ids).
+    float bound = -INFINITY;
+    bool open = false;
+    if (rules.top_k || rules.by_mass) {
+        const bool sure = rules.top_k && rules.top_k <= T / 4;
+        const float ids = rules.top_k ? 1.25f * rules.top_k + 64.0f : 3.0f * T;
+        const int want = sure ? rules.top_k : min((int)(T * (1.0f - __expf(-ids / T))), T - T / 64);
+        bound = bound_of(sh, z, most, want);
+        open = !sure && bound > -INFINITY;
+    }
+    // (min_p bounds it too, but the mass of top_p's ids is that of all that top_k keeps)
+    if (rules.least > 0.0 && !(rules.top_k && rules.by_mass)) {
+        const float down = -logf(fminf(min_p, 1.0f)) * t;
+        const float lowest = peak - down - 1e-5f * (fabsf(peak) + down) - 1e-30f;
+        if (lowest > bound) {
+            bound = lowest;
+            open = false;
         }
-        __syncthreads();
-        if (most > -INFINITY) atomicAdd(&counts[first_bin(z, most)], 1u);
-        __syncthreads();
-        u64 sum = 0, all;
-        uint32_t c[B];
+    }
+
+    Chosen found = {-1, 0.0f, true};
+    if (bound > -INFINITY || r.n <= Shared<T>::LIST) {
+        const bool weigh = rules.by_mass && !rules.top_k;
+        u64 total = 0;
+        auto gather = [&](int id, f4 l) {
+            int taken = 0;
 #pragma unroll
-        for (int k = 0; k < B; k++) {
-            c[k] = B * threadIdx.x + k < kBins - 1 ? counts[B * threadIdx.x + k] : 0;
-            sum += c[k];
-        }
-        u64 upto = block_before<T>(sum, sh.waves, &all);
-#pragma unroll
-        for (int k = 0; k < B; k++) {
-            if (upto < (u64)top_k && upto + c[k] >= (u64)top_k) sh.bin = B * threadIdx.x + k;
-            upto += c[k];
-        }
-        __syncthreads();
-        const int bin = sh.bin;
-        each4<T, 4>(r, [&](int id, f4 l) {
+            for (int e = 0; e < 4; e++) taken |= (l[e] >= bound && l[e] > -INFINITY ? 1 : 0) << e;
+            if (__ballot(taken) == 0) return;
+            uint32_t at = taken ? atomicAdd(&sh.listed, (uint32_t)__builtin_popcount(taken)) : 0;
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                if (first_bin(z, l[e]) <= bin) {
-                    const uint32_t at = atomicAdd(&sh.listed, 1u);
-                    if (at < kList) sh.list[at] = composite(l[e], id + e);
+                if ((taken >> e) & 1) {
+                    if (at < (uint32_t)Shared<T>::LIST) sh.list[at] = composite(l[e], id + e);
+                    at++;
                 }
-        });
+        };
+        if (weigh) {
+            each4<T, 2>(r, [&](int id, f4 l) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) total += weight(z, l[e]);
+                gather(id, l);
+            });
+            total = block_sum(sh, total);
+        } else {
+            each4<T, 4>(r, gather);
+        }
         __syncthreads();
         const int listed = sh.listed;
-        if (listed <= kList) {
-            // ranks, then what each rule keeps of them, all of the list's prefixes
-            u64 first_k = 0;
-            weigh_list(sh, taylor, z, listed);
-            rank_list(sh, listed, true, [&](int e, u64, u64, u64 larger) { sh.segments[e] = larger; });
-            __syncthreads();
-            const bool mine = (int)threadIdx.x < listed, more = (int)threadIdx.x + T < listed;
-            u64 before[2] = {0, 0}, w[2] = {0, 0}, kept = 0, total;
-            static_assert(kList <= 2 * 256, "two ids a thread at most");
-            const bool in[2] = {mine && sh.segments[threadIdx.x] < (u64)top_k,
-                                more && sh.segments[threadIdx.x + T] < (u64)top_k};
-            if (in[0]) w[0] = sh.weights[threadIdx.x];
-            if (in[1]) w[1] = sh.weights[threadIdx.x + T];
-            block_before<T>(w[0] + w[1], sh.waves, &first_k);
-            if (by_mass) {
-                rank_list(sh, listed, false, [&](int e, u64, u64, u64 larger) { sh.segments[e] = larger; });
-                __syncthreads();
-                if (in[0]) before[0] = sh.segments[threadIdx.x];
-                if (in[1]) before[1] = sh.segments[threadIdx.x + T];
-            }
-            const double mass = (double)top_p * (double)first_k;
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                if (by_mass && before[k] != 0 && !((double)before[k] < mass)) w[k] = 0;
-                if ((double)w[k] < least) w[k] = 0;
-                kept += w[k];
-                if ((int)threadIdx.x + k * T < listed) sh.weights[threadIdx.x + k * T] = w[k];
-            }
-            block_before<T>(kept, sh.waves, &total);
-            // the draw, in the order of the ids: composites' low halves, inverted
-            const u64 at = drawn(random, total);
-            for (int e = threadIdx.x; e < listed; e += T) sh.list[e] = (sh.list[e] << 32) | (sh.list[e] >> 32);
-            __syncthreads();
-            rank_list(sh, listed, false, [&](int, u64 own, u64 weight, u64 larger) {
-                if (larger <= at && at < larger + weight) {
-                    const int id = ~(int)(uint32_t)(own >> 32);
-                    p.ids[row] = id;
-                    if (p.logprobs) p.logprobs[row] = log_probability(z, logit_of((uint32_t)own), total);
-                }
-            });
-            return;
+        if (listed <= Shared<T>::LIST && !(open && listed < rules.top_k)) {
+            if (listed <= kFew)
+                found = draw_of_few(sh, z, rules, listed, total, open);
+            else
+                found = draw_of_many(sh, z, rules, listed, total, open);
         }
-        __syncthreads();
     }
-
-    if (threadIdx.x == 0) sh.cut = 0;
-    __syncthreads();
-    const bool by_count = top_k > 0 && top_k < r.n;
-    for (int rule = by_count ? 0 : 1; rule < (by_mass ? 2 : 1); rule++) keep(sh, taylor, r, z, rule == 0 ? top_k : 0, top_p);
-
-    // the draw, in the order of the ids
-    const u64 cut = sh.cut;
-    auto kept = [&](float l, int id) {
-        if (!(l > -INFINITY && composite(l, id) >= cut)) return (u64)0;
-        const u64 w = weight(taylor, z, l);
-        return (double)w < least ? (u64)0 : w;
-    };
-    const int segments = (r.n + kSegment - 1) / kSegment;
-    each4<T, 2>(r, [&](int id, f4 l) {
-        u64 sum = 0;
-#pragma unroll
-        for (int e = 0; e < 4; e++) sum += kept(l[e], id + e);
-        sum = __ballot(sum != 0) ? wave_sum_u64(sum) : 0;
-        if (lane == 0) sh.segments[id / kSegment] = sum;
-    });
-    __syncthreads();
-    constexpr int S = sizeof(sh.segments) / sizeof(u64) / T > 1 ? sizeof(sh.segments) / sizeof(u64) / T : 1;
-    u64 m[S], sum = 0, total;
-#pragma unroll
-    for (int k = 0; k < S; k++) {
-        const int g = S * threadIdx.x + k;
-        m[k] = g < segments ? sh.segments[g] : 0;
-        sum += m[k];
-    }
-    u64 before = block_before<T>(sum, sh.waves, &total);
-    const u64 at = drawn(random, total);
-#pragma unroll
-    for (int k = 0; k < S; k++) {
-        if (before <= at && at < before + m[k]) {
-            sh.bin = S * threadIdx.x + k;
-            sh.before = before;
+    if (found.missed) {
+        const RowIds<T> ids = {r};
+        u64 cut = 0;
+#pragma unroll 1
+        for (int rule = rules.top_k ? 0 : 1; rule < (rules.by_mass ? 2 : 1); rule++) {
+            __syncthreads();
+            cut = max(cut, last_kept(sh, z, ids, cut, rule == 0 ? rules.top_k : 0, top_p, 0));
         }
-        before += m[k];
+        found = draw_of_row(sh, r, z, rules, cut);
     }
-    __syncthreads();
-    if (threadIdx.x >= 64) return;
-    const int id = (int)sh.bin * kSegment + 4 * lane;
-    const f4 l = allowed4(load4(r, id), mask4(r, id));
-    u64 w[4], upto = 0;
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-        w[e] = kept(l[e], id + e);
-        upto += w[e];
-    }
-    const u64 own = upto;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const u64 other = __shfl_up(upto, off);
-        if (lane >= off) upto += other;
-    }
-    u64 from = sh.before + upto - own;
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-        if (from <= at && at < from + w[e]) {
-            p.ids[row] = id + e;
-            if (p.logprobs) p.logprobs[row] = log_probability(z, l[e], total);
-        }
-        from += w[e];
+    if (found.id >= 0) {
+        p.ids[row] = found.id;
+        if (p.logprobs) p.logprobs[row] = found.logprob;
     }
 }
 
@@ -663,8 +817,7 @@ int32_t nhip_sample_dev(const float* d_logits, int32_t ldx, int32_t n, int32_t r
     (void)d_workspace;
     (void)workspace_bytes;
     SampleParams p = {d_logits, d_mask, *s, d_ids, d_logprobs, ldx, n, mask_ld, words, {}};
-    p.taylor[0] = 1.0;
-    for (int k = 1; k < kTerms; k++) p.taylor[k] = p.taylor[k - 1] * 0.6931471805599453 / k;
+    std::copy(kPower, kPower + kTerms, p.power);
     if (n <= 4096)
         hipLaunchKernelGGL((sample_kernel<256>), dim3(rows), dim3(256), 0, as_stream(stream), p);
     else
