@@ -22,7 +22,6 @@ namespace nhip {
 namespace {
 
 constexpr int kBins = 1024;    // of a histogram; in the first the last one holds what weighs nothing
-constexpr int kFew = 512;      // ids that are ranked against one another
 constexpr int kSegment = 256;  // ids of a wave's step, four a lane
 constexpr int kMaxIds = 1 << 19;
 constexpr int kTerms = 10;
@@ -46,6 +45,7 @@ struct SampleParams {
     float* logprobs;
     int32_t ldx, n, mask_ld, words;
     double power[kTerms];  // kPower, as arguments: they stay in scalar registers
+    float none;            // -inf, which the compiler does not know (it would take NaN for a number)
 };
 
 // A larger key for a larger logit; +0 and -0 alike.
@@ -68,12 +68,13 @@ struct Row {
     const float* x;
     const uint32_t* mask;
     int n;
+    float none;  // -inf
     bool infinite;
 };
 __device__ __forceinline__ f4 counted4(const Row& r, f4 v, uint32_t bits)
 {
 #pragma unroll
-    for (int e = 0; e < 4; e++) v[e] = v[e] > -INFINITY ? v[e] : -INFINITY;
+    for (int e = 0; e < 4; e++) v[e] = __builtin_amdgcn_fmed3f(v[e], r.none, INFINITY);  // (of a NaN the least)
     if (r.mask) {
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] = (bits >> e) & 1 ? v[e] : -INFINITY;
@@ -208,6 +209,7 @@ __device__ __forceinline__ u64 wave_upto(u64 v)
 template <int T>
 struct Shared {
     static constexpr int COPIES = T == 1024 ? 16 : 4, LIST = kBins * COPIES / 2;
+    static constexpr int RANKED = T / 2, FEW = T / 2;  // ids that are ranked against one another
     union {
         u64 bins[kBins * COPIES];
         struct {
@@ -215,7 +217,7 @@ struct Shared {
         };
     };
     u64 counts[kBins];
-    u64 few[kFew], few_weights[kFew];
+    u64 few[FEW], few_weights[FEW];
     u64 waves[T / 64];
     uint32_t listed, few_listed, bin, key;
     u64 cut, before, mass, total, least, most;
@@ -255,7 +257,7 @@ struct Rules {
     int top_k;  // 0: all
     bool by_mass;
     float top_p, random;
-    double least;  // min_p's weight
+    u64 least;  // min_p's weight, rounded up
 };
 
 // The bin of a histogram (copies of it side by side) in which a rule ends, and
@@ -343,7 +345,7 @@ template <int T>
 __device__ __forceinline__ Shares shares(int listed)
 {
     Shares s;
-    s.threads = listed <= 64 ? min(16, T / 64) : listed <= 256 ? T / 256 : max(1, T / 512);
+    s.threads = listed <= T / 16 ? 16 : listed <= T / 4 ? 4 : 2;
     s.place = threadIdx.x & (s.threads - 1);
     s.step = T / s.threads;
     s.first = threadIdx.x / s.threads;
@@ -394,7 +396,7 @@ __device__ __forceinline__ u64 last_kept(Shared<T>& sh, const Scale& z, const Id
                 least = min(least, c);
                 most = max(most, c);
                 const uint32_t at = atomicAdd(&sh.few_listed, 1u);
-                if (at < (uint32_t)kFew) {
+                if (at < (uint32_t)Shared<T>::FEW) {
                     sh.few[at] = c;
                     sh.few_weights[at] = quantity(l, place);
                 }
@@ -406,7 +408,7 @@ __device__ __forceinline__ u64 last_kept(Shared<T>& sh, const Scale& z, const Id
         }
         __syncthreads();
         listed = sh.few_listed;
-        if (listed <= kFew) break;
+        if (listed <= Shared<T>::FEW) break;
         lo = sh.least;
         hi = sh.most;
         const int shift = hi > lo ? max(0, 64 - __builtin_clzll(hi - lo) - 10) : 0;
@@ -420,22 +422,20 @@ __device__ __forceinline__ u64 last_kept(Shared<T>& sh, const Scale& z, const Id
         hi -= (u64)min(sh.bin, (uint32_t)kBins - 1) << shift;
         lo = max(lo, hi - (((u64)1 << shift) - 1));
     }
-    listed = min(listed, kFew);
+    listed = min(listed, Shared<T>::FEW);
     if (threadIdx.x == 0) sh.cut = cut;
     __syncthreads();
     const Shares s = shares<T>(listed);
-    for (int e0 = 0; e0 < listed; e0 += s.step) {
-        const int e = e0 + s.first;
-        const u64 own = e < listed ? sh.few[e] : 0;
-        u64 larger = 0;
-        for (int i = s.place; i < listed; i += s.threads) {
-            const u64 q = sh.few_weights[i];
-            larger += sh.few[i] > own ? q : 0;
-        }
-        for (int off = 1; off < s.threads; off <<= 1) larger += __shfl_xor(larger, off);
-        larger += before;
-        if (e < listed && s.place == 0 && limit.inside(larger) && !limit.inside(larger + sh.few_weights[e])) sh.cut = own;
+    const u64 own = s.first < listed ? sh.few[s.first] : 0;
+    u64 larger = 0;
+    for (int i = s.place; i < listed; i += s.threads) {
+        const u64 q = sh.few_weights[i];
+        larger += sh.few[i] > own ? q : 0;
     }
+    for (int off = 1; off < s.threads; off <<= 1) larger += __shfl_xor(larger, off);
+    larger += before;
+    if (s.first < listed && s.place == 0 && limit.inside(larger) && !limit.inside(larger + sh.few_weights[s.first]))
+        sh.cut = own;
     __syncthreads();
     return sh.cut;
 }
@@ -460,7 +460,7 @@ struct Chosen {
     bool missed;
 };
 
-// The rules and the draw over sh.list of up to kFew ids, by ranks.  total0: the
+// The rules and the draw over sh.list of up to RANKED ids, by ranks.  total0: the
 // weight of all ids, for top_p without top_k.  open: ids below the list may be
 // kept too.
 template <int T>
@@ -468,64 +468,50 @@ __device__ __forceinline__ Chosen draw_of_few(Shared<T>& sh, const Scale& z, con
                                               bool open)
 {
     const Shares s = shares<T>(listed);
-    for (int e = threadIdx.x; e < listed; e += T) sh.weights[e] = weight(z, logit_in(sh.list[e]));
+    if ((int)threadIdx.x < listed) sh.weights[threadIdx.x] = weight(z, logit_in(sh.list[threadIdx.x]));
     if (threadIdx.x == 0) sh.mass = sh.total = 0;
     __syncthreads();
-    constexpr int K = T == 1024 ? 1 : 2;  // ids of a thread
-    u64 own[K], w[K], before[K];
-    bool kept[K];
-#pragma unroll
-    for (int k = 0; k < K; k++) {
-        const int e = s.first + s.step * k;
-        own[k] = e < listed ? sh.list[e] : 0;
-        w[k] = e < listed ? sh.weights[e] : 0;
-        u64 larger = 0;
-        uint32_t rank = 0;
-        for (int i = s.place; i < listed; i += s.threads) {
-            const u64 c = sh.list[i], x = sh.weights[i];
-            larger += c > own[k] ? x : 0;
-            rank += c > own[k] ? 1 : 0;
-        }
-        for (int off = 1; off < s.threads; off <<= 1) {
-            larger += __shfl_xor(larger, off);
-            rank += __shfl_xor(rank, off);
-        }
-        before[k] = larger;
-        kept[k] = e < listed && s.place == 0 && (rules.top_k == 0 || rank < (uint32_t)rules.top_k);
-        if (kept[k]) atomicMax(&sh.mass, larger + w[k]);  // (the last one has all)
+    const bool first = s.first < listed && s.place == 0;
+    const u64 own = s.first < listed ? sh.list[s.first] : 0, w = s.first < listed ? sh.weights[s.first] : 0;
+    u64 larger = 0;
+    uint32_t rank = 0;
+    for (int i = s.place; i < listed; i += s.threads) {
+        const u64 c = sh.list[i], x = sh.weights[i];
+        larger += c > own ? x : 0;
+        rank += c > own ? 1 : 0;
     }
-    __syncthreads();
-    const u64 mass = sh.mass;
-    const Limit limit = mass_limit(rules.top_p, rules.top_k ? mass : total0);
-    if (open && rules.by_mass && rules.top_k == 0 && limit.inside(mass)) return {-1, 0.0f, true};
-#pragma unroll
-    for (int k = 0; k < K; k++) {
-        kept[k] = kept[k] && (!rules.by_mass || limit.inside(before[k])) && (double)w[k] >= rules.least;
-        if (kept[k]) atomicMax(&sh.total, before[k] + w[k]);
-        const int e = s.first + s.step * k;
-        if (e < listed && s.place == 0) sh.weights[e] = kept[k] ? w[k] : 0;
+    for (int off = 1; off < s.threads; off <<= 1) {
+        larger += __shfl_xor(larger, off);
+        rank += __shfl_xor(rank, off);
     }
+    bool kept = first && (rules.top_k == 0 || rank < (uint32_t)rules.top_k);
+    if (rules.by_mass) {
+        if (kept) atomicMax(&sh.mass, larger + w);  // (the last one has all)
+        __syncthreads();
+        const u64 mass = sh.mass;
+        const Limit limit = mass_limit(rules.top_p, rules.top_k ? mass : total0);
+        if (open && rules.top_k == 0 && limit.inside(mass)) return {-1, 0.0f, true};
+        kept = kept && limit.inside(larger);
+    }
+    kept = kept && w >= rules.least;
+    if (kept) atomicMax(&sh.total, larger + w);
+    if (first) sh.weights[s.first] = kept ? w : 0;
     __syncthreads();
     const u64 total = sh.total, at = drawn(rules.random, total);
-    Chosen found = {-1, 0.0f, false};
-#pragma unroll
-    for (int k = 0; k < K; k++) {
-        u64 lower = 0;  // the kept weight of lower ids
-        for (int i = s.place; i < listed; i += s.threads) {
-            const u64 x = sh.weights[i];
-            lower += (uint32_t)sh.list[i] > (uint32_t)own[k] ? x : 0;
-        }
-        for (int off = 1; off < s.threads; off <<= 1) lower += __shfl_xor(lower, off);
-        if (kept[k] && lower <= at && at < lower + w[k])
-            found = {id_in(own[k]), log_probability(z, logit_in(own[k]), total), false};
+    u64 lower = 0;  // the kept weight of lower ids
+    for (int i = s.place; i < listed; i += s.threads) {
+        const u64 x = sh.weights[i];
+        lower += (uint32_t)sh.list[i] > (uint32_t)own ? x : 0;
     }
-    return found;
+    for (int off = 1; off < s.threads; off <<= 1) lower += __shfl_xor(lower, off);
+    if (kept && lower <= at && at < lower + w) return {id_in(own), log_probability(z, logit_in(own), total), false};
+    return {-1, 0.0f, false};
 }
 
 // The same of more ids, by histograms.
 template <int T>
 __device__ __forceinline__ Chosen draw_of_many(Shared<T>& sh, const Scale& z, const Rules& rules, int listed, u64 total0,
-                                               bool open)
+                                               bool open, int n)
 {
     u64 sum = 0;
 #pragma unroll 1
@@ -539,45 +525,41 @@ __device__ __forceinline__ Chosen draw_of_many(Shared<T>& sh, const Scale& z, co
         cut = max(cut, last_kept(sh, z, ids, cut, rule == 0 ? rules.top_k : 0, rules.top_p, rules.top_k ? 0 : total0));
     sum = 0;
     for (int e = threadIdx.x; e < listed; e += T) {
-        const u64 w = sh.list[e] >= cut && (double)sh.weights[e] >= rules.least ? sh.weights[e] : 0;
+        const u64 w = sh.list[e] >= cut && sh.weights[e] >= rules.least ? sh.weights[e] : 0;
         sh.weights[e] = w;
         sum += w;
     }
     const u64 total = block_sum(sh, sum), at = drawn(rules.random, total);
-    // in the order of the ids: the 512 ids, then the id
-    constexpr int SPAN = kMaxIds / kBins;
-    static_assert(SPAN <= kFew, "a bin's ids are few");  // (the list has an id once)
+    // in the order of the ids: a few neighbours of them, then the id
+    static_assert(kMaxIds / kBins <= Shared<1024>::FEW, "a bin's ids are few");  // (the list has an id once)
+    const int shift = max(0, 32 - __builtin_clz(n) - 10);  // (n <= 4096 for 256 threads)
     clear_bins<T>(sh.counts, kBins);
-    for (int e = threadIdx.x; e < listed; e += T) atomicAdd(&sh.counts[id_in(sh.list[e]) / SPAN], sh.weights[e]);
+    for (int e = threadIdx.x; e < listed; e += T) atomicAdd(&sh.counts[min(id_in(sh.list[e]) >> shift, kBins - 1)], sh.weights[e]);
     if (threadIdx.x == 0) sh.few_listed = 0;
     __syncthreads();
     find_bin<T, false>(sh, sh.counts, 1, 0, Limit{at + 1, 0.0}, 0.0f);
     const int bin = sh.bin;
     const u64 before = sh.before;
     for (int e = threadIdx.x; e < listed; e += T)
-        if (id_in(sh.list[e]) / SPAN == bin && sh.weights[e]) {
-            const uint32_t to = atomicAdd(&sh.few_listed, 1u);
+        if (id_in(sh.list[e]) >> shift == bin && sh.weights[e]) {
+            const uint32_t to = min(atomicAdd(&sh.few_listed, 1u), (uint32_t)Shared<T>::FEW - 1);
             sh.few[to] = sh.list[e];
             sh.few_weights[to] = sh.weights[e];
         }
     __syncthreads();
-    const int few = sh.few_listed;
+    const int few = min(sh.few_listed, (uint32_t)Shared<T>::FEW);
     const Shares s = shares<T>(few);
-    Chosen found = {-1, 0.0f, false};
-    for (int e0 = 0; e0 < few; e0 += s.step) {
-        const int e = e0 + s.first;
-        const u64 own = e < few ? sh.few[e] : 0;
-        u64 lower = 0;
-        for (int i = s.place; i < few; i += s.threads) {
-            const u64 x = sh.few_weights[i];
-            lower += (uint32_t)sh.few[i] > (uint32_t)own ? x : 0;
-        }
-        for (int off = 1; off < s.threads; off <<= 1) lower += __shfl_xor(lower, off);
-        lower += before;
-        if (e < few && s.place == 0 && lower <= at && at < lower + sh.few_weights[e])
-            found = {id_in(own), log_probability(z, logit_in(own), total), false};
+    const u64 own = s.first < few ? sh.few[s.first] : 0;
+    u64 lower = 0;
+    for (int i = s.place; i < few; i += s.threads) {
+        const u64 x = sh.few_weights[i];
+        lower += (uint32_t)sh.few[i] > (uint32_t)own ? x : 0;
     }
-    return found;
+    for (int off = 1; off < s.threads; off <<= 1) lower += __shfl_xor(lower, off);
+    lower += before;
+    if (s.first < few && s.place == 0 && lower <= at && at < lower + sh.few_weights[s.first])
+        return {id_in(own), log_probability(z, logit_in(own), total), false};
+    return {-1, 0.0f, false};
 }
 
 // The draw over the row itself, of what `cut` and min_p leave: its waves' parts, then
@@ -589,7 +571,7 @@ __device__ __forceinline__ Chosen draw_of_row(Shared<T>& sh, const Row& r, const
     const int lane = threadIdx.x & 63, wave = wave_id(), segments = (r.n + kSegment - 1) / kSegment;
     auto kept = [&](float l, int id) {
         const u64 w = weight(z, l);
-        return (cut == 0 || composite(l, id) >= cut) && (double)w >= rules.least ? w : (u64)0;
+        return (cut == 0 || composite(l, id) >= cut) && w >= rules.least ? w : (u64)0;
     };
     u64 total = 0, at = 0, before = 0;
     int first = 0, end = segments;
@@ -667,7 +649,7 @@ __global__ __launch_bounds__(T) void sample_kernel(SampleParams p)
     __shared__ Shared<T> sh;
     const int row = blockIdx.x;
     Row r = {p.logits + (size_t)row * p.ldx, p.mask ? p.mask + (size_t)row * p.mask_ld : nullptr,
-             p.mask ? min(p.n, 32 * min(p.words, kMaxIds / 32)) : p.n, false};
+             p.mask ? min(p.n, 32 * min(p.words, kMaxIds / 32)) : p.n, p.none, false};
     const float t = p.s.temperature ? p.s.temperature[row] : 1.0f;
     const int top_k = p.s.top_k ? p.s.top_k[row] : 0;
     const float top_p = p.s.top_p ? p.s.top_p[row] : 1.0f;
@@ -701,12 +683,12 @@ __global__ __launch_bounds__(T) void sample_kernel(SampleParams p)
         }
         return;
     }
-    r.infinite = logit_in(best) == INFINITY;
+    r.infinite = __builtin_amdgcn_readfirstlane(logit_in(best) == INFINITY);
     if (r.infinite) most = most == INFINITY ? 0.0f : -INFINITY;
     const float peak = r.infinite ? 0.0f : logit_in(best);
     const Scale z = scale_of(peak, t, p.power);
     const Rules rules = {top_k > 0 && top_k < r.n ? top_k : 0, top_p < 1.0f, top_p, random,
-                         min_p > 0.0f ? (double)fminf(min_p, 1.0f) * kOne : 0.0};
+                         min_p > 0.0f ? (u64)ceil((double)fminf(min_p, 1.0f) * kOne) : 0};
 
     // A logit that nothing kept is below, or that hardly anything will be (open): as
     // many of the threads' largest are not below it as top_k keeps, or some more ids in
@@ -721,7 +703,7 @@ __global__ __launch_bounds__(T) void sample_kernel(SampleParams p)
         open = !sure && bound > -INFINITY;
     }
     // (min_p bounds it too, but the mass of top_p's ids is that of all that top_k keeps)
-    if (rules.least > 0.0 && !(rules.top_k && rules.by_mass)) {
+    if (rules.least && !(rules.top_k && rules.by_mass)) {
         const float down = -logf(fminf(min_p, 1.0f)) * t;
         const float lowest = peak - down - 1e-5f * (fabsf(peak) + down) - 1e-30f;
         if (lowest > bound) {
@@ -731,14 +713,15 @@ __global__ __launch_bounds__(T) void sample_kernel(SampleParams p)
     }
 
     Chosen found = {-1, 0.0f, true};
-    if (bound > -INFINITY || r.n <= Shared<T>::LIST) {
+    if (bound > -INFINITY || (r.n <= Shared<T>::LIST && (rules.top_k || rules.by_mass))) {
+        bound = fmaxf(bound, -3.4028235e38f);  // (never -inf, which is no id's)
         const bool weigh = rules.by_mass && !rules.top_k;
         u64 total = 0;
         auto gather = [&](int id, f4 l) {
+            if (__ballot(fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= bound) == 0) return;
             int taken = 0;
 #pragma unroll
-            for (int e = 0; e < 4; e++) taken |= (l[e] >= bound && l[e] > -INFINITY ? 1 : 0) << e;
-            if (__ballot(taken) == 0) return;
+            for (int e = 0; e < 4; e++) taken |= (l[e] >= bound ? 1 : 0) << e;
             uint32_t at = taken ? atomicAdd(&sh.listed, (uint32_t)__builtin_popcount(taken)) : 0;
 #pragma unroll
             for (int e = 0; e < 4; e++)
@@ -760,10 +743,10 @@ __global__ __launch_bounds__(T) void sample_kernel(SampleParams p)
         __syncthreads();
         const int listed = sh.listed;
         if (listed <= Shared<T>::LIST && !(open && listed < rules.top_k)) {
-            if (listed <= kFew)
+            if (listed <= Shared<T>::RANKED)
                 found = draw_of_few(sh, z, rules, listed, total, open);
             else
-                found = draw_of_many(sh, z, rules, listed, total, open);
+                found = draw_of_many(sh, z, rules, listed, total, open, r.n);
         }
     }
     if (found.missed) {
@@ -816,7 +799,7 @@ int32_t nhip_sample_dev(const float* d_logits, int32_t ldx, int32_t n, int32_t r
     if (rc) return rc;
     (void)d_workspace;
     (void)workspace_bytes;
-    SampleParams p = {d_logits, d_mask, *s, d_ids, d_logprobs, ldx, n, mask_ld, words, {}};
+    SampleParams p = {d_logits, d_mask, *s, d_ids, d_logprobs, ldx, n, mask_ld, words, {}, -INFINITY};
     std::copy(kPower, kPower + kTerms, p.power);
     if (n <= 4096)
         hipLaunchKernelGGL((sample_kernel<256>), dim3(rows), dim3(256), 0, as_stream(stream), p);
