@@ -113,6 +113,32 @@ __device__ __forceinline__ u64 weight(const Scale& z, float l)
     return (u64)__double_as_longlong(x) & 0xFFFFFFFFFFFFFull;
 }
 
+// Four of them, a chain of 20 dependent operations each, side by side.
+struct Weights {
+    u64 w[4];
+};
+__device__ __forceinline__ Weights weights4(const Scale& z, f4 l)
+{
+    double y[4], f[4];
+    int n[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const double t = fmax(fma((double)l[e] - z.peak, z.log2e, 42.0), -22.0), whole = rint(t);
+        f[e] = t - whole;
+        n[e] = (int)whole;
+        y[e] = z.power[kTerms - 1];
+    }
+#pragma unroll
+    for (int k = kTerms - 2; k >= 0; k--)
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = fma(y[e], f[e], z.power[k]);
+    Weights r;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        r.w[e] = (u64)__double_as_longlong(ldexp(y[e], n[e]) + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+    return r;
+}
+
 // The bin of the first histogram, which descends with the logit: kBins - 1 for what weighs nothing.
 __device__ __forceinline__ int first_bin(const Scale& z, float l)
 {
@@ -208,18 +234,19 @@ __device__ __forceinline__ u64 wave_upto(u64 v)
 // has their place, and its histograms are short.
 template <int T>
 struct Shared {
-    static constexpr int COPIES = T == 1024 ? 16 : 4, LIST = kBins * COPIES / 2;
+    static constexpr int COPIES = T == 1024 ? 16 : 4, LIST = kBins * COPIES / 2, WAVES = T / 64, OWN = LIST / WAVES;
     static constexpr int RANKED = T / 2, FEW = T / 2;  // ids that are ranked against one another
     union {
         u64 bins[kBins * COPIES];
         struct {
-            u64 list[LIST], weights[LIST];
+            u64 list[WAVES][OWN], weights[WAVES][OWN];  // each wave's own
         };
     };
     u64 counts[kBins];
     u64 few[FEW], few_weights[FEW];
     u64 waves[T / 64];
-    uint32_t listed, few_listed, bin, key;
+    uint32_t listed[WAVES];
+    uint32_t few_listed, bin, key;
     u64 cut, before, mass, total, least, most;
 };
 
@@ -307,34 +334,38 @@ __device__ __forceinline__ void clear_bins(u64* bins, int n)
     __syncthreads();
 }
 
-// The ids in order, as the rules below take them: f(composite, logit, place).
+// The ids in order, as the rules below take them: f(composite, logit, its weight
+// (WEIGHTS) or 1).
 template <int T>
 struct RowIds {  // of the row itself
     static constexpr int COPIES = Shared<T>::COPIES;
     const Row& r;
-    template <typename F>
-    __device__ __forceinline__ void each(const Shared<T>&, F f) const
+    template <bool WEIGHTS, typename F>
+    __device__ __forceinline__ void each(const Shared<T>&, const Scale& z, F f) const
     {
         each4<T, 2>(r, [&](int id, f4 l) {
+            Weights w = {{1, 1, 1, 1}};
+            if (WEIGHTS) w = weights4(z, l);
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                if (l[e] > -INFINITY) f(composite(l[e], id + e), l[e], 0);
+                if (l[e] > -INFINITY) f(composite(l[e], id + e), l[e], w.w[e]);
         });
     }
     __device__ __forceinline__ u64* bins(Shared<T>& sh) const { return sh.bins; }
-    __device__ __forceinline__ u64 weight_of(const Shared<T>&, const Scale& z, float l, int) const { return weight(z, l); }
 };
 template <int T>
-struct ListIds {  // of sh.list, with their weights
+struct ListIds {  // of sh.list, with their weights, every wave its own
     static constexpr int COPIES = 1;
-    int listed;
-    template <typename F>
-    __device__ __forceinline__ void each(const Shared<T>& sh, F f) const
+    template <bool WEIGHTS, typename F>
+    __device__ __forceinline__ void each(const Shared<T>& sh, const Scale&, F f) const
     {
-        for (int e = threadIdx.x; e < listed; e += T) f(sh.list[e], logit_in(sh.list[e]), e);
+        const int wave = wave_id(), listed = sh.listed[wave];
+        for (int e = threadIdx.x & 63; e < listed; e += 64) {
+            const u64 c = sh.list[wave][e];
+            f(c, logit_in(c), WEIGHTS ? sh.weights[wave][e] : 1);
+        }
     }
     __device__ __forceinline__ u64* bins(Shared<T>& sh) const { return sh.counts; }
-    __device__ __forceinline__ u64 weight_of(const Shared<T>& sh, const Scale&, float, int e) const { return sh.weights[e]; }
 };
 
 // The place of a thread among those that share the ids of a short list, `threads` to one.
@@ -364,12 +395,15 @@ __device__ __forceinline__ u64 last_kept(Shared<T>& sh, const Scale& z, const Id
     constexpr int C = Ids::COPIES;
     u64* bins = ids.bins(sh);
     const int copy = threadIdx.x & (C - 1);
-    auto quantity = [&](float l, int place) { return masses ? ids.weight_of(sh, z, l, place) : (u64)1; };
     clear_bins<T>(bins, kBins * C);
-    ids.each(sh, [&](u64 c, float l, int place) {
+    auto add = [&](u64 c, float l, u64 q) {
         const int b = first_bin(z, l);
-        if (b < kBins - 1 && c >= cut) atomicAdd(&bins[b * C + copy], quantity(l, place));
-    });
+        if (b < kBins - 1 && c >= cut) atomicAdd(&bins[b * C + copy], q);
+    };
+    if (masses)
+        ids.template each<true>(sh, z, add);
+    else
+        ids.template each<false>(sh, z, add);
     __syncthreads();
     Limit limit = masses ? mass_limit(top_p, total0) : Limit{(u64)count, 0.0};
     if (masses && total0 == 0)
@@ -391,15 +425,12 @@ __device__ __forceinline__ u64 last_kept(Shared<T>& sh, const Scale& z, const Id
         }
         __syncthreads();
         u64 least = ~(u64)0, most = 0;
-        ids.each(sh, [&](u64 c, float l, int place) {
+        ids.template each<false>(sh, z, [&](u64 c, float l, u64) {
             if (inside(c, l)) {
                 least = min(least, c);
                 most = max(most, c);
                 const uint32_t at = atomicAdd(&sh.few_listed, 1u);
-                if (at < (uint32_t)Shared<T>::FEW) {
-                    sh.few[at] = c;
-                    sh.few_weights[at] = quantity(l, place);
-                }
+                if (at < (uint32_t)Shared<T>::FEW) sh.few[at] = c;
             }
         });
         if (most) {
@@ -413,8 +444,8 @@ __device__ __forceinline__ u64 last_kept(Shared<T>& sh, const Scale& z, const Id
         hi = sh.most;
         const int shift = hi > lo ? max(0, 64 - __builtin_clzll(hi - lo) - 10) : 0;
         clear_bins<T>(bins, kBins * C);
-        ids.each(sh, [&](u64 c, float l, int place) {
-            if (inside(c, l)) atomicAdd(&bins[(int)((hi - c) >> shift) * C + copy], quantity(l, place));
+        ids.template each<true>(sh, z, [&](u64 c, float l, u64 w) {
+            if (inside(c, l)) atomicAdd(&bins[(int)((hi - c) >> shift) * C + copy], masses ? w : 1);
         });
         __syncthreads();
         find_bin<T, false>(sh, bins, C, before, limit, 0.0f);
@@ -424,6 +455,7 @@ __device__ __forceinline__ u64 last_kept(Shared<T>& sh, const Scale& z, const Id
     }
     listed = min(listed, Shared<T>::FEW);
     if (threadIdx.x == 0) sh.cut = cut;
+    if ((int)threadIdx.x < listed) sh.few_weights[threadIdx.x] = masses ? weight(z, logit_in(sh.few[threadIdx.x])) : 1;
     __syncthreads();
     const Shares s = shares<T>(listed);
     const u64 own = s.first < listed ? sh.few[s.first] : 0;
@@ -468,15 +500,24 @@ __device__ __forceinline__ Chosen draw_of_few(Shared<T>& sh, const Scale& z, con
                                               bool open)
 {
     const Shares s = shares<T>(listed);
-    if ((int)threadIdx.x < listed) sh.weights[threadIdx.x] = weight(z, logit_in(sh.list[threadIdx.x]));
+    // the waves' lists one behind the other
+    const int wave = wave_id(), here = sh.listed[wave];
+    int at_few = threadIdx.x & 63;
+#pragma unroll
+    for (int w = 0; w < T / 64; w++) at_few += w < wave ? sh.listed[w] : 0;
+    for (int e = threadIdx.x & 63; e < here; e += 64, at_few += 64) {
+        const u64 c = sh.list[wave][e];
+        sh.few[at_few] = c;
+        sh.few_weights[at_few] = weight(z, logit_in(c));
+    }
     if (threadIdx.x == 0) sh.mass = sh.total = 0;
     __syncthreads();
     const bool first = s.first < listed && s.place == 0;
-    const u64 own = s.first < listed ? sh.list[s.first] : 0, w = s.first < listed ? sh.weights[s.first] : 0;
+    const u64 own = s.first < listed ? sh.few[s.first] : 0, w = s.first < listed ? sh.few_weights[s.first] : 0;
     u64 larger = 0;
     uint32_t rank = 0;
     for (int i = s.place; i < listed; i += s.threads) {
-        const u64 c = sh.list[i], x = sh.weights[i];
+        const u64 c = sh.few[i], x = sh.few_weights[i];
         larger += c > own ? x : 0;
         rank += c > own ? 1 : 0;
     }
@@ -495,13 +536,13 @@ __device__ __forceinline__ Chosen draw_of_few(Shared<T>& sh, const Scale& z, con
     }
     kept = kept && w >= rules.least;
     if (kept) atomicMax(&sh.total, larger + w);
-    if (first) sh.weights[s.first] = kept ? w : 0;
+    if (first) sh.few_weights[s.first] = kept ? w : 0;
     __syncthreads();
     const u64 total = sh.total, at = drawn(rules.random, total);
     u64 lower = 0;  // the kept weight of lower ids
     for (int i = s.place; i < listed; i += s.threads) {
-        const u64 x = sh.weights[i];
-        lower += (uint32_t)sh.list[i] > (uint32_t)own ? x : 0;
+        const u64 x = sh.few_weights[i];
+        lower += (uint32_t)sh.few[i] > (uint32_t)own ? x : 0;
     }
     for (int off = 1; off < s.threads; off <<= 1) lower += __shfl_xor(lower, off);
     if (kept && lower <= at && at < lower + w) return {id_in(own), log_probability(z, logit_in(own), total), false};
@@ -510,13 +551,16 @@ __device__ __forceinline__ Chosen draw_of_few(Shared<T>& sh, const Scale& z, con
 
 // The same of more ids, by histograms.
 template <int T>
-__device__ __forceinline__ Chosen draw_of_many(Shared<T>& sh, const Scale& z, const Rules& rules, int listed, u64 total0,
-                                               bool open, int n)
+__device__ __forceinline__ Chosen draw_of_many(Shared<T>& sh, const Scale& z, const Rules& rules, u64 total0, bool open,
+                                               int n)
 {
+    const int lane = threadIdx.x & 63, wave = wave_id(), listed = sh.listed[wave];
+    const u64* list = sh.list[wave];
+    u64* weights = sh.weights[wave];
     u64 sum = 0;
 #pragma unroll 1
-    for (int e = threadIdx.x; e < listed; e += T) sum += sh.weights[e] = weight(z, logit_in(sh.list[e]));
-    const ListIds<T> ids = {listed};
+    for (int e = lane; e < listed; e += 64) sum += weights[e] = weight(z, logit_in(list[e]));
+    const ListIds<T> ids;
     u64 cut = 0;
     if (open && rules.by_mass && rules.top_k == 0 && mass_limit(rules.top_p, total0).inside(block_sum(sh, sum)))
         return {-1, 0.0f, true};
@@ -524,9 +568,9 @@ __device__ __forceinline__ Chosen draw_of_many(Shared<T>& sh, const Scale& z, co
     for (int rule = rules.top_k ? 0 : 1; rule < (rules.by_mass ? 2 : 1); rule++)
         cut = max(cut, last_kept(sh, z, ids, cut, rule == 0 ? rules.top_k : 0, rules.top_p, rules.top_k ? 0 : total0));
     sum = 0;
-    for (int e = threadIdx.x; e < listed; e += T) {
-        const u64 w = sh.list[e] >= cut && sh.weights[e] >= rules.least ? sh.weights[e] : 0;
-        sh.weights[e] = w;
+    for (int e = lane; e < listed; e += 64) {
+        const u64 w = list[e] >= cut && weights[e] >= rules.least ? weights[e] : 0;
+        weights[e] = w;
         sum += w;
     }
     const u64 total = block_sum(sh, sum), at = drawn(rules.random, total);
@@ -534,17 +578,17 @@ __device__ __forceinline__ Chosen draw_of_many(Shared<T>& sh, const Scale& z, co
     static_assert(kMaxIds / kBins <= Shared<1024>::FEW, "a bin's ids are few");  // (the list has an id once)
     const int shift = max(0, 32 - __builtin_clz(n) - 10);  // (n <= 4096 for 256 threads)
     clear_bins<T>(sh.counts, kBins);
-    for (int e = threadIdx.x; e < listed; e += T) atomicAdd(&sh.counts[min(id_in(sh.list[e]) >> shift, kBins - 1)], sh.weights[e]);
+    for (int e = lane; e < listed; e += 64) atomicAdd(&sh.counts[min(id_in(list[e]) >> shift, kBins - 1)], weights[e]);
     if (threadIdx.x == 0) sh.few_listed = 0;
     __syncthreads();
     find_bin<T, false>(sh, sh.counts, 1, 0, Limit{at + 1, 0.0}, 0.0f);
     const int bin = sh.bin;
     const u64 before = sh.before;
-    for (int e = threadIdx.x; e < listed; e += T)
-        if (id_in(sh.list[e]) >> shift == bin && sh.weights[e]) {
+    for (int e = lane; e < listed; e += 64)
+        if (id_in(list[e]) >> shift == bin && weights[e]) {
             const uint32_t to = min(atomicAdd(&sh.few_listed, 1u), (uint32_t)Shared<T>::FEW - 1);
-            sh.few[to] = sh.list[e];
-            sh.few_weights[to] = sh.weights[e];
+            sh.few[to] = list[e];
+            sh.few_weights[to] = weights[e];
         }
     __syncthreads();
     const int few = min(sh.few_listed, (uint32_t)Shared<T>::FEW);
@@ -569,9 +613,14 @@ __device__ __forceinline__ Chosen draw_of_row(Shared<T>& sh, const Row& r, const
 {
     constexpr int W = T / 64;
     const int lane = threadIdx.x & 63, wave = wave_id(), segments = (r.n + kSegment - 1) / kSegment;
-    auto kept = [&](float l, int id) {
-        const u64 w = weight(z, l);
-        return (cut == 0 || composite(l, id) >= cut) && w >= rules.least ? w : (u64)0;
+    const bool all = cut == 0 && rules.least == 0;
+    auto kept4 = [&](int id, f4 l) {
+        Weights w = weights4(z, l);
+        if (!all) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) w.w[e] = composite(l[e], id + e) >= cut && w.w[e] >= rules.least ? w.w[e] : 0;
+        }
+        return w;
     };
     u64 total = 0, at = 0, before = 0;
     int first = 0, end = segments;
@@ -579,8 +628,8 @@ __device__ __forceinline__ Chosen draw_of_row(Shared<T>& sh, const Row& r, const
         const int each = (end - first + W - 1) / W, from = first + wave * each, to = min(end, from + each);
         u64 sum = 0;
         auto add = [&](int id, f4 l) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) sum += kept(l[e], id + e);
+            const Weights w = kept4(id, l);
+            sum += (w.w[0] + w.w[1]) + (w.w[2] + w.w[3]);
         };
         walk<2>(r, from, min(to, r.n / kSegment), 1, add);
         if (to == segments && from < to && r.n % kSegment) {
@@ -611,17 +660,13 @@ __device__ __forceinline__ Chosen draw_of_row(Shared<T>& sh, const Row& r, const
     if (threadIdx.x < 64) {
         const int id = first * kSegment + 4 * lane;
         const f4 l = segment4(r, id);
-        u64 w[4], own = 0;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            w[e] = kept(l[e], id + e);
-            own += w[e];
-        }
+        const Weights w = kept4(id, l);
+        const u64 own = (w.w[0] + w.w[1]) + (w.w[2] + w.w[3]);
         u64 from = before + wave_upto(own) - own;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            if (from <= at && at < from + w[e]) found = {id + e, log_probability(z, l[e], total), false};
-            from += w[e];
+            if (from <= at && at < from + w.w[e]) found = {id + e, log_probability(z, l[e], total), false};
+            from += w.w[e];
         }
     }
     return found;
@@ -671,7 +716,6 @@ __global__ __launch_bounds__(T) void sample_kernel(SampleParams p)
 #pragma unroll
     for (int off = 32; off; off >>= 1) best = max(best, (u64)__shfl_xor(best, off));
     if ((threadIdx.x & 63) == 0) sh.waves[threadIdx.x >> 6] = best;
-    if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < T / 64; w++) best = max(best, sh.waves[w]);
@@ -697,8 +741,8 @@ __global__ __launch_bounds__(T) void sample_kernel(SampleParams p)
     bool open = false;
     if (rules.top_k || rules.by_mass) {
         const bool sure = rules.top_k && rules.top_k <= T / 4;
-        const float ids = rules.top_k ? 1.25f * rules.top_k + 64.0f : 3.0f * T;
-        const int want = sure ? rules.top_k : min((int)(T * (1.0f - __expf(-ids / T))), T - T / 64);
+        const float ids = rules.top_k ? 1.25f * rules.top_k + 64.0f : 5.0f * T;
+        const int want = sure ? rules.top_k : min((int)(T * (1.0f - __expf(-ids / T))), T - T / 100);
         bound = bound_of(sh, z, most, want);
         open = !sure && bound > -INFINITY;
     }
@@ -716,37 +760,43 @@ __global__ __launch_bounds__(T) void sample_kernel(SampleParams p)
     if (bound > -INFINITY || (r.n <= Shared<T>::LIST && (rules.top_k || rules.by_mass))) {
         bound = fmaxf(bound, -3.4028235e38f);  // (never -inf, which is no id's)
         const bool weigh = rules.by_mass && !rules.top_k;
+        const int wave = wave_id();
+        int here = 0;  // ids of this wave
         u64 total = 0;
         auto gather = [&](int id, f4 l) {
             if (__ballot(fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= bound) == 0) return;
-            int taken = 0;
 #pragma unroll
-            for (int e = 0; e < 4; e++) taken |= (l[e] >= bound ? 1 : 0) << e;
-            uint32_t at = taken ? atomicAdd(&sh.listed, (uint32_t)__builtin_popcount(taken)) : 0;
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                if ((taken >> e) & 1) {
-                    if (at < (uint32_t)Shared<T>::LIST) sh.list[at] = composite(l[e], id + e);
-                    at++;
-                }
+            for (int e = 0; e < 4; e++) {
+                const uint64_t taken = __ballot(l[e] >= bound);
+                const int at = here + __builtin_amdgcn_mbcnt_hi((uint32_t)(taken >> 32),
+                                                                __builtin_amdgcn_mbcnt_lo((uint32_t)taken, 0));
+                if (l[e] >= bound && at < Shared<T>::OWN) sh.list[wave][at] = composite(l[e], id + e);
+                here += __popcll(taken);
+            }
         };
         if (weigh) {
             each4<T, 2>(r, [&](int id, f4 l) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) total += weight(z, l[e]);
+                const Weights w = weights4(z, l);
+                total += (w.w[0] + w.w[1]) + (w.w[2] + w.w[3]);
                 gather(id, l);
             });
             total = block_sum(sh, total);
         } else {
             each4<T, 4>(r, gather);
         }
+        if ((threadIdx.x & 63) == 0) sh.listed[wave] = here;
         __syncthreads();
-        const int listed = sh.listed;
-        if (listed <= Shared<T>::LIST && !(open && listed < rules.top_k)) {
+        int listed = 0, longest = 0;
+#pragma unroll
+        for (int w = 0; w < T / 64; w++) {
+            listed += sh.listed[w];
+            longest = max(longest, (int)sh.listed[w]);
+        }
+        if (longest <= Shared<T>::OWN && !(open && listed < rules.top_k)) {
             if (listed <= Shared<T>::RANKED)
                 found = draw_of_few(sh, z, rules, listed, total, open);
             else
-                found = draw_of_many(sh, z, rules, listed, total, open, r.n);
+                found = draw_of_many(sh, z, rules, total, open, r.n);
         }
     }
     if (found.missed) {
