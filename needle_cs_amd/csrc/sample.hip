@@ -11,8 +11,10 @@
 // A workgroup takes a row.  It finds the largest logit, from its threads' own
 // largest a logit that what is kept will hardly fall below, and gathers the ids
 // above that into LDS, where the rules and the draw are ranks of few ids or
-// histograms of many.  Rows that keep more than the list holds or than the
-// guess allowed, and rows without rules, are walked instead.
+// histograms of many.  A share of the mass is found by a histogram of the row,
+// which every wave has of its own part, so that it says where the draw falls
+// too.  Rows that keep more than the list holds or than the guess allowed, and
+// rows without rules, are walked instead.
 #include <algorithm>
 #include <cmath>
 
@@ -229,22 +231,21 @@ __device__ __forceinline__ u64 wave_upto(u64 v)
     return v;
 }
 
-// COPIES of a histogram of the row side by side, a lane's own: lanes of a wave
-// that meet in a bin would wait for one another.  Where ids are listed the list
-// has their place, and its histograms are short.
+// A histogram of the row for every wave, of the wave's part of it.  Where ids are
+// listed the list has their place, and its histograms are short.
 template <int T>
 struct Shared {
-    static constexpr int COPIES = T == 1024 ? 16 : 4, LIST = kBins * COPIES / 2, WAVES = T / 64, OWN = LIST / WAVES;
+    static constexpr int WAVES = T / 64, LIST = kBins * WAVES / 2, OWN = LIST / WAVES;
     static constexpr int RANKED = T / 2, FEW = T / 2;  // ids that are ranked against one another
     union {
-        u64 bins[kBins * COPIES];
+        u64 bins[WAVES * kBins];
         struct {
             u64 list[WAVES][OWN], weights[WAVES][OWN];  // each wave's own
         };
     };
     u64 counts[kBins];
     u64 few[FEW], few_weights[FEW];
-    u64 waves[T / 64];
+    u64 waves[T / 64], parts[T / 64];
     uint32_t listed[WAVES];
     uint32_t few_listed, bin, key;
     u64 cut, before, mass, total, least, most;
@@ -287,11 +288,12 @@ struct Rules {
     u64 least;  // min_p's weight, rounded up
 };
 
-// The bin of a histogram (copies of it side by side) in which a rule ends, and
+// The bin of a histogram (the sum of `copies`) in which a rule ends, and
 // the sum before it, in sh.bin and sh.before; kBins where it does not end.
 // SHARE: the rule is the share top_p of all bins.  The sum of all bins.
 template <int T, bool SHARE>
-__device__ __forceinline__ u64 find_bin(Shared<T>& sh, const u64* bins, int copies, u64 before, Limit limit, float top_p)
+__device__ __forceinline__ u64 find_bin(Shared<T>& sh, const u64* bins, int copies, u64 before, Limit limit,
+                                        float top_p)
 {
     constexpr int B = kBins / T;
     u64 q[B], own = 0;
@@ -299,7 +301,7 @@ __device__ __forceinline__ u64 find_bin(Shared<T>& sh, const u64* bins, int copi
     for (int k = 0; k < B; k++) {
         const int b = B * threadIdx.x + k;
         q[k] = 0;
-        for (int c = 0; c < copies; c++) q[k] += bins[b * copies + ((c + b) & (copies - 1))];
+        for (int c = 0; c < copies; c++) q[k] += bins[c * kBins + b];
         own += q[k];
     }
     const u64 upto = wave_upto(own);
@@ -334,16 +336,37 @@ __device__ __forceinline__ void clear_bins(u64* bins, int n)
     __syncthreads();
 }
 
-// The ids in order, as the rules below take them: f(composite, logit, its weight
-// (WEIGHTS) or 1).
+// A wave's part of a row, or of the segments [first, end) of it.
+struct Part {
+    int each, from, to;
+};
+template <int T>
+__device__ __forceinline__ Part part_of(int wave, int first, int end)
+{
+    const int each = (end - first + T / 64 - 1) / (T / 64), from = min(first + wave * each, end);
+    return {each, from, min(end, from + each)};
+}
+__device__ __forceinline__ int segments_of(const Row& r) { return (r.n + kSegment - 1) / kSegment; }
+// f(first id, logits) for every four ids of a part.
+template <typename F>
+__device__ __forceinline__ void walk_part(const Row& r, const Part& p, F f)
+{
+    walk<2>(r, p.from, p.to, 1, f);
+    if (p.from < p.to && p.to == segments_of(r) && r.n % kSegment) {
+        const int i = kSegment * (p.to - 1) + 4 * (int)(threadIdx.x & 63);
+        f(i, segment4(r, i));
+    }
+}
+
+// The ids that the rules below are about: f(composite, logit, its weight (WEIGHTS) or 1) for each.
 template <int T>
 struct RowIds {  // of the row itself
-    static constexpr int COPIES = Shared<T>::COPIES;
+    static constexpr int COPIES = Shared<T>::WAVES;
     const Row& r;
     template <bool WEIGHTS, typename F>
     __device__ __forceinline__ void each(const Shared<T>&, const Scale& z, F f) const
     {
-        each4<T, 2>(r, [&](int id, f4 l) {
+        walk_part(r, part_of<T>(wave_id(), 0, segments_of(r)), [&](int id, f4 l) {
             Weights w = {{1, 1, 1, 1}};
             if (WEIGHTS) w = weights4(z, l);
 #pragma unroll
@@ -368,6 +391,17 @@ struct ListIds {  // of sh.list, with their weights, every wave its own
     __device__ __forceinline__ u64* bins(Shared<T>& sh) const { return sh.counts; }
 };
 
+// The wave's own list with the lanes' ids for which `taken`, `here` before and the result after,
+// which is more than OWN where it has no place for them.
+template <int T>
+__device__ __forceinline__ int list_id(Shared<T>& sh, int here, bool taken, float l, int id)
+{
+    const uint64_t all = __ballot(taken);
+    const int at = here + __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
+    if (taken && at < Shared<T>::OWN) sh.list[wave_id()][at] = composite(l, id);
+    return here + __popcll(all);
+}
+
 // The place of a thread among those that share the ids of a short list, `threads` to one.
 struct Shares {
     int threads, place, step, first;
@@ -383,36 +417,17 @@ __device__ __forceinline__ Shares shares(int listed)
     return s;
 }
 
-// The composite of the last id that a rule keeps of `ids` from `cut` on: the first
-// `count` (0: the share top_p of them, or with total0 the ids that weigh less than that
-// share of it before them).  0 where it keeps all.  A histogram by logit, finer ones by
-// composites where a bin has many ids, and ranks within the last.
+// The composite of the last id that a rule keeps (masses: by weights, or by ones), where
+// that is in a bin of the first histogram and `before` stands before it; cut where it is not.
+// Finer histograms by composites while more ids are left than are ranked.
 template <int T, typename Ids>
-__device__ __forceinline__ u64 last_kept(Shared<T>& sh, const Scale& z, const Ids& ids, u64 cut, int count, float top_p,
-                                         u64 total0)
+__device__ __forceinline__ u64 last_in_bin(Shared<T>& sh, const Scale& z, const Ids& ids, u64 cut, int bin, bool masses,
+                                           const Limit& limit, u64 before)
 {
-    const bool masses = count == 0;
     constexpr int C = Ids::COPIES;
     u64* bins = ids.bins(sh);
-    const int copy = threadIdx.x & (C - 1);
-    clear_bins<T>(bins, kBins * C);
-    auto add = [&](u64 c, float l, u64 q) {
-        const int b = first_bin(z, l);
-        if (b < kBins - 1 && c >= cut) atomicAdd(&bins[b * C + copy], q);
-    };
-    if (masses)
-        ids.template each<true>(sh, z, add);
-    else
-        ids.template each<false>(sh, z, add);
-    __syncthreads();
-    Limit limit = masses ? mass_limit(top_p, total0) : Limit{(u64)count, 0.0};
-    if (masses && total0 == 0)
-        limit = mass_limit(top_p, find_bin<T, true>(sh, bins, C, 0, limit, top_p));
-    else
-        find_bin<T, false>(sh, bins, C, 0, limit, 0.0f);
-    const int bin = sh.bin;
-    if (bin == kBins) return 0;
-    u64 lo = 0, hi = ~(u64)0, before = sh.before;
+    u64* own_bins = bins + (C > 1 ? wave_id() * kBins : 0);
+    u64 lo = 0, hi = ~(u64)0;
     auto inside = [&](u64 c, float l) { return first_bin(z, l) == bin && c >= cut && c >= lo && c <= hi; };
     int listed = 0;
     // (64 bits, ten at a time: seven rounds end it, whatever a second look at the logits says)
@@ -445,7 +460,7 @@ __device__ __forceinline__ u64 last_kept(Shared<T>& sh, const Scale& z, const Id
         const int shift = hi > lo ? max(0, 64 - __builtin_clzll(hi - lo) - 10) : 0;
         clear_bins<T>(bins, kBins * C);
         ids.template each<true>(sh, z, [&](u64 c, float l, u64 w) {
-            if (inside(c, l)) atomicAdd(&bins[(int)((hi - c) >> shift) * C + copy], masses ? w : 1);
+            if (inside(c, l)) atomicAdd(&own_bins[(int)((hi - c) >> shift)], masses ? w : 1);
         });
         __syncthreads();
         find_bin<T, false>(sh, bins, C, before, limit, 0.0f);
@@ -472,6 +487,38 @@ __device__ __forceinline__ u64 last_kept(Shared<T>& sh, const Scale& z, const Id
     return sh.cut;
 }
 
+// The composite of the last id that a rule keeps of `ids` from `cut` on: the first
+// `count` (0: the share top_p of them, or with total0 the ids that weigh less than that
+// share of it before them).  0 where it keeps all.  A histogram by logit, then the bin
+// in which the rule ends.
+template <int T, typename Ids>
+__device__ __forceinline__ u64 last_kept(Shared<T>& sh, const Scale& z, const Ids& ids, u64 cut, int count, float top_p,
+                                         u64 total0)
+{
+    const bool masses = count == 0;
+    constexpr int C = Ids::COPIES;
+    u64* bins = ids.bins(sh);
+    u64* own_bins = bins + (C > 1 ? wave_id() * kBins : 0);
+    clear_bins<T>(bins, kBins * C);
+    auto add = [&](u64 c, float l, u64 q) {
+        const int b = first_bin(z, l);
+        if (b < kBins - 1 && c >= cut) atomicAdd(&own_bins[b], q);
+    };
+    if (masses)
+        ids.template each<true>(sh, z, add);
+    else
+        ids.template each<false>(sh, z, add);
+    __syncthreads();
+    Limit limit = masses ? mass_limit(top_p, total0) : Limit{(u64)count, 0.0};
+    if (masses && total0 == 0)
+        limit = mass_limit(top_p, find_bin<T, true>(sh, bins, C, 0, limit, top_p));
+    else
+        find_bin<T, false>(sh, bins, C, 0, limit, 0.0f);
+    const int bin = sh.bin;
+    if (bin == kBins) return 0;
+    return last_in_bin(sh, z, ids, cut, bin, masses, limit, sh.before);
+}
+
 __device__ __forceinline__ float log_probability(const Scale& z, float l, u64 total)
 {
     return (float)(((double)l - z.peak) * z.log2e * 0.6931471805599453 - log((double)total / kOne));
@@ -493,11 +540,9 @@ struct Chosen {
 };
 
 // The rules and the draw over sh.list of up to RANKED ids, by ranks.  total0: the
-// weight of all ids, for top_p without top_k.  open: ids below the list may be
-// kept too.
+// weight of all ids, for top_p without top_k.
 template <int T>
-__device__ __forceinline__ Chosen draw_of_few(Shared<T>& sh, const Scale& z, const Rules& rules, int listed, u64 total0,
-                                              bool open)
+__device__ __forceinline__ Chosen draw_of_few(Shared<T>& sh, const Scale& z, const Rules& rules, int listed, u64 total0)
 {
     const Shares s = shares<T>(listed);
     // the waves' lists one behind the other
@@ -531,7 +576,6 @@ __device__ __forceinline__ Chosen draw_of_few(Shared<T>& sh, const Scale& z, con
         __syncthreads();
         const u64 mass = sh.mass;
         const Limit limit = mass_limit(rules.top_p, rules.top_k ? mass : total0);
-        if (open && rules.top_k == 0 && limit.inside(mass)) return {-1, 0.0f, true};
         kept = kept && limit.inside(larger);
     }
     kept = kept && w >= rules.least;
@@ -551,23 +595,19 @@ __device__ __forceinline__ Chosen draw_of_few(Shared<T>& sh, const Scale& z, con
 
 // The same of more ids, by histograms.
 template <int T>
-__device__ __forceinline__ Chosen draw_of_many(Shared<T>& sh, const Scale& z, const Rules& rules, u64 total0, bool open,
-                                               int n)
+__device__ __forceinline__ Chosen draw_of_many(Shared<T>& sh, const Scale& z, const Rules& rules, u64 total0, int n)
 {
     const int lane = threadIdx.x & 63, wave = wave_id(), listed = sh.listed[wave];
     const u64* list = sh.list[wave];
     u64* weights = sh.weights[wave];
-    u64 sum = 0;
 #pragma unroll 1
-    for (int e = lane; e < listed; e += 64) sum += weights[e] = weight(z, logit_in(list[e]));
+    for (int e = lane; e < listed; e += 64) weights[e] = weight(z, logit_in(list[e]));
     const ListIds<T> ids;
     u64 cut = 0;
-    if (open && rules.by_mass && rules.top_k == 0 && mass_limit(rules.top_p, total0).inside(block_sum(sh, sum)))
-        return {-1, 0.0f, true};
 #pragma unroll 1
     for (int rule = rules.top_k ? 0 : 1; rule < (rules.by_mass ? 2 : 1); rule++)
         cut = max(cut, last_kept(sh, z, ids, cut, rule == 0 ? rules.top_k : 0, rules.top_p, rules.top_k ? 0 : total0));
-    sum = 0;
+    u64 sum = 0;
     for (int e = lane; e < listed; e += 64) {
         const u64 w = list[e] >= cut && weights[e] >= rules.least ? weights[e] : 0;
         weights[e] = w;
@@ -607,12 +647,14 @@ __device__ __forceinline__ Chosen draw_of_many(Shared<T>& sh, const Scale& z, co
 }
 
 // The draw over the row itself, of what `cut` and min_p leave: its waves' parts, then
-// the parts of the one that the draw falls into, down to a segment.
+// the parts of the one that the draw falls into, down to a segment.  known: it falls
+// into the segments [first, end), whose lower neighbours weigh `before`, and all is `total`.
 template <int T>
-__device__ __forceinline__ Chosen draw_of_row(Shared<T>& sh, const Row& r, const Scale& z, const Rules& rules, u64 cut)
+__device__ __forceinline__ Chosen draw_of_row(Shared<T>& sh, const Row& r, const Scale& z, const Rules& rules, u64 cut,
+                                              bool known, int first, int end, u64 before, u64 total)
 {
     constexpr int W = T / 64;
-    const int lane = threadIdx.x & 63, wave = wave_id(), segments = (r.n + kSegment - 1) / kSegment;
+    const int lane = threadIdx.x & 63, wave = wave_id();
     const bool all = cut == 0 && rules.least == 0;
     auto kept4 = [&](int id, f4 l) {
         Weights w = weights4(z, l);
@@ -622,39 +664,33 @@ __device__ __forceinline__ Chosen draw_of_row(Shared<T>& sh, const Row& r, const
         }
         return w;
     };
-    u64 total = 0, at = 0, before = 0;
-    int first = 0, end = segments;
-    while (true) {
-        const int each = (end - first + W - 1) / W, from = first + wave * each, to = min(end, from + each);
+    u64 at = known ? drawn(rules.random, total) : 0;
+    while (!known || end - first > 1) {
+        const Part part = part_of<T>(wave, first, end);
         u64 sum = 0;
-        auto add = [&](int id, f4 l) {
+        walk_part(r, part, [&](int id, f4 l) {
             const Weights w = kept4(id, l);
             sum += (w.w[0] + w.w[1]) + (w.w[2] + w.w[3]);
-        };
-        walk<2>(r, from, min(to, r.n / kSegment), 1, add);
-        if (to == segments && from < to && r.n % kSegment) {
-            const int i = kSegment * (segments - 1) + 4 * lane;
-            add(i, segment4(r, i));
-        }
+        });
         sum = wave_sum_u64(sum);
         __syncthreads();
         if (lane == 0) sh.waves[wave] = sum;
         __syncthreads();
-        if (end - first == segments) {
+        if (!known) {
 #pragma unroll
             for (int w = 0; w < W; w++) total += sh.waves[w];
             at = drawn(rules.random, total);
+            known = true;
         }
         // (the last part at most, whatever a second look at the logits says: another stream may be writing them)
-        int part = 0;
-        for (int w = 0; w + 1 < W && first + (part + 1) * each < end; w++) {
+        int of = 0;
+        for (int w = 0; w + 1 < W && first + (of + 1) * part.each < end; w++) {
             if (before + sh.waves[w] > at) break;
             before += sh.waves[w];
-            part++;
+            of++;
         }
-        end = min(end, first + (part + 1) * each);
-        first += part * each;
-        if (each == 1) break;
+        end = min(end, first + (of + 1) * part.each);
+        first += of * part.each;
     }
     Chosen found = {-1, 0.0f, false};
     if (threadIdx.x < 64) {
@@ -670,6 +706,67 @@ __device__ __forceinline__ Chosen draw_of_row(Shared<T>& sh, const Row& r, const
         }
     }
     return found;
+}
+
+// top_p alone: one pass for the histograms, one that lists the ids of the bin in
+// which the share ends; with those every wave knows what its part keeps.  `missed`
+// where the list does not hold them.
+template <int T>
+__device__ __forceinline__ Chosen draw_by_mass(Shared<T>& sh, const Row& r, const Scale& z, const Rules& rules)
+{
+    const int lane = threadIdx.x & 63, wave = wave_id();
+    const Part part = part_of<T>(wave, 0, segments_of(r));
+    u64* own_bins = sh.bins + wave * kBins;
+    clear_bins<T>(sh.bins, T / 64 * kBins);
+    walk_part(r, part, [&](int, f4 l) {
+        const Weights w = weights4(z, l);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (w.w[e]) atomicAdd(&own_bins[first_bin(z, l[e])], w.w[e]);
+    });
+    __syncthreads();
+    const u64 all = find_bin<T, true>(sh, sh.bins, T / 64, 0, Limit{0, 0.0}, rules.top_p);
+    const Limit limit = mass_limit(rules.top_p, all);
+    const int bin = sh.bin;
+    u64 before = sh.before, mine = 0;
+    if (bin == kBins) return {-1, 0.0f, true};
+    for (int b = lane; b < bin; b += 64) mine += own_bins[b];
+    __syncthreads();  // (the list takes the histograms' place)
+    // (a bin's logits, and a little more, by their values alone)
+    const bool any_logit = z.bins < 1e-30f;  // (bins so wide that what follows might overflow)
+    const float width = 2.0f / z.bins, slack = 0.02f * width + 1e-6f * fabsf((float)z.peak);
+    const float above = any_logit ? INFINITY : (float)z.peak - bin * width + slack;
+    const float below = any_logit ? -INFINITY : (float)z.peak - (bin + 1) * width - slack;
+    int here = 0;
+    walk_part(r, part, [&](int id, f4 l) {
+        bool any = false;
+#pragma unroll
+        for (int e = 0; e < 4; e++) any = any || (l[e] <= above && l[e] >= below);
+        if (__ballot(any) == 0) return;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            here = list_id(sh, here, l[e] > -INFINITY && first_bin(z, l[e]) == bin, l[e], id + e);
+    });
+    const bool missed = here > Shared<T>::OWN;
+    here = min(here, Shared<T>::OWN);
+    for (int e = lane; e < here; e += 64) sh.weights[wave][e] = weight(z, logit_in(sh.list[wave][e]));
+    if (lane == 0) sh.listed[wave] = here;
+    if (__syncthreads_or(missed)) return {-1, 0.0f, true};
+    const u64 cut = last_in_bin(sh, z, ListIds<T>(), 0, bin, true, limit, before);
+    for (int e = lane; e < here; e += 64) mine += sh.list[wave][e] >= cut ? sh.weights[wave][e] : 0;
+    mine = wave_sum_u64(mine);
+    if (lane == 0) sh.parts[wave] = mine;
+    __syncthreads();
+    u64 total = 0;
+#pragma unroll
+    for (int k = 0; k < T / 64; k++) total += sh.parts[k];
+    const u64 at = drawn(rules.random, total);
+    int of = 0;
+    before = 0;
+    while (of + 1 < T / 64 && before + sh.parts[of] <= at) before += sh.parts[of++];
+    const Part there = part_of<T>(of, 0, segments_of(r));
+    if (there.from >= there.to) return {-1, 0.0f, true};
+    return draw_of_row(sh, r, z, rules, cut, true, there.from, there.to, before, total);
 }
 
 // A logit that at least `want` of the threads' largest are not below.
@@ -734,14 +831,15 @@ __global__ __launch_bounds__(T) void sample_kernel(SampleParams p)
     const Rules rules = {top_k > 0 && top_k < r.n ? top_k : 0, top_p < 1.0f, top_p, random,
                          min_p > 0.0f ? (u64)ceil((double)fminf(min_p, 1.0f) * kOne) : 0};
 
-    // A logit that nothing kept is below, or that hardly anything will be (open): as
-    // many of the threads' largest are not below it as top_k keeps, or some more ids in
-    // all, as far as ids fall to the threads by chance (that many of T threads: T ln(T / (T - many)) ids).
+    // A logit that nothing that top_k keeps is below, or hardly anything (open): as many
+    // of the threads' largest are not below it as top_k keeps, or so many that some more ids
+    // than it keeps are not, as far as ids fall to threads by chance (where `many` of T
+    // threads have one, T ln(T / (T - many)) ids).
     float bound = -INFINITY;
     bool open = false;
-    if (rules.top_k || rules.by_mass) {
-        const bool sure = rules.top_k && rules.top_k <= T / 4;
-        const float ids = rules.top_k ? 1.25f * rules.top_k + 64.0f : 5.0f * T;
+    if (rules.top_k) {
+        const bool sure = rules.top_k <= T / 4;
+        const float ids = 1.25f * rules.top_k + 64.0f;
         const int want = sure ? rules.top_k : min((int)(T * (1.0f - __expf(-ids / T))), T - T / 100);
         bound = bound_of(sh, z, most, want);
         open = !sure && bound > -INFINITY;
@@ -757,7 +855,9 @@ __global__ __launch_bounds__(T) void sample_kernel(SampleParams p)
     }
 
     Chosen found = {-1, 0.0f, true};
-    if (bound > -INFINITY || (r.n <= Shared<T>::LIST && (rules.top_k || rules.by_mass))) {
+    if (rules.by_mass && !rules.top_k && !rules.least) {
+        found = draw_by_mass(sh, r, z, rules);
+    } else if (bound > -INFINITY || (r.n <= Shared<T>::LIST && rules.top_k)) {
         bound = fmaxf(bound, -3.4028235e38f);  // (never -inf, which is no id's)
         const bool weigh = rules.by_mass && !rules.top_k;
         const int wave = wave_id();
@@ -766,13 +866,7 @@ __global__ __launch_bounds__(T) void sample_kernel(SampleParams p)
         auto gather = [&](int id, f4 l) {
             if (__ballot(fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= bound) == 0) return;
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const uint64_t taken = __ballot(l[e] >= bound);
-                const int at = here + __builtin_amdgcn_mbcnt_hi((uint32_t)(taken >> 32),
-                                                                __builtin_amdgcn_mbcnt_lo((uint32_t)taken, 0));
-                if (l[e] >= bound && at < Shared<T>::OWN) sh.list[wave][at] = composite(l[e], id + e);
-                here += __popcll(taken);
-            }
+            for (int e = 0; e < 4; e++) here = list_id(sh, here, l[e] >= bound, l[e], id + e);
         };
         if (weigh) {
             each4<T, 2>(r, [&](int id, f4 l) {
@@ -794,9 +888,9 @@ __global__ __launch_bounds__(T) void sample_kernel(SampleParams p)
         }
         if (longest <= Shared<T>::OWN && !(open && listed < rules.top_k)) {
             if (listed <= Shared<T>::RANKED)
-                found = draw_of_few(sh, z, rules, listed, total, open);
+                found = draw_of_few(sh, z, rules, listed, total);
             else
-                found = draw_of_many(sh, z, rules, total, open, r.n);
+                found = draw_of_many(sh, z, rules, total, r.n);
         }
     }
     if (found.missed) {
@@ -807,7 +901,7 @@ __global__ __launch_bounds__(T) void sample_kernel(SampleParams p)
             __syncthreads();
             cut = max(cut, last_kept(sh, z, ids, cut, rule == 0 ? rules.top_k : 0, top_p, 0));
         }
-        found = draw_of_row(sh, r, z, rules, cut);
+        found = draw_of_row(sh, r, z, rules, cut, false, 0, segments_of(r), 0, 0);
     }
     if (found.id >= 0) {
         p.ids[row] = found.id;
@@ -842,7 +936,8 @@ int32_t nhip_sample_dev(const float* d_logits, int32_t ldx, int32_t n, int32_t r
     int32_t rc = check_sample(rows, n);
     if (rc) return rc;
     NHIP_REQUIRE(ldx >= n, "sample: stride %d is less than %d ids", ldx, n);
-    NHIP_REQUIRE(!d_mask || (words >= 0 && mask_ld >= words), "sample: a mask of %d words with stride %d", words, mask_ld);
+    NHIP_REQUIRE(!d_mask || (words >= 0 && mask_ld >= words), "sample: a mask of %d words with stride %d", words,
+                 mask_ld);
     if (rows == 0) return NHIP_OK;
     NHIP_REQUIRE(d_logits && s && s->random && d_ids, "sample: null pointer");
     rc = ensure_device();
