@@ -576,7 +576,9 @@ struct Split {
 //   256 workgroups,     dims of 64    8.2 10.4 12.8 17.4             11.3 13.9 16.8 21.3
 //                       dims of 128  12.0 15.9 20.9 31.3             15.7 19.8 24.4 37.3
 // So rows stay whole up to 18 blocks (for few workgroups the two meet a little
-// above for dims of 64, a little below for 128), or up to 40 where the
+// above for dims of 64, a little below for 128; so a block of sinks beside a
+// window of 1024 makes 19 for dims of 64, where 3 rows on 3 kv heads take 7.4 us
+// whole and 8.2 in parts, 11.5 and 10.2 for dims of 128), or up to 40 where the
 // workgroups fill half the CUs (where 128 of them meet at 40 for dims of 128;
 // rows of very different lengths gain there by parts: 16 of 32 to 2400, 8 kv
 // heads of 128: 21.1 whole, 18.0 in parts).  Longer ones are cut into parts of
@@ -591,9 +593,10 @@ Split decode_split(const nhip_paged_cache* c, int32_t rows, int32_t max_count, i
 {
     const int64_t units = (int64_t)rows * c->kv_heads;
     // blocks of a row: its ends need not be a block's, and its sinks have some of their own
-    const int most = max_count / 64 + 2 + (std::min(sinks, c->width * c->page_size) + 63) / 64;
+    const int sink_blocks = (std::min(sinks, c->width * c->page_size) + 63) / 64;
+    const int most = max_count / 64 + 2 + sink_blocks;
     Split s;
-    if (most <= 18 || (most <= 40 && units >= 128)) {
+    if (most <= 18 + (c->v_dim <= 64 ? std::min(sink_blocks, 1) : 0) || (most <= 40 && units >= 128)) {
         s.blocks = most;
     } else {
         const int64_t even = (most * units + 2047) / 2048, fewest = (most + kMaxParts - 1) / kMaxParts;

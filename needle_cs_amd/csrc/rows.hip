@@ -51,6 +51,7 @@ struct NormParams {
     float* scales;
     int32_t ldx, ldd, lds, rows, cols, zero_centered;
     float eps;
+    double inverse_cols;
 };
 
 __device__ __forceinline__ float4 gain4(const NormParams& p, int i)
@@ -89,12 +90,19 @@ __device__ __forceinline__ float peak4(float m, float4 v)
     return fmaxf(fmaxf(m, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
 }
 
+template <int S>
+__device__ __forceinline__ double add_lane_xor(double v)
+{
+    return v + __hiloint2double((int)lane_xor<S>((uint32_t)__double2hiint(v)),
+                                (int)lane_xor<S>((uint32_t)__double2loint(v)));
+}
+
 // The sum and the maximum over the T threads of a row, in every thread.  (A
 // row's two uses alternate, each behind a barrier of its own.)
 template <int T>
 __device__ __forceinline__ double row_sum(double v, double* lds)
 {
-    for (int off = 32; off; off >>= 1) v += __shfl_xor(v, off);
+    v = add_lane_xor<1>(add_lane_xor<2>(add_lane_xor<4>(add_lane_xor<8>(add_lane_xor<16>(add_lane_xor<32>(v))))));
     if constexpr (T > 64) {
         if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
         __syncthreads();
@@ -118,13 +126,14 @@ __device__ __forceinline__ float row_max(float v, float* lds)
 
 __device__ __forceinline__ float inverse_rms(const NormParams& p, double squares)
 {
-    return (float)(1.0 / sqrt(squares / (double)p.cols + (double)p.eps));
+    return (float)rsqrt(squares * p.inverse_cols + (double)p.eps);
 }
 
+__device__ __forceinline__ float scale_of(float peak) { return peak > 0.0f ? peak / 127.0f : 1.0f; }
+
 // T threads a row, which they hold in registers, G groups of four elements
-// each (HELD), or read again for each of the three passes.  A held row is
-// read once and written once.
-template <int T, int G, bool HELD>
+// each: it is read once and written once.
+template <int T, int G>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void add_rms_quantize_kernel(NormParams p)
 {
     constexpr int WG = T < 256 ? 256 : T;
@@ -133,68 +142,67 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void add_rms_quantize_kernel(Nor
     const int t = threadIdx.x % T;
     for (size_t row = (size_t)blockIdx.x * (WG / T) + threadIdx.x / T; row < (size_t)p.rows;
          row += (size_t)gridDim.x * (WG / T)) {
-        float4 v[G];
+        float4 v[G], g[G];
         double squares = 0.0;
-        const int passes = HELD ? G : (p.cols + 4 * T - 1) / (4 * T);
-        if constexpr (HELD) {
 #pragma unroll
-            for (int j = 0; j < G; j++) v[j] = sum4(p, row, 4 * (t + T * j));
+        for (int j = 0; j < G; j++) v[j] = sum4(p, row, 4 * (t + T * j));
 #pragma unroll
-            for (int j = 0; j < G; j++) squares = squares4(v[j], squares);
-        }
-        if (p.sum || !HELD) {
+        for (int j = 0; j < G; j++) g[j] = gain4(p, 4 * (t + T * j));
 #pragma unroll
-            for (int j = 0; j < passes; j++) {
-                const int i = 4 * (t + T * j);
-                float4 s;
-                if constexpr (HELD) {
-                    s = v[j];
-                } else {
-                    s = sum4(p, row, i);
-                    squares = squares4(s, squares);
-                }
-                if (p.sum) store4(p.sum + row * p.lds, i, p.cols, s);
-            }
+        for (int j = 0; j < G; j++) squares = squares4(v[j], squares);
+        if (p.sum) {
+#pragma unroll
+            for (int j = 0; j < G; j++) store4(p.sum + row * p.lds, 4 * (t + T * j), p.cols, v[j]);
         }
         const float r = inverse_rms(p, row_sum<T>(squares, sums));
-        // (a row that is not held comes back from the sums, where they are kept: x may be the same memory)
-        auto again = [&](int i) {
-            return normed4(p.sum ? load4(p.sum + row * p.lds, i, p.cols) : sum4(p, row, i), r, gain4(p, i));
-        };
         float peak = 0.0f;
 #pragma unroll
-        for (int j = 0; j < passes; j++) {
-            const int i = 4 * (t + T * j);
-            if constexpr (HELD) {
-                v[j] = normed4(v[j], r, gain4(p, i));
-                peak = peak4(peak, v[j]);
-            } else {
-                peak = peak4(peak, again(i));
-            }
+        for (int j = 0; j < G; j++) {
+            v[j] = normed4(v[j], r, g[j]);
+            peak = peak4(peak, v[j]);
         }
-        peak = row_max<T>(peak, peaks);
-        const float scale = peak > 0.0f ? peak / 127.0f : 1.0f;
-        const float inverse = 1.0f / scale;
+        const float scale = scale_of(row_max<T>(peak, peaks)), inverse = 1.0f / scale;
 #pragma unroll
-        for (int j = 0; j < passes; j++) {
-            const int i = 4 * (t + T * j);
-            float4 h;
-            if constexpr (HELD)
-                h = v[j];
-            else
-                h = again(i);
-            store_codes4(p.q + row * p.cols, i, p.cols, ref_quantize4(h, inverse));
-        }
+        for (int j = 0; j < G; j++)
+            store_codes4(p.q + row * p.cols, 4 * (t + T * j), p.cols, ref_quantize4(v[j], inverse));
         if (t == 0) p.scales[row] = scale;
     }
 }
 
-template <int T, int G, bool HELD>
+// Rows of any length, by T threads, read for each of the three passes: from the
+// sums, where they are kept (x may be the same memory).
+template <int T>
+__global__ __launch_bounds__(T) void add_rms_quantize_long_kernel(NormParams p)
+{
+    __shared__ double sums[T / 64];
+    __shared__ float peaks[T / 64];
+    const int first = 4 * threadIdx.x;
+    for (size_t row = blockIdx.x; row < (size_t)p.rows; row += gridDim.x) {
+        double squares = 0.0;
+        for (int i = first; i < p.cols; i += 4 * T) {
+            const float4 v = sum4(p, row, i);
+            squares = squares4(v, squares);
+            if (p.sum) store4(p.sum + row * p.lds, i, p.cols, v);
+        }
+        const float r = inverse_rms(p, row_sum<T>(squares, sums));
+        auto again = [&](int i) {
+            return normed4(p.sum ? load4(p.sum + row * p.lds, i, p.cols) : sum4(p, row, i), r, gain4(p, i));
+        };
+        float peak = 0.0f;
+        for (int i = first; i < p.cols; i += 4 * T) peak = peak4(peak, again(i));
+        const float scale = scale_of(row_max<T>(peak, peaks)), inverse = 1.0f / scale;
+        for (int i = first; i < p.cols; i += 4 * T)
+            store_codes4(p.q + row * p.cols, i, p.cols, ref_quantize4(again(i), inverse));
+        if (threadIdx.x == 0) p.scales[row] = scale;
+    }
+}
+
+template <int T, int G>
 void launch_norm(const NormParams& p, hipStream_t stream)
 {
     constexpr int WG = T < 256 ? 256 : T, ROWS = WG / T;
-    hipLaunchKernelGGL((add_rms_quantize_kernel<T, G, HELD>), dim3(std::min((p.rows + ROWS - 1) / ROWS, kMaxGroups)),
-                       dim3(WG), 0, stream, p);
+    hipLaunchKernelGGL((add_rms_quantize_kernel<T, G>), dim3(std::min((p.rows + ROWS - 1) / ROWS, kMaxGroups)), dim3(WG),
+                       0, stream, p);
 }
 
 // L lanes a row.
@@ -258,16 +266,16 @@ int32_t nhip_add_rms_quantize_dev(const float* d_x, int32_t ldx, const float* d_
     rc = ensure_device();
     if (rc) return rc;
     const NormParams p = {d_x,      d_delta, d_gain, d_sum, d_q,  d_scales, ldx,
-                          ldd, ld_sum,  rows,   cols,  zero_centered, eps};
+                          ldd, ld_sum,  rows,   cols,  zero_centered, eps, 1.0 / cols};
     hipStream_t s = as_stream(stream);
     if (cols <= 1024)
-        launch_norm<64, 4, true>(p, s);
+        launch_norm<64, 4>(p, s);
     else if (cols <= 4096)
-        launch_norm<256, 4, true>(p, s);
+        launch_norm<256, 4>(p, s);
     else if (cols <= 16384)
-        launch_norm<1024, 4, true>(p, s);
+        launch_norm<1024, 4>(p, s);
     else
-        launch_norm<1024, 1, false>(p, s);
+        hipLaunchKernelGGL((add_rms_quantize_long_kernel<1024>), dim3(std::min(rows, kMaxGroups)), dim3(1024), 0, s, p);
     NHIP_CHECK_HIP(hipGetLastError());
     return NHIP_OK;
 }

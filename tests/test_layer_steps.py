@@ -162,7 +162,7 @@ def test_sinks_workspaces():
     assert c.decode_sinks_workspace(4, 12, 4, 300) == 0
     assert c.decode_sinks_workspace(4, 12, 0, 60000) == c.decode_workspace(4, 12, 60000)
     # 1 row of 2 kv heads, 1024 / 64 + 2 + 1 = 19 blocks: 8 a part, 3 parts
-    assert c.decode_sinks_workspace(1, 12, 4, 1024) == 12 * 3 * 264
+    assert c.decode_sinks_workspace(1, 12, 4, 1088) == 12 * 3 * 264
     # sinks past what a sequence holds count as all of it
     assert c.decode_sinks_workspace(1, 12, 2 ** 31 - 1, 1024) == c.decode_sinks_workspace(1, 12, 4096 * 16, 1024)
     need = c.prompt_workspace(20, 12, 1, 60000)
