@@ -209,26 +209,55 @@ __device__ __forceinline__ void each4(const Row& r, F f)
     }
 }
 
-// Sum over the wave, in every lane.
+template <int S>
+__device__ __forceinline__ u64 lane_xor_u64(u64 v)
+{
+    return (u64)lane_xor<S>((uint32_t)(v >> 32)) << 32 | lane_xor<S>((uint32_t)v);
+}
 template <int S>
 __device__ __forceinline__ u64 add_lane_xor(u64 v)
 {
-    return v + ((u64)lane_xor<S>((uint32_t)(v >> 32)) << 32 | lane_xor<S>((uint32_t)v));
+    return v + lane_xor_u64<S>(v);
 }
+template <int S>
+__device__ __forceinline__ u64 max_lane_xor(u64 v)
+{
+    return max(v, lane_xor_u64<S>(v));
+}
+// Sum over the wave, in every lane, and the largest.
 __device__ __forceinline__ u64 wave_sum_u64(u64 v)
 {
     return add_lane_xor<32>(add_lane_xor<16>(add_lane_xor<8>(add_lane_xor<4>(add_lane_xor<2>(add_lane_xor<1>(v))))));
 }
-// Sum of the lanes up to this one.
+__device__ __forceinline__ u64 wave_max_u64(u64 v)
+{
+    return max_lane_xor<32>(max_lane_xor<16>(max_lane_xor<8>(max_lane_xor<4>(max_lane_xor<2>(max_lane_xor<1>(v))))));
+}
+// Sum over the 2, 4 or 16 neighbours that share an id, in each of them.
+__device__ __forceinline__ u64 shared_sum(u64 v, int threads)
+{
+    v = add_lane_xor<1>(v);
+    if (threads > 2) v = add_lane_xor<2>(v);
+    if (threads > 4) v = add_lane_xor<8>(add_lane_xor<4>(v));
+    return v;
+}
+// Sum of the lanes up to this one: within rows of 16 lanes, then the last
+// lane's of a row to the next one's, and lane 31's to the upper half.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 add_lane_below(u64 v)
+{
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xF, false);
+    return v + ((u64)hi << 32 | lo);
+}
 __device__ __forceinline__ u64 wave_upto(u64 v)
 {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const u64 other = __shfl_up(v, off);
-        if (lane >= off) v += other;
-    }
-    return v;
+    v = add_lane_below<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
+    v = add_lane_below<0x112, 0xF>(v);
+    v = add_lane_below<0x114, 0xF>(v);
+    v = add_lane_below<0x118, 0xF>(v);
+    v = add_lane_below<0x142, 0xA>(v);  // row_bcast:15 to rows 1 and 3
+    return add_lane_below<0x143, 0xC>(v);  // row_bcast:31 to rows 2 and 3
 }
 
 // A histogram of the row for every wave, of the wave's part of it.  Where ids are
@@ -410,7 +439,7 @@ template <int T>
 __device__ __forceinline__ Shares shares(int listed)
 {
     Shares s;
-    s.threads = listed <= T / 16 ? 16 : listed <= T / 4 ? 4 : 2;
+    s.threads = __builtin_amdgcn_readfirstlane(listed <= T / 16 ? 16 : listed <= T / 4 ? 4 : 2);
     s.place = threadIdx.x & (s.threads - 1);
     s.step = T / s.threads;
     s.first = threadIdx.x / s.threads;
@@ -479,7 +508,7 @@ __device__ __forceinline__ u64 last_in_bin(Shared<T>& sh, const Scale& z, const 
         const u64 q = sh.few_weights[i];
         larger += sh.few[i] > own ? q : 0;
     }
-    for (int off = 1; off < s.threads; off <<= 1) larger += __shfl_xor(larger, off);
+    larger = shared_sum(larger, s.threads);
     larger += before;
     if (s.first < listed && s.place == 0 && limit.inside(larger) && !limit.inside(larger + sh.few_weights[s.first]))
         sh.cut = own;
@@ -559,18 +588,15 @@ __device__ __forceinline__ Chosen draw_of_few(Shared<T>& sh, const Scale& z, con
     __syncthreads();
     const bool first = s.first < listed && s.place == 0;
     const u64 own = s.first < listed ? sh.few[s.first] : 0, w = s.first < listed ? sh.few_weights[s.first] : 0;
-    u64 larger = 0;
-    uint32_t rank = 0;
+    u64 larger = 0, rank = 0;
     for (int i = s.place; i < listed; i += s.threads) {
         const u64 c = sh.few[i], x = sh.few_weights[i];
         larger += c > own ? x : 0;
         rank += c > own ? 1 : 0;
     }
-    for (int off = 1; off < s.threads; off <<= 1) {
-        larger += __shfl_xor(larger, off);
-        rank += __shfl_xor(rank, off);
-    }
-    bool kept = first && (rules.top_k == 0 || rank < (uint32_t)rules.top_k);
+    larger = shared_sum(larger, s.threads);
+    rank = shared_sum(rank, s.threads);
+    bool kept = first && (rules.top_k == 0 || rank < (u64)rules.top_k);
     if (rules.by_mass) {
         if (kept) atomicMax(&sh.mass, larger + w);  // (the last one has all)
         __syncthreads();
@@ -588,7 +614,7 @@ __device__ __forceinline__ Chosen draw_of_few(Shared<T>& sh, const Scale& z, con
         const u64 x = sh.few_weights[i];
         lower += (uint32_t)sh.few[i] > (uint32_t)own ? x : 0;
     }
-    for (int off = 1; off < s.threads; off <<= 1) lower += __shfl_xor(lower, off);
+    lower = shared_sum(lower, s.threads);
     if (kept && lower <= at && at < lower + w) return {id_in(own), log_probability(z, logit_in(own), total), false};
     return {-1, 0.0f, false};
 }
@@ -639,7 +665,7 @@ __device__ __forceinline__ Chosen draw_of_many(Shared<T>& sh, const Scale& z, co
         const u64 x = sh.few_weights[i];
         lower += (uint32_t)sh.few[i] > (uint32_t)own ? x : 0;
     }
-    for (int off = 1; off < s.threads; off <<= 1) lower += __shfl_xor(lower, off);
+    lower = shared_sum(lower, s.threads);
     lower += before;
     if (s.first < few && s.place == 0 && lower <= at && at < lower + sh.few_weights[s.first])
         return {id_in(own), log_probability(z, logit_in(own), total), false};
@@ -810,8 +836,7 @@ __global__ __launch_bounds__(T) void sample_kernel(SampleParams p)
         }
     });
     u64 best = most > -INFINITY ? composite(most, most_id) : 0;
-#pragma unroll
-    for (int off = 32; off; off >>= 1) best = max(best, (u64)__shfl_xor(best, off));
+    best = wave_max_u64(best);
     if ((threadIdx.x & 63) == 0) sh.waves[threadIdx.x >> 6] = best;
     __syncthreads();
 #pragma unroll
