@@ -909,6 +909,12 @@ __device__ __forceinline__ int32_t scalar_load(const int32_t* a, int64_t i)
     return ((const __attribute__((address_space(4))) int32_t*)a)[i];
 }
 
+// The lowest n bits: none of n <= 0, all of n >= 32.
+__device__ __forceinline__ uint32_t lowest_bits(int n)
+{
+    return n <= 0 ? 0u : ~0u >> (32 - min(n, 32));
+}
+
 #define NHIP_INLINE __attribute__((always_inline))
 
 // SINKS: as the decode kernel's.  A tile's rows begin to attend at different
@@ -1114,18 +1120,17 @@ __global__ __launch_bounds__(256, QK <= 64 ? 3 : 2) void paged_prompt_kernel(Pro
                 const float largest = fmaxf(vs[0], vs[1]);  // of the lane's two positions
                 const bool masked = !whole | (tile_pos + 63 > wave_first) | (tile_pos < wave_last - from_window);
                 if (masked) {
-                    const int last = q_pos - tile_pos - 8 * g, first = q_first - tile_pos - 8 * g;
-                    const int sunk = SINKS ? p.sinks - tile_pos - 8 * g : 0;
+                    // a bit for each position that the row attends, and a score's bits or those of -inf by it
+                    const int behind = q_pos + 1 - tile_pos, first = q_first - tile_pos, sunk = p.sinks - tile_pos;
 #pragma unroll
                     for (int t = 0; t < 2; t++) {
-                        const uint32_t bits = (t ? counted.y : counted.x) >> (8 * g);
+                        uint32_t bits = ~lowest_bits(first - 32 * t);
+                        if (SINKS) bits |= lowest_bits(sunk - 32 * t);
+                        bits = (bits & lowest_bits(behind - 32 * t) & (t ? counted.y : counted.x)) >> (8 * g);
 #pragma unroll
                         for (int r = 0; r < 16; r++) {
-                            const int at = 16 * (r / 8) + r % 8;
-                            const bool attends = (32 * t + at <= last) &
-                                                 ((32 * t + at >= first) | (SINKS && 32 * t + at < sunk)) &
-                                                 ((bits >> at) & 1);
-                            z[t][r] = attends ? z[t][r] : -INFINITY;
+                            const uint32_t kept = __builtin_amdgcn_sbfe((int)bits, 16 * (r / 8) + r % 8, 1);
+                            z[t][r] = __uint_as_float((__float_as_uint(z[t][r]) & kept) | (0xFF800000u & ~kept));
                         }
                     }
                 }
