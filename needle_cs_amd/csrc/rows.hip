@@ -102,7 +102,9 @@ __device__ __forceinline__ double add_lane_xor(double v)
 template <int T>
 __device__ __forceinline__ double row_sum(double v, double* lds)
 {
-    v = add_lane_xor<1>(add_lane_xor<2>(add_lane_xor<4>(add_lane_xor<8>(add_lane_xor<16>(add_lane_xor<32>(v))))));
+    if constexpr (T > 32) v = add_lane_xor<32>(v);
+    if constexpr (T > 16) v = add_lane_xor<16>(v);
+    v = add_lane_xor<1>(add_lane_xor<2>(add_lane_xor<4>(add_lane_xor<8>(v))));
     if constexpr (T > 64) {
         if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
         __syncthreads();
@@ -114,7 +116,12 @@ __device__ __forceinline__ double row_sum(double v, double* lds)
 template <int T>
 __device__ __forceinline__ float row_max(float v, float* lds)
 {
-    v = wave_max(v);
+    if constexpr (T > 32) v = fmaxf(v, lane_xor<32>(v));
+    if constexpr (T > 16) v = fmaxf(v, lane_xor<16>(v));
+    v = fmaxf(v, lane_xor<8>(v));
+    v = fmaxf(v, lane_xor<4>(v));
+    v = fmaxf(v, lane_xor<2>(v));
+    v = fmaxf(v, lane_xor<1>(v));
     if constexpr (T > 64) {
         if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
         __syncthreads();
@@ -132,7 +139,10 @@ __device__ __forceinline__ float inverse_rms(const NormParams& p, double squares
 __device__ __forceinline__ float scale_of(float peak) { return peak > 0.0f ? peak / 127.0f : 1.0f; }
 
 // T threads a row, which they hold in registers, G groups of four elements
-// each: it is read once and written once.
+// each: it is read once and written once (13 bytes an element with the addition
+// and the sums; 4099 rows of 4096 in 42.5 us are 5.1 TB/s).  What a group's
+// code costs shows where there are few rows, also where no element is left for
+// it: 3 rows of 512 with a wave take 4.1 us by G = 4, 3.4 by 2.
 template <int T, int G>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void add_rms_quantize_kernel(NormParams p)
 {
@@ -197,6 +207,13 @@ __global__ __launch_bounds__(T) void add_rms_quantize_long_kernel(NormParams p)
     }
 }
 
+// The fewest groups that hold a row, by as many threads as have four elements
+// each; more rows than there are CUs keep more elements a thread.  us, 3 rows
+// and 8192 rows: 512 columns <256, 1> 3.1 and 15.8, <64, 2> 3.4 and 11.3 (equal
+// for 512 rows); 1024 columns <256, 1> 3.2 and 21.9, <64, 4> 4.2 and 19.6 (equal
+// for 2048 rows); 4096 columns <1024, 1> 4.3 and 91, <256, 4> 4.7 and 87 (5.3
+// and 5.6 for 256 rows, 7.0 and 6.8 for 512).  200,000 rows of 48 columns:
+// 25 us by 16 threads, 72 by 64.
 template <int T, int G>
 void launch_norm(const NormParams& p, hipStream_t stream)
 {
@@ -205,7 +222,11 @@ void launch_norm(const NormParams& p, hipStream_t stream)
                        0, stream, p);
 }
 
-// L lanes a row.
+// L lanes a row, of four elements each: as few as the row has for rows of up to
+// 64 columns (200,000 of 48: 9.8 us with 16 lanes, 13.8 with 32), then few enough
+// (8192 rows of 256: 3.9 with 32, 5.4 with 256; of 512: 5.4 with 64, 6.2 with 256;
+// of 1024: 8.5 with 64, 8.3 with 256).  Bytes bound it: 8185 rows of 4096 columns
+// 25.6 us, 6.5 TB/s.
 template <int L>
 __global__ __launch_bounds__(256) void dequantize_rows_kernel(const int8_t* q, const float* scales, int rows, int cols,
                                                              float* x, int ldx)
@@ -268,10 +289,26 @@ int32_t nhip_add_rms_quantize_dev(const float* d_x, int32_t ldx, const float* d_
     const NormParams p = {d_x,      d_delta, d_gain, d_sum, d_q,  d_scales, ldx,
                           ldd, ld_sum,  rows,   cols,  zero_centered, eps, 1.0 / cols};
     hipStream_t s = as_stream(stream);
-    if (cols <= 1024)
+    if (cols <= 64)
+        launch_norm<16, 1>(p, s);
+    else if (cols <= 128)
+        launch_norm<32, 1>(p, s);
+    else if (cols <= 256)
+        launch_norm<64, 1>(p, s);
+    else if (cols <= 1024 && rows <= 512)
+        launch_norm<256, 1>(p, s);
+    else if (cols <= 512)
+        launch_norm<64, 2>(p, s);
+    else if (cols <= 1024)
         launch_norm<64, 4>(p, s);
+    else if (cols <= 2048)
+        launch_norm<256, 2>(p, s);
+    else if (cols <= 4096 && rows <= 256)
+        launch_norm<1024, 1>(p, s);
     else if (cols <= 4096)
         launch_norm<256, 4>(p, s);
+    else if (cols <= 8192)
+        launch_norm<1024, 2>(p, s);
     else if (cols <= 16384)
         launch_norm<1024, 4>(p, s);
     else
@@ -295,6 +332,8 @@ int32_t nhip_dequantize_rows_dev(const int8_t* d_q, const float* d_scales, int32
         launch_dequantize<16>(d_q, d_scales, rows, cols, d_x, ldx, s);
     else if (cols <= 128)
         launch_dequantize<32>(d_q, d_scales, rows, cols, d_x, ldx, s);
+    else if (cols <= 512)
+        launch_dequantize<64>(d_q, d_scales, rows, cols, d_x, ldx, s);
     else
         launch_dequantize<256>(d_q, d_scales, rows, cols, d_x, ldx, s);
     NHIP_CHECK_HIP(hipGetLastError());

@@ -971,7 +971,11 @@ int32_t nhip_sample_dev(const float* d_logits, int32_t ldx, int32_t n, int32_t r
     (void)workspace_bytes;
     SampleParams p = {d_logits, d_mask, *s, d_ids, d_logprobs, ldx, n, mask_ld, words, {}, -INFINITY};
     std::copy(kPower, kPower + kTerms, p.power);
-    if (n <= 4096)
+    // Short rows, and rows that are short enough to share a CU by threes where there are more of them
+    // than CUs: us by 256 and by 1024 threads for top_k 50 with top_p 0.95, and for top_p 0.9, 1 row of
+    // 4096 10.3 and 10.7, 13.3 and 13.5; of 8192 12.2 and 11.2, 18.4 and 16.8; 300 rows of 8192 13.3 and
+    // 21.5, 22.3 and 31.6; of 32000 25.2 and 30.1, 60.5 and 58.1 (top_k 1000 80.0 and 45.2).
+    if (n <= 4096 || (n <= 16384 && rows > 256))
         hipLaunchKernelGGL((sample_kernel<256>), dim3(rows), dim3(256), 0, as_stream(stream), p);
     else
         hipLaunchKernelGGL((sample_kernel<1024>), dim3(rows), dim3(1024), 0, as_stream(stream), p);

@@ -96,6 +96,13 @@ def test_norm_row_counts(hip, rows, cols):
     NormCall(hip, np.random.default_rng(rows), rows, cols).check()
 
 
+@pytest.mark.parametrize("rows", [256, 257, 512, 513])
+@pytest.mark.parametrize("cols", [33, 65, 128, 129, 300, 512, 513, 1000, 1024, 1030, 4093, 4100, 8192, 8193])
+def test_norm_rows_by_columns(hip, rows, cols):
+    """Every number of threads a row and of elements a thread, full and with ends inside a thread's four."""
+    NormCall(hip, np.random.default_rng(rows + cols), rows, cols, pads=(0, 3, 1)).check()
+
+
 def test_norm_rows_of_zeros_and_of_nothing(hip):
     call = NormCall(hip, np.random.default_rng(1), 6, 520)
     call.x[1] = call.delta[1] = 0
@@ -123,7 +130,8 @@ def test_norm_is_the_rows_calls_one_after_the_other(hip):
 
 
 @pytest.mark.parametrize("rows,cols,pad", [(1, 1, 0), (7, 3, 2), (1000, 48, 0), (333, 50, 1), (99, 64, 0), (65, 65, 3), (64, 128, 0),
-                                           (300000, 5, 0), (20, 4096, 8), (3, 70001, 0)])
+                                           (300000, 5, 0), (20, 4096, 8), (3, 70001, 0),
+                                           (40, 129, 1), (9, 511, 0), (33, 512, 4), (31, 513, 0)])
 def test_dequantize(hip, rows, cols, pad):
     from needle_cs_amd.rows import dequantize_rows
     rng = np.random.default_rng(rows + cols)

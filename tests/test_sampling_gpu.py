@@ -159,6 +159,30 @@ def test_ties(hip, n):
                 Call(hip, x, [0.0, 0.3, 0.8, 0.99999], 0.9, k, p, 0.0, rng.random((4, n)) < 0.8).check()
 
 
+@pytest.mark.parametrize("n", [300, 4096, 4097, 5119, 40001, 262147])
+@pytest.mark.parametrize("temperature", [0.3, 1.0, 2.0, 10.0, 1e6, 1e30, np.inf])
+def test_a_share_of_the_mass(hip, n, temperature):
+    """top_p alone, from bins of one id to bins of the whole row; draws in every part of a row and at its ends."""
+    rng = np.random.default_rng(n)
+    rows = 8 if n < 100000 else 4
+    u = np.concatenate([[0.0, 1.0 - 2.0 ** -24], rng.random(rows - 2)])
+    for grid in (0.0, 0.5):
+        x = logits(rng, rows, n, grid)
+        for p in (0.02, 0.5, 0.9, 0.999, 1.0 - 2.0 ** -24):
+            Call(hip, x, u, temperature, None, p).check()
+    Call(hip, x, u, temperature, None, 0.9, None, rng.random((rows, n)) < 0.3).check()
+    wide = x.clip(-11.3, 11.3) * np.float32(3e37)
+    Call(hip, wide, u, temperature, None, 0.7).check()
+
+
+@pytest.mark.parametrize("rows,n", [(257, 16384), (257, 16385), (256, 16384), (300, 5000)])
+def test_many_rows(hip, rows, n):
+    rng = np.random.default_rng(rows + n)
+    Call(hip, logits(rng, rows, n, 0.125), rng.random(rows), rng.choice([0.0, 0.7, 1.0, 1.5], rows),
+         rng.choice([0, 1, 40, 700, 3000, n - 1], rows), rng.choice([0.2, 0.9, 0.99, 1.0], rows),
+         rng.choice([0.0, 0.0, 0.02], rows), rng.random((rows, n)) < 0.9).check()
+
+
 def test_near_ties(hip):
     """Logits one step of fp32 apart, in one bin of the first histogram."""
     rng = np.random.default_rng(4)
