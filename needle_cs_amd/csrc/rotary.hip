@@ -33,8 +33,8 @@ struct TableParams {
 // A workgroup takes kSpan positions and 32 frequencies.  The cos and sin of
 // first + 16 a + b are one complex product of those of first + 16 a and b, all
 // in 64 bits: 24 of either for 128 positions instead of 128, and an error of
-// three roundings of 2^-53 more.  131,072 positions of 64 pairs (67 MB): TABLE_US us,
-// 32.2 with a cos and sin for each.
+// three roundings of 2^-53 more.  131,072 positions of 64 pairs, 67 MB to be written:
+// 14.0 us, 4.8 TB/s; 32.2 with a cos and sin for each.
 constexpr int kCoarse = 8, kFine = 16, kSpan = kCoarse * kFine;
 __global__ __launch_bounds__(256) void rotary_table_kernel(TableParams p)
 {
@@ -113,7 +113,10 @@ struct RotateParams {
 };
 
 // L threads a head, a unit each, and further heads of the row in turn, so that
-// a unit's cos and sin are read once a row.
+// a unit's cos and sin are read once a row.  Bytes bound it: 8185 rows of 40 heads
+// of 128 with 64 dimensions rotated, 337 MB read and written, take 63.5 us, 5.3
+// TB/s (113 with a pair a thread, whose accesses are 4 bytes wide); 3 rows of 12
+// heads 2 us beside a launch.
 constexpr int kHeadsAhead = 4;  // loads in flight
 template <int L>
 __global__ __launch_bounds__(256) void rotate_kernel(RotateParams p)
@@ -147,7 +150,8 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateParams p)
     }
 }
 
-// Dimensions that are no multiple of 8: a thread takes a pair or, behind them, an element that stays.
+// Dimensions that are no multiple of 8, where a unit of four pairs would pass
+// them: a thread takes a pair or, behind them, an element that stays.
 __global__ __launch_bounds__(256) void rotate_pairs_kernel(RotateParams p)
 {
     const int half = p.r.dim / 2, units = half + p.head_dim - p.r.dim;

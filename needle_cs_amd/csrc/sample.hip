@@ -8,13 +8,22 @@
 // summation shows, those by atomics into LDS among them; a sum of 2^19 weights
 // stays below 2^62.
 //
-// A workgroup takes a row.  It finds the largest logit, from its threads' own
+// A workgroup takes a row, which it reads two to four times, from L2 or the last
+// cache after the first.  It finds the largest logit, from its threads' own
 // largest a logit that what is kept will hardly fall below, and gathers the ids
 // above that into LDS, where the rules and the draw are ranks of few ids or
 // histograms of many.  A share of the mass is found by a histogram of the row,
 // which every wave has of its own part, so that it says where the draw falls
 // too.  Rows that keep more than the list holds or than the guess allowed, and
 // rows without rules, are walked instead.
+//
+// One row is bound by the latency of the steps behind each pass: 32000 ids, the
+// first 50 and 0.95 of the mass 13.2 us, greedy 5.2.  250 rows of 131071 ids, a
+// CU each, in us: greedy 27 (131 MB, 4.9 TB/s), the first 50 48, 0.9 of the mass
+// 90, no rule 64, the first 30000 153, and 120 with a mask and settings of every
+// kind, where the row that takes longest counts.  A pass costs about 22 by the
+// reads, and 35 where it weighs: some 30 instructions an id, which all four SIMDs
+// of a CU issue without a gap.
 #include <algorithm>
 #include <cmath>
 
