@@ -651,7 +651,7 @@ __device__ __forceinline__ Chosen draw_of_many(Shared<T>& sh, const Scale& z, co
     const u64 total = block_sum(sh, sum), at = drawn(rules.random, total);
     // in the order of the ids: a few neighbours of them, then the id
     static_assert(kMaxIds / kBins <= Shared<1024>::FEW, "a bin's ids are few");  // (the list has an id once)
-    const int shift = max(0, 32 - __builtin_clz(n) - 10);  // (n <= 4096 for 256 threads)
+    const int shift = max(0, 32 - __builtin_clz(n - 1) - 10);  // (n > 1; at most 16384 for 256 threads)
     clear_bins<T>(sh.counts, kBins);
     for (int e = lane; e < listed; e += 64) atomicAdd(&sh.counts[min(id_in(list[e]) >> shift, kBins - 1)], weights[e]);
     if (threadIdx.x == 0) sh.few_listed = 0;

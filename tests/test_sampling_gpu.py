@@ -175,6 +175,18 @@ def test_a_share_of_the_mass(hip, n, temperature):
     Call(hip, wide, u, temperature, None, 0.7).check()
 
 
+@pytest.mark.parametrize("n", [700, 4096, 16384, 1 << 17, (1 << 19) - 1, 1 << 19])
+def test_neighbours(hip, n):
+    """What is kept side by side in the row, at its start, its end and across powers of two."""
+    rng = np.random.default_rng(n)
+    kept = min(n // 2, 2000)
+    for first in (0, n // 2 - kept // 2, n - kept, n // 4):
+        x = rng.standard_normal((3, n)).astype(np.float32) - 12
+        x[:, first:first + kept] += 11
+        for k, p in ((kept - 100, 1.0), (kept, 0.9), (0, 0.8)):
+            Call(hip, x, rng.random(3), 1.5, k, p).check()
+
+
 @pytest.mark.parametrize("rows,n", [(257, 16384), (257, 16385), (256, 16384), (300, 5000)])
 def test_many_rows(hip, rows, n):
     rng = np.random.default_rng(rows + n)
