@@ -880,7 +880,8 @@ __global__ __launch_bounds__(T) void sample_kernel(SampleParams p)
     }
     // (min_p bounds it too, but the mass of top_p's ids is that of all that top_k keeps)
     if (rules.least && !(rules.top_k && rules.by_mass)) {
-        const float down = -logf(fminf(min_p, 1.0f)) * t;
+        // (half a unit below the least weight is what rounds to it)
+        const float down = (float)((1e-12 - log(((double)rules.least - 0.5) / kOne)) * t);
         const float lowest = peak - down - 1e-5f * (fabsf(peak) + down) - 1e-30f;
         if (lowest > bound) {
             bound = lowest;

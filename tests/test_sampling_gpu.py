@@ -187,6 +187,29 @@ def test_neighbours(hip, n):
             Call(hip, x, rng.random(3), 1.5, k, p).check()
 
 
+@pytest.mark.parametrize("min_p", [1e-13, 1.5e-13, 2.0 ** -42, 4e-13, 7e-12])
+def test_the_least_weights(hip, min_p):
+    """Weights around min_p's, a few units of 2^-42 each, which round to it from below, in sum as much as the draw has left."""
+    n, units = 1 << 19, min_p * 2.0 ** 42
+    for first in (0.51, 0.9, 1.0, 1.1):
+        x = np.full((2, n), np.float32(np.log((np.ceil(units) - 1 + first) / 2.0 ** 42)), dtype=np.float32)
+        x[:, 0] = 0.0
+        Call(hip, x, [1.0 - 2.0 ** -24, 0.5], 1.0, 0, 1.0, min_p).check()
+        Call(hip, x, [1.0 - 2.0 ** -24, 0.5], 1.0, 0, 1.0 - 2.0 ** -24, min_p).check()
+
+
+def test_the_largest_weights(hip):
+    """min_p = 1 keeps what rounds to the largest weight, also beside a largest logit of 0."""
+    x = np.full((4, 5000), -30, dtype=np.float32)
+    x[:, 40:60] = -np.float32(10.0) ** -np.arange(20)
+    x[:, 60] = 0.0
+    for t in (1e-5, 0.5, 1.0, 1e4):
+        call = Call(hip, x, [0.0, 0.3, 0.7, 0.99], t, 0, 1.0, 1.0)
+        call.check()
+        call = Call(hip, x, [0.0, 0.3, 0.7, 0.99], t, 0, 0.8, 1.0)
+        call.check()
+
+
 @pytest.mark.parametrize("rows,n", [(257, 16384), (257, 16385), (256, 16384), (300, 5000)])
 def test_many_rows(hip, rows, n):
     rng = np.random.default_rng(rows + n)
