@@ -126,8 +126,10 @@ __device__ __forceinline__ Place place_of(const PagedLayer& c, const int32_t* re
 // sin are read once a row.  Heads from p.heads on are the keys'.  A lane's eight
 // elements are two 16-byte loads and two 4-byte stores of codes; the peak is the
 // maximum over L lanes.  Bytes bound it: 8185 rows of 32 + 8 heads of 128 and
-// their values, 201 MB read and 52 written, take 57 to 68 us, 3.7 to 4.4 TB/s
-// (84 where the values' workgroups came first on every XCD and these last).
+// their values, 205 MB read and 52 written, take 54 to 65 us, 4.0 to 4.8 TB/s
+// (84 where the XCDs' shares of these workgroups and the values' were uneven; 58
+// to 68 with a row's heads far apart in the grid, for the table came from memory
+// again for every four of them).
 template <int QK, int H, bool MIXED>
 __device__ __forceinline__ void append_rotated(const RotaryAppendParams& p, int first_head, int row0)
 {
@@ -210,10 +212,10 @@ __global__ __launch_bounds__(256) void paged_append_kernel(Params p)
     if constexpr (ROTARY) {
         if (id / 8 >= share) {
             constexpr int heads = rotated_heads<QK, H>();
-            const uint32_t rotated = groups * ((p.heads + c.kv_heads + heads - 1) / heads);
-            const uint32_t part = (id & 7) * ((rotated + 7) / 8) + id / 8 - share;
+            const uint32_t sides = (p.heads + c.kv_heads + heads - 1) / heads, rotated = groups * sides;
+            const uint32_t part = (id & 7) * ((rotated + 7) / 8) + id / 8 - share, group = part / sides;
             if (id / 8 - share < (rotated + 7) / 8 && part < rotated)
-                append_rotated<QK, H, MIXED>(p, part / groups * heads, (int)(part % groups) * N);
+                append_rotated<QK, H, MIXED>(p, (part - group * sides) * heads, (int)group * N);
             return;
         }
     }
