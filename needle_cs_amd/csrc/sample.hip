@@ -8,8 +8,8 @@
 // summation shows, those by atomics into LDS among them; a sum of 2^19 weights
 // stays below 2^62.
 //
-// A workgroup takes a row, which it reads two to four times, from L2 or the last
-// cache after the first.  It finds the largest logit, from its threads' own
+// A workgroup takes a row, which it reads one to four times, from L2 or the last
+// cache after the first, and keeps in registers where it is short.  It finds the largest logit, from its threads' own
 // largest a logit that what is kept will hardly fall below, and gathers the ids
 // above that into LDS, where the rules and the draw are ranks of few ids or
 // histograms of many.  A share of the mass is found by a histogram of the row,
@@ -18,10 +18,10 @@
 // rows without rules, are walked instead.
 //
 // One row is bound by the latency of the steps behind each pass: 32000 ids, the
-// first 50 and 0.95 of the mass 13.2 us, greedy 5.2.  250 rows of 131071 ids, a
+// first 50 and 0.95 of the mass 12.8 us (13.3 read twice), greedy 5.2.  250 rows of 131071 ids, a
 // CU each, in us: greedy 27 (131 MB, 4.9 TB/s), the first 50 48, 0.9 of the mass
-// 90, no rule 64, the first 30000 153, and 120 with a mask and settings of every
-// kind, where the row that takes longest counts.  A pass costs about 22 by the
+// 90, no rule 64, the first 5000 72, the first 30000 155, and 113 to 120 with a
+// mask and settings of every kind, where the row that takes longest counts.  A pass costs about 22 by the
 // reads, and 35 where it weighs: some 30 instructions an id, which all four SIMDs
 // of a CU issue without a gap.
 #include <algorithm>
@@ -233,6 +233,35 @@ __device__ __forceinline__ u64 max_lane_xor(u64 v)
 {
     return max(v, lane_xor_u64<S>(v));
 }
+// The same of a row of up to 4 G T ids, which each thread keeps, G fours of it.
+template <int T>
+__device__ __forceinline__ int held_id(int j)
+{
+    return kSegment * (wave_id() + T / 64 * j) + 4 * (int)(threadIdx.x & 63);
+}
+template <int T, int G>
+__device__ __forceinline__ void hold(const Row& r, f4 (&v)[G])
+{
+    const int whole = r.n / kSegment;
+    uint32_t bits[G];
+#pragma unroll
+    for (int j = 0; j < G; j++) {
+        const int segment = wave_id() + T / 64 * j, i = held_id<T>(j);
+        v[j] = f4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        bits[j] = 0;
+        if (segment < whole) {
+            v[j] = *reinterpret_cast<const f4*>(r.x + i);
+            bits[j] = mask_bits(r, i);
+        } else if (segment == whole && i < r.n) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[j][e] = i + e < r.n ? r.x[i + e] : -INFINITY;
+            bits[j] = mask_bits(r, i);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < G; j++) v[j] = counted4(r, v[j], bits[j]);
+}
+
 // Sum over the wave, in every lane, and the largest.
 __device__ __forceinline__ u64 wave_sum_u64(u64 v)
 {
@@ -804,18 +833,21 @@ __device__ __forceinline__ Chosen draw_by_mass(Shared<T>& sh, const Row& r, cons
     return draw_of_row(sh, r, z, rules, cut, true, there.from, there.to, before, total);
 }
 
-// A logit that at least `want` of the threads' largest are not below.
+// A logit that at least `want` of the threads' largest are not below: of `most` each,
+// or with `two` of `other` too.
 template <int T>
-__device__ __forceinline__ float bound_of(Shared<T>& sh, const Scale& z, float most, int want)
+__device__ __forceinline__ float bound_of(Shared<T>& sh, const Scale& z, float most, float other, bool two, int want)
 {
     if (threadIdx.x == 0) sh.key = ~0u;
     clear_bins<T>(sh.counts, kBins);
-    const int b = first_bin(z, most);
+    const int b = first_bin(z, most), b2 = two ? first_bin(z, other) : kBins - 1;
     if (b < kBins - 1) atomicAdd(&sh.counts[b], (u64)1);
+    if (two && b2 < kBins - 1) atomicAdd(&sh.counts[b2], (u64)1);
     __syncthreads();
     find_bin<T, false>(sh, sh.counts, 1, 0, Limit{(u64)want, 0.0}, 0.0f);
     if (sh.bin == kBins) return -INFINITY;
     if (b == (int)sh.bin) atomicMin(&sh.key, key_of(most));
+    if (two && b2 == (int)sh.bin) atomicMin(&sh.key, key_of(other));
     __syncthreads();
     return logit_of(sh.key);
 }
@@ -833,18 +865,30 @@ __global__ __launch_bounds__(T) void sample_kernel(SampleParams p)
     const float min_p = p.s.min_p ? p.s.min_p[row] : 0.0f;
     const float random = p.s.random[row];
 
-    // the thread's first id, then the row's
-    float most = -INFINITY;
-    int most_id = 0;
-    each4<T, 4>(r, [&](int id, f4 l) {
+    // the first of the thread's ids, by halves, then of the row's
+    float halves[2] = {-INFINITY, -INFINITY};
+    int first_id[2] = {0, 0};
+    constexpr int G = 8;
+    const bool held = r.n <= 4 * G * T;
+    f4 own[G];
+    auto largest = [&](int id, f4 l) {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const bool more = l[e] > most;
-            most = more ? l[e] : most;
-            most_id = more ? id + e : most_id;
+            const bool more = l[e] > halves[e / 2];
+            halves[e / 2] = more ? l[e] : halves[e / 2];
+            first_id[e / 2] = more ? id + e : first_id[e / 2];
         }
-    });
-    u64 best = most > -INFINITY ? composite(most, most_id) : 0;
+    };
+    if (held) {
+        hold<T>(r, own);
+#pragma unroll
+        for (int j = 0; j < G; j++) largest(held_id<T>(j), own[j]);
+    } else {
+        each4<T, 4>(r, largest);
+    }
+    const bool second = halves[1] > halves[0] || (halves[1] == halves[0] && first_id[1] < first_id[0]);
+    float most = second ? halves[1] : halves[0];
+    u64 best = most > -INFINITY ? composite(most, second ? first_id[1] : first_id[0]) : 0;
     best = wave_max_u64(best);
     if ((threadIdx.x & 63) == 0) sh.waves[threadIdx.x >> 6] = best;
     __syncthreads();
@@ -859,23 +903,28 @@ __global__ __launch_bounds__(T) void sample_kernel(SampleParams p)
         return;
     }
     r.infinite = __builtin_amdgcn_readfirstlane(logit_in(best) == INFINITY);
-    if (r.infinite) most = most == INFINITY ? 0.0f : -INFINITY;
+    if (r.infinite) {
+        most = most == INFINITY ? 0.0f : -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 2; k++) halves[k] = halves[k] == INFINITY ? 0.0f : -INFINITY;
+    }
     const float peak = r.infinite ? 0.0f : logit_in(best);
     const Scale z = scale_of(peak, t, p.power);
     const Rules rules = {top_k > 0 && top_k < r.n ? top_k : 0, top_p < 1.0f, top_p, random,
                          min_p > 0.0f ? (u64)ceil((double)fminf(min_p, 1.0f) * kOne) : 0};
 
-    // A logit that nothing that top_k keeps is below, or hardly anything (open): as many
-    // of the threads' largest are not below it as top_k keeps, or so many that some more ids
-    // than it keeps are not, as far as ids fall to threads by chance (where `many` of T
-    // threads have one, T ln(T / (T - many)) ids).
+    // A logit that nothing that top_k keeps is below: as many of the threads' largest are not
+    // below it as top_k keeps.  Where those are too few, one that most probably (open) has
+    // somewhat more ids not below it: of N = 2 T shares of the row, to which ids fall by chance,
+    // `want` have one where N ln(N / (N - want)) ids are spread.  Short rows are listed whole.
     float bound = -INFINITY;
     bool open = false;
-    if (rules.top_k) {
-        const bool sure = rules.top_k <= T / 4;
-        const float ids = 1.25f * rules.top_k + 64.0f;
-        const int want = sure ? rules.top_k : min((int)(T * (1.0f - __expf(-ids / T))), T - T / 100);
-        bound = bound_of(sh, z, most, want);
+    const bool sure = __builtin_amdgcn_readfirstlane(rules.top_k) <= T / 4;
+    if (rules.top_k && (sure || r.n > Shared<T>::LIST)) {
+        constexpr int N = 2 * T;
+        const float ids = 1.12f * rules.top_k + 64.0f;
+        const int want = sure ? rules.top_k : min((int)(N * (1.0f - __expf(-ids / N))), N - N / 100);
+        bound = bound_of(sh, z, sure ? most : halves[0], halves[1], !sure, want);
         open = !sure && bound > -INFINITY;
     }
     // (min_p bounds it too, but the mass of top_p's ids is that of all that top_k keeps)
@@ -910,6 +959,15 @@ __global__ __launch_bounds__(T) void sample_kernel(SampleParams p)
                 gather(id, l);
             });
             total = block_sum(sh, total);
+        } else if (held) {
+#pragma unroll
+            for (int j = 0; j < G; j++) {
+                if (r.infinite) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) own[j][e] = own[j][e] == INFINITY ? 0.0f : -INFINITY;
+                }
+                gather(held_id<T>(j), own[j]);
+            }
         } else {
             each4<T, 4>(r, gather);
         }

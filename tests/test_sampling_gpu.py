@@ -198,6 +198,19 @@ def test_the_least_weights(hip, min_p):
         Call(hip, x, [1.0 - 2.0 ** -24, 0.5], 1.0, 0, 1.0 - 2.0 ** -24, min_p).check()
 
 
+@pytest.mark.parametrize("rows,n", [(2, 2049), (2, 8192), (2, 8193), (2, 32767), (2, 32768), (2, 32769), (2, 100003), (258, 2048),
+                                    (258, 2049), (258, 8192), (258, 8193)])
+@pytest.mark.parametrize("top_k", [64, 65, 256, 257, 1800, 2300, 5000, 7900, 8300])
+def test_many_kept(hip, rows, n, top_k):
+    """Up to what a list holds and above, from rows that threads hold and from those that they read again."""
+    rng = np.random.default_rng(n + top_k)
+    for grid in (0.0, 0.125):
+        Call(hip, logits(rng, rows, n, grid), rng.random(rows), 1.3, top_k, rng.choice([0.97, 1.0], rows)).check()
+    x = np.sort(logits(rng, rows, n), axis=1)[:, ::-1]  # (all of them in a few threads' shares)
+    x[0, 5] = np.inf
+    Call(hip, np.ascontiguousarray(x), rng.random(rows), 1.3, top_k, None, None, rng.random((rows, n)) < 0.9).check()
+
+
 def test_the_largest_weights(hip):
     """min_p = 1 keeps what rounds to the largest weight, also beside a largest logit of 0."""
     x = np.full((4, 5000), -30, dtype=np.float32)
