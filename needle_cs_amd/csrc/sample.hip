@@ -1039,11 +1039,12 @@ int32_t nhip_sample_dev(const float* d_logits, int32_t ldx, int32_t n, int32_t r
     (void)workspace_bytes;
     SampleParams p = {d_logits, d_mask, *s, d_ids, d_logprobs, ldx, n, mask_ld, words, {}, -INFINITY};
     std::copy(kPower, kPower + kTerms, p.power);
-    // Short rows, and rows that are short enough to share a CU by threes where there are more of them
-    // than CUs: us by 256 and by 1024 threads for top_k 50 with top_p 0.95, and for top_p 0.9, 1 row of
-    // 4096 10.3 and 10.7, 13.3 and 13.5; of 8192 12.2 and 11.2, 18.4 and 16.8; 300 rows of 8192 13.3 and
-    // 21.5, 22.3 and 31.6; of 32000 25.2 and 30.1, 60.5 and 58.1 (top_k 1000 80.0 and 45.2).
-    if (n <= 4096 || (n <= 16384 && rows > 256))
+    // Rows that 256 threads hold, and somewhat longer ones, which share a CU by threes, where there are
+    // more of them than CUs: us by 256 and by 1024 threads for top_k 50 with top_p 0.95, for top_p 0.9 and
+    // for top_k 1000: 1 row of 4096 11.1 and 12.6, 14.0 and 15.2, 14.3 and 17.5; of 8192 12.0 and 12.9,
+    // 18.1 and 17.4, 17.0 and 21.8; 300 rows of 8192 13.4 and 24.7, 23.3 and 34.3, 26.7 and 42.6; of 16384
+    // 18.8 and 28.3, 34.4 and 42.7, 46.3 and 41.4; 128 rows of 32000 20.0 and 14.8, 48.4 and 30.1.
+    if (n <= 8192 || (n <= 16384 && rows > 256))
         hipLaunchKernelGGL((sample_kernel<256>), dim3(rows), dim3(256), 0, as_stream(stream), p);
     else
         hipLaunchKernelGGL((sample_kernel<1024>), dim3(rows), dim3(1024), 0, as_stream(stream), p);
