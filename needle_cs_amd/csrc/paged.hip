@@ -106,11 +106,11 @@ __device__ __forceinline__ float group_max(float v)
 struct Place {
     int page, at;
 };
-// Heads that one workgroup rotates.
-template <int QK, int H>
+// Heads that one workgroup rotates, side by side.
+template <int QK>
 __host__ __device__ constexpr int rotated_heads()
 {
-    return H * (256 / (QK <= 64 ? 8 : 16) / kAppendRows);
+    return 256 / (QK <= 64 ? 8 : 16) / kAppendRows;
 }
 __device__ __forceinline__ Place place_of(const PagedLayer& c, const int32_t* refs, int seq, int pos)
 {
@@ -122,78 +122,58 @@ __device__ __forceinline__ Place place_of(const PagedLayer& c, const int32_t* re
 }
 
 // Query and key heads rotated and quantized: 16 rows, L lanes a head, a unit of
-// eight elements each, and H x 16 / L heads in turn, so that a unit's cos and
-// sin are read once a row.  Heads from p.heads on are the keys'.  A lane's eight
+// eight elements each.  Heads from p.heads on are the keys'.  A lane's eight
 // elements are two 16-byte loads and two 4-byte stores of codes; the peak is the
 // maximum over L lanes.  Bytes bound it: 8185 rows of 32 + 8 heads of 128 and
-// their values, 205 MB read and 52 written, take 54 to 65 us, 4.0 to 4.8 TB/s
+// their values, 205 MB read and 52 written, take 54 to 64 us, 4.0 to 4.8 TB/s
 // (84 where the XCDs' shares of these workgroups and the values' were uneven; 58
 // to 68 with a row's heads far apart in the grid, for the table came from memory
-// again for every four of them).
-template <int QK, int H, bool MIXED>
+// again for each).  Side by side they find the table in L2: two or four heads a
+// lane, for which it is read once, take 39.2 and 41.0 us in place of 40.0 where
+// all of it is in the last cache, and 5.3 and 6.3 in place of 5.1 for 512 rows.
+template <int QK, bool MIXED>
 __device__ __forceinline__ void append_rotated(const RotaryAppendParams& p, int first_head, int row0)
 {
-    constexpr int L = QK <= 64 ? 8 : 16, SIDE = 256 / L / kAppendRows;  // heads side by side
+    constexpr int L = QK <= 64 ? 8 : 16;
     const PagedLayer& c = p.c;
-    const int l = threadIdx.x % L, slot = threadIdx.x / L, side = slot / kAppendRows;
+    const int l = threadIdx.x % L, slot = threadIdx.x / L;
     const int row = row0 + slot % kAppendRows, at = min(row, p.rows - 1);
-    const int heads = p.heads + c.kv_heads;
+    const int heads = p.heads + c.kv_heads, head = min(first_head + slot / kAppendRows, heads - 1);
     const int pos = p.row_pos[at];
     const bool known = pos >= 0 && pos < p.r.positions, mine = 8 * l < QK;
     const RotaryUnit unit = rotary_unit<MIXED>(p.r, mine ? l : 0, known ? pos : 0);
-    auto from = [&](int head) {
-        return head < p.heads ? p.q + (size_t)at * p.ldq + head * QK
-                              : p.k + (size_t)at * p.ldk + (head - p.heads) * QK;
-    };
-    f4 a[H], b[H];
-#pragma unroll
-    for (int k = 0; k < H; k++) {
-        const float* head = from(min(first_head + side + SIDE * k, heads - 1));
-        a[k] = *reinterpret_cast<const f4*>(head + unit.a);
-        b[k] = *reinterpret_cast<const f4*>(head + unit.b);
-    }
+    const float* from = head < p.heads ? p.q + ((size_t)at * p.ldq + head * QK)
+                                       : p.k + ((size_t)at * p.ldk + (head - p.heads) * QK);
+    f4 a = *reinterpret_cast<const f4*>(from + unit.a), b = *reinterpret_cast<const f4*>(from + unit.b);
     Place place = {-1, 0};
-    if (first_head + SIDE * H > p.heads && known) place = place_of(c, p.refs, p.row_seq[at], pos);
+    if (head >= p.heads && known) place = place_of(c, p.refs, p.row_seq[at], pos);
+    rotate_unit<MIXED>(p.r, unit, from, a, b);
+    if (!known || !mine) a = b = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    float peak = 0.0f;
 #pragma unroll
-    for (int k = 0; k < H; k++) {
-        const int head = first_head + side + SIDE * k;
-        if (head >= heads) continue;
-        rotate_unit<MIXED>(p.r, unit, from(head), a[k], b[k]);
-        if (!known || !mine) a[k] = b[k] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-        float peak = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 4; e++) peak = fmaxf(peak, fmaxf(fabsf(a[k][e]), fabsf(b[k][e])));
-        peak = fmaxf(peak, lane_xor<1>(peak));
-        peak = fmaxf(peak, lane_xor<2>(peak));
-        peak = fmaxf(peak, lane_xor<4>(peak));
-        if (L == 16) peak = fmaxf(peak, lane_xor<8>(peak));
-        const float scale = peak > 0.0f ? peak / 127.0f : 1.0f, inverse = 1.0f / scale;
-        int8_t* codes;
-        float* scales;
-        if (head < p.heads) {
-            const size_t to = (size_t)row * p.heads + head;
-            codes = p.codes + to * QK;
-            scales = p.q_scales + to;
-        } else {
-            const size_t cell = (((size_t)place.page * c.kv_heads + head - p.heads) << c.page_shift) + place.at;
-            codes = c.keys + cell * QK;
-            scales = c.kscale + cell;
-            if (place.page < 0) continue;
-        }
-        if (row >= p.rows) continue;
+    for (int e = 0; e < 4; e++) peak = fmaxf(peak, fmaxf(fabsf(a[e]), fabsf(b[e])));
+    peak = fmaxf(peak, lane_xor<1>(peak));
+    peak = fmaxf(peak, lane_xor<2>(peak));
+    peak = fmaxf(peak, lane_xor<4>(peak));
+    if (L == 16) peak = fmaxf(peak, lane_xor<8>(peak));
+    const float scale = peak > 0.0f ? peak / 127.0f : 1.0f, inverse = 1.0f / scale;
+    if (row >= p.rows || first_head + slot / kAppendRows >= heads) return;
+    auto put = [&](int8_t* codes, float* scales, size_t to) {
+        codes += to * QK;
         if (mine) {
-            *reinterpret_cast<uint32_t*>(codes + unit.a) =
-                ref_quantize4(make_float4(a[k][0], a[k][1], a[k][2], a[k][3]), inverse);
-            *reinterpret_cast<uint32_t*>(codes + unit.b) =
-                ref_quantize4(make_float4(b[k][0], b[k][1], b[k][2], b[k][3]), inverse);
+            *reinterpret_cast<uint32_t*>(codes + unit.a) = ref_quantize4(make_float4(a[0], a[1], a[2], a[3]), inverse);
+            *reinterpret_cast<uint32_t*>(codes + unit.b) = ref_quantize4(make_float4(b[0], b[1], b[2], b[3]), inverse);
         }
-        if (l == 0) *scales = scale;
-    }
+        if (l == 0) scales[to] = scale;
+    };
+    if (head < p.heads)
+        put(p.codes, p.q_scales, (size_t)row * p.heads + head);
+    else if (place.page >= 0)
+        put(c.keys, c.kscale, (((size_t)place.page * c.kv_heads + head - p.heads) << c.page_shift) + place.at);
 }
 
-// ROTARY: the keys go with the queries, H heads to a lane, in workgroups of
-// their own.
-template <int QK, int V, int H, bool MIXED, typename Params>
+// ROTARY: the keys go with the queries, in workgroups of their own.
+template <int QK, int V, bool MIXED, typename Params>
 __global__ __launch_bounds__(256) void paged_append_kernel(Params p)
 {
     constexpr bool ROTARY = std::is_same<Params, RotaryAppendParams>::value;
@@ -211,11 +191,11 @@ __global__ __launch_bounds__(256) void paged_append_kernel(Params p)
     const uint32_t share = ROTARY ? (all + 7) / 8 : gridDim.x * gridDim.y / 8;
     if constexpr (ROTARY) {
         if (id / 8 >= share) {
-            constexpr int heads = rotated_heads<QK, H>();
+            constexpr int heads = rotated_heads<QK>();
             const uint32_t sides = (p.heads + c.kv_heads + heads - 1) / heads, rotated = groups * sides;
             const uint32_t part = (id & 7) * ((rotated + 7) / 8) + id / 8 - share, group = part / sides;
             if (id / 8 - share < (rotated + 7) / 8 && part < rotated)
-                append_rotated<QK, H, MIXED>(p, (part - group * sides) * heads, (int)group * N);
+                append_rotated<QK, MIXED>(p, (part - group * sides) * heads, (int)group * N);
             return;
         }
     }
@@ -323,36 +303,30 @@ __global__ __launch_bounds__(256) void paged_append_kernel(Params p)
     }
 }
 
-template <int QK, int V, int H, bool MIXED, typename Params>
+template <int QK, int V, bool MIXED, typename Params>
 void launch_append(const Params& p, unsigned groups, hipStream_t stream)
 {
     const unsigned x = std::min((groups + 7) / 8 * 8, 1u << 20);  // (a multiple of 8)
-    hipLaunchKernelGGL((paged_append_kernel<QK, V, H, MIXED, Params>), dim3(x, (groups + x - 1) / x), dim3(256), 0,
-                       stream, p);
+    hipLaunchKernelGGL((paged_append_kernel<QK, V, MIXED, Params>), dim3(x, (groups + x - 1) / x), dim3(256), 0, stream,
+                       p);
 }
 unsigned row_groups(int rows) { return (unsigned)(rows + kAppendRows - 1) / kAppendRows; }
 template <int QK, int V>
 void launch_append(const AppendParams& p, hipStream_t stream)
 {
-    launch_append<QK, V, 1, false>(p, row_groups(p.rows) * p.c.kv_heads, stream);
+    launch_append<QK, V, false>(p, row_groups(p.rows) * p.c.kv_heads, stream);
 }
 template <int QK, int V>
 void launch_append(const RotaryAppendParams& p, hipStream_t stream)
 {
+    constexpr unsigned side = rotated_heads<QK>();
     const unsigned heads = p.heads + p.c.kv_heads, groups = row_groups(p.rows);
     // (each XCD's share of either kind of workgroup, rounded up)
-    auto workgroups = [&](unsigned side) {
-        return (groups * p.c.kv_heads + 7) / 8 * 8 + (groups * ((heads + side - 1) / side) + 7) / 8 * 8;
-    };
-    // Four heads a lane read a unit's cos and sin once for them: us with one and with four for
-    // 1024 rows of 40 heads of 128 7.9 and 8.3, 4096 rows 32.0 and 27.2, 2048 of 14 heads of 48
-    // 4.5 and 5.1, 8192 of them 11.3 and 10.2.
+    const unsigned all = (groups * p.c.kv_heads + 7) / 8 * 8 + (groups * ((heads + side - 1) / side) + 7) / 8 * 8;
     if (p.r.dim % 8)
-        launch_append<QK, V, 1, true>(p, workgroups(rotated_heads<QK, 1>()), stream);
-    else if ((int64_t)p.rows * heads >= 1 << 16)
-        launch_append<QK, V, 4, false>(p, workgroups(rotated_heads<QK, 4>()), stream);
+        launch_append<QK, V, true>(p, all, stream);
     else
-        launch_append<QK, V, 1, false>(p, workgroups(rotated_heads<QK, 1>()), stream);
+        launch_append<QK, V, false>(p, all, stream);
 }
 
 template <typename Params>
