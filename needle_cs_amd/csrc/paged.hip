@@ -106,11 +106,12 @@ __device__ __forceinline__ float group_max(float v)
 struct Place {
     int page, at;
 };
-// Heads that one workgroup rotates, side by side.
+// Heads and rows that one workgroup rotates.
+constexpr int kRotatedHeads = 4;
 template <int QK>
-__host__ __device__ constexpr int rotated_heads()
+__host__ __device__ constexpr int rotated_rows()
 {
-    return 256 / (QK <= 64 ? 8 : 16) / kAppendRows;
+    return 256 / (QK <= 64 ? 8 : 16) / kRotatedHeads;
 }
 __device__ __forceinline__ Place place_of(const PagedLayer& c, const int32_t* refs, int seq, int pos)
 {
@@ -137,8 +138,8 @@ __device__ __forceinline__ void append_rotated(const RotaryAppendParams& p, int 
     constexpr int L = QK <= 64 ? 8 : 16;
     const PagedLayer& c = p.c;
     const int l = threadIdx.x % L, slot = threadIdx.x / L;
-    const int row = row0 + slot % kAppendRows, at = min(row, p.rows - 1);
-    const int heads = p.heads + c.kv_heads, head = min(first_head + slot / kAppendRows, heads - 1);
+    const int row = row0 + slot / kRotatedHeads, at = min(row, p.rows - 1);
+    const int heads = p.heads + c.kv_heads, head = min(first_head + slot % kRotatedHeads, heads - 1);
     const int pos = p.row_pos[at];
     const bool known = pos >= 0 && pos < p.r.positions, mine = 8 * l < QK;
     const RotaryUnit unit = rotary_unit<MIXED>(p.r, mine ? l : 0, known ? pos : 0);
@@ -157,7 +158,7 @@ __device__ __forceinline__ void append_rotated(const RotaryAppendParams& p, int 
     peak = fmaxf(peak, lane_xor<4>(peak));
     if (L == 16) peak = fmaxf(peak, lane_xor<8>(peak));
     const float scale = peak > 0.0f ? peak / 127.0f : 1.0f, inverse = 1.0f / scale;
-    if (row >= p.rows || first_head + slot / kAppendRows >= heads) return;
+    if (row >= p.rows || first_head + slot % kRotatedHeads >= heads) return;
     auto put = [&](int8_t* codes, float* scales, size_t to) {
         codes += to * QK;
         if (mine) {
@@ -191,11 +192,12 @@ __global__ __launch_bounds__(256) void paged_append_kernel(Params p)
     const uint32_t share = ROTARY ? (all + 7) / 8 : gridDim.x * gridDim.y / 8;
     if constexpr (ROTARY) {
         if (id / 8 >= share) {
-            constexpr int heads = rotated_heads<QK>();
-            const uint32_t sides = (p.heads + c.kv_heads + heads - 1) / heads, rotated = groups * sides;
+            constexpr int R = rotated_rows<QK>();
+            const uint32_t sides = (p.heads + c.kv_heads + kRotatedHeads - 1) / kRotatedHeads;
+            const uint32_t rotated = (p.rows + R - 1) / R * sides;
             const uint32_t part = (id & 7) * ((rotated + 7) / 8) + id / 8 - share, group = part / sides;
             if (id / 8 - share < (rotated + 7) / 8 && part < rotated)
-                append_rotated<QK, MIXED>(p, (part - group * sides) * heads, (int)group * N);
+                append_rotated<QK, MIXED>(p, (part - group * sides) * kRotatedHeads, (int)group * R);
             return;
         }
     }
@@ -319,10 +321,10 @@ void launch_append(const AppendParams& p, hipStream_t stream)
 template <int QK, int V>
 void launch_append(const RotaryAppendParams& p, hipStream_t stream)
 {
-    constexpr unsigned side = rotated_heads<QK>();
-    const unsigned heads = p.heads + p.c.kv_heads, groups = row_groups(p.rows);
+    constexpr unsigned R = rotated_rows<QK>();
+    const unsigned sides = (p.heads + p.c.kv_heads + kRotatedHeads - 1) / kRotatedHeads;
     // (each XCD's share of either kind of workgroup, rounded up)
-    const unsigned all = (groups * p.c.kv_heads + 7) / 8 * 8 + (groups * ((heads + side - 1) / side) + 7) / 8 * 8;
+    const unsigned all = (row_groups(p.rows) * p.c.kv_heads + 7) / 8 * 8 + ((p.rows + R - 1) / R * sides + 7) / 8 * 8;
     if (p.r.dim % 8)
         launch_append<QK, V, true>(p, all, stream);
     else
