@@ -738,7 +738,8 @@ typedef struct nhip_sampling {
     const float* top_p;
     const float* min_p;
 } nhip_sampling;
-/* The workspace needs no initialisation; calls that may overlap need one each. */
+/* (None is needed at present: 0, and d_workspace may be NULL.  One that is needs
+ * no initialisation, and calls that may overlap need one each.) */
 size_t nhip_sample_workspace(int32_t rows, int32_t n);
 int32_t nhip_sample_dev(const float* d_logits, int32_t ldx, int32_t n, int32_t rows, const nhip_sampling* s,
                         const uint32_t* d_mask, int32_t mask_ld, int32_t words, void* d_workspace,
