@@ -19,6 +19,7 @@
 
 #include "paged.hpp"
 #include "rotary.hpp"
+#include "stores.hpp"
 
 namespace nhip {
 
@@ -89,7 +90,6 @@ struct RotaryAppendParams : AppendParams {
 // One step's 16 rows take 4.5 us: a launch (2.5) and the chain sequence, page,
 // holders, store, which the codes are formed beside.
 constexpr int kAppendRows = 16;
-typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
 
 template <int L>
 __device__ __forceinline__ float group_max(float v)
@@ -144,7 +144,7 @@ __device__ __forceinline__ void append_rotated(const RotaryAppendParams& p, int 
     const int heads = p.heads + c.kv_heads, head = min(first_head + slot % kRotatedHeads, heads - 1);
     const int pos = p.row_pos[at];
     const bool known = pos >= 0 && pos < p.r.positions, mine = 8 * l < QK;
-    const RotaryUnit unit = rotary_unit<MIXED>(p.r, mine ? l : 0, known ? pos : 0);
+    const RotaryUnit unit = rotary_unit<MIXED>(p.r, QK, mine ? l : 0, known ? pos : 0);
     const float* from = head < p.heads ? p.q + ((size_t)at * p.ldq + head * QK)
                                        : p.k + ((size_t)at * p.ldk + (head - p.heads) * QK);
     f4 a = *reinterpret_cast<const f4*>(from + unit.a), b = *reinterpret_cast<const f4*>(from + unit.b);
@@ -364,6 +364,7 @@ struct ReadParams {
     float* k;
     float* v;
     int32_t ldk, ldv, rows;
+    bool away;
 };
 
 // 4 L threads take the keys or the values (blockIdx.y) of 16 rows of one kv
@@ -416,8 +417,7 @@ __global__ __launch_bounds__(256) void paged_read_kernel(ReadParams p)
             f4 y;
 #pragma unroll
             for (int e = 0; e < 4; e++) y[e] = (float)(int8_t)(codes[k] >> (8 * e)) * scale[k];
-            *reinterpret_cast<f4*>(p.k + (size_t)(row0 + i) * p.ldk + kvh * QK + 4 * l) =
-                cells[u][i] == (size_t)-1 ? none : y;
+            store_f4(p.k + (size_t)(row0 + i) * p.ldk + kvh * QK + 4 * l, cells[u][i] == (size_t)-1 ? none : y, p.away);
         }
         return;
     }
@@ -441,7 +441,7 @@ __global__ __launch_bounds__(256) void paged_read_kernel(ReadParams p)
                 f4 y;
 #pragma unroll
                 for (int e = 0; e < 4; e++) y[e] = (float)(int8_t)(codes[e] >> (8 * k)) * scale[k];
-                *reinterpret_cast<f4*>(to + (size_t)(first + k) * p.ldv) = y;
+                store_f4(to + (size_t)(first + k) * p.ldv, y, p.away);
             }
         }
         return;
@@ -456,7 +456,7 @@ __global__ __launch_bounds__(256) void paged_read_kernel(ReadParams p)
         f4 y;
 #pragma unroll
         for (int e = 0; e < 4; e++) y[e] = (float)from[16 * e] * scale;
-        *reinterpret_cast<f4*>(to + (size_t)i * p.ldv) = cell == (size_t)-1 ? none : y;
+        store_f4(to + (size_t)i * p.ldv, cell == (size_t)-1 ? none : y, p.away);
     }
 }
 
@@ -1016,7 +1016,8 @@ int32_t nhip_paged_read_dev(const nhip_paged_cache* c, int32_t layer, const int3
                  "paged read: row strides %d, %d below a row's columns", ldk, ldv);
     rc = ensure_device();
     if (rc) return rc;
-    const ReadParams p{paged_layer(c, layer), d_row_seq, d_row_pos, d_k, d_v, ldk, ldv, rows};
+    const ReadParams p{paged_layer(c, layer), d_row_seq, d_row_pos, d_k, d_v, ldk, ldv, rows,
+                       stored_away((int64_t)rows * c->kv_heads * ((d_k ? c->qk_dim : 0) + (d_v ? c->v_dim : 0)))};
     const unsigned units = row_groups(rows) * c->kv_heads, of_one = c->v_dim <= 64 ? 4 : 2;
     const dim3 grid((units + of_one - 1) / of_one, d_k && d_v ? 2 : 1);
     if (c->qk_dim == 48)

@@ -4,6 +4,7 @@
 #include <cmath>
 
 #include "rotary.hpp"
+#include "stores.hpp"
 
 namespace nhip {
 
@@ -110,6 +111,7 @@ struct RotateParams {
     const int32_t* row_pos;
     float* y;
     int32_t ldx, ldy, heads, head_dim, rows;
+    bool away;
 };
 
 // L threads a head, a unit each, and further heads of the row in turn, so that
@@ -128,7 +130,7 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateParams p)
         const float* from = p.x + (size_t)row * p.ldx;
         float* to = p.y + (size_t)row * p.ldy;
         for (int u = threadIdx.x % L; u < units; u += L) {
-            const RotaryUnit unit = rotary_unit<false>(p.r, u, pos);
+            const RotaryUnit unit = rotary_unit<false>(p.r, p.head_dim, u, pos);
             for (int h0 = slot; h0 < p.heads; h0 += kHeadsAhead * (256 / L)) {
                 rotary_f4 a[kHeadsAhead], b[kHeadsAhead];
 #pragma unroll
@@ -142,8 +144,8 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateParams p)
                     const int h = h0 + k * (256 / L);
                     if (h >= p.heads) break;
                     rotate_unit<false>(p.r, unit, nullptr, a[k], b[k]);
-                    *reinterpret_cast<rotary_f4*>(to + h * p.head_dim + unit.a) = a[k];
-                    *reinterpret_cast<rotary_f4*>(to + h * p.head_dim + unit.b) = b[k];
+                    store_f4(to + h * p.head_dim + unit.a, a[k], p.away);
+                    store_f4(to + h * p.head_dim + unit.b, b[k], p.away);
                 }
             }
         }
@@ -233,7 +235,8 @@ int32_t nhip_rotary_dev(const nhip_rotary* r, const float* d_x, int32_t ldx, int
     NHIP_REQUIRE(d_y != d_x || ldy == ldx, "rotary: heads rotated in place have their rows' stride");
     rc = ensure_device();
     if (rc) return rc;
-    const RotateParams p = {rotary_table(r), d_x, d_row_pos, d_y, ldx, ldy, heads, head_dim, rows};
+    const RotateParams p = {rotary_table(r), d_x, d_row_pos, d_y, ldx, ldy, heads, head_dim, rows,
+                            stored_away((int64_t)rows * heads * head_dim)};
     hipStream_t st = as_stream(stream);
     if (r->dim % 8 || head_dim % 8)
         hipLaunchKernelGGL(rotate_pairs_kernel, dim3(rows), dim3(256), 0, st, p);

@@ -21,13 +21,15 @@ struct RotaryTable {
 inline RotaryTable rotary_table(const nhip_rotary* r) { return {r->cos, r->sin, r->positions, r->dim, r->interleaved}; }
 
 typedef float rotary_f4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef float rotary_f2 __attribute__((ext_vector_type(2), aligned(4)));
 
 // Unit u of a head: eight of its elements, a .. a + 3 and b .. b + 3, with the
-// cos and sin of its pairs.  Where dim is a multiple of 8 a unit is four whole
-// pairs (or elements that stay), so that it is rotated in registers, and its
-// cos and sin, read once, serve every head of the row; else (MIXED, a variant
-// of its own for the registers) the partners and the table come from memory,
-// element by element.
+// cos and sin of its pairs.  Where dim and head_dim are multiples of 8 a unit is
+// four whole pairs (or elements that stay), so that it is rotated in registers,
+// and its cos and sin, read once, serve every head of the row; a and b lie half
+// of the rotated part (or of the rest) apart, so that neighbouring lanes' fours
+// make whole lines.  Else (MIXED, a variant of its own for the registers) the
+// partners and the table come from memory, element by element.
 struct RotaryUnit {
     int a, b;
     enum Kind { STAYS, HALVES, NEIGHBOURS, ANY } kind;
@@ -36,22 +38,26 @@ struct RotaryUnit {
 };
 
 template <bool MIXED>
-__device__ __forceinline__ RotaryUnit rotary_unit(const RotaryTable& r, int u, int pos)
+__device__ __forceinline__ RotaryUnit rotary_unit(const RotaryTable& r, int head_dim, int u, int pos)
 {
     const size_t row = (size_t)pos * (r.dim / 2);
     RotaryUnit x = {8 * u, 8 * u + 4, RotaryUnit::STAYS, {}, {}, r.cos + row, r.sin + row};
-    if (8 * u < r.dim) {
-        if (MIXED) {
-            x.kind = RotaryUnit::ANY;
-        } else {
-            x.kind = r.interleaved ? RotaryUnit::NEIGHBOURS : RotaryUnit::HALVES;
-            x.c = *reinterpret_cast<const rotary_f4*>(x.cos_row + 4 * u);
-            x.s = *reinterpret_cast<const rotary_f4*>(x.sin_row + 4 * u);
-            if (!r.interleaved) {
-                x.a = 4 * u;
-                x.b = 4 * u + r.dim / 2;
-            }
-        }
+    if (MIXED) {
+        if (8 * u < r.dim) x.kind = RotaryUnit::ANY;
+    } else if (8 * u >= r.dim) {
+        x.a = r.dim / 2 + 4 * u;
+        x.b = x.a + (head_dim - r.dim) / 2;
+    } else {
+        x.a = 4 * u;
+        x.b = 4 * u + r.dim / 2;
+        x.kind = r.interleaved ? RotaryUnit::NEIGHBOURS : RotaryUnit::HALVES;
+        const int pair = r.interleaved ? 2 * u : 4 * u, other = r.interleaved ? r.dim / 4 + 2 * u : 4 * u + 2;
+        const rotary_f2 c0 = *reinterpret_cast<const rotary_f2*>(x.cos_row + pair);
+        const rotary_f2 c1 = *reinterpret_cast<const rotary_f2*>(x.cos_row + other);
+        const rotary_f2 s0 = *reinterpret_cast<const rotary_f2*>(x.sin_row + pair);
+        const rotary_f2 s1 = *reinterpret_cast<const rotary_f2*>(x.sin_row + other);
+        x.c = rotary_f4{c0.x, c0.y, c1.x, c1.y};
+        x.s = rotary_f4{s0.x, s0.y, s1.x, s1.y};
     }
     return x;
 }

@@ -4,6 +4,7 @@
 #include <algorithm>
 
 #include "common.hpp"
+#include "stores.hpp"
 
 namespace nhip {
 namespace {
@@ -11,7 +12,6 @@ namespace {
 constexpr int32_t kMaxRows = 1 << 26, kMaxCols = 1 << 20;
 constexpr int kMaxGroups = 1 << 20;  // workgroups of a launch; they take the further rows in turn
 
-typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32_bytes __attribute__((aligned(1)));
 
 // Elements i .. i + 3 of a row of n, 0 past its end.
@@ -23,10 +23,10 @@ __device__ __forceinline__ float4 load4(const float* row, int i, int n)
     }
     return make_float4(i < n ? row[i] : 0.0f, i + 1 < n ? row[i + 1] : 0.0f, i + 2 < n ? row[i + 2] : 0.0f, 0.0f);
 }
-__device__ __forceinline__ void store4(float* row, int i, int n, float4 v)
+__device__ __forceinline__ void store4(float* row, int i, int n, float4 v, bool away)
 {
     if (i + 4 <= n) {
-        *reinterpret_cast<f4*>(row + i) = f4{v.x, v.y, v.z, v.w};
+        store_f4(row + i, f4{v.x, v.y, v.z, v.w}, away);
         return;
     }
     if (i < n) row[i] = v.x;
@@ -52,6 +52,7 @@ struct NormParams {
     int32_t ldx, ldd, lds, rows, cols, zero_centered;
     float eps;
     double inverse_cols;
+    bool away;
 };
 
 __device__ __forceinline__ float4 gain4(const NormParams& p, int i)
@@ -162,7 +163,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void add_rms_quantize_kernel(Nor
         for (int j = 0; j < G; j++) squares = squares4(v[j], squares);
         if (p.sum) {
 #pragma unroll
-            for (int j = 0; j < G; j++) store4(p.sum + row * p.lds, 4 * (t + T * j), p.cols, v[j]);
+            for (int j = 0; j < G; j++) store4(p.sum + row * p.lds, 4 * (t + T * j), p.cols, v[j], p.away);
         }
         const float r = inverse_rms(p, row_sum<T>(squares, sums));
         float peak = 0.0f;
@@ -192,7 +193,7 @@ __global__ __launch_bounds__(T) void add_rms_quantize_long_kernel(NormParams p)
         for (int i = first; i < p.cols; i += 4 * T) {
             const float4 v = sum4(p, row, i);
             squares = squares4(v, squares);
-            if (p.sum) store4(p.sum + row * p.lds, i, p.cols, v);
+            if (p.sum) store4(p.sum + row * p.lds, i, p.cols, v, p.away);
         }
         const float r = inverse_rms(p, row_sum<T>(squares, sums));
         auto again = [&](int i) {
@@ -229,7 +230,7 @@ void launch_norm(const NormParams& p, hipStream_t stream)
 // 25.6 us, 6.5 TB/s.
 template <int L>
 __global__ __launch_bounds__(256) void dequantize_rows_kernel(const int8_t* q, const float* scales, int rows, int cols,
-                                                             float* x, int ldx)
+                                                             float* x, int ldx, bool away)
 {
     const int l = threadIdx.x % L;
     for (size_t row = (size_t)blockIdx.x * (256 / L) + threadIdx.x / L; row < (size_t)rows;
@@ -244,7 +245,8 @@ __global__ __launch_bounds__(256) void dequantize_rows_kernel(const int8_t* q, c
                 for (int e = 0; i + e < cols; e++) c |= (uint32_t)(uint8_t)from[i + e] << (8 * e);
             store4(x + row * ldx, i, cols,
                    make_float4((float)(int8_t)c * scale, (float)(int8_t)(c >> 8) * scale,
-                               (float)(int8_t)(c >> 16) * scale, (float)(int8_t)(c >> 24) * scale));
+                               (float)(int8_t)(c >> 16) * scale, (float)(int8_t)(c >> 24) * scale),
+                   away);
         }
     }
 }
@@ -253,7 +255,7 @@ template <int L>
 void launch_dequantize(const int8_t* q, const float* scales, int rows, int cols, float* x, int ldx, hipStream_t stream)
 {
     hipLaunchKernelGGL((dequantize_rows_kernel<L>), dim3(std::min((rows + 256 / L - 1) / (256 / L), kMaxGroups)),
-                       dim3(256), 0, stream, q, scales, rows, cols, x, ldx);
+                       dim3(256), 0, stream, q, scales, rows, cols, x, ldx, stored_away((int64_t)rows * cols));
 }
 
 int32_t check_rows(const char* what, int32_t rows, int32_t cols)
@@ -287,7 +289,8 @@ int32_t nhip_add_rms_quantize_dev(const float* d_x, int32_t ldx, const float* d_
     rc = ensure_device();
     if (rc) return rc;
     const NormParams p = {d_x,      d_delta, d_gain, d_sum, d_q,  d_scales, ldx,
-                          ldd, ld_sum,  rows,   cols,  zero_centered, eps, 1.0 / cols};
+                          ldd, ld_sum,  rows,   cols,  zero_centered, eps, 1.0 / cols,
+                          stored_away((int64_t)rows * cols)};
     hipStream_t s = as_stream(stream);
     if (cols <= 64)
         launch_norm<16, 1>(p, s);
