@@ -103,6 +103,13 @@ def test_norm_rows_by_columns(hip, rows, cols):
     NormCall(hip, np.random.default_rng(rows + cols), rows, cols, pads=(0, 3, 1)).check()
 
 
+@pytest.mark.parametrize("rows,cols", [(2101, 4003), (1030, 8192), (420, 20001), (140001, 60)])
+@pytest.mark.parametrize("total", ["sum", "x"])
+def test_norm_of_many_rows(hip, rows, cols, total):
+    """More than 32 MB, whose sums are stored past the caches."""
+    NormCall(hip, np.random.default_rng(cols), rows, cols, pads=(1, 2, 1)).check(total)
+
+
 def test_norm_rows_of_zeros_and_of_nothing(hip):
     call = NormCall(hip, np.random.default_rng(1), 6, 520)
     call.x[1] = call.delta[1] = 0
@@ -131,7 +138,8 @@ def test_norm_is_the_rows_calls_one_after_the_other(hip):
 
 @pytest.mark.parametrize("rows,cols,pad", [(1, 1, 0), (7, 3, 2), (1000, 48, 0), (333, 50, 1), (99, 64, 0), (65, 65, 3), (64, 128, 0),
                                            (300000, 5, 0), (20, 4096, 8), (3, 70001, 0),
-                                           (40, 129, 1), (9, 511, 0), (33, 512, 4), (31, 513, 0)])
+                                           (40, 129, 1), (9, 511, 0), (33, 512, 4), (31, 513, 0),
+                                           (70001, 121, 2), (8200, 1024, 0)])
 def test_dequantize(hip, rows, cols, pad):
     from needle_cs_amd.rows import dequantize_rows
     rng = np.random.default_rng(rows + cols)
@@ -243,6 +251,13 @@ def test_rotate(hip, rows, heads, head_dim, dim, pad, offset, interleaved):
     r.rotate(dx.ptr + 4 * offset, width + pad, heads, head_dim, dp.ptr, rows, dx.ptr + 4 * offset, width + pad)  # in place
     got = dx.download(np.float32)[offset:].reshape(rows, -1)
     assert np.array_equal(got[:, :width], want) and np.array_equal(got[:, width:], x[:, width:])
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("heads,head_dim,dim", [(32, 128, 128), (32, 128, 72), (40, 104, 8), (33, 64, 56)])
+def test_rotate_many_rows(hip, heads, head_dim, dim, interleaved):
+    """More than 32 MB, stored past the caches."""
+    test_rotate(hip, 8500000 // (heads * head_dim) + 1, heads, head_dim, dim, 3, 1, interleaved)
 
 
 @pytest.mark.parametrize("dim,head_dim", [(64, 64), (12, 20)])

@@ -164,6 +164,16 @@ def test_read(hip, qk, v, kv, page):
     check_read(hip, gpu, 1, [(1, int(p)) for p in rng.permutation(150)[:60]] + [(2, 3)] * 5)
 
 
+@pytest.mark.parametrize("consecutive", [False, True])
+def test_read_many_rows(hip, consecutive):
+    """More than 32 MB, stored past the caches."""
+    rng = np.random.default_rng(7)
+    pool = Pool(rng, 1, 40, 64, 4, 128, 128, 2, 8)
+    pool.give(rng, [500, 300])
+    at = np.tile(np.arange(499), 17) if consecutive else rng.integers(0, 500, 8400)
+    check_read(hip, Gpu(hip, pool), 0, [(0, int(p)) for p in at], pads=(1, 2))
+
+
 def test_read_out_of_range(hip):
     rng = np.random.default_rng(2)
     pool = Pool(rng, 1, 12, 16, 2, 48, 64, 3, 6)
