@@ -126,8 +126,9 @@ __device__ __forceinline__ Place place_of(const PagedLayer& c, const int32_t* re
 // L lanes a head, a unit of eight elements each.  Heads from p.heads on are the
 // keys'.  A lane's eight elements are two 16-byte loads and two 4-byte stores of
 // codes; the peak is the maximum over L lanes.  Bytes bound it: 8185 rows of
-// 32 + 8 heads of 128 and their values, 205 MB read and 52 written, take 56 to
-// 61 us, 4.2 to 4.6 TB/s.  What it took before: 84 where the XCDs' shares of
+// 32 + 8 heads of 128 and their values, 205 MB read and 52 written, take 46 us,
+// 5.6 TB/s, behind passes that store past the caches; 56 to 61 behind others, as
+// all that follows here:  84 where the XCDs' shares of
 // these workgroups and the values' were uneven; 58 to 68 with a row's heads far
 // apart in the grid, for the table came from memory again for each; 62 to 65
 // with 16 rows of one head, whose reads are 512 bytes apart from one another.
@@ -373,7 +374,8 @@ struct ReadParams {
 // positions have in each of four dimensions, and has four rows' values; else a
 // value is a byte by itself, and a line of the cache is read 16 times (from L2).
 // Bytes bound it, four out for one in: 8185 rows of 8 kv heads of 128, 17 MB
-// read and 67 written, 19.3 to 20.4 us, 4.3 TB/s.
+// read and 67 written, 16.5 to 17.6 us, 4.8 to 5.1 TB/s (19.3 to 20.4 by
+// ordinary stores).
 template <int QK, int V>
 __global__ __launch_bounds__(256) void paged_read_kernel(ReadParams p)
 {

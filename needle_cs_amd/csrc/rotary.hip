@@ -116,8 +116,9 @@ struct RotateParams {
 
 // L threads a head, a unit each, and further heads of the row in turn, so that
 // a unit's cos and sin are read once a row.  Bytes bound it: 8185 rows of 40 heads
-// of 128 with 64 dimensions rotated, 337 MB read and written, take 63.5 us, 5.3
-// TB/s (113 with a pair a thread, whose accesses are 4 bytes wide); 3 rows of 12
+// of 128 with 64 dimensions rotated, 337 MB read and written, take 57.6 us, 5.9
+// TB/s (113 with a pair a thread, whose accesses are 4 bytes wide; 63.6 with two
+// neighbouring fours a lane for neighbouring pairs, by ordinary stores 62.3); 3 rows of 12
 // heads 2 us beside a launch.
 constexpr int kHeadsAhead = 4;  // loads in flight
 template <int L>
