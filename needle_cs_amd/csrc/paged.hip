@@ -127,14 +127,14 @@ __device__ __forceinline__ Place place_of(const PagedLayer& c, const int32_t* re
 // keys'.  A lane's eight elements are two 16-byte loads and two 4-byte stores of
 // codes; the peak is the maximum over L lanes.  Bytes bound it: 8185 rows of
 // 32 + 8 heads of 128 and their values, 205 MB read and 52 written, take 46 us,
-// 5.6 TB/s, behind passes that store past the caches; 56 to 61 behind others, as
-// all that follows here:  84 where the XCDs' shares of
-// these workgroups and the values' were uneven; 58 to 68 with a row's heads far
-// apart in the grid, for the table came from memory again for each; 62 to 65
-// with 16 rows of one head, whose reads are 512 bytes apart from one another.
-// Two or four heads a lane, for which the table is read once, take 39.2 and
-// 41.0 us in place of 40.0 from the last cache, for 512 rows 5.3 and 6.3 in
-// place of 5.1; eight neighbouring heads in place of four the same.
+// 5.6 TB/s, behind passes that store past the caches, and 56 to 61 behind others,
+// as all that follows here: 84 where the XCDs' shares of these workgroups and the
+// values' were uneven; 58 to 68 with a row's heads far apart in the grid, for the
+// table came from memory again for each; 62 to 65 with 16 rows of one head, whose
+// reads are 512 bytes apart from one another.  Two or four heads a lane, for which
+// the table is read once, take 39.2 and 41.0 us in place of 40.0 from the last
+// cache, for 512 rows 5.3 and 6.3 in place of 5.1; eight neighbouring heads in
+// place of four the same.
 template <int QK, bool MIXED>
 __device__ __forceinline__ void append_rotated(const RotaryAppendParams& p, int first_head, int row0)
 {
