@@ -41,15 +41,15 @@ class Rotary:
         self.ptr = C.addressof(self.view)
 
     @classmethod
-    def make(cls, positions: int, dim: int, interleaved: bool = False, **scaling) -> "Rotary":
-        """With a table of its own for `positions` positions (``rotary_table``'s `scaling`)."""
+    def make(cls, positions: int, dim: int, interleaved: bool = False, stream=None, **scaling) -> "Rotary":
+        """With a table of its own for `positions` positions (``rotary_table``'s `scaling`), filled on `stream`."""
         if positions <= 0 or dim <= 0:
             raise ValueError("a rotary table's sizes are positive")
         buffers = DeviceBuffer(2 * positions * dim), DeviceBuffer(2 * positions * dim)
         made = cls(buffers[0].ptr, buffers[1].ptr, positions, dim, interleaved)
         made.buffers = buffers
-        rotary_table(buffers[0].ptr, buffers[1].ptr, 0, positions, dim, **scaling)
-        check(lib().nhip_stream_sync(None))  # calls on any stream find it made
+        rotary_table(buffers[0].ptr, buffers[1].ptr, 0, positions, dim, stream=stream, **scaling)
+        check(lib().nhip_stream_sync(stream))  # calls on any stream find it made
         return made
 
     def rotate(self, x, ldx: int, heads: int, head_dim: int, row_pos, rows: int, y, ldy: int, stream=None) -> None:

@@ -329,3 +329,20 @@ def test_rows_on_a_stream_captured_and_replayed(hip):
         turned.zero()
         steps(None)
         assert np.array_equal(turned.download(np.float32).reshape(17, 768), want)
+
+
+def test_a_table_made_on_a_stream_is_read_by_another(hip):
+    """Behind work of that stream; the other reads at once."""
+    from needle_cs_amd.rotary import Rotary, rotary_table
+    stream, other = hip.Stream(), hip.Stream()
+    want = [b.download(np.float32) for b in Rotary.make(3000, 64, theta=500.0).buffers]
+    room = hip.DeviceBuffer(4 << 20), hip.DeviceBuffer(4 << 20)
+    for _ in range(20):
+        rotary_table(room[0].ptr, room[1].ptr, 0, 1 << 15, 64, stream=stream.ptr)
+    r = Rotary.make(3000, 64, theta=500.0, stream=stream.ptr)
+    x, pos = np.ones((3000, 64), dtype=np.float32), np.arange(3000, dtype=np.int32)
+    dx, dp, dy = hip.DeviceBuffer.from_array(x), hip.DeviceBuffer.from_array(pos), hip.DeviceBuffer(x.nbytes)
+    r.rotate(dx.ptr, 64, 1, 64, dp.ptr, 3000, dy.ptr, 64, other.ptr)
+    other.sync()
+    cos, sin = (w.reshape(3000, 32) for w in want)
+    assert np.array_equal(dy.download(np.float32).reshape(3000, 64), np.concatenate([cos - sin, cos + sin], axis=1))

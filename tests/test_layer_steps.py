@@ -214,3 +214,38 @@ def test_nothing_to_do_is_no_error():
     c.decode_sinks(0, None, None, 0, 12, None, None, None, 4, 16, None, 0, None)
     c.prompt_sinks(0, None, None, 0, 12, 0, None, None, None, 8, 4, 16, None, 0, None)
     sample(None, 100, 100, 0, Sampling(), None, 0, 0, None, 0, None, None)
+
+
+class Recorded:
+    """A library that does nothing and says what was called, in order, and on which stream."""
+
+    def __init__(self):
+        self.calls, self.at = [], 0x100000
+
+    def nhip_malloc(self, p, size):
+        p._obj.value = self.at
+        self.at += size
+        return 0
+
+    def nhip_free(self, p):
+        return 0
+
+    def nhip_rotary_table_dev(self, *args):
+        self.calls.append(("table", args[-1]))
+        return 0
+
+    def nhip_stream_sync(self, stream):
+        self.calls.append(("sync", stream))
+        return 0
+
+
+@pytest.mark.parametrize("stream", [None, 0x7000])
+def test_a_table_is_whole_when_it_is_given_out(monkeypatch, stream):
+    """Rotary.make waits for the stream that fills its table, whichever that is."""
+    import needle_cs_amd.rotary
+    fake = Recorded()
+    for module in (N, needle_cs_amd.rotary):
+        monkeypatch.setattr(module, "lib", lambda: fake)
+    made = Rotary.make(10, 8, True, theta=500.0, stream=stream)
+    assert fake.calls == [("table", stream), ("sync", stream)]
+    made.close()
