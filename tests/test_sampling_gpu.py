@@ -262,6 +262,28 @@ def test_values_that_are_no_numbers(hip):
             Call(hip, x, rng.random(12), t, k, p, m).check()
 
 
+@pytest.mark.parametrize("n", [3, 900, 3001, 40003])
+def test_signalling_nans(hip, n):
+    """A NaN of any pattern is no id: quiet and signalling ones of both signs, in every row but the last alone
+    among numbers, beside an infinity, and everywhere."""
+    rng = np.random.default_rng(n)
+    patterns = np.array([0x7F800001, 0xFF800001, 0x7FBFFFFF, 0xFFBFFFFF, 0x7FC00000, 0xFFFFFFFF], dtype=np.uint32)
+    for k, p, m in ((0, 1.0, 0.0), (1, 1.0, 0.0), (40, 0.9, 0.0), (0, 0.5, 0.0), (700, 0.9, 0.01)):
+        x = logits(rng, 16, n)
+        bits = x.view(np.uint32)
+        for r in range(6):
+            bits[r, ::2] = patterns[r]
+            bits[r + 6, 0] = patterns[r]
+        bits[12, 1:] = rng.choice(patterns, n - 1)
+        bits[13] = rng.choice(patterns, n)
+        bits[14, 2:] = rng.choice(patterns, n - 2)
+        x[14, 1] = INF
+        mask = rng.random((16, n)) < 0.9
+        for t in (0.0, 1.0):
+            Call(hip, x, rng.random(16), t, k, p, m).check()
+            Call(hip, x, rng.random(16), t, k, p, m, mask, pad=1, offset=1).check()
+
+
 def test_masks(hip):
     rng = np.random.default_rng(6)
     x = logits(rng, 9, 10000)
