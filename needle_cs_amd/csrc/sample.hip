@@ -635,9 +635,9 @@ __device__ __forceinline__ Chosen draw_of_few(Shared<T>& sh, const Scale& z, con
     larger = shared_sum(larger, s.threads);
     rank = shared_sum(rank, s.threads);
     bool kept = first && (rules.top_k == 0 || rank < (u64)rules.top_k);
+    if (rules.by_mass && kept) atomicMax(&sh.mass, larger + w);  // (the last one has all)
+    __syncthreads();  // (and every thread has read the weights, of which those below are set to 0)
     if (rules.by_mass) {
-        if (kept) atomicMax(&sh.mass, larger + w);  // (the last one has all)
-        __syncthreads();
         const u64 mass = sh.mass;
         const Limit limit = mass_limit(rules.top_p, rules.top_k ? mass : total0);
         kept = kept && limit.inside(larger);

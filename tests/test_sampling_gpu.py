@@ -262,6 +262,18 @@ def test_values_that_are_no_numbers(hip):
             Call(hip, x, rng.random(12), t, k, p, m).check()
 
 
+@pytest.mark.parametrize("rows,n", [(64, 5000), (300, 9000), (64, 20000)])
+@pytest.mark.parametrize("top_k", [3, 16, 17, 64, 65, 128, 200, 512])
+def test_few_kept_of_those_listed(hip, rows, n, top_k):
+    """min_p behind top_k alone: of the ids that are ranked against one another, by 16, 4 and 2 threads each, any
+    number is dropped before the draw, none among them."""
+    rng = np.random.default_rng(n + top_k)
+    for grid in (0.0, 0.5):
+        x = logits(rng, rows, n, grid)
+        for min_p in (0.9, 0.3, 0.05, 1e-4):
+            Call(hip, x, rng.random(rows), 1.0, top_k, None, min_p).check()
+
+
 @pytest.mark.parametrize("n", [3, 900, 3001, 40003])
 def test_signalling_nans(hip, n):
     """A NaN of any pattern is no id: quiet and signalling ones of both signs, in every row but the last alone
