@@ -579,10 +579,13 @@ struct Split {
 //                       dims of 128   9.5 12.6 16.7 21.8             11.9 17.3 17.2 21.3
 //   256 workgroups,     dims of 64    8.2 10.4 12.8 17.4             11.3 13.9 16.8 21.3
 //                       dims of 128  12.0 15.9 20.9 31.3             15.7 19.8 24.4 37.3
-// So rows stay whole up to 18 blocks (for few workgroups the two meet a little
-// above for dims of 64, a little below for 128; so a block of sinks beside a
-// window of 1024 makes 19 for dims of 64, where 3 rows on 3 kv heads take 7.4 us
-// whole and 8.2 in parts, 11.5 and 10.2 for dims of 128), or up to 40 where the
+// So rows stay whole up to 18 blocks, for dims of 64 up to 19, whichever of them
+// hold sinks: 3 rows on 2 kv heads of 48 / 64, 12 heads, take at 18 to 22 blocks
+//   without sinks     7.4 7.5 7.5 7.5 8.4 us   parts  8.3 8.3 8.3 8.2 8.3
+//   one block of them 7.5 7.5 7.6 7.6 8.5             8.3 8.3 8.3 8.3 8.3
+// (20 would gain as much), 8 rows on 4 7.4 at 19 and 7.7 in parts, 16 on 6 7.4 and
+// 8.7; for dims of 128 they meet at 17 or 18 (3 rows on 2 11.8 and 10.5 at 18, 16
+// on 6 12.0 and 11.8).  Or up to 40 where the
 // workgroups fill half the CUs (where 128 of them meet at 40 for dims of 128;
 // rows of very different lengths gain there by parts: 16 of 32 to 2400, 8 kv
 // heads of 128: 21.1 whole, 18.0 in parts).  Longer ones are cut into parts of
@@ -600,7 +603,7 @@ Split decode_split(const nhip_paged_cache* c, int32_t rows, int32_t max_count, i
     const int sink_blocks = (std::min(sinks, c->width * c->page_size) + 63) / 64;
     const int most = max_count / 64 + 2 + sink_blocks;
     Split s;
-    if (most <= 18 + (c->v_dim <= 64 ? std::min(sink_blocks, 1) : 0) || (most <= 40 && units >= 128)) {
+    if (most <= (c->v_dim <= 64 ? 19 : 18) || (most <= 40 && units >= 128)) {
         s.blocks = most;
     } else {
         const int64_t even = (most * units + 2047) / 2048, fewest = (most + kMaxParts - 1) / kMaxParts;

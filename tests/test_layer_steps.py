@@ -216,6 +216,22 @@ def test_nothing_to_do_is_no_error():
     sample(None, 100, 100, 0, Sampling(), None, 0, 0, None, 0, None, None)
 
 
+@pytest.mark.parametrize("dims,whole", [((48, 64), 19), ((64, 64), 19), ((128, 128), 18)])
+@pytest.mark.parametrize("sinks", [0, 1, 64, 65, 300])
+def test_rows_are_cut_by_their_blocks_alone(dims, whole, sinks):
+    """Where a decode call of few workgroups keeps a row in one part (and needs no workspace) is a number of blocks
+    of 64 positions, whichever of them hold sinks."""
+    c = cache(pages=4096, width=4096, qk_dim=dims[0], v_dim=dims[1])
+    for blocks in range(10, 24):
+        for extra in (0, 63):
+            max_count = 64 * (blocks - 2 - -(-sinks // 64)) + extra
+            need = c.decode_sinks_workspace(3, 12, sinks, max_count)
+            parts = -(-blocks // 8)
+            assert need == (0 if blocks <= whole else 3 * 12 * parts * (dims[1] + 2) * 4)
+            if sinks == 0:
+                assert need == c.decode_workspace(3, 12, max_count)
+
+
 class Recorded:
     """A library that does nothing and says what was called, in order, and on which stream."""
 

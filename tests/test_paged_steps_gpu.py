@@ -320,6 +320,21 @@ def test_decode_sinks_split(hip, qk, v, rows, kv, group):
         check_decode(gpu, 0, q, qs, spec, sinks, 5001)
 
 
+@pytest.mark.parametrize("qk,v", DIMS)
+@pytest.mark.parametrize("sinks", [0, 4, 65])
+def test_decode_sinks_at_the_longest_whole_rows(hip, qk, v, sinks):
+    """Rows of 17 to 21 blocks, with and without sinks: whole, and in parts."""
+    rng = np.random.default_rng(qk + sinks)
+    pool = Pool(rng, 1, 200, 16, 2, qk, v, 2, 110)
+    pool.give(rng, [1700, 1450])
+    gpu = Gpu(hip, pool)
+    q, qs = queries(rng, 4, 12, qk)
+    for blocks in range(17, 22):
+        n = 64 * (blocks - 2 - -(-sinks // 64)) + 20
+        # (63 positions into a block: as many blocks as a row of n can have)
+        check_decode(gpu, 0, q, qs, [(0, 127, n), (1, 191, n - 200), (1, 1450 - n, n), (0, 66, 5)], sinks, n)
+
+
 @pytest.mark.parametrize("kv", [16, 48])
 def test_decode_sinks_sorted(hip, kv):
     """Many whole rows, dealt out by their length."""
