@@ -1018,7 +1018,7 @@ extern "C" {
 
 size_t nhip_sample_workspace(int32_t rows, int32_t n)
 {
-    if (check_sample(rows, n)) return 0;
+    check_sample(rows, n);  // (for last_error; no call needs a workspace)
     return 0;
 }
 
@@ -1035,8 +1035,7 @@ int32_t nhip_sample_dev(const float* d_logits, int32_t ldx, int32_t n, int32_t r
     NHIP_REQUIRE(d_logits && s && s->random && d_ids, "sample: null pointer");
     rc = ensure_device();
     if (rc) return rc;
-    (void)d_workspace;
-    (void)workspace_bytes;
+    (void)d_workspace, (void)workspace_bytes;  // (none is needed: nhip_sample_workspace)
     SampleParams p = {d_logits, d_mask, *s, d_ids, d_logprobs, ldx, n, mask_ld, words, {}, -INFINITY};
     std::copy(kPower, kPower + kTerms, p.power);
     // Rows that 256 threads hold, and somewhat longer ones, which share a CU by threes, where there are

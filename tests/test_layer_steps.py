@@ -203,6 +203,19 @@ def test_sample_needs_its_settings_and_workspace():
                 sample(A, 1 << 19, 1 << 19, 1, Sampling(A), None, 0, 0, ws, size, A, A)
 
 
+@pytest.mark.parametrize("rows,n", [(1, 1), (1, 1 << 19), (65536, 100), (300, 131071), (0, 5)])
+def test_sampling_needs_no_workspace(rows, n):
+    """Of whatever size; that it is not asked for says tests/test_sampling_gpu.py."""
+    assert sample_workspace(rows, n) == 0
+
+
+@pytest.mark.parametrize("rows,n", [(65537, 100), (-1, 100), (1, 0), (1, (1 << 19) + 1)])
+def test_a_workspace_of_no_call_is_an_error(rows, n):
+    """0 like those that need none, so the reason is left for last_error."""
+    N.lib().nhip_rotary_table_dev(A, A, 0, 1, 3, None, None)
+    assert sample_workspace(rows, n) == 0 and "sample" in N.last_error()
+
+
 def test_nothing_to_do_is_no_error():
     c = cache()
     add_rms_quantize(None, 64, None, 0, None, 0, 1e-5, 0, 64, None, 0, None, None)

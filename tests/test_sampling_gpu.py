@@ -342,6 +342,18 @@ def test_without_logprobs_and_settings(hip):
     assert np.array_equal(ids, call.want()[0]) and (logprobs == 3).all()
 
 
+@pytest.mark.parametrize("n", [700, 32000, 131071])
+def test_without_a_workspace(hip, n):
+    """None of 0 bytes serves every way to a draw."""
+    from needle_cs_amd.sampling import sample, sample_workspace
+    rng = np.random.default_rng(n)
+    for t, k, p, m in ((0.0, 0, 1.0, 0.0), (1.0, 0, 1.0, 0.0), (1.0, 50, 0.9, 0.0), (1.0, 0, 0.9, 0.0), (1.0, 600, 1.0, 0.01)):
+        call = Call(hip, logits(rng, 3, n), rng.random(3), t, k, p, m)
+        assert sample_workspace(3, n) == 0
+        sample(call.dx.ptr, n, n, 3, call.sampling, None, 0, 0, None, 0, call.ids.ptr, call.logprobs.ptr)
+        assert np.array_equal(call.get()[0], call.want()[0])
+
+
 @pytest.mark.parametrize("rows,n", [(1, 32000), (3, 200000), (40, 32000)])
 def test_captured_and_replayed(hip, rows, n):
     """A graph on a stream of its own with new logits and numbers for every replay, eager calls on the same
