@@ -35,6 +35,7 @@ namespace {
 constexpr int kBins = 1024;    // of a histogram; in the first the last one holds what weighs nothing
 constexpr int kSegment = 256;  // ids of a wave's step, four a lane
 constexpr int kMaxIds = 1 << 19;
+constexpr int kFewIds = 16384;  // at most, of a row by 256 threads
 constexpr int kTerms = 10;
 constexpr double kOne = 4398046511104.0;  // 2^42, the weight of the largest logit
 constexpr float kLeastScore = -30.0f;     // e^-30 2^42 < 1/2: no weight
@@ -316,7 +317,15 @@ struct Shared {
     uint32_t listed[WAVES];
     uint32_t few_listed, bin, key;
     u64 cut, before, mass, total, least, most;
+
+    // what the sizes ask of one another
+    static_assert(kBins % T == 0, "find_bin gives every thread as many bins");
+    static_assert(OWN % kSegment == 0, "a row of LIST ids, its segments dealt to the waves in turn, fits their lists");
+    static_assert(2 * RANKED <= T && 2 * FEW <= T, "an id that is ranked has two threads or more (shares)");
+    static_assert(RANKED <= FEW, "draw_of_few's ids are copied into few");
+    static_assert((T == 256 ? kFewIds : kMaxIds) / kBins <= FEW, "draw_of_many's bin of neighbours fits few");
 };
+static_assert(sizeof(Shared<1024>) <= 160 * 1024 && 3 * sizeof(Shared<256>) <= 160 * 1024, "LDS of a CU");
 
 // The sum over the workgroup, in every thread.
 template <int T>
@@ -679,8 +688,8 @@ __device__ __forceinline__ Chosen draw_of_many(Shared<T>& sh, const Scale& z, co
     }
     const u64 total = block_sum(sh, sum), at = drawn(rules.random, total);
     // in the order of the ids: a few neighbours of them, then the id
-    static_assert(kMaxIds / kBins <= Shared<1024>::FEW, "a bin's ids are few");  // (the list has an id once)
-    const int shift = max(0, 32 - __builtin_clz(n - 1) - 10);  // (n > 1; at most 16384 for 256 threads)
+    // (the list has an id once, so that a bin has at most 2^shift)
+    const int shift = max(0, 32 - __builtin_clz(n - 1) - 10);  // (n > 1)
     clear_bins<T>(sh.counts, kBins);
     for (int e = lane; e < listed; e += 64) atomicAdd(&sh.counts[min(id_in(list[e]) >> shift, kBins - 1)], weights[e]);
     if (threadIdx.x == 0) sh.few_listed = 0;
@@ -1043,7 +1052,7 @@ int32_t nhip_sample_dev(const float* d_logits, int32_t ldx, int32_t n, int32_t r
     // for top_k 1000: 1 row of 4096 11.1 and 12.6, 14.0 and 15.2, 14.3 and 17.5; of 8192 12.0 and 12.9,
     // 18.1 and 17.4, 17.0 and 21.8; 300 rows of 8192 13.4 and 24.7, 23.3 and 34.3, 26.7 and 42.6; of 16384
     // 18.8 and 28.3, 34.4 and 42.7, 46.3 and 41.4; 128 rows of 32000 20.0 and 14.8, 48.4 and 30.1.
-    if (n <= 8192 || (n <= 16384 && rows > 256))
+    if (n <= 8192 || (n <= kFewIds && rows > 256))
         hipLaunchKernelGGL((sample_kernel<256>), dim3(rows), dim3(256), 0, as_stream(stream), p);
     else
         hipLaunchKernelGGL((sample_kernel<1024>), dim3(rows), dim3(1024), 0, as_stream(stream), p);
