@@ -374,8 +374,8 @@ struct ReadParams {
 // positions have in each of four dimensions, and has four rows' values; else a
 // value is a byte by itself, and a line of the cache is read 16 times (from L2).
 // Bytes bound it, four out for one in: 8185 rows of 8 kv heads of 128, 17 MB
-// read and 67 written, 16.5 to 17.6 us, 4.8 to 5.1 TB/s (19.3 to 20.4 by
-// ordinary stores).
+// read and 67 written, 19.3 to 20.4 us, 4.1 to 4.4 TB/s (16.5 to 17.6 past the
+// caches, which the call that reads them pays for: stores.hpp).
 template <int QK, int V>
 __global__ __launch_bounds__(256) void paged_read_kernel(ReadParams p)
 {
@@ -1018,8 +1018,9 @@ int32_t nhip_paged_read_dev(const nhip_paged_cache* c, int32_t layer, const int3
                  "paged read: row strides %d, %d below a row's columns", ldk, ldv);
     rc = ensure_device();
     if (rc) return rc;
+    const int64_t elements = (int64_t)rows * c->kv_heads * ((d_k ? c->qk_dim : 0) + (d_v ? c->v_dim : 0));
     const ReadParams p{paged_layer(c, layer), d_row_seq, d_row_pos, d_k, d_v, ldk, ldv, rows,
-                       stored_away((int64_t)rows * c->kv_heads * ((d_k ? c->qk_dim : 0) + (d_v ? c->v_dim : 0)))};
+                       stored_away(elements, kReadAway)};
     const unsigned units = row_groups(rows) * c->kv_heads, of_one = c->v_dim <= 64 ? 4 : 2;
     const dim3 grid((units + of_one - 1) / of_one, d_k && d_v ? 2 : 1);
     if (c->qk_dim == 48)

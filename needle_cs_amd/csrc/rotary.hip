@@ -237,7 +237,7 @@ int32_t nhip_rotary_dev(const nhip_rotary* r, const float* d_x, int32_t ldx, int
     rc = ensure_device();
     if (rc) return rc;
     const RotateParams p = {rotary_table(r), d_x, d_row_pos, d_y, ldx, ldy, heads, head_dim, rows,
-                            stored_away((int64_t)rows * heads * head_dim)};
+                            stored_away((int64_t)rows * heads * head_dim, kReadAway)};
     hipStream_t st = as_stream(stream);
     if (r->dim % 8 || head_dim % 8)
         hipLaunchKernelGGL(rotate_pairs_kernel, dim3(rows), dim3(256), 0, st, p);

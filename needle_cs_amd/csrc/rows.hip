@@ -257,7 +257,8 @@ template <int L>
 void launch_dequantize(const int8_t* q, const float* scales, int rows, int cols, float* x, int ldx, hipStream_t stream)
 {
     hipLaunchKernelGGL((dequantize_rows_kernel<L>), dim3(std::min((rows + 256 / L - 1) / (256 / L), kMaxGroups)),
-                       dim3(256), 0, stream, q, scales, rows, cols, x, ldx, stored_away((int64_t)rows * cols));
+                       dim3(256), 0, stream, q, scales, rows, cols, x, ldx,
+                       stored_away((int64_t)rows * cols, kSumsAway));
 }
 
 int32_t check_rows(const char* what, int32_t rows, int32_t cols)
@@ -292,7 +293,7 @@ int32_t nhip_add_rms_quantize_dev(const float* d_x, int32_t ldx, const float* d_
     if (rc) return rc;
     const NormParams p = {d_x,      d_delta, d_gain, d_sum, d_q,  d_scales, ldx,
                           ldd, ld_sum,  rows,   cols,  zero_centered, eps, 1.0 / cols,
-                          stored_away((int64_t)rows * cols)};
+                          stored_away((int64_t)rows * cols, kSumsAway)};
     hipStream_t s = as_stream(stream);
     if (cols <= 64)
         launch_norm<16, 1>(p, s);

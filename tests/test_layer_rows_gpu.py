@@ -260,6 +260,12 @@ def test_rotate_many_rows(hip, heads, head_dim, dim, interleaved):
     test_rotate(hip, 8500000 // (heads * head_dim) + 1, heads, head_dim, dim, 3, 1, interleaved)
 
 
+@pytest.mark.parametrize("heads,head_dim,dim,interleaved", [(32, 128, 128, False), (33, 64, 56, True)])
+def test_rotate_more_than_the_last_cache_keeps(hip, heads, head_dim, dim, interleaved):
+    """160 MB and more, apart and in place."""
+    test_rotate(hip, 40_000_000 // (heads * head_dim) + 1, heads, head_dim, dim, 3, 1, interleaved)
+
+
 @pytest.mark.parametrize("dim,head_dim", [(64, 64), (12, 20)])
 def test_rotate_leaves_rows_out_of_range(hip, dim, head_dim):
     from needle_cs_amd.rotary import Rotary

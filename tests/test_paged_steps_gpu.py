@@ -174,6 +174,23 @@ def test_read_many_rows(hip, consecutive):
     check_read(hip, Gpu(hip, pool), 0, [(0, int(p)) for p in at], pads=(1, 2))
 
 
+@pytest.mark.parametrize("qk,v", DIMS)
+@pytest.mark.parametrize("consecutive", [False, True])
+def test_read_more_than_the_last_cache_keeps(hip, qk, v, consecutive):
+    """160 MB and more: the rows of a few positions over and over, as small calls give them."""
+    rng = np.random.default_rng(8)
+    pool = Pool(rng, 1, 40, 64, 4, qk, v, 2, 8)
+    pool.give(rng, [500, 300])
+    gpu = Gpu(hip, pool)
+    few = np.arange(497) if consecutive else rng.integers(0, 500, 497)
+    check_read(hip, gpu, 0, [(0, int(p)) for p in few], pads=(1, 2))
+    want = read(hip, gpu, 0, [0] * 497, few, (1, 2))
+    times = 40_000_000 // (497 * 4 * (qk + v)) + 1
+    got = read(hip, gpu, 0, np.zeros(497 * times), np.tile(few, times), (1, 2))
+    for a, b in zip(got, want):
+        assert (a.reshape(times, *b.shape) == b).all()
+
+
 def test_read_out_of_range(hip):
     rng = np.random.default_rng(2)
     pool = Pool(rng, 1, 12, 16, 2, 48, 64, 3, 6)
