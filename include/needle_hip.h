@@ -218,7 +218,7 @@ int32_t nhip_dequantize_rows_dev(const int8_t* d_q, const float* d_scales, int32
  * d_sum have row strides ldx, ldd and ld_sum >= cols (columns of wider
  * matrices); d_sum may be d_x or d_delta (with its stride), and overlaps
  * nothing else.  A row with a NaN or an infinity has codes of no meaning, and
- * no effect on the others.  rows <= 2^26, cols <= 2^20. */
+ * no effect on the others.  0 < eps <= 1, rows <= 2^26, cols <= 2^20. */
 int32_t nhip_add_rms_quantize_dev(const float* d_x, int32_t ldx, const float* d_delta, int32_t ldd,
                                   const float* d_gain, int32_t zero_centered, float eps, int32_t rows, int32_t cols,
                                   float* d_sum, int32_t ld_sum, int8_t* d_q, float* d_scales, void* stream);
@@ -375,8 +375,11 @@ typedef struct nhip_rotary {
  *   NHIP_ROTARY_BANDS   the same by the turns themselves: r = clamp((original *
  *                       f_i / (2 pi) - low) / (high - low), 0, 1),
  *                       f_i / factor * (1 - r) + f_i * r
- * cos and sin are multiplied by magnitude (1 for none).  low, high and
- * original are used by the last two (0 < low < high, original > 0). */
+ * (PARTS is its formula where that leaves the words: with a hi below 0 every
+ * pair keeps f_i, with a lo above hi every one takes f_i / factor.)  cos and sin
+ * are multiplied by magnitude (1 for none).  theta in (1, 10^12], factor in [1,
+ * 10^6] (but for PLAIN, which has none), magnitude in (0, 10^6]; low, high and
+ * original are used by the last two (0 < low < high <= 10^9, 0 < original <= 10^9). */
 enum {
     NHIP_ROTARY_PLAIN = 0,
     NHIP_ROTARY_LINEAR = 1,
@@ -723,7 +726,8 @@ int32_t nhip_argmax_dev(const float* d_x, int32_t ldx, int32_t n, int32_t rows, 
  *          times all of them; always the first (>= 1 or NaN: all);
  *   min_p  of those, ids of weight >= min_p (at most 1; NaN: all).
  * With t = floor(random * total weight of the kept ids), d_ids[r] is the lowest
- * kept id for which the weights of the kept ids up to it exceed t.  A
+ * kept id for which the weights of the kept ids up to it exceed t.  (Sums are
+ * exact; the products random * and top_p * total are rounded to 64-bit floats.)  A
  * temperature <= 0 or NaN takes the first id; where the largest logit is +inf,
  * the ids that have it weigh 1 and the others 0.  random counts as
  * clamped to [0, 1) (NaN: 0).  d_logprobs (may be NULL) is ln(weight / total
@@ -738,8 +742,9 @@ typedef struct nhip_sampling {
     const float* top_p;
     const float* min_p;
 } nhip_sampling;
-/* (None is needed at present: 0, and d_workspace may be NULL.  One that is needs
- * no initialisation, and calls that may overlap need one each.) */
+/* (None is needed at present: 0, as for sizes that are refused, and d_workspace
+ * may be NULL.  One that is needs no initialisation, and calls that may overlap
+ * need one each.) */
 size_t nhip_sample_workspace(int32_t rows, int32_t n);
 int32_t nhip_sample_dev(const float* d_logits, int32_t ldx, int32_t n, int32_t rows, const nhip_sampling* s,
                         const uint32_t* d_mask, int32_t mask_ld, int32_t words, void* d_workspace,

@@ -134,7 +134,9 @@ __device__ __forceinline__ Place place_of(const PagedLayer& c, const int32_t* re
 // reads are 512 bytes apart from one another.  Two or four heads a lane, for which
 // the table is read once, take 39.2 and 41.0 us in place of 40.0 from the last
 // cache, for 512 rows 5.3 and 6.3 in place of 5.1; eight neighbouring heads in
-// place of four the same.
+// place of four the same.  MIXED, for dimensions that are no multiple of 8, is bound
+// by the element-wise reads of partners and table: the same rows with 60 rotated 97
+// (halves) and 107 (neighbours), 54.5 with 64; 16 rows 5.2 and 4.0.
 template <int QK, bool MIXED>
 __device__ __forceinline__ void append_rotated(const RotaryAppendParams& p, int first_head, int row0)
 {
@@ -374,8 +376,9 @@ struct ReadParams {
 // positions have in each of four dimensions, and has four rows' values; else a
 // value is a byte by itself, and a line of the cache is read 16 times (from L2).
 // Bytes bound it, four out for one in: 8185 rows of 8 kv heads of 128, 17 MB
-// read and 67 written, 19.3 to 20.4 us, 4.1 to 4.4 TB/s (16.5 to 17.6 past the
-// caches, which the call that reads them pays for: stores.hpp).
+// read and 67 written, 16.4 to 20.4 us, 4.1 to 5.1 TB/s (up to 2 less past the
+// caches, which the call that reads them pays for: stores.hpp); in no order, where a
+// value is a byte by itself, 26.4.
 template <int QK, int V>
 __global__ __launch_bounds__(256) void paged_read_kernel(ReadParams p)
 {

@@ -241,12 +241,19 @@ __device__ __forceinline__ int ordered_row(const DecodeParams& p, int place, Spa
 // Registers: the general form for dims of 128 has to stay within 168, which
 // three waves a SIMD share (32 rows of up to 32768: 276 us, 289 with 169).
 //
+// Loads overlap the products in part only: the wait for a block's table entries,
+// which are checked where they are loaded, is one for the next keys too (vector
+// loads return in order), and the scales that go from one block to the next are
+// waited for at its end, and the next values with them.
+//
 // SINKS: the row's blocks are its first positions' and its window's, one behind
-// the other; its own variant, so that the others keep their registers.  48 rows
+// the other; its own variant, so that the others keep their registers.  The
+// general form for dims of 128 has 168 itself by 12 bytes of scratch a lane, an
+// address that is read back before each block's keys.  48 rows
 // of up to 8192 positions and 16 sinks, 32 heads on 8 of 128: 159 us and 6 for
-// the join, 5.1 TB/s of reads, bound as the rows without sinks; 3 rows of 1024
-// and 4 sinks, 12 heads on 2 of 48 / 64: 7.7 us, by the latency of 19 blocks on
-// eight waves.
+// the join, 5.1 TB/s of reads, bound by these waits as the rows without sinks; 3
+// rows of 1024 and 4 sinks, 12 heads on 2 of 48 / 64: 7.7 us, by them in each of
+// the three rounds of 19 blocks on eight waves.
 template <int QK, int V, int W, bool ONE, bool SORTED, bool SINKS>
 __global__ __launch_bounds__(64 * W, QK <= 64 ? 4 : ONE || SORTED ? 2 : 3) void paged_decode_kernel(DecodeParams p)
 {

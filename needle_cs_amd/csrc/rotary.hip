@@ -154,7 +154,9 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateParams p)
 }
 
 // Dimensions that are no multiple of 8, where a unit of four pairs would pass
-// them: a thread takes a pair or, behind them, an element that stays.
+// them: a thread takes a pair or, behind them, an element that stays, by accesses
+// of 4 bytes, which bound it: 8000 rows of 40 heads of 80 with 20 rotated 85 us, 2.4
+// TB/s (41 by the other kernel with 24 rotated), of 64 heads of 50 67.
 __global__ __launch_bounds__(256) void rotate_pairs_kernel(RotateParams p)
 {
     const int half = p.r.dim / 2, units = half + p.head_dim - p.r.dim;

@@ -8,20 +8,27 @@
 // summation shows, those by atomics into LDS among them; a sum of 2^19 weights
 // stays below 2^62.
 //
-// A workgroup takes a row, which it reads one to four times, from L2 or the last
-// cache after the first, and keeps in registers where it is short.  It finds the largest logit, from its threads' own
-// largest a logit that what is kept will hardly fall below, and gathers the ids
-// above that into LDS, where the rules and the draw are ranks of few ids or
-// histograms of many.  A share of the mass is found by a histogram of the row,
-// which every wave has of its own part, so that it says where the draw falls
-// too.  Rows that keep more than the list holds or than the guess allowed, and
-// rows without rules, are walked instead.
+// A workgroup takes a row, which it keeps in registers where it is short, and reads
+// from L2 or the last cache after the first pass.  It finds the largest logit, from
+// its threads' own largest a logit that what is kept will hardly fall below, and
+// gathers the ids above that into LDS, where the rules and the draw are ranks of
+// few ids or histograms of many.  A share of the mass is found by a histogram of
+// the row, which every wave has of its own part, so that it says where the draw
+// falls too.  So a row whose kept ids fit the list is read one to four times.  Rows
+// that keep more than the list holds or than the guess allowed, and rows without
+// rules, are walked instead, behind the passes that found that out: for each rule
+// a histogram and the ids of the bin in which it ends (and where those are more
+// than are ranked, a finer histogram and its ids, seven times at most), then the
+// weights for the draw and the parts of the row in which it falls.
 //
 // One row is bound by the latency of the steps behind each pass: 32000 ids, the
-// first 50 and 0.95 of the mass 12.8 us (13.3 read twice), greedy 5.2.  250 rows of 131071 ids, a
-// CU each, in us: greedy 27 (131 MB, 4.9 TB/s), the first 50 48, 0.9 of the mass
-// 90, no rule 64, the first 5000 72, the first 30000 155, and 113 to 120 with a
-// mask and settings of every kind, where the row that takes longest counts.  A pass costs about 22 by the
+// first 50 and 0.95 of the mass 12.8 us (13.3 read twice), greedy 5.2.  Rows of
+// 131071 ids have a CU each however few they are; us for 1, 64 and 250 rows from
+// memory (normal logits of deviation 2.5): greedy 11, 14 and 29 (131 MB, 4.5 TB/s),
+// the first 50 and 0.95 of the mass 24, 27 and 51, 0.9 of the mass 77, 84 and 105,
+// no rule 41, 45 and 62, the first 5000 50, 53 and 70, the first 30000, which are
+// walked, 131, 158 and 193; 250 rows with a mask and settings of every kind 113 to
+// 120, where the row that takes longest counts.  A pass costs about 22 by the
 // reads, and 35 where it weighs: some 30 instructions an id, which all four SIMDs
 // of a CU issue without a gap.
 #include <algorithm>
